@@ -30,6 +30,10 @@
  *                          index rule of loopfuse/torch_backend/__init__.py:46-63
  *                          (out = buffer[block_table]), used as a store address. The reference
  *                          fills its caches on the host with torch.randn.
+ *   lf_plan_pages, lf_kv_append_packed_bf16, lf_packed_prefill_bf16, lf_shared_prefix_decode_bf16
+ *                          no counterpart in the reference, whose batches hold sequences of one
+ *                          length: a serving step over requests of different lengths, on the same
+ *                          cache layout and index rule.
  */
 #ifndef LF_SM100_H_
 #define LF_SM100_H_
@@ -41,7 +45,7 @@
 extern "C" {
 #endif
 
-#define LF_ABI_VERSION 5
+#define LF_ABI_VERSION 6
 
 typedef enum {
   LF_OK = 0,
@@ -60,6 +64,9 @@ typedef enum {
 #define LF_DEV_BAD_PAGE 2       /* block_table entry outside [0, n_pages)                   */
 #define LF_DEV_BOUNDS 3         /* debug-bounds build only: an index left its range; bits 8..
                                    say where. The access was skipped or clamped.            */
+
+#define LF_DEV_BAD_LENGTHS 4    /* a request's length is negative or the batch has more tokens than
+                                   the caller's buffers; lengths are cut to what fits          */
 
 /* Mask kinds (what the capture layer deduces from loopfuse::causal_mask / sliding_mask). */
 #define LF_MASK_NONE 0
@@ -204,6 +211,91 @@ typedef struct {
   int32_t* status;              /* optional device word */
 } LfKvAppendArgs;
 
+/* Requests of one lf_plan_pages call. */
+#define LF_MAX_REQUESTS 16384
+
+typedef struct {
+  const int32_t* kv_lens;     /* [B] tokens of each request that are in the cache already        */
+  const int32_t* new_lens;    /* [B] tokens that this step adds                                  */
+  const int32_t* free_pages;  /* [n_free] pages that nobody holds, taken from the front          */
+  int32_t* block_table;       /* [B, bt_blocks], in and out: entries of the new pages are written */
+  int32_t* cu_seqlens;        /* out [B + 1]: first row of each request in the packed batch      */
+  int32_t* seq_lens;          /* out [B]: kv_lens + new_lens                                     */
+  int32_t* slots;             /* out [num_tokens]: page * page_size + slot of each row; -1 past the
+                                 last token and where no page was left                          */
+  int32_t* positions;         /* out [num_tokens]: position in its request; 0 past the last token */
+  int32_t* pages_used;        /* out [1]: pages the step needs (may be more than n_free)         */
+  int64_t bt_stride;          /* elements between rows of block_table                           */
+  int32_t B, n_free, bt_blocks, page_size;
+  int32_t num_tokens;         /* rows of the packed batch, padding included                     */
+  int32_t* status;            /* optional device word                                           */
+} LfPagePlanArgs;
+
+typedef struct {
+  const void* k_new;    /* bf16 [T, Hkv, D], innermost stride 1 */
+  const void* v_new;
+  void* k_pool;         /* bf16 [n_pages, page_size, Hkv, D] */
+  void* v_pool;
+  const int32_t* slots; /* [T]: page * page_size + slot; negative = the row is not stored */
+  int32_t T, Hkv, D;    /* D in {64, 128} */
+  int32_t page_size, n_pages;
+  int64_t kn_stride[2], vn_stride[2];  /* element strides of (token, kv head) */
+  int64_t kp_stride[3], vp_stride[3];  /* (page, slot, kv head) */
+  int32_t* status;
+} LfKvAppendPackedArgs;
+
+typedef struct {
+  const void* q;          /* bf16 [T, Hq, D]: the requests' tokens one after the other */
+  const void* k;          /* dense: bf16 [Tk, Hkv, D]. paged: pool [n_pages, page_size, Hkv, D] */
+  const void* v;
+  void* out;              /* bf16 [T, Hq, D] */
+  const int32_t* cu_q;    /* device [B + 1]: request b has the query rows [cu_q[b], cu_q[b + 1]) */
+  const int32_t* cu_k;    /* dense: device [B + 1], the same for the keys */
+  const int32_t* kv_lens; /* paged: device [B], keys of each request (its query rows are the last) */
+  const int32_t* block_table;  /* paged: device [B, bt_blocks]; NULL = dense */
+  int32_t B, T, Tk, Hq, Hkv, D;  /* D in {64, 128}; Hq % Hkv == 0, Hq / Hkv <= 128 */
+  int64_t q_stride[2];    /* element strides of (token, head), multiples of 8 */
+  int64_t k_stride[3];    /* dense: (token, kv head, -). paged: (page, slot, kv head) */
+  int64_t v_stride[3];
+  int64_t o_stride[2];
+  int64_t bt_stride;
+  int32_t bt_blocks, page_size, n_pages;
+  float scale;
+  int32_t n_mod;
+  int32_t mod_op[LF_MAX_MODS];
+  float mod_arg[LF_MAX_MODS];
+  int32_t mask_kind;      /* LF_MASK_*: a request's query i of n sees key j of m up to j = i + m - n */
+  int32_t window;
+  void* workspace;        /* device, >= lf_packed_workspace_bytes(...) */
+  size_t workspace_bytes;
+  int32_t* status;
+} LfPackedArgs;
+
+typedef struct {
+  const void* q;          /* bf16 [B, Hkv, G, D]: the G query heads that share a kv head */
+  const void* k;          /* pool bf16 [n_pages, page_size, Hkv, D] */
+  const void* v;
+  void* out;              /* bf16 [B, Hkv, G, D] */
+  const int32_t* block_table;  /* device [B, bt_blocks] */
+  const int32_t* seq_lens;     /* device [B]: keys of each request, the shared ones included; 0 = none */
+  int32_t B, Hkv, G, D;   /* D in {64, 128}; G <= 128 */
+  int64_t q_stride[3];    /* (b, kv head, g) */
+  int64_t o_stride[3];
+  int64_t k_stride[3];    /* (page, slot, kv head) */
+  int64_t v_stride[3];
+  int64_t bt_stride;
+  int32_t bt_blocks, page_size, n_pages;
+  int32_t prefix_len;     /* keys below it are read through row 0 of the table, for all requests */
+  int32_t max_seq_len;    /* no request is longer (one that is, is cut); sizes the workspace */
+  float scale;
+  int32_t n_mod;
+  int32_t mod_op[LF_MAX_MODS];
+  float mod_arg[LF_MAX_MODS];
+  void* workspace;        /* device, >= lf_shared_prefix_workspace_bytes(...), 32-byte aligned */
+  size_t workspace_bytes;
+  int32_t* status;
+} LfSharedPrefixArgs;
+
 typedef struct {
   int32_t abi_version;
   int32_t device;         /* current CUDA device ordinal */
@@ -340,6 +432,41 @@ int lf_selftest_wait_timeout(int64_t limit_cycles, int32_t* status, int64_t* wai
  * [0, n_pages), is reported as LF_DEV_BAD_PAGE in `status` and that row is not written (the
  * kernel never stores outside the pools). Rows of different sequences must not share a page. */
 int lf_kv_append_bf16(const LfKvAppendArgs* args, void* stream);
+
+/* Where the new tokens of a step go: block tables, slots and positions of a batch of requests of
+ * different lengths, from the lengths alone, on the device. Request b holds ceil(kv_lens[b] /
+ * page_size) pages, named by its row of the table, and gets
+ * ceil((kv_lens[b] + new_lens[b]) / page_size) less those from the free list, requests in order.
+ * Too few free pages, a table that is too narrow or an old entry that is negative: LF_DEV_BAD_PAGE in
+ * `status`, entry and slot -1. A negative length counts as 0, tokens past num_tokens are dropped
+ * (LF_DEV_BAD_LENGTHS). The outputs must not overlap the inputs. */
+int lf_plan_pages(const LfPagePlanArgs* args, void* stream);
+
+/* The store that goes with it: row t of k_new / v_new to slot slots[t] of the pools (bit-exact). A
+ * slot outside the pool is reported as LF_DEV_BAD_PAGE and not written. Of rows with the same slot
+ * one wins. */
+int lf_kv_append_packed_bf16(const LfKvAppendPackedArgs* args, void* stream);
+
+/* Attention of packed requests of different lengths, one launch (or two: batches that do not fit the
+ * machine at once are ordered by length first, which takes the workspace). The mask is per request and
+ * aligned at its end; a row that sees no key is zeros (lf_prefill_bf16 gives NaN there). Offsets that
+ * are out of order or outside the tensors are cut to them; rows that no request holds are not written.
+ * The mod chain may hold multipliers, or the softcap form (MUL|DIV)* TANH (MUL|DIV)*, with a product of
+ * scale and multipliers that is not negative; anything else is LF_ERR_UNSUPPORTED. Keys and values of
+ * other requests, or of a page's unused slots, never reach a result, whatever they hold; within a
+ * request, a value row that a query does not see must be finite (its weight is zero). */
+int lf_packed_prefill_bf16(const LfPackedArgs* args, void* stream);
+/* Workspace of a call on the current device; 0 = none. */
+size_t lf_packed_workspace_bytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv);
+
+/* Decode attention of requests that share their first prefix_len tokens, with the pages of the shared
+ * ones read once for the whole batch: equal to lf_decode_paged_bf16 on each request with a table whose
+ * first entries are those of row 0, up to rounding. Score functions as for lf_packed_prefill_bf16. A
+ * request of length 0 gets zeros. The page that holds key prefix_len may hold shared keys too: they are
+ * read through row 0, the others through the request's own row. */
+int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* args, void* stream);
+size_t lf_shared_prefix_workspace_bytes(int32_t B, int32_t Hkv, int32_t G, int32_t D, int32_t prefix_len,
+                                        int32_t max_seq_len);
 
 /* 1 when the library was built with -DLF_DEBUG_BOUNDS (python -m loopfuse_b200.build
  * --debug-bounds -> liblf_sm100_dbg.so): every index that a kernel forms for a plain global

@@ -20,6 +20,8 @@ EXPORTS = [
     "lf_decode_bf16_static", "lf_prefill_kv_tile", "lf_prefill_q_tile", "lf_tile_map_cache_stats",
     "lf_kv_append_bf16", "lf_selftest_wait_timeout", "lf_add_bf16", "lf_debug_bounds",
     "lf_prefill_row_bias_bf16", "lf_prefill_form",
+    "lf_plan_pages", "lf_kv_append_packed_bf16", "lf_packed_prefill_bf16",
+    "lf_packed_workspace_bytes", "lf_shared_prefix_decode_bf16", "lf_shared_prefix_workspace_bytes",
 ]
 
 LF_STATIC_SCRATCH_BYTES = 8 << 20
@@ -71,6 +73,60 @@ class LfKvAppendArgs(C.Structure):
         ("kp_stride", C.c_int64 * 3), ("vp_stride", C.c_int64 * 3),
         ("bt_stride", C.c_int64), ("bt_blocks", C.c_int32), ("page_size", C.c_int32),
         ("n_pages", C.c_int32), ("status", C.c_void_p),
+    ]
+
+
+class LfPagePlanArgs(C.Structure):
+    _fields_ = [
+        ("kv_lens", C.c_void_p), ("new_lens", C.c_void_p), ("free_pages", C.c_void_p),
+        ("block_table", C.c_void_p), ("cu_seqlens", C.c_void_p), ("seq_lens", C.c_void_p),
+        ("slots", C.c_void_p), ("positions", C.c_void_p), ("pages_used", C.c_void_p),
+        ("bt_stride", C.c_int64), ("B", C.c_int32), ("n_free", C.c_int32),
+        ("bt_blocks", C.c_int32), ("page_size", C.c_int32), ("num_tokens", C.c_int32),
+        ("status", C.c_void_p),
+    ]
+
+
+class LfKvAppendPackedArgs(C.Structure):
+    _fields_ = [
+        ("k_new", C.c_void_p), ("v_new", C.c_void_p), ("k_pool", C.c_void_p),
+        ("v_pool", C.c_void_p), ("slots", C.c_void_p),
+        ("T", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32),
+        ("page_size", C.c_int32), ("n_pages", C.c_int32),
+        ("kn_stride", C.c_int64 * 2), ("vn_stride", C.c_int64 * 2),
+        ("kp_stride", C.c_int64 * 3), ("vp_stride", C.c_int64 * 3), ("status", C.c_void_p),
+    ]
+
+
+class LfPackedArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
+        ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("kv_lens", C.c_void_p),
+        ("block_table", C.c_void_p),
+        ("B", C.c_int32), ("T", C.c_int32), ("Tk", C.c_int32), ("Hq", C.c_int32),
+        ("Hkv", C.c_int32), ("D", C.c_int32),
+        ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3),
+        ("o_stride", C.c_int64 * 2), ("bt_stride", C.c_int64),
+        ("bt_blocks", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32),
+        ("scale", C.c_float), ("n_mod", C.c_int32),
+        ("mod_op", C.c_int32 * LF_MAX_MODS), ("mod_arg", C.c_float * LF_MAX_MODS),
+        ("mask_kind", C.c_int32), ("window", C.c_int32),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p),
+    ]
+
+
+class LfSharedPrefixArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
+        ("block_table", C.c_void_p), ("seq_lens", C.c_void_p),
+        ("B", C.c_int32), ("Hkv", C.c_int32), ("G", C.c_int32), ("D", C.c_int32),
+        ("q_stride", C.c_int64 * 3), ("o_stride", C.c_int64 * 3),
+        ("k_stride", C.c_int64 * 3), ("v_stride", C.c_int64 * 3), ("bt_stride", C.c_int64),
+        ("bt_blocks", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32),
+        ("prefix_len", C.c_int32), ("max_seq_len", C.c_int32),
+        ("scale", C.c_float), ("n_mod", C.c_int32),
+        ("mod_op", C.c_int32 * LF_MAX_MODS), ("mod_arg", C.c_float * LF_MAX_MODS),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p),
     ]
 
 
@@ -147,6 +203,17 @@ def load() -> C.CDLL:
                                          C.POINTER(C.c_int64), C.c_int64, C.c_void_p,
                                          C.c_void_p]
     lib.lf_paged_gather_bf16.restype = C.c_int
+    for name, args in (("lf_plan_pages", LfPagePlanArgs),
+                       ("lf_kv_append_packed_bf16", LfKvAppendPackedArgs),
+                       ("lf_packed_prefill_bf16", LfPackedArgs),
+                       ("lf_shared_prefix_decode_bf16", LfSharedPrefixArgs)):
+        fn = getattr(lib, name)
+        fn.argtypes = [C.POINTER(args), C.c_void_p]
+        fn.restype = C.c_int
+    lib.lf_packed_workspace_bytes.argtypes = [C.c_int32] * 4
+    lib.lf_packed_workspace_bytes.restype = C.c_size_t
+    lib.lf_shared_prefix_workspace_bytes.argtypes = [C.c_int32] * 6
+    lib.lf_shared_prefix_workspace_bytes.restype = C.c_size_t
     _lib = lib
     return lib
 

@@ -18,6 +18,31 @@ namespace lf {
 void set_cuda_error(cudaError_t e, const char* where);
 int check_launch(const char* where);
 
+// Division by a divisor fixed at launch time: q = (mulhi(n, mul) + n) >> shift (Granlund &
+// Montgomery's round-up method; exact for every 0 <= n < 2^31). The item decode of the
+// persistent kernels runs on one warp that gets few issue slots; real divisions (a few dozen
+// dependent instructions each) made it take thousands of clocks.
+struct FastDiv {
+  uint32_t mul, shift, d;
+  static FastDiv make(int32_t divisor) {
+    FastDiv f;
+    f.d = static_cast<uint32_t>(divisor);
+    f.shift = 0;
+    while ((1u << f.shift) < f.d) ++f.shift;
+    f.mul = static_cast<uint32_t>(((static_cast<uint64_t>(1) << 32) *
+                                   ((static_cast<uint64_t>(1) << f.shift) - f.d)) / f.d + 1);
+    return f;
+  }
+  __host__ __device__ __forceinline__ uint32_t div(uint32_t n) const {
+#ifdef __CUDA_ARCH__
+    const uint32_t hi = __umulhi(n, mul);
+#else
+    const uint32_t hi = static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> 32);
+#endif
+    return static_cast<uint32_t>((static_cast<uint64_t>(hi) + n) >> shift);
+  }
+};
+
 // ---------------------------------------------------------------------------------------
 // Programmatic dependent launch: a launch of several kernels (append -> decode, add -> attention ->
 // add), or call after call, hides each kernel's launch and set-up behind the end of the one before.

@@ -78,6 +78,12 @@ struct Lib {
   int (*kv_append)(const LfKvAppendArgs*, void*) = nullptr;
   int (*add)(const void*, const void*, void*, int32_t, int32_t, int32_t, int32_t, const int64_t*,
              const int64_t*, const int64_t*, void*) = nullptr;
+  int (*plan_pages)(const LfPagePlanArgs*, void*) = nullptr;
+  int (*kv_append_packed)(const LfKvAppendPackedArgs*, void*) = nullptr;
+  int (*packed_prefill)(const LfPackedArgs*, void*) = nullptr;
+  size_t (*packed_workspace)(int32_t, int32_t, int32_t, int32_t) = nullptr;
+  int (*shared_prefix)(const LfSharedPrefixArgs*, void*) = nullptr;
+  size_t (*shared_prefix_workspace)(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) = nullptr;
   PyObject* check = nullptr;  // _native.check(rc, what): raises LfError
 } lib;
 
@@ -649,6 +655,270 @@ void run_decode(const Tensor& q, const DecodeQuery& dq, const Tensor& k_in, cons
 }
 
 // ---------------------------------------------------------------------------------------
+// Requests of different lengths: page plan, packed append, packed prefill, shared-prefix decode
+// ---------------------------------------------------------------------------------------
+// Lengths, offsets and page lists are int32 vectors on the device (the host never reads them).
+void check_i32(const Tensor& t, const c10::Device& dev, const char* name, int64_t size) {
+  require_cuda(t, dev);
+  if (t.scalar_type() != at::kInt) type_error(std::string(name) + " must be int32");
+  if (t.dim() != 1 || (size >= 0 && t.size(0) != size) || (t.size(0) > 1 && t.stride(0) != 1))
+    value_error(std::string(name) + " must be a contiguous vector" +
+                (size >= 0 ? " of " + std::to_string(size) + " elements" : "") + ", got " +
+                shape_text(t.sizes()));
+}
+const int32_t* i32_ptr(const Tensor& t) { return static_cast<const int32_t*>(t.data_ptr()); }
+
+int32_t narrow_i32(int64_t v, const char* name) {
+  if (v < 0 || v > 0x7fffffff) value_error(std::string(name) + " is out of range: " + std::to_string(v));
+  return static_cast<int32_t>(v);
+}
+
+// Scratch of a call: from the caller's DecodeWorkspace, or an allocation of the call on its stream.
+struct Scratch {
+  Tensor held;
+  c10::DataPtr own;
+  void* get(size_t nbytes, PyObject* workspace, const Tensor& like) {
+    if (!nbytes) return nullptr;
+    if (workspace == Py_None) {
+      own = c10::cuda::CUDACachingAllocator::get()->allocate(nbytes);
+      return own.get();
+    }
+    held = workspace_tensor(workspace, nbytes, like,
+                            c10::cuda::getCurrentCUDAStream(like.device().index()).stream());
+    return held.data_ptr();
+  }
+};
+
+struct PagePlan {
+  Tensor cu, seq_lens, slots, positions, pages_used;
+};
+
+PagePlan run_plan_pages(const Tensor& kv_lens, const Tensor& new_lens, const Tensor& free_pages,
+                        const Tensor& table, int64_t page_size, int64_t num_tokens,
+                        const Tensor* status) {
+  const c10::Device dev = kv_lens.device();
+  check_i32(kv_lens, dev, "kv_lens", -1);
+  const int64_t B = kv_lens.size(0);
+  check_i32(new_lens, dev, "new_lens", B);
+  check_i32(free_pages, dev, "free_pages", -1);
+  require_cuda(table, dev);
+  // (Written in place: a converted copy would leave the caller's table as it was.)
+  if (table.scalar_type() != at::kInt) type_error("block_table must be int32");
+  if (table.dim() != 2 || table.size(0) != B || (table.size(1) > 1 && table.stride(1) != 1))
+    value_error("block_table must be [batch, blocks] with contiguous rows, got " +
+                shape_text(table.sizes()));
+  if (page_size <= 0) value_error("page_size must be positive");
+  const int64_t T = narrow_i32(num_tokens, "num_tokens");
+  // One allocation: slots, positions, offsets, lengths, count.
+  const Tensor all = at::empty({2 * T + 2 * B + 2}, at::TensorOptions().dtype(at::kInt).device(dev));
+  PagePlan r{all.narrow(0, 2 * T, B + 1), all.narrow(0, 2 * T + B + 1, B), all.narrow(0, 0, T),
+             all.narrow(0, T, T), all.narrow(0, 2 * T + 2 * B + 1, 1)};
+  LfPagePlanArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.kv_lens = i32_ptr(kv_lens);
+  a.new_lens = i32_ptr(new_lens);
+  a.free_pages = i32_ptr(free_pages);
+  a.block_table = static_cast<int32_t*>(table.data_ptr());
+  int32_t* base = static_cast<int32_t*>(all.data_ptr());
+  a.slots = base;
+  a.positions = base + T;
+  a.cu_seqlens = base + 2 * T;
+  a.seq_lens = base + 2 * T + B + 1;
+  a.pages_used = base + 2 * T + 2 * B + 1;
+  a.bt_stride = table.stride(0);
+  a.B = narrow_i32(B, "batch");
+  a.n_free = narrow_i32(free_pages.size(0), "free_pages");
+  a.bt_blocks = narrow_i32(table.size(1), "blocks");
+  a.page_size = narrow_i32(page_size, "page_size");
+  a.num_tokens = i32(T);
+  a.status = status_ptr(status);
+  check_rc(launch(dev, [&](void* st) { return lib.plan_pages(&a, st); }), "lf_plan_pages");
+  return r;
+}
+
+void run_kv_append_packed(const Tensor& kn, const Tensor& vn, const Tensor& k_pool,
+                          const Tensor& v_pool, const Tensor& slots, const Tensor* status) {
+  const c10::Device dev = kn.device();
+  for (const Tensor* t : {&kn, &vn, &k_pool, &v_pool}) require_cuda(*t, dev);
+  check_bf16(kn, "k_new");
+  check_bf16(vn, "v_new");
+  if (kn.dim() != 3 || vn.sizes() != kn.sizes())
+    value_error("k_new and v_new must be [T, Hkv, D], got " + shape_text(kn.sizes()) + " and " +
+                shape_text(vn.sizes()));
+  const Tensor kp = pool_view(k_pool, "k_pool"), vp = pool_view(v_pool, "v_pool");
+  if (kp.size(2) != kn.size(1) || kp.size(3) != kn.size(2) || vp.sizes() != kp.sizes())
+    value_error("pool shape mismatch: new " + shape_text(kn.sizes()) + " pool " +
+                shape_text(kp.sizes()));
+  check_i32(slots, dev, "slots", -1);
+  if (slots.size(0) < kn.size(0)) value_error("slots must have an entry for each new row");
+  LfKvAppendPackedArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.k_new = kn.data_ptr();
+  a.v_new = vn.data_ptr();
+  a.k_pool = kp.data_ptr();
+  a.v_pool = vp.data_ptr();
+  a.slots = i32_ptr(slots);
+  a.T = narrow_i32(kn.size(0), "T");
+  a.Hkv = i32(kn.size(1)), a.D = i32(kn.size(2));
+  a.page_size = narrow_i32(kp.size(1), "page_size");
+  a.n_pages = narrow_i32(kp.size(0), "pages");
+  for (int i = 0; i < 2; ++i) {
+    a.kn_stride[i] = kn.stride(i);
+    a.vn_stride[i] = vn.stride(i);
+  }
+  strides3(a.kp_stride, kp);
+  strides3(a.vp_stride, vp);
+  a.status = status_ptr(status);
+  check_rc(launch(dev, [&](void* st) { return lib.kv_append_packed(&a, st); }),
+           "lf_kv_append_packed_bf16");
+}
+
+struct PackedOptions {
+  double scale = 1.0;
+  Mods mods;
+  int mask_kind = 0, window = 0;
+};
+
+Tensor run_packed_prefill(const Tensor& q, const Tensor& k_in, const Tensor& v_in, const Tensor& cu_q,
+                          const Tensor* cu_k, const Tensor* table, const Tensor* seq_lens, Tensor out,
+                          PyObject* workspace, const Tensor* status, const PackedOptions& o) {
+  const c10::Device dev = q.device();
+  for (const Tensor* t : {&q, &k_in, &v_in}) require_cuda(*t, dev);
+  check_bf16(q, "q");
+  check_bf16(k_in, "k");
+  check_bf16(v_in, "v");
+  if (q.dim() != 3) value_error("q must be [T, Hq, D], got " + shape_text(q.sizes()));
+  check_i32(cu_q, dev, "cu_seqlens", -1);
+  const int64_t B = cu_q.size(0) - 1;
+  if (B <= 0) value_error("cu_seqlens must have an entry more than there are requests");
+  if (!table != !seq_lens) value_error("block_table and seq_lens go together");
+  if (table && cu_k) value_error("cu_seqlens_k is for packed keys: paged ones have seq_lens");
+  LfPackedArgs a;
+  std::memset(&a, 0, sizeof(a));
+  Tensor k = k_in, v = v_in, bt;
+  if (table) {
+    k = pool_view(k_in, "k");
+    v = pool_view(v_in, "v");
+    require_cuda(*table, dev);
+    bt = table_i32(*table);
+    check_i32(*seq_lens, dev, "seq_lens", B);
+    if (bt.size(0) != B) value_error("block_table batch mismatch");
+    if (bt.size(1) == 0) value_error("block_table has no blocks");
+    a.kv_lens = i32_ptr(*seq_lens);
+    a.block_table = i32_ptr(bt);
+    a.bt_stride = bt.stride(0);
+    a.bt_blocks = narrow_i32(bt.size(1), "blocks");
+    a.page_size = narrow_i32(k.size(1), "page_size");
+    a.n_pages = narrow_i32(k.size(0), "pages");
+    strides3(a.k_stride, k);
+    strides3(a.v_stride, v);
+  } else {
+    if (k.dim() != 3 || v.dim() != 3)
+      value_error("k and v must be [T, Hkv, D], got " + shape_text(k.sizes()) + " and " +
+                  shape_text(v.sizes()));
+    if (cu_k) check_i32(*cu_k, dev, "cu_seqlens_k", B + 1);
+    if (!cu_k && k.size(0) != q.size(0)) value_error("k and q must have the same tokens, or cu_seqlens_k");
+    a.cu_k = i32_ptr(cu_k ? *cu_k : cu_q);
+    a.Tk = narrow_i32(k.size(0), "keys");
+    for (int i = 0; i < 2; ++i) {
+      a.k_stride[i] = k.stride(i);
+      a.v_stride[i] = v.stride(i);
+    }
+  }
+  if (v.sizes() != k.sizes() || k.size(-1) != q.size(2))
+    value_error("shape mismatch: q " + shape_text(q.sizes()) + " k " + shape_text(k.sizes()) + " v " +
+                shape_text(v.sizes()));
+  const int64_t Hq = q.size(1), Hkv = k.size(-2);
+  if (Hkv == 0 || Hq % Hkv) value_error("Hq must be a multiple of Hkv");
+  if (!out.defined()) {
+    out = new_bf16(q.sizes(), dev);
+  } else {
+    require_cuda(out, dev);
+    check_bf16(out, "out");
+    if (out.sizes() != q.sizes()) value_error("out must have the shape of q");
+  }
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.out = out.data_ptr();
+  a.cu_q = i32_ptr(cu_q);
+  a.B = narrow_i32(B, "batch");
+  a.T = narrow_i32(q.size(0), "tokens");
+  a.Hq = i32(Hq), a.Hkv = i32(Hkv), a.D = i32(q.size(2));
+  for (int i = 0; i < 2; ++i) {
+    a.q_stride[i] = q.stride(i);
+    a.o_stride[i] = out.stride(i);
+  }
+  fill_mods(a, o.scale, o.mods);
+  a.mask_kind = o.mask_kind;
+  a.window = o.window;
+  a.status = status_ptr(status);
+  const c10::cuda::CUDAGuard guard(dev);
+  a.workspace_bytes = lib.packed_workspace(a.B, a.T, a.Hq, a.Hkv);
+  Scratch scratch;
+  a.workspace = scratch.get(a.workspace_bytes, workspace, q);
+  check_rc(launch(dev, [&](void* st) { return lib.packed_prefill(&a, st); }), "lf_packed_prefill_bf16");
+  return out;
+}
+
+Tensor run_shared_prefix(const Tensor& q, const Tensor& k_pool, const Tensor& v_pool, const Tensor& table,
+                         const Tensor& seq_lens, int64_t prefix_len, int64_t max_len, Tensor out,
+                         PyObject* workspace, const Tensor* status, double scale, const Mods& mods) {
+  const c10::Device dev = q.device();
+  for (const Tensor* t : {&q, &k_pool, &v_pool, &table}) require_cuda(*t, dev);
+  check_bf16(q, "q");
+  if (q.dim() != 4) value_error("q must be [B, Hkv, G, D], got " + shape_text(q.sizes()));
+  const Tensor k = pool_view(k_pool, "k_pool"), v = pool_view(v_pool, "v_pool");
+  const int64_t B = q.size(0);
+  if (k.size(2) != q.size(1) || k.size(3) != q.size(3) || v.sizes() != k.sizes())
+    value_error("pool shape mismatch: q " + shape_text(q.sizes()) + " pool " + shape_text(k.sizes()));
+  const Tensor bt = table_i32(table);
+  if (bt.size(0) != B) value_error("block_table batch mismatch");
+  check_i32(seq_lens, dev, "seq_lens", B);
+  const int64_t held = bt.size(1) * k.size(1);
+  if (max_len < 0) max_len = held;
+  if (prefix_len < 0 || prefix_len > held || max_len > held)
+    value_error("prefix_len and max_seq_len must lie in what the block table holds (" +
+                std::to_string(held) + " tokens)");
+  if (!out.defined()) {
+    out = new_bf16(q.sizes(), dev);
+  } else {
+    require_cuda(out, dev);
+    check_bf16(out, "out");
+    if (out.sizes() != q.sizes()) value_error("out must have the shape of q");
+  }
+  LfSharedPrefixArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.out = out.data_ptr();
+  a.block_table = i32_ptr(bt);
+  a.seq_lens = i32_ptr(seq_lens);
+  a.B = narrow_i32(B, "batch"), a.Hkv = i32(q.size(1)), a.G = i32(q.size(2)), a.D = i32(q.size(3));
+  strides3(a.q_stride, q);
+  strides3(a.o_stride, out);
+  strides3(a.k_stride, k);
+  strides3(a.v_stride, v);
+  a.bt_stride = bt.stride(0);
+  a.bt_blocks = narrow_i32(bt.size(1), "blocks");
+  a.page_size = narrow_i32(k.size(1), "page_size");
+  a.n_pages = narrow_i32(k.size(0), "pages");
+  a.prefix_len = narrow_i32(prefix_len, "prefix_len");
+  a.max_seq_len = narrow_i32(max_len, "max_seq_len");
+  fill_mods(a, scale, mods);
+  a.status = status_ptr(status);
+  const c10::cuda::CUDAGuard guard(dev);
+  a.workspace_bytes =
+      lib.shared_prefix_workspace(a.B, a.Hkv, a.G, a.D, a.prefix_len, a.max_seq_len);
+  Scratch scratch;
+  a.workspace = scratch.get(a.workspace_bytes, workspace, q);
+  check_rc(launch(dev, [&](void* st) { return lib.shared_prefix(&a, st); }),
+           "lf_shared_prefix_decode_bf16");
+  return out;
+}
+
+// ---------------------------------------------------------------------------------------
 // Python functions (positional arguments only; functional.py has the keyword forms)
 // ---------------------------------------------------------------------------------------
 void want_args(Py_ssize_t n, Py_ssize_t want) {
@@ -753,6 +1023,61 @@ PyObject* py_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
     strides3(os, out);
     run_decode(q, dq, k, v, nullptr, o, a[4], status, out, os);
     return THPVariable_Wrap(out);
+  });
+}
+
+// kv_lens, new_lens, free_pages, block_table, page_size, num_tokens, status
+PyObject* py_plan_pages(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    want_args(n, 7);
+    const PagePlan r = run_plan_pages(tensor_arg(a[0], "kv_lens"), tensor_arg(a[1], "new_lens"),
+                                      tensor_arg(a[2], "free_pages"), tensor_arg(a[3], "block_table"),
+                                      int_arg(a[4]), int_arg(a[5]), optional_tensor(a[6], "status"));
+    return Py_BuildValue("(NNNNN)", THPVariable_Wrap(r.cu), THPVariable_Wrap(r.seq_lens),
+                         THPVariable_Wrap(r.slots), THPVariable_Wrap(r.positions),
+                         THPVariable_Wrap(r.pages_used));
+  });
+}
+
+// k_new, v_new, k_pool, v_pool, slots, status
+PyObject* py_kv_append_packed(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    want_args(n, 6);
+    run_kv_append_packed(tensor_arg(a[0], "k_new"), tensor_arg(a[1], "v_new"),
+                         tensor_arg(a[2], "k_pool"), tensor_arg(a[3], "v_pool"),
+                         tensor_arg(a[4], "slots"), optional_tensor(a[5], "status"));
+    Py_RETURN_NONE;
+  });
+}
+
+// q, k, v, cu_seqlens, cu_seqlens_k, block_table, seq_lens, out, workspace, status, scale, mods,
+// mask_kind, window
+PyObject* py_packed_prefill(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    want_args(n, 14);
+    PackedOptions o;
+    o.scale = float_arg(a[10]);
+    o.mods = mods_arg(a[11]);
+    o.mask_kind = static_cast<int>(int_arg(a[12]));
+    o.window = narrow_i32(int_arg(a[13]), "window");
+    return THPVariable_Wrap(run_packed_prefill(
+        tensor_arg(a[0], "q"), tensor_arg(a[1], "k"), tensor_arg(a[2], "v"),
+        tensor_arg(a[3], "cu_seqlens"), optional_tensor(a[4], "cu_seqlens_k"),
+        optional_tensor(a[5], "block_table"), optional_tensor(a[6], "seq_lens"), out_arg(a[7]), a[8],
+        optional_tensor(a[9], "status"), o));
+  });
+}
+
+// q, k_pool, v_pool, block_table, seq_lens, prefix_len, max_seq_len, out, workspace, status, scale,
+// mods
+PyObject* py_shared_prefix_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    want_args(n, 12);
+    const int64_t max_len = a[6] == Py_None ? -1 : narrow_i32(int_arg(a[6]), "max_seq_len");
+    return THPVariable_Wrap(run_shared_prefix(
+        tensor_arg(a[0], "q"), tensor_arg(a[1], "k_pool"), tensor_arg(a[2], "v_pool"),
+        tensor_arg(a[3], "block_table"), tensor_arg(a[4], "seq_lens"), int_arg(a[5]), max_len,
+        out_arg(a[7]), a[8], optional_tensor(a[9], "status"), float_arg(a[10]), mods_arg(a[11])));
   });
 }
 
@@ -1063,6 +1388,12 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     get("lf_decode_launches", lib.launches);
     get("lf_kv_append_bf16", lib.kv_append);
     get("lf_add_bf16", lib.add);
+    get("lf_plan_pages", lib.plan_pages);
+    get("lf_kv_append_packed_bf16", lib.kv_append_packed);
+    get("lf_packed_prefill_bf16", lib.packed_prefill);
+    get("lf_packed_workspace_bytes", lib.packed_workspace);
+    get("lf_shared_prefix_decode_bf16", lib.shared_prefix);
+    get("lf_shared_prefix_workspace_bytes", lib.shared_prefix_workspace);
     Py_INCREF(a[1]);
     Py_XSETREF(lib.check, a[1]);
     Py_RETURN_NONE;
@@ -1078,6 +1409,10 @@ PyMethodDef methods[] = {
     {"paged_decode", LF_FAST(py_paged_decode), "launch lf_decode_paged_bf16"},
     {"kv_append", LF_FAST(py_kv_append), "launch lf_kv_append_bf16"},
     {"add", LF_FAST(py_add), "launch lf_add_bf16"},
+    {"plan_pages", LF_FAST(py_plan_pages), "launch lf_plan_pages"},
+    {"kv_append_packed", LF_FAST(py_kv_append_packed), "launch lf_kv_append_packed_bf16"},
+    {"packed_prefill", LF_FAST(py_packed_prefill), "launch lf_packed_prefill_bf16"},
+    {"shared_prefix_decode", LF_FAST(py_shared_prefix_decode), "launch lf_shared_prefix_decode_bf16"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host",

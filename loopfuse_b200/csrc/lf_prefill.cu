@@ -34,9 +34,8 @@
 // between the CTAs of one kv head.
 #include "lf_common.cuh"
 #include "lf_skip_range.h"
+#include "lf_tensor_map.h"
 
-#include <cuda.h>
-#include <cudaTypedefs.h>
 #include <float.h>
 #include <math.h>
 
@@ -84,31 +83,6 @@ constexpr float kBoundedMaxC2 = 80.f;
 // logit2 = (raw * a + bias) * c2: the usual biased attention, a scale and an additive score bias with
 // nothing behind it. (Any other chain around a bias is generic.)
 constexpr int kModeBias = 4;
-
-// Division by a divisor fixed at launch time: q = (mulhi(n, mul) + n) >> shift (Granlund &
-// Montgomery's round-up method; exact for every 0 <= n < 2^31). The item decode of the
-// persistent kernels runs on one warp that gets few issue slots; real divisions (a few dozen
-// dependent instructions each) made it take thousands of clocks.
-struct FastDiv {
-  uint32_t mul, shift, d;
-  static FastDiv make(int32_t divisor) {
-    FastDiv f;
-    f.d = static_cast<uint32_t>(divisor);
-    f.shift = 0;
-    while ((1u << f.shift) < f.d) ++f.shift;
-    f.mul = static_cast<uint32_t>(((static_cast<uint64_t>(1) << 32) *
-                                   ((static_cast<uint64_t>(1) << f.shift) - f.d)) / f.d + 1);
-    return f;
-  }
-  __host__ __device__ __forceinline__ uint32_t div(uint32_t n) const {
-#ifdef __CUDA_ARCH__
-    const uint32_t hi = __umulhi(n, mul);
-#else
-    const uint32_t hi = static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> 32);
-#endif
-    return static_cast<uint32_t>((static_cast<uint64_t>(hi) + n) >> shift);
-  }
-};
 
 struct PrefillParams {
   __nv_bfloat16* out;
@@ -1359,7 +1333,7 @@ namespace lf {
 // ---------------------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------------------
-static PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
+PFN_cuTensorMapEncodeTiled_v12000 get_encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
   std::call_once(once, [] {

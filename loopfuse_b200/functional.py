@@ -9,15 +9,16 @@ The argument checks, the output allocation and the launch are in the native host
 from __future__ import annotations
 
 import ctypes as C
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import torch
 
 from . import _native
-from .spec import MASK_NONE, ScoreMod
+from .spec import MASK_CAUSAL, MASK_NONE, ScoreMod
 
 _DEV_TIMEOUT = 1
 _DEV_BAD_PAGE = 2
+_DEV_BAD_LENGTHS = 4
 
 
 def _require_cuda(*tensors: torch.Tensor) -> torch.device:
@@ -56,6 +57,9 @@ def check_status(status: torch.Tensor, what: str = "kernel") -> None:
         raise RuntimeError(f"{what}: a bounded device-side wait ran out (site {code >> 8})")
     if (code & 0xFF) == _DEV_BAD_PAGE:
         raise RuntimeError(f"{what}: block_table holds a page id outside the pool")
+    if (code & 0xFF) == _DEV_BAD_LENGTHS:
+        raise RuntimeError(f"{what}: a request's length is negative, or the batch has more tokens "
+                           "than num_tokens")
     raise RuntimeError(f"{what}: device status {code}")
 
 
@@ -300,3 +304,83 @@ def kv_append(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor,
     ``paged_decode_attention`` reads."""
     _native.host().kv_append(k_new, v_new, k_pool, v_pool, block_table, block_table_v, seq_pos,
                              start_pos, status)
+
+
+class PagePlan(NamedTuple):
+    """What ``plan_pages`` makes of a step's requests; int32 tensors on the device."""
+    cu_seqlens: torch.Tensor   # [B + 1] first row of each request in the packed batch
+    seq_lens: torch.Tensor     # [B] tokens of each request after the step
+    slots: torch.Tensor        # [num_tokens] page * page_size + slot of each row; -1: none
+    positions: torch.Tensor    # [num_tokens] position of each row in its request
+    pages_used: torch.Tensor   # [1] pages taken from the front of the free list
+
+
+def plan_pages(kv_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor,
+               block_table: torch.Tensor, *, page_size: int, num_tokens: int,
+               status: Optional[torch.Tensor] = None) -> PagePlan:
+    """Pages and places for the new tokens of a step, from the requests' lengths, on the device.
+
+    Request ``b`` has ``kv_lens[b]`` tokens in the pages that row ``b`` of ``block_table`` (int32
+    ``[B, blocks]``) names and adds ``new_lens[b]``; the pages that it lacks come from the front of
+    ``free_pages``, requests in order, and are written into its row in place. A row may begin with
+    pages that other requests hold too (a shared prefix), as long as the last one is full.
+    ``num_tokens`` is the number of rows of the packed batch: rows past the last token get slot -1
+    and position 0. If pages run out, ``pages_used`` says how many were needed, and what got none
+    has entry and slot -1 (reported in ``status``)."""
+    return PagePlan(*_native.host().plan_pages(kv_lens, new_lens, free_pages, block_table, page_size,
+                                               num_tokens, status))
+
+
+def kv_append_packed(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor,
+                     v_pool: torch.Tensor, slots: torch.Tensor, *,
+                     status: Optional[torch.Tensor] = None) -> None:
+    """Write the K/V rows ``[T, Hkv, D]`` of a packed batch into a paged cache, in place: row ``t``
+    goes to ``pool[slots[t] // page_size, slots[t] % page_size]``; a negative slot is skipped. The
+    ``slots`` of ``plan_pages`` put every token where ``packed_prefill_attention`` and the paged
+    decodes read it."""
+    _native.host().kv_append_packed(k_new, v_new, k_pool, v_pool, slots, status)
+
+
+def packed_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                             cu_seqlens: torch.Tensor, *,
+                             cu_seqlens_k: Optional[torch.Tensor] = None,
+                             block_table: Optional[torch.Tensor] = None,
+                             seq_lens: Optional[torch.Tensor] = None, scale: float = 1.0,
+                             mods: Sequence[ScoreMod] = (), mask_kind: int = MASK_CAUSAL,
+                             window: int = 0, out: Optional[torch.Tensor] = None,
+                             workspace: Optional[DecodeWorkspace] = None,
+                             status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of a batch of prompts of different lengths, packed: ``q`` ``[T, Hq, D]`` holds the
+    requests' tokens one after the other, request ``b`` those in ``[cu_seqlens[b],
+    cu_seqlens[b + 1])``; Hq may be a multiple of Hkv.
+
+    Keys and values are packed the same way (``[Tk, Hkv, D]``, by ``cu_seqlens_k`` where the keys
+    are others than the queries), or, with ``block_table`` (int32 ``[B, blocks]``) and ``seq_lens``
+    (int32 ``[B]``), read from a paged cache ``[pages, page_size, Hkv, D]``, the new tokens' own
+    among them: chunks of prompts and single tokens of running requests in one batch.
+
+    The mask is per request and aligned at its end: query ``i`` of ``n`` sees key ``j`` of ``m`` up
+    to ``i + m - n``, with ``MASK_CAUSAL_WINDOW`` the last ``window`` of those. A query that sees no
+    key gets zeros. ``mods`` may hold multipliers or a softcap chain (multipliers around one
+    tanh). No length is read by the host."""
+    return _native.host().packed_prefill(q, k, v, cu_seqlens, cu_seqlens_k, block_table, seq_lens, out,
+                                         workspace, status, scale, mods, mask_kind, window)
+
+
+def shared_prefix_decode_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                                   block_table: torch.Tensor, seq_lens: torch.Tensor,
+                                   prefix_len: int, *, max_seq_len: Optional[int] = None,
+                                   scale: float = 1.0, mods: Sequence[ScoreMod] = (),
+                                   out: Optional[torch.Tensor] = None,
+                                   workspace: Optional[DecodeWorkspace] = None,
+                                   status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Decode attention over a paged cache for requests that share their first ``prefix_len`` tokens:
+    ``q`` ``[B, Hkv, G, D]``, any G up to 128; ``seq_lens`` (int32 ``[B]``) counts the shared tokens
+    too. Those are read once for the whole batch, through row 0 of ``block_table``; each request's
+    other tokens through its own row. A request of length 0 (a row of a padded batch) gets zeros.
+
+    ``max_seq_len`` is a bound on the lengths that the host knows (default: all that the table
+    holds); the closer it is, the better the work is cut. ``mods`` as for
+    ``packed_prefill_attention``."""
+    return _native.host().shared_prefix_decode(q, k_pool, v_pool, block_table, seq_lens, prefix_len,
+                                               max_seq_len, out, workspace, status, scale, mods)
