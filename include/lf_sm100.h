@@ -266,7 +266,7 @@ typedef struct {
   float mod_arg[LF_MAX_MODS];
   int32_t mask_kind;      /* LF_MASK_*: a request's query i of n sees key j of m up to j = i + m - n */
   int32_t window;
-  void* workspace;        /* device, >= lf_packed_workspace_bytes(...) */
+  void* workspace;        /* device, >= lf_packed_workspace_bytes(this), 32-byte aligned */
   size_t workspace_bytes;
   int32_t* status;
 } LfPackedArgs;
@@ -447,8 +447,9 @@ int lf_plan_pages(const LfPagePlanArgs* args, void* stream);
  * one wins. */
 int lf_kv_append_packed_bf16(const LfKvAppendPackedArgs* args, void* stream);
 
-/* Attention of packed requests of different lengths, one launch (or two: batches that do not fit the
- * machine at once are ordered by length first, which takes the workspace). The mask is per request and
+/* Attention of packed requests of different lengths, one launch (or two: batches of many or long tiles
+ * are ordered by length first, and long tiles cut, which takes the workspace; requests of up to 2048
+ * keys are never cut, and have the same result in every batch). The mask is per request and
  * aligned at its end; a row that sees no key is zeros (lf_prefill_bf16 gives NaN there). Offsets that
  * are out of order or outside the tensors are cut to them; rows that no request holds are not written.
  * The mod chain may hold multipliers, or the softcap form (MUL|DIV)* TANH (MUL|DIV)*, with a product of
@@ -456,8 +457,8 @@ int lf_kv_append_packed_bf16(const LfKvAppendPackedArgs* args, void* stream);
  * other requests, or of a page's unused slots, never reach a result, whatever they hold; within a
  * request, a value row that a query does not see must be finite (its weight is zero). */
 int lf_packed_prefill_bf16(const LfPackedArgs* args, void* stream);
-/* Workspace of a call on the current device; 0 = none. */
-size_t lf_packed_workspace_bytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv);
+/* Workspace of a call with these sizes on the current device; 0 = none. */
+size_t lf_packed_workspace_bytes(const LfPackedArgs* args);
 
 /* Decode attention of requests that share their first prefix_len tokens, with the pages of the shared
  * ones read once for the whole batch: equal to lf_decode_paged_bf16 on each request with a table whose

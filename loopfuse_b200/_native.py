@@ -210,7 +210,7 @@ def load() -> C.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = [C.POINTER(args), C.c_void_p]
         fn.restype = C.c_int
-    lib.lf_packed_workspace_bytes.argtypes = [C.c_int32] * 4
+    lib.lf_packed_workspace_bytes.argtypes = [C.POINTER(LfPackedArgs)]
     lib.lf_packed_workspace_bytes.restype = C.c_size_t
     lib.lf_shared_prefix_workspace_bytes.argtypes = [C.c_int32] * 6
     lib.lf_shared_prefix_workspace_bytes.restype = C.c_size_t

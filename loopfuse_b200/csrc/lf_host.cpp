@@ -81,7 +81,7 @@ struct Lib {
   int (*plan_pages)(const LfPagePlanArgs*, void*) = nullptr;
   int (*kv_append_packed)(const LfKvAppendPackedArgs*, void*) = nullptr;
   int (*packed_prefill)(const LfPackedArgs*, void*) = nullptr;
-  size_t (*packed_workspace)(int32_t, int32_t, int32_t, int32_t) = nullptr;
+  size_t (*packed_workspace)(const LfPackedArgs*) = nullptr;
   int (*shared_prefix)(const LfSharedPrefixArgs*, void*) = nullptr;
   size_t (*shared_prefix_workspace)(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) = nullptr;
   PyObject* check = nullptr;  // _native.check(rc, what): raises LfError
@@ -854,7 +854,7 @@ Tensor run_packed_prefill(const Tensor& q, const Tensor& k_in, const Tensor& v_i
   a.window = o.window;
   a.status = status_ptr(status);
   const c10::cuda::CUDAGuard guard(dev);
-  a.workspace_bytes = lib.packed_workspace(a.B, a.T, a.Hq, a.Hkv);
+  a.workspace_bytes = lib.packed_workspace(&a);
   Scratch scratch;
   a.workspace = scratch.get(a.workspace_bytes, workspace, q);
   check_rc(launch(dev, [&](void* st) { return lib.packed_prefill(&a, st); }), "lf_packed_prefill_bf16");

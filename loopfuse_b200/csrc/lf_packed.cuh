@@ -8,12 +8,19 @@
 // domain, o = sum_j 2^(f(s_j) - m) v_j, l = sum_j 2^(f(s_j) - m), with a reference m that moves when
 // the row maximum passes it by more than 2^8 (the rescale is rare) and out = o / l.
 //
-// One CTA per tile, two CTAs per SM: the start and end of one lie under the blocks of the other, which
-// is what short requests are made of. 256 threads:
+// Two CTAs per SM, each of which takes tiles (or slices of the keys of long ones) from a list until it is
+// empty. 256 threads:
 //   warps 0-3   softmax (one thread per score row)
-//   warp  4     producer: Q once, then pairs of 64-key tiles into a ring, in the order of their use:
-//               {K(lo), K(lo+1)}, {V(lo), K(lo+2)}, {V(lo+1), K(lo+3)}, ...
-//   warp  5     MMA issuer: S[buf] = Q K^T, O += P V; QK of block j+2 is issued right behind PV of block j
+//   warp  4     takes the items from the list and hands them to the other warps; Q, and the K blocks
+//   warp  5     issues S[g & 1] = Q K^T, as soon as PV of block g - 2 is done with the buffer
+//   warp  6     the V blocks
+//   warp  7     issues O += P V
+// (One warp for both products takes longer over a block than the softmax warps: beside them it gets few
+// issue slots. 8 prompts up to 8192 tokens 718 us, and 806 with every other wait in front of that for P.)
+// Blocks are numbered through over all items of a CTA (g): the producers and the issuer run on into the
+// next item while the softmax warps finish the last one, so the look-ups, copies and first scores of a
+// tile lie under the blocks of the tile before it. (Short prompts are mostly starts and ends: one CTA per
+// tile, 28 prompts of 512 tokens, 32 heads on 8, took 144 us.)
 // Tensor memory (256 columns): S of buffer b at column b * 64, P (bf16) over its first 32 columns, O at 128.
 //
 // What a packed batch adds to the tiles of the prefill kernels: the last key block of a request holds
@@ -41,58 +48,85 @@ enum PackedKind {
   kPackedPrefix = 2,  // one query token per request against a slice of the shared prefix; partial results
 };
 
+// A tile, or a slice of its keys, as the list has it (the kv head comes with the place in the order).
+struct __align__(16) PackedItem {
+  int32_t q_row;    // first query row (token of the packed batch; request, for the prefix)
+  int32_t count;    // tokens; 0: none, the end of a CTA's items
+  int32_t k_from;   // dense: row of the request's first key; paged: row of the block table
+  int32_t m;        // the request's keys
+  int32_t pos;      // last key that the first token sees
+  int32_t lo, hi;   // key blocks
+  int32_t hkv;      // (in shared memory)
+  int32_t part;     // slices of one tile: the first one's place in the workspace, else -1
+  int32_t n_parts, index;
+  int32_t counter;  // ... and the count of those that are done
+};
+
 struct PackedParams {
   __nv_bfloat16* out;
   int64_t o_stride[2];        // (token, head)
+  int32_t out_sectors;        // output rows are 32-byte aligned
   const int32_t* cu_q;        // [B + 1] first query token of each request
   const int32_t* cu_k;        // dense: [B + 1] first key
   const int32_t* kv_lens;     // paged, prefix: [B] keys of each request
   const int32_t* table;       // block table
   int64_t bt_stride;
-  const int2* items;          // (request, tile) in the order of the launch, or null: looked up by the CTA
-  const int32_t* n_items;     // how many there are
+  const PackedItem* items;    // the list, or null: a CTA has one tile, which it looks up
+  uint32_t* list;             // [0] items of a kv head, [1] ticket, [2 ..] slices done, by counter
   int32_t B, T, Tk, Hkv, G;
   int32_t tq;                 // tokens (requests) per tile: 128 / G
   int32_t mask_kind, window;
   float a;                    // softcap: score = tanh(raw * a) * c2
   float c2;                   // logit in the log2 domain = score * c2; > 0
+  float m_first;              // a row's first reference: -inf, or 0 where no logit is far from it
   int32_t bt_blocks, page_size, page_shift, n_pages;
   int32_t box;                // keys per copy of a paged operand: they lie in one page
-  int32_t n_tiles;            // grid: tiles of a kv head (an upper bound)
-  FastDiv div_chunk;          // heads of a chunk of kv heads (see the launch)
-  FastDiv div_tiles;          // tiles
+  int32_t n_tiles;            // tiles of a kv head (no list: an upper bound)
+  FastDiv div_chunk;          // heads of a chunk of kv heads (see the launch); prefix: kv heads
+  FastDiv div_tiles;          // tiles (no list)
   FastDiv div_g;              // query heads per kv head
-  // Prefix: rows [B, Hkv, G], keys [split * chunk, ...) below prefix_len.
-  int32_t prefix_len, chunk, splits;
-  float* part_o;              // [split][row][D]
-  float2* part_ml;            // [split][row] (reference, sum)
+  int32_t prefix_len, chunk;  // prefix: keys [split * chunk, ...) below prefix_len
+  float* part_o;              // [slice][row][D] un-normalised
+  float2* part_ml;            // [slice][row] (reference, sum)
   int32_t* status;
 };
 
 template <int D>
 struct PackedShape {
-  static constexpr int kStages = D == 64 ? 4 : 2;
-  // Output staging (2 KB per softmax warp; with D = 64 the CTA has to stay above a third of the SM's
-  // shared memory, so that a third one does not wait for tensor memory).
-  static constexpr uint32_t kStaging = 4 * 2048 + 4096;
+  static constexpr int kStages = D == 64 ? 4 : 2;  // of K, and of V: blocks in flight
+  // Behind the rings: a CTA has to stay above a third of the SM's shared memory, so that a third one does
+  // not wait for tensor memory.
+  static constexpr uint32_t kRest = 13 * 1024;
   static constexpr uint32_t kTmemColumns = 256;
   static constexpr uint32_t kQBlockBytes = kPackedRows * 128;  // [128][64] bf16
   static constexpr uint32_t kKVBlockBytes = kPackedKeys * 128;
   static constexpr uint32_t kTileBytes = kKVBlockBytes * (D / 64);
-  static constexpr size_t kSmem = 1024 /*align slack*/ + 1024 /*barriers*/ + kStaging +
+  static constexpr size_t kSmem = 1024 /*barriers*/ + kRest +
                                   kQBlockBytes * (D / 64) + kStages * 2 * kTileBytes;
 };
 
-struct __align__(8) PackedBarriers {
-  uint64_t q_full;
-  uint64_t kv_full[4];
-  uint64_t kv_empty[4];
+constexpr int kItemSlots = 4;
+
+struct __align__(16) PackedBarriers {
+  PackedItem item[kItemSlots];
+  uint64_t item_full[kItemSlots], item_empty[kItemSlots];
+  uint64_t q_full, q_empty;
+  uint64_t k_full[4], k_empty[4];
+  uint64_t v_full[4], v_empty[4];
   uint64_t s_full[2];   // MMA -> softmax
   uint64_t p_full[2];   // softmax -> MMA
-  uint64_t pv_done;     // second-to-last PV done
-  uint64_t o_final;     // last PV done
+  uint64_t s_free[2];   // PV done: the buffer may take other scores
+  uint64_t pv_done;     // second-to-last PV of an item done
+  uint64_t o_final;     // last PV of an item done
+  uint64_t o_empty;     // softmax -> MMA: O has been read
   uint32_t tmem_base;
+  uint32_t last_part;
 };
+static_assert(sizeof(PackedBarriers) <= 1024, "the block in front of the staging");
+
+// A value that is the same in all lanes, as one that the compiler knows to be: loops and branches on it
+// need no registers to bring the lanes together again.
+__device__ __forceinline__ int warp_uniform(int x) { return __reduce_max_sync(0xffffffffu, x); }
 
 __device__ __forceinline__ void packed_timeout(int32_t* status, int where) {
   if (status) atomicCAS(status, LF_DEV_OK, LF_DEV_TIMEOUT | (where << 8));
@@ -114,11 +148,32 @@ __device__ __forceinline__ PackedRequest packed_request(const PackedParams& p, i
     r.k0 = clamp_to(p.cu_k[b], p.Tk);
     r.m = max(clamp_to(p.cu_k[b + 1], p.Tk) - r.k0, 0);
   } else {
-    r.k0 = 0;
+    r.k0 = b;
     const int64_t held = static_cast<int64_t>(p.bt_blocks) * p.page_size;
     r.m = clamp_to(p.kv_lens[b], held > 0x7fffffff ? 0x7fffffff : static_cast<int>(held));
   }
   return r;
+}
+
+// Tile `tile` of request r as one item.
+__device__ __forceinline__ PackedItem packed_item(const PackedParams& p, const PackedRequest& r, int tile) {
+  PackedItem it;
+  const int t0 = tile * p.tq;
+  it.q_row = r.q0 + t0;
+  it.count = min(p.tq, r.n - t0);
+  it.k_from = r.k0;
+  it.m = r.m;
+  it.pos = t0 + r.m - r.n;
+  int first = 0, end = r.m;
+  if (p.mask_kind != LF_MASK_NONE) end = min(end, it.pos + it.count);
+  if (p.mask_kind == LF_MASK_CAUSAL_WINDOW) first = max(0, it.pos - (p.window - 1));
+  it.lo = first / kPackedKeys;
+  it.hi = end > first ? (end + kPackedKeys - 1) / kPackedKeys : it.lo;
+  it.hkv = 0;
+  it.part = -1;
+  it.n_parts = 1;
+  it.index = it.counter = 0;
+  return it;
 }
 
 // Request and tile of place `rank`, requests in order and a request's heaviest tile first; the whole
@@ -149,101 +204,174 @@ __device__ __forceinline__ int2 find_tile(const PackedParams& p, int rank) {
   return make_int2(-1, 0);
 }
 
+// Item at place `at` of the order: chunks of kv heads, in each the list, longest first, for every head of
+// the chunk. `n`: items of the list.
+__device__ __forceinline__ PackedItem listed_item(const PackedParams& p, uint32_t at, uint32_t n) {
+  PackedItem it;
+  it.count = 0;
+  const uint32_t r = p.div_chunk.div(at);
+  const uint32_t chunk = r / n;
+  const uint32_t hkv = chunk * p.div_chunk.d + (at - r * p.div_chunk.d);
+  if (chunk * p.div_chunk.d >= static_cast<uint32_t>(p.Hkv)) return it;  // past the last one
+  const int4* src = reinterpret_cast<const int4*>(p.items + (r - chunk * n));
+  const int4 x = src[0], y = src[1], z = src[2];
+  it.q_row = x.x, it.count = x.y, it.k_from = x.z, it.m = x.w;
+  it.pos = y.x, it.lo = y.y, it.hi = y.z;
+  it.part = z.x, it.n_parts = z.y, it.index = z.z, it.counter = z.w;
+  it.hkv = static_cast<int>(hkv);
+  if (it.hkv >= p.Hkv) it.lo = it.hi = it.hkv = -1;  // a place of the last chunk that has no head
+  return it;
+}
+
+// The only item of a CTA without a list.
+template <int KIND>
+__device__ __forceinline__ PackedItem own_item(const PackedParams& p, int cta) {
+  PackedItem it;
+  it.count = 0;
+  if constexpr (KIND == kPackedPrefix) {
+    const int unit = static_cast<int>(p.div_tiles.div(cta));  // (split, kv head); tiles of it together
+    it.q_row = (cta - unit * static_cast<int>(p.div_tiles.d)) * p.tq;
+    it.index = static_cast<int>(p.div_chunk.div(unit));       // split
+    it.hkv = unit - it.index * static_cast<int>(p.div_chunk.d);
+    it.count = min(p.tq, p.B - it.q_row);
+    it.k_from = 0;
+    it.pos = 0;
+    it.m = min(p.prefix_len, (it.index + 1) * p.chunk);
+    it.lo = it.index * (p.chunk / kPackedKeys);
+    it.hi = (it.m + kPackedKeys - 1) / kPackedKeys;
+    it.part = it.n_parts = it.counter = 0;
+  } else {
+    const int r = static_cast<int>(p.div_chunk.div(cta));
+    const int chunk = static_cast<int>(p.div_tiles.div(r));
+    const int hkv = chunk * static_cast<int>(p.div_chunk.d) + cta - r * static_cast<int>(p.div_chunk.d);
+    if (hkv < p.Hkv) {
+      const int2 at = find_tile(p, r - chunk * static_cast<int>(p.div_tiles.d));
+      if (at.x >= 0) {
+        it = packed_item(p, packed_request<KIND>(p, at.x), at.y);
+        it.hkv = hkv;
+      }
+    }
+  }
+  return it;
+}
+
+// 32 bytes (a whole sector) per thread.
+__device__ __forceinline__ void stg_32(void* p, const uint32_t* r) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// Output rows of a tile from its slices, a warp for its 32 rows, lanes along the columns: o = sum_s o_s
+// 2^(m_s - m) / sum_s l_s 2^(m_s - m). Four rows at a time, so that their loads are in flight together.
+template <int D>
+__device__ __forceinline__ void join_slices(const PackedParams& p, const PackedItem& it, int warp, int lane,
+                                         int rows) {
+  constexpr int kCols = D / 32;
+  const int n = it.n_parts, hkv = it.hkv, q_row = it.q_row;
+  const int64_t part0 = (static_cast<int64_t>(it.part) * p.Hkv + hkv) * kPackedRows;
+  const int64_t step = static_cast<int64_t>(p.Hkv) * kPackedRows;
+  const int end = min(warp * 32 + 32, rows);
+  #pragma unroll 1
+  for (int r0 = warp * 32; r0 < end; r0 += 4) {
+    float acc[4][kCols], l[4], m[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      m[u] = -INFINITY;
+      l[u] = 0.f;
+#pragma unroll
+      for (int c = 0; c < kCols; ++c) acc[u][c] = 0.f;
+    }
+    for (int s = 0; s < n; ++s) {
+      float2 ml[4];
+      float x[4][kCols];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t at = part0 + s * step + min(r0 + u, end - 1);
+        ml[u] = __ldcg(&p.part_ml[at]);
+        const float* src = p.part_o + at * D + lane * kCols;
+        if constexpr (kCols == 4) {
+          const float4 v = __ldcg(reinterpret_cast<const float4*>(src));
+          x[u][0] = v.x, x[u][1] = v.y, x[u][2] = v.z, x[u][3] = v.w;
+        } else {
+          const float2 v = __ldcg(reinterpret_cast<const float2*>(src));
+          x[u][0] = v.x, x[u][1] = v.y;
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if (ml[u].y == 0.f) continue;  // (no key of this row: what its accumulator holds is of no value)
+        const float top = fmaxf(m[u], ml[u].x);
+        const float back = ex2_approx(m[u] - top), w = ex2_approx(ml[u].x - top);
+        m[u] = top;
+        l[u] = fmaf(l[u], back, ml[u].y * w);
+#pragma unroll
+        for (int c = 0; c < kCols; ++c) acc[u][c] = fmaf(acc[u][c], back, x[u][c] * w);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if (r0 + u >= end) break;
+      const int tok = static_cast<int>(p.div_g.div(r0 + u));
+      __nv_bfloat16* dst = p.out + static_cast<int64_t>(q_row + tok) * p.o_stride[0] +
+                           static_cast<int64_t>(hkv * p.G + r0 + u - tok * p.G) * p.o_stride[1] + lane * kCols;
+      const float inv = l[u] == 0.f ? 0.f : 1.f / l[u];
+      if constexpr (kCols == 4)
+        *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(acc[u][0] * inv, acc[u][1] * inv),
+                                                    pack_bf16x2(acc[u][2] * inv, acc[u][3] * inv));
+      else
+        *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(acc[u][0] * inv, acc[u][1] * inv);
+    }
+  }
+}
+
 template <int D, int KIND, bool SOFTCAP>
-__device__ __forceinline__ void packed_tile(const CUtensorMap& tmap_q, const CUtensorMap& tmap_k,
-                                            const CUtensorMap& tmap_v, const PackedParams& p,
-                                            unsigned char* smem_unaligned, int cta) {
+__device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CUtensorMap& tmap_k,
+                                             const CUtensorMap& tmap_v, const PackedParams& p, int cta) {
   using Shape = PackedShape<D>;
   constexpr int kStages = Shape::kStages;
   constexpr int kBlocksD = D / 64;
   constexpr uint32_t kIdescQK = make_idesc_bf16(128, kPackedKeys, 0);
   constexpr uint32_t kIdescPV = make_idesc_bf16(128, D, 1);
   constexpr uint32_t kColO = 128;
-  constexpr int kProducerWarp = 4, kMmaWarp = 5;
+  constexpr int kKWarp = 4, kQkWarp = 5, kVWarp = 6, kPvWarp = 7;
   constexpr bool kPages = KIND != kPackedDense;
 
-  unsigned char* smem = reinterpret_cast<unsigned char*>(
-      (reinterpret_cast<uintptr_t>(smem_unaligned) + 1023) & ~static_cast<uintptr_t>(1023));
+  // (Aligned by declaration: every address is a constant then, and none of them takes registers.)
+  extern __shared__ __align__(1024) unsigned char smem[];
   PackedBarriers* bars = reinterpret_cast<PackedBarriers*>(smem);
-  unsigned char* sStage = smem + 1024;
-  unsigned char* sQ = sStage + Shape::kStaging;
-  unsigned char* sKV = sQ + Shape::kQBlockBytes * kBlocksD;
+  unsigned char* sQ = smem + 1024;
+  unsigned char* sK = sQ + Shape::kQBlockBytes * kBlocksD;
+  unsigned char* sV = sK + kStages * Shape::kTileBytes;
 
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
 
-  // ---------------- which tile ----------------
-  int hkv, t0, count;      // kv head; first token of the tile and how many it has
-  int table_row = 0, split = 0;
-  PackedRequest rq;
-  int key_lo, key_hi;      // keys that some row of the tile sees
-  int off = 0;             // query token i sees the keys up to i + off
-  if constexpr (KIND == kPackedPrefix) {
-    const int unit = static_cast<int>(p.div_tiles.div(cta));  // (kv head, split); tiles of it together
-    const int tile = cta - unit * static_cast<int>(p.div_tiles.d);
-    split = static_cast<int>(p.div_chunk.div(unit));          // div_chunk: kv heads
-    hkv = unit - split * static_cast<int>(p.div_chunk.d);
-    t0 = tile * p.tq;
-    count = min(p.tq, p.B - t0);
-    rq = {0, p.B, 0, 0};
-    key_lo = split * p.chunk;
-    key_hi = min(p.prefix_len, key_lo + p.chunk);
-    rq.m = key_hi;
-  } else {
-    const int r = static_cast<int>(p.div_chunk.div(cta));     // place in the order of this chunk of heads
-    const int head_chunk = static_cast<int>(p.div_tiles.div(r));
-    hkv = head_chunk * static_cast<int>(p.div_chunk.d) + cta - r * static_cast<int>(p.div_chunk.d);
-    if (hkv >= p.Hkv) return;
-    const int rank = r - head_chunk * static_cast<int>(p.div_tiles.d);
-    int2 at;
-    if (p.items) {
-      if (rank >= *p.n_items) return;
-      at = p.items[rank];
-    } else {
-      at = find_tile(p, rank);
-      if (at.x < 0) return;
-    }
-    rq = packed_request<KIND>(p, at.x);
-    table_row = at.x;
-    t0 = at.y * p.tq;
-    count = min(p.tq, rq.n - t0);
-    off = rq.m - rq.n;
-    key_lo = 0;
-    key_hi = rq.m;
-    if (p.mask_kind != LF_MASK_NONE) key_hi = min(key_hi, t0 + count + off);
-    if (p.mask_kind == LF_MASK_CAUSAL_WINDOW) key_lo = max(0, t0 + off - (p.window - 1));
-  }
-  const int rows = count * p.G;
-  // Rows that see a handful of keys do not average the rounding of P away: where the first row of the tile
-  // does (the start of a prompt, a tiny window), P enters the second product as two bf16, its rounding and
-  // what that leaves, in the half of the S buffer that P does not need.
-  bool fine = false;
-  if constexpr (KIND != kPackedPrefix) {
-    int sees = rq.m;
-    if (p.mask_kind != LF_MASK_NONE) sees = min(sees, t0 + off + 1);
-    if (p.mask_kind == LF_MASK_CAUSAL_WINDOW) sees = min(sees, p.window);
-    fine = sees < 16;
-  }
-  const int lo = key_lo / kPackedKeys;
-  const int hi = key_hi > key_lo ? (key_hi + kPackedKeys - 1) / kPackedKeys : lo;
-  const int nblk = hi - lo;
-
   // ---------------- setup ----------------
-  if (warp == kProducerWarp && lane == 0) {
+  if (warp == kKWarp && lane == 0) {
     tma_prefetch_desc(&tmap_q);
     tma_prefetch_desc(&tmap_k);
     tma_prefetch_desc(&tmap_v);
+    for (int i = 0; i < kItemSlots; ++i) {
+      mbar_init(&bars->item_full[i], 1);
+      mbar_init(&bars->item_empty[i], 7);  // (softmax, QK, V, PV)
+    }
     mbar_init(&bars->q_full, 1);
+    mbar_init(&bars->q_empty, 1);
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&bars->kv_full[s], 1);
-      mbar_init(&bars->kv_empty[s], 1);
+      mbar_init(&bars->k_full[s], 1);
+      mbar_init(&bars->k_empty[s], 1);
+      mbar_init(&bars->v_full[s], 1);
+      mbar_init(&bars->v_empty[s], 1);
     }
     for (int bf = 0; bf < 2; ++bf) {
       mbar_init(&bars->s_full[bf], 1);
       mbar_init(&bars->p_full[bf], 4);
+      mbar_init(&bars->s_free[bf], 1);
     }
     mbar_init(&bars->pv_done, 1);
     mbar_init(&bars->o_final, 1);
+    mbar_init(&bars->o_empty, 4);
     mbar_fence_init();
   }
   if (warp == 0) {
@@ -254,201 +382,262 @@ __device__ __forceinline__ void packed_tile(const CUtensorMap& tmap_q, const CUt
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem_base = bars->tmem_base;
+  pdl_wait();  // (nothing in global memory has been touched so far)
 
   // 128 registers per thread at two CTAs of 256: 184 for the softmax warps, 72 for the others (one
   // instruction per warpgroup, in front of the dispatch of roles).
   if (warp >= 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
 
-  if (warp == kProducerWarp) {
-    // ---------------- producer ----------------
+  // A wait that runs out is reported, and the waits after it are passed over: the warp runs through what
+  // is left without a loop to leave in the middle (lanes that may leave one apart cost the registers that
+  // bring them together again).
+  bool lost = false;
+  auto wait = [&](uint64_t* bar, uint32_t parity, int where) {
+    if (!lost && !mbar_wait(bar, parity)) {
+      packed_timeout(p.status, where);
+      lost = true;
+    }
+  };
+  // Item number i of this CTA, once warp 4 has put it there.
+  auto take_item = [&](int i, PackedItem* it) {
+    wait(&bars->item_full[i % kItemSlots], (i / kItemSlots) & 1, 80);
+    *it = bars->item[i % kItemSlots];
+    if (__any_sync(0xffffffffu, lost)) it->count = 0;
+  };
+  auto free_item = [&](int i) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars->item_empty[i % kItemSlots]);
+  };
+  // Rows that see a handful of keys do not average the rounding of P away: where the first row of the tile
+  // does (the start of a prompt, a tiny window), P enters the second product as two bf16, its rounding and
+  // what that leaves, in the half of the S buffer that P does not need.
+  auto is_fine = [&](const PackedItem& it) {
+    if constexpr (KIND == kPackedPrefix) return false;
+    int sees = it.m;
+    if (p.mask_kind != LF_MASK_NONE) sees = min(sees, it.pos + 1);
+    if (p.mask_kind == LF_MASK_CAUSAL_WINDOW) sees = min(sees, p.window);
+    return sees < 16;
+  };
+
+  // Next place in the order (without a list there is none).
+  auto take_place = [&]() -> uint32_t {
+    uint32_t at = 0xffffffffu;
+    if (p.items) {
+      if (lane == 0) at = atomicAdd(&p.list[1], 1u);
+      at = gridDim.x + __shfl_sync(0xffffffffu, at, 0);
+    }
+    return at;
+  };
+
+  if (warp == kKWarp || warp == kVWarp) {
+    // ---------------- producers ----------------
+    // The whole warp runs the loops and waits; the elected lane issues the copies.
+    const bool is_k = warp == kKWarp;
     const bool elected = elect_one_sync();
-    if (nblk > 0) {
-      if (elected) {
-        // (A box is always tq tokens; those past the end of the request are strangers' rows or zeros.)
-        mbar_arrive_expect_tx(&bars->q_full, static_cast<uint32_t>(p.tq * p.G) * 128 * kBlocksD);
-#pragma unroll
-        for (int kb = 0; kb < kBlocksD; ++kb)
-          tma_load_4d(sQ + kb * Shape::kQBlockBytes, &tmap_q, &bars->q_full, kb * 64, 0, hkv,
-                      rq.q0 + t0);
+    const CUtensorMap* map = is_k ? &tmap_k : &tmap_v;
+    unsigned char* ring = is_k ? sK : sV;
+    uint64_t* full = is_k ? bars->k_full : bars->v_full;
+    uint64_t* empty = is_k ? bars->k_empty : bars->v_empty;
+    auto page_of = [&](int t) { return p.page_shift >= 0 ? (t >> p.page_shift) : (t / p.page_size); };
+    const int boxes = kPages ? kPackedKeys / p.box : 1;
+
+    // K warp: the item behind the present one goes to the others as soon as Q of this one is on its way.
+    uint32_t n_list = 0, at = cta;
+    auto read_item = [&](bool first) {
+      PackedItem x;
+      x.count = 0;
+      if (p.items) {
+        if (n_list > 0) x = listed_item(p, at, n_list);
+        at = take_place();
+      } else if (first) {
+        x = own_item<KIND>(p, cta);
       }
-      bool ok = true;
-      auto page_of = [&](int t) { return p.page_shift >= 0 ? (t >> p.page_shift) : (t / p.page_size); };
-      const int32_t* table = p.table + static_cast<int64_t>(table_row) * p.bt_stride;
-      const int boxes = kPages ? kPackedKeys / p.box : 1;
-      // Boxes of block j that hold a key (the rest of the last block is not fetched).
-      auto live_boxes = [&](int j) {
-        return min(boxes, (rq.m - j * kPackedKeys + p.box - 1) / p.box);
-      };
-      // Table entries of a block's boxes, one or two per lane, requested a block ahead of their use.
-      auto request = [&](int j, int32_t (&e)[2]) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = i * 32 + lane;
-          e[i] = 0;
-          if (j < hi && r < live_boxes(j)) e[i] = table[page_of(j * kPackedKeys + r * p.box)];
+      return x;
+    };
+    auto hand_on = [&](PackedItem x, int i) {
+      // (A tile that sees no key is not handed on: its rows are zeros, written here.)
+      while (KIND != kPackedPrefix && x.count > 0 && x.hi <= x.lo) {
+        const int pieces = x.hkv < 0 ? 0 : x.count * p.G * (D / 8);
+        for (int e = lane; e < pieces; e += 32) {
+          const int r = e / (D / 8), t = static_cast<int>(p.div_g.div(r));
+          *reinterpret_cast<uint4*>(p.out + static_cast<int64_t>(x.q_row + t) * p.o_stride[0] +
+                                    static_cast<int64_t>(x.hkv * p.G + r - t * p.G) * p.o_stride[1] +
+                                    (e % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
         }
-      };
-      // Block j of K or V into `dst`. Paged: the page ids are checked, then the elected lane issues a copy
-      // per box.
-      auto load = [&](const CUtensorMap* map, unsigned char* dst, uint64_t* bar, int j, int32_t (&e)[2]) {
-        if constexpr (!kPages) {
+        x = read_item(false);
+      }
+      wait(&bars->item_empty[i % kItemSlots], ((i / kItemSlots) & 1) ^ 1, 87);
+      __syncwarp();
+      if (lane == 0) {
+        bars->item[i % kItemSlots] = x;
+        mbar_arrive(&bars->item_full[i % kItemSlots]);
+      }
+      __syncwarp();
+    };
+    if (is_k) {
+      if (p.items) n_list = p.list[0];
+      hand_on(read_item(true), 0);
+    }
+    int g = 0;  // blocks
+    for (int i = 0;; ++i) {
+      PackedItem it;
+      take_item(i, &it);
+      if (!is_k) free_item(i);
+      if (it.count <= 0) break;
+      const int lo = it.lo, hi = it.hi;
+      {
+        if (is_k) {
+          const PackedItem next = read_item(false);
+          if (i > 0) wait(&bars->q_empty, (i - 1) & 1, 81);
+          __syncwarp();
           if (elected) {
+            // (A box is always tq tokens; those past the end of the request are strangers' rows or zeros.)
+            mbar_arrive_expect_tx(&bars->q_full, static_cast<uint32_t>(p.tq * p.G) * 128 * kBlocksD);
 #pragma unroll
             for (int kb = 0; kb < kBlocksD; ++kb)
-              tma_load_4d(dst + kb * Shape::kKVBlockBytes, map, bar, kb * 64, rq.k0 + j * kPackedKeys,
-                          hkv, 0);
+              tma_load_4d(sQ + kb * Shape::kQBlockBytes, &tmap_q, &bars->q_full, kb * 64, 0, it.hkv, it.q_row);
           }
-        } else {
-          const int live = live_boxes(j);
+          hand_on(next, i + 1);
+        }
+        const int32_t* table = p.table + static_cast<int64_t>(it.k_from) * p.bt_stride;
+        // Boxes of block j that hold a key (the rest of the last block is not fetched).
+        auto live_boxes = [&](int j) { return min(boxes, (it.m - j * kPackedKeys + p.box - 1) / p.box); };
+        // Table entries of a block's boxes, one or two per lane, requested a block ahead of their use.
+        int32_t entry[2] = {0, 0};
+        auto request = [&](int j) {
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            if (i * 32 + lane < live && (e[i] < 0 || e[i] >= p.n_pages)) {
-              if (p.status) atomicExch(p.status, LF_DEV_BAD_PAGE);
-              e[i] = 0;
-            }
+          for (int e = 0; e < 2; ++e) {
+            const int r = e * 32 + lane;
+            entry[e] = 0;
+            if (j < hi && r < live_boxes(j)) entry[e] = table[page_of(j * kPackedKeys + r * p.box)];
           }
-          for (int r = 0; r < live; ++r) {
-            const int page = __shfl_sync(0xffffffffu, r < 32 ? e[0] : e[1], r & 31);
-            const int t = j * kPackedKeys + r * p.box;
-            const int slot = t - page_of(t) * p.page_size;
+        };
+        if constexpr (kPages) request(lo);
+        for (int j = lo; j < hi; ++j, ++g) {
+          int32_t page[2];
+          if constexpr (kPages) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              page[e] = entry[e];
+              if (page[e] < 0 || page[e] >= p.n_pages) {
+                if (p.status) atomicExch(p.status, LF_DEV_BAD_PAGE);
+                page[e] = 0;
+              }
+            }
+            request(j + 1);
+          }
+          const int stage = g % kStages;
+          wait(&empty[stage], ((g / kStages) & 1) ^ 1, 81);
+          if (__any_sync(0xffffffffu, lost)) break;
+          unsigned char* dst = ring + stage * Shape::kTileBytes;
+          if constexpr (!kPages) {
             if (elected) {
+              mbar_arrive_expect_tx(&full[stage], Shape::kTileBytes);
 #pragma unroll
               for (int kb = 0; kb < kBlocksD; ++kb)
-                tma_load_4d(dst + kb * Shape::kKVBlockBytes + r * p.box * 128, map, bar, kb * 64, slot,
-                            hkv, page);
+                tma_load_4d(dst + kb * Shape::kKVBlockBytes, map, &full[stage], kb * 64,
+                            it.k_from + j * kPackedKeys, it.hkv, 0);
+            }
+          } else {
+            const int live = live_boxes(j);
+            if (elected)
+              mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(live * p.box) * 128 * kBlocksD);
+            for (int r = 0; r < live; ++r) {
+              const int pg = __shfl_sync(0xffffffffu, r < 32 ? page[0] : page[1], r & 31);
+              const int t = j * kPackedKeys + r * p.box;
+              const int slot = t - page_of(t) * p.page_size;
+              if (elected) {
+#pragma unroll
+                for (int kb = 0; kb < kBlocksD; ++kb)
+                  tma_load_4d(dst + kb * Shape::kKVBlockBytes + r * p.box * 128, map, &full[stage], kb * 64,
+                              slot, it.hkv, pg);
+              }
             }
           }
-        }
-      };
-      auto bytes = [&](int j) -> uint32_t {
-        return kPages ? static_cast<uint32_t>(live_boxes(j) * p.box) * 128 * kBlocksD : Shape::kTileBytes;
-      };
-      int32_t ek[2] = {0, 0}, ek2[2] = {0, 0}, ev[2] = {0, 0};
-      // Entries of the blocks whose V is still to come: those of K(j), K(j+1) serve V again.
-      if constexpr (kPages) {
-        request(lo, ev);
-        request(lo + 1, ek);
-        request(lo + 2, ek2);
-      }
-      {
-        if (elected) mbar_arrive_expect_tx(&bars->kv_full[0], bytes(lo) + (nblk > 1 ? bytes(lo + 1) : 0u));
-        load(&tmap_k, sKV, &bars->kv_full[0], lo, ev);
-        if (nblk > 1) load(&tmap_k, sKV + Shape::kTileBytes, &bars->kv_full[0], lo + 1, ek);
-      }
-      for (int j = lo, n = 1; j < hi && ok; ++j, ++n) {
-        const int stage = n % kStages;
-        ok = mbar_wait(&bars->kv_empty[stage], ((n / kStages) & 1) ^ 1);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) {
-          packed_timeout(p.status, 81);
-          break;
-        }
-        unsigned char* dst = sKV + stage * (2 * Shape::kTileBytes);
-        const bool more = j + 2 < hi;
-        if (elected)
-          mbar_arrive_expect_tx(&bars->kv_full[stage], bytes(j) + (more ? bytes(j + 2) : 0u));
-        load(&tmap_v, dst, &bars->kv_full[stage], j, ev);
-        if (more) load(&tmap_k, dst + Shape::kTileBytes, &bars->kv_full[stage], j + 2, ek2);
-        if constexpr (kPages) {
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            ev[i] = ek[i];
-            ek[i] = ek2[i];
-          }
-          request(j + 3, ek2);
         }
       }
     }
-  } else if (warp == kMmaWarp) {
-    // ---------------- MMA issuer ----------------
+  } else if (warp == kQkWarp) {
+    // ---------------- S = Q K^T ----------------
     // The whole warp runs the loop (every lane waits on the barriers); the elected lane alone issues.
-    if (nblk > 0) {
-      const bool elected = elect_one_sync();
-      bool ok = __all_sync(0xffffffffu, mbar_wait(&bars->q_full, 0));
-      constexpr uint32_t kStageUnits = (2 * Shape::kTileBytes) >> 4;
-      constexpr uint32_t kHalfUnits = Shape::kTileBytes >> 4;
-      const uint64_t qdesc = make_smem_desc_sw128(smem_u32(sQ), 16, 1024);
-      const uint64_t kdesc0 = make_smem_desc_sw128(smem_u32(sKV), 16, 1024);
-      const uint64_t vdesc0 = make_smem_desc_sw128(smem_u32(sKV), Shape::kKVBlockBytes, 1024);
-      const uint32_t o_col = tmem_base + kColO;
-      auto wait_stage = [&](int n) {
-        if (!mbar_wait(&bars->kv_full[n % kStages], (n / kStages) & 1)) ok = false;
-        return n % kStages;
-      };
-      auto issue_qk = [&](int stage, int half, int kt) {
-        const uint64_t kd = kdesc0 + static_cast<uint64_t>(stage * kStageUnits + half * kHalfUnits);
-        const uint32_t d = tmem_base + (kt & 1) * 64;
+    const bool elected = elect_one_sync();
+    constexpr uint32_t kStageUnits = Shape::kTileBytes >> 4;
+    const uint64_t qdesc = make_smem_desc_sw128(smem_u32(sQ), 16, 1024);
+    const uint64_t kdesc0 = make_smem_desc_sw128(smem_u32(sK), 16, 1024);
+    int g = 0;
+    for (int i = 0;; ++i) {
+      PackedItem it;
+      take_item(i, &it);
+      free_item(i);
+      if (it.count <= 0) break;
+      wait(&bars->q_full, i & 1, 82);
+      for (int j = it.lo; j < it.hi; ++j, ++g) {
+        const int stage = g % kStages;
+        wait(&bars->k_full[stage], (g / kStages) & 1, 82);
+        wait(&bars->s_free[g & 1], ((g >> 1) & 1) ^ 1, 82);
+        // The lanes meet before anything is issued that lets a barrier they wait on complete its next phase.
+        const bool run = __all_sync(0xffffffffu, !lost) && elected;
+        tc_fence_after();
+        const uint64_t kd = kdesc0 + static_cast<uint64_t>(stage * kStageUnits);
+        const uint32_t d = tmem_base + (g & 1) * 64;
 #pragma unroll
         for (int ks = 0; ks < D / 16; ++ks)
-          mma_ss_if(elected, d,
+          mma_ss_if(run, d,
                     qdesc + static_cast<uint64_t>((ks / 4) * (Shape::kQBlockBytes >> 4) + (ks % 4) * 2),
                     kd + static_cast<uint64_t>((ks / 4) * (Shape::kKVBlockBytes >> 4) + (ks % 4) * 2),
                     kIdescQK, ks > 0 ? 1u : 0u);
-        tc_commit_if(elected, &bars->s_full[kt & 1]);
-      };
-      if (ok) {
-        const int st = wait_stage(0);
-        tc_fence_after();
-        ok = __all_sync(0xffffffffu, ok);
-        if (ok) {
-          issue_qk(st, 0, 0);
-          if (nblk > 1) issue_qk(st, 1, 1);
-          tc_commit_if(elected, &bars->kv_empty[st]);
-        }
+        tc_commit_if(run, &bars->s_full[g & 1]);
+        tc_commit_if(run, &bars->k_empty[stage]);
+        tc_commit_if(run && j + 1 == it.hi, &bars->q_empty);
       }
-      __syncwarp();
-      for (int kt = 0; kt < nblk && ok; ++kt) {
-        const int st = wait_stage(kt + 1);  // {V(kt), K(kt + 2)}
-        if (ok) ok = mbar_wait(&bars->p_full[kt & 1], (kt >> 1) & 1);
+    }
+  } else if (warp == kPvWarp) {
+    // ---------------- O += P V ----------------
+    const bool elected = elect_one_sync();
+    constexpr uint32_t kStageUnits = Shape::kTileBytes >> 4;
+    const uint64_t vdesc0 = make_smem_desc_sw128(smem_u32(sV), Shape::kKVBlockBytes, 1024);
+    const uint32_t o_col = tmem_base + kColO;
+    int g = 0;
+    for (int i = 0;; ++i) {
+      PackedItem it;
+      take_item(i, &it);
+      free_item(i);
+      if (it.count <= 0) break;
+      const bool fine = is_fine(it);
+      if (i > 0) wait(&bars->o_empty, (i - 1) & 1, 88);
+      for (int j = it.lo; j < it.hi; ++j, ++g) {
+        const int stage = g % kStages;
+        wait(&bars->v_full[stage], (g / kStages) & 1, 88);
+        wait(&bars->p_full[g & 1], (g >> 1) & 1, 88);
+        const bool run = __all_sync(0xffffffffu, !lost) && elected;
         tc_fence_after();
-        const uint64_t vd = vdesc0 + static_cast<uint64_t>(st * kStageUnits);
-        const bool run = elected && ok;
+        const uint64_t vd = vdesc0 + static_cast<uint64_t>(stage * kStageUnits);
+        const uint32_t a = tmem_base + (g & 1) * 64;
 #pragma unroll
         for (int ks = 0; ks < kPackedKeys / 16; ++ks)
-          mma_ts_if(run, o_col, tmem_base + (kt & 1) * 64 + ks * 8,
-                    vd + static_cast<uint64_t>(ks * (2048 >> 4)), kIdescPV, (kt > 0 || ks > 0) ? 1u : 0u);
+          mma_ts_if(run, o_col, a + ks * 8, vd + static_cast<uint64_t>(ks * (2048 >> 4)), kIdescPV,
+                    ks > 0 || j > it.lo ? 1u : 0u);
         if (fine) {
 #pragma unroll
           for (int ks = 0; ks < kPackedKeys / 16; ++ks)
-            mma_ts_if(run, o_col, tmem_base + (kt & 1) * 64 + 32 + ks * 8,
-                      vd + static_cast<uint64_t>(ks * (2048 >> 4)), kIdescPV, 1u);
+            mma_ts_if(run, o_col, a + 32 + ks * 8, vd + static_cast<uint64_t>(ks * (2048 >> 4)), kIdescPV, 1u);
         }
-        // Completion points the softmax warps may wait on: the second-to-last PV (for a rescale in the
-        // last block) and the last one (for the epilogue).
-        tc_commit_if(run && kt == nblk - 2, &bars->pv_done);
-        tc_commit_if(run && kt == nblk - 1, &bars->o_final);
-        // The lanes meet before anything is issued that lets a barrier they wait on complete its next
-        // phase, and leave together when a wait ran out.
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (kt + 2 < nblk) issue_qk(st, 1, kt + 2);
-        tc_commit_if(elected, &bars->kv_empty[st]);
+        tc_commit_if(run, &bars->s_free[g & 1]);
+        tc_commit_if(run, &bars->v_empty[stage]);
+        // Completion points the softmax warps may wait on: the second-to-last PV (for a rescale in the last
+        // block) and the last one (for the epilogue).
+        tc_commit_if(run && j + 2 == it.hi, &bars->pv_done);
+        tc_commit_if(run && j + 1 == it.hi, &bars->o_final);
       }
-      if (!ok) packed_timeout(p.status, 82);
     }
   } else if (warp < 4) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
     // ---------------- softmax warps ----------------
     const int row = warp * 32 + lane;  // of the tile == tensor-memory lane
-    const bool valid = row < rows;
-    const int row_tok = static_cast<int>(p.div_g.div(valid ? row : 0));
-    const int head = row - row_tok * p.G;  // of the kv head's query heads
-    const int tok = t0 + row_tok;
     const uint32_t lane_addr = static_cast<uint32_t>(warp * 32) << 16;
     const uint32_t s_base = tmem_base + lane_addr;
     const uint32_t o_addr = tmem_base + lane_addr + kColO;
-    // Keys that this row sees: [c_lo, c_hi].
-    int c_lo = 0, c_hi = key_hi - 1;
-    if constexpr (KIND == kPackedPrefix) {
-      if (valid) c_hi = min(c_hi, p.kv_lens[tok] - 1);
-    } else {
-      if (p.mask_kind != LF_MASK_NONE) c_hi = min(rq.m - 1, tok + off);
-      if (p.mask_kind == LF_MASK_CAUSAL_WINDOW) c_lo = max(0, tok + off - (p.window - 1));
-    }
-    float m_used = -INFINITY;  // reference that P and O are scaled by (log2 domain)
-    float l_run = 0.f;
-    bool ok = true;
-    const bool idle = warp * 32 >= rows;  // no row of this warp is one of the tile's
+    int g = 0, twos = 0;  // blocks; items of two or more
 
     auto rescale_o = [&](int c, float alpha) {
       uint32_t orr[32];
@@ -458,249 +647,297 @@ __device__ __forceinline__ void packed_tile(const CUtensorMap& tmap_q, const CUt
       for (int i = 0; i < 32; ++i) orr[i] = __float_as_uint(__uint_as_float(orr[i]) * alpha);
       tmem_st_32x32b_x32(o_addr + c * 32, orr);
     };
-    for (int k = 0; k < nblk && ok; ++k) {
-      const int c0 = (lo + k) * kPackedKeys;
-      const int buf = k & 1;
-      const uint32_t s_addr = s_base + buf * 64;
-      if (!mbar_wait(&bars->s_full[buf], (k >> 1) & 1)) {
-        packed_timeout(p.status, 83);
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      if (c0 + kPackedKeys > rq.m) {
-        // V rows past the last key become zeros (the stage's next fill waits for this block's PV).
-        const int stage = (k + 1) % kStages;
-        if (!mbar_wait(&bars->kv_full[stage], ((k + 1) / kStages) & 1)) {
-          packed_timeout(p.status, 84);
-          ok = false;
-          break;
-        }
-        unsigned char* v = sKV + stage * (2 * Shape::kTileBytes);
-        const int first = rq.m - c0;  // (0 < first < 64)
-        for (int i = first * 8 + row; i < kPackedKeys * 8; i += 128)
-#pragma unroll
-          for (int kb = 0; kb < kBlocksD; ++kb)
-            *reinterpret_cast<uint4*>(v + kb * Shape::kKVBlockBytes + i * 16) = make_uint4(0, 0, 0, 0);
-        fence_proxy_async_smem();
-      }
-      if (!idle) {
-        uint32_t sr[2][32];
-        tmem_ld_32x32b_x32(s_addr, sr[0]);
-        tmem_ld_32x32b_x32(s_addr + 32, sr[1]);
-        tmem_wait_ld();
-        const int rel_lo = c_lo - c0, rel_hi = c_hi - c0;  // visible columns of this row in the block
-        const bool masked = valid && (rel_lo > 0 || rel_hi < kPackedKeys - 1);
 
-        if constexpr (SOFTCAP) {
-          // tanh(x), x = raw * a: x (1 - x^2 / 3) up to |x| = 0.125 (error below 4.1e-6), its series to
-          // x^7 up to 0.4 (below 6e-6), the unit's approximation beyond.
-          float mx[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int i = 0;; ++i) {
+      // (Only what the block loop needs is held in registers; the rest is read again behind it. With all the
+      // SM's memory taken as shared memory a spilled register comes from L2.)
+      int nblk, c0, c_lo, c_hi, m, rows;
+      bool fine;
+      {
+        PackedItem it;
+        take_item(i, &it);
+        it.count = warp_uniform(it.count);
+        if (it.count <= 0) break;
+        rows = it.count * p.G;
+        fine = warp_uniform(is_fine(it)) != 0;
+        nblk = warp_uniform(it.hi - it.lo);
+        c0 = warp_uniform(it.lo) * kPackedKeys;
+        m = warp_uniform(it.m);
+        // Keys that this row sees: [c_lo, c_hi].
+        const int tok = row < rows ? static_cast<int>(p.div_g.div(row)) : 0;
+        c_lo = 0, c_hi = m - 1;
+        if constexpr (KIND == kPackedPrefix) {
+          if (row < rows) c_hi = min(c_hi, p.kv_lens[it.q_row + tok] - 1);
+        } else {
+          const int last = it.pos + tok;
+          if (p.mask_kind != LF_MASK_NONE) c_hi = min(c_hi, last);
+          if (p.mask_kind == LF_MASK_CAUSAL_WINDOW) c_lo = max(0, last - (p.window - 1));
+        }
+      }
+      const bool valid = row < rows;
+      const bool idle = warp_uniform(warp * 32) >= rows;  // no row of this warp is one of the tile's
+      float m_used = p.m_first;  // reference that P and O are scaled by (log2 domain)
+      float l_run = 0.f;
+
+      for (int k = 0; k < nblk; ++k, ++g, c0 += kPackedKeys) {
+        const uint32_t s_addr = s_base + (g & 1) * 64;
+        wait(&bars->s_full[g & 1], (g >> 1) & 1, 83);
+        tc_fence_after();
+        if (c0 + kPackedKeys > m) {
+          // V rows past the last key become zeros (the stage's next fill waits for this block's PV).
+          const int stage = g % kStages;
+          wait(&bars->v_full[stage], (g / kStages) & 1, 84);
+          unsigned char* v = sV + stage * Shape::kTileBytes;
+          const int first = m - c0;  // (0 < first < 64)
+          for (int e = first * 8 + row; e < kPackedKeys * 8; e += 128)
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+            for (int kb = 0; kb < kBlocksD; ++kb)
+              *reinterpret_cast<uint4*>(v + kb * Shape::kKVBlockBytes + e * 16) = make_uint4(0, 0, 0, 0);
+          fence_proxy_async_smem();
+        }
+        if (!idle) {
+          uint32_t sr[2][32];
+          tmem_ld_32x32b_x32(s_addr, sr[0]);
+          tmem_ld_32x32b_x32(s_addr + 32, sr[1]);
+          tmem_wait_ld();
+
+          if constexpr (SOFTCAP) {
+            // tanh(x), x = raw * a: x (1 - x^2 / 3) up to |x| = 0.125 (error below 4.1e-6), its series to
+            // x^7 up to 0.4 (below 6e-6), the unit's approximation beyond.
+            float mx[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              mx[2 * c] = max3(mx[2 * c], fabsf(__uint_as_float(sr[c][i])),
-                               fabsf(__uint_as_float(sr[c][i + 1])));
-              mx[2 * c + 1] = max3(mx[2 * c + 1], fabsf(__uint_as_float(sr[c][i + 2])),
-                                   fabsf(__uint_as_float(sr[c][i + 3])));
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                mx[2 * c] = max3(mx[2 * c], fabsf(__uint_as_float(sr[c][e])),
+                                 fabsf(__uint_as_float(sr[c][e + 1])));
+                mx[2 * c + 1] = max3(mx[2 * c + 1], fabsf(__uint_as_float(sr[c][e + 2])),
+                                     fabsf(__uint_as_float(sr[c][e + 3])));
+              }
+            const float bound = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * fabsf(p.a);
+            const float a2 = p.a * p.a;
+            const float b1 = a2 * (-1.f / 3.f);
+            if (!__any_sync(0xffffffffu, valid && !(bound <= 0.125f))) {
+              const uint64_t a_2 = pack2(p.a, p.a), b_2 = pack2(b1 * p.a, b1 * p.a);
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                  const uint64_t r = pack2u(sr[c][e], sr[c][e + 1]);
+                  float t0, t1;
+                  unpack2(mul2(r, fma2(mul2(r, r), b_2, a_2)), t0, t1);
+                  sr[c][e] = __float_as_uint(t0);
+                  sr[c][e + 1] = __float_as_uint(t1);
+                }
+            } else if (!__any_sync(0xffffffffu, valid && !(bound <= 0.4f))) {
+              const float b2 = a2 * a2 * (2.f / 15.f);
+              const float b3 = a2 * a2 * a2 * (-17.f / 315.f);
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                  const float r = __uint_as_float(sr[c][e]), y = r * r;
+                  sr[c][e] = __float_as_uint((r * p.a) * fmaf(fmaf(fmaf(y, b3, b2), y, b1), y, 1.f));
+                }
+            } else {
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  sr[c][e] = __float_as_uint(tanh_approx(__uint_as_float(sr[c][e]) * p.a));
             }
-          const float bound = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * fabsf(p.a);
-          const float a2 = p.a * p.a;
-          const float b1 = a2 * (-1.f / 3.f);
-          if (!__any_sync(0xffffffffu, valid && !(bound <= 0.125f))) {
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float r = __uint_as_float(sr[c][i]);
-                sr[c][i] = __float_as_uint((r * p.a) * fmaf(r * r, b1, 1.f));
-              }
-          } else if (!__any_sync(0xffffffffu, valid && !(bound <= 0.4f))) {
-            const float b2 = a2 * a2 * (2.f / 15.f);
-            const float b3 = a2 * a2 * a2 * (-17.f / 315.f);
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int i = 0; i < 32; ++i) {
-                const float r = __uint_as_float(sr[c][i]), y = r * r;
-                sr[c][i] = __float_as_uint((r * p.a) * fmaf(fmaf(fmaf(y, b3, b2), y, b1), y, 1.f));
-              }
-          } else {
-#pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-              for (int i = 0; i < 32; ++i)
-                sr[c][i] = __float_as_uint(tanh_approx(__uint_as_float(sr[c][i]) * p.a));
           }
-        }
 
-        // Where every row of the warp has a reference and sees the whole block, P is taken against that
-        // reference without looking for the block's maximum first; P may then exceed 1, which bf16 and
-        // fp32 hold as exactly as any other magnitude (a row sum past 2^14 takes the other pass). Row sums
-        // are taken over the bf16 that the PV product sees: numerator and denominator carry the same
-        // rounding, and a row that one key dominates has none.
-        uint32_t pk[32];
-        bool own_max = __any_sync(0xffffffffu, fine || masked || (valid && m_used == -INFINITY));
-        if (!own_max) {
-          float fs[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float p0 = ex2_approx(fmaf(__uint_as_float(sr[c][i]), p.c2, -m_used));
-              const float p1 = ex2_approx(fmaf(__uint_as_float(sr[c][i + 1]), p.c2, -m_used));
-              const uint32_t pkv = pack_bf16x2(p0, p1);
-              pk[c * 16 + (i >> 1)] = pkv;
-              if ((i >> 1) & 1) add_bf16x2_to_f32(fs[2], fs[3], pkv);
-              else add_bf16x2_to_f32(fs[0], fs[1], pkv);
-            }
-          const float sum = (fs[0] + fs[1]) + (fs[2] + fs[3]);
-          own_max = __any_sync(0xffffffffu, valid && !(sum <= 16384.f));
-          if (!own_max) l_run += sum;
-        }
-        if (own_max) {
-          if (__any_sync(0xffffffffu, masked)) {
+          const int rel_lo = c_lo - c0, rel_hi = c_hi - c0;  // visible columns of this row in the block
+          if (__any_sync(0xffffffffu, valid && (rel_lo > 0 || rel_hi < kPackedKeys - 1))) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-              // Bit i: column c * 32 + i is visible (shifts by 32 and more give 0).
+              // Bit e: column c * 32 + e is visible (shifts by 32 and more give 0).
               uint32_t seen, upto;
               asm("shl.b32 %0, 0xffffffff, %1;" : "=r"(seen) : "r"(max(rel_lo - c * 32, 0)));
               asm("shl.b32 %0, 0xfffffffe, %1;" : "=r"(upto) : "r"(max(rel_hi - c * 32, 0)));
               seen = rel_hi < c * 32 ? 0u : seen & ~upto;
 #pragma unroll
-              for (int i = 0; i < 32; ++i)
-                if (!(seen & (1u << i))) sr[c][i] = 0xff800000u;  // -inf
+              for (int e = 0; e < 32; ++e)
+                if (!(seen & (1u << e))) sr[c][e] = 0xff800000u;  // -inf
             }
           }
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          // Where every row of the warp has a reference, P is taken against it without looking for the
+          // block's maximum first; P may then exceed 1, which bf16 and fp32 hold as exactly as any other
+          // magnitude (a row sum past 2^14 takes the other pass). Row sums are taken over the bf16 that the
+          // PV product sees: numerator and denominator carry the same rounding, and a row that one key
+          // dominates has none.
+          uint32_t pk[32];
+          bool own_max = __any_sync(0xffffffffu, fine || (valid && m_used == -INFINITY));
+          if (!own_max) {
+            float fs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              mx[2 * c] = max3(mx[2 * c], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
-              mx[2 * c + 1] = max3(mx[2 * c + 1], __uint_as_float(sr[c][i + 2]),
-                                   __uint_as_float(sr[c][i + 3]));
-            }
-          const float m_new = fmaxf(m_used, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.c2);
-          float alpha = 1.f;  // lazy rescale: the reference moves only when it is passed by 2^8
-          if (m_new > -INFINITY && (m_used == -INFINITY || m_new - m_used > 8.f)) {
-            alpha = ex2_approx(m_used - m_new);
-            m_used = m_new;
+              for (int e = 0; e < 32; e += 2) {
+                const float p0 = ex2_approx(fmaf(__uint_as_float(sr[c][e]), p.c2, -m_used));
+                const float p1 = ex2_approx(fmaf(__uint_as_float(sr[c][e + 1]), p.c2, -m_used));
+                const uint32_t pkv = pack_bf16x2(p0, p1);
+                pk[c * 16 + (e >> 1)] = pkv;
+                if ((e >> 1) & 1) add_bf16x2_to_f32(fs[2], fs[3], pkv);
+                else add_bf16x2_to_f32(fs[0], fs[1], pkv);
+              }
+            const float sum = (fs[0] + fs[1]) + (fs[2] + fs[3]);
+            own_max = __any_sync(0xffffffffu, valid && !(sum <= 16384.f));
+            if (!own_max) l_run += sum;
           }
-          if (k > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-            // O must hold every PV up to k-1: QK(k+1) is issued behind PV(k-1), so "S(k+1) is ready" says
-            // so; in the last block there is no S(k+1).
-            const bool last = k + 1 == nblk;
-            if (!mbar_wait(last ? &bars->pv_done : &bars->s_full[(k + 1) & 1],
-                           last ? 0u : (((k + 1) >> 1) & 1))) {
-              packed_timeout(p.status, 85);
-              ok = false;
-              break;
+          if (own_max) {
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; e += 4) {
+                mx[2 * c] = max3(mx[2 * c], __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
+                mx[2 * c + 1] = max3(mx[2 * c + 1], __uint_as_float(sr[c][e + 2]),
+                                     __uint_as_float(sr[c][e + 3]));
+              }
+            const float m_new = fmaxf(m_used, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.c2);
+            float alpha = 1.f;  // lazy rescale: the reference moves only when it is passed by 2^8
+            if (m_new > -INFINITY && (m_used == -INFINITY || m_new - m_used > 8.f)) {
+              alpha = ex2_approx(m_used - m_new);
+              m_used = m_new;
             }
-            tc_fence_after();
+            if (k > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
+              // O must hold every PV up to the block before: QK(g+1) is issued behind PV(g-1), so "S(g+1) is
+              // ready" says so; behind an item's last block that may be another item's, or none.
+              const bool last = k + 1 == nblk;
+              wait(last ? &bars->pv_done : &bars->s_full[(g + 1) & 1],
+                   last ? (twos & 1) : (((g + 1) >> 1) & 1), 85);
+              tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < D / 32; ++c) rescale_o(c, alpha);
-          }
-          const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
-          float ps[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; i += 2) {
-              const float p0 = ex2_approx(fmaf(__uint_as_float(sr[c][i]), p.c2, neg_m));
-              const float p1 = ex2_approx(fmaf(__uint_as_float(sr[c][i + 1]), p.c2, neg_m));
-              const uint32_t pkv = pack_bf16x2(p0, p1);
-              pk[c * 16 + (i >> 1)] = pkv;
-              if ((i >> 1) & 1) add_bf16x2_to_f32(ps[2], ps[3], pkv);
-              else add_bf16x2_to_f32(ps[0], ps[1], pkv);
+              for (int c = 0; c < D / 32; ++c) rescale_o(c, alpha);
             }
-          if (fine) {
-            uint32_t rest[32];
+            const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+            float ps[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              const int c = i >> 4, e = (2 * i) & 31;
-              const float p0 = ex2_approx(fmaf(__uint_as_float(sr[c][e]), p.c2, neg_m));
-              const float p1 = ex2_approx(fmaf(__uint_as_float(sr[c][e + 1]), p.c2, neg_m));
-              rest[i] = pack_bf16x2(p0 - bf16lo_to_f32(pk[i]), p1 - bf16hi_to_f32(pk[i]));
-              add_bf16x2_to_f32(ps[i & 2], ps[(i & 2) + 1], rest[i]);
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float p0 = ex2_approx(fmaf(__uint_as_float(sr[c][e]), p.c2, neg_m));
+                const float p1 = ex2_approx(fmaf(__uint_as_float(sr[c][e + 1]), p.c2, neg_m));
+                const uint32_t pkv = pack_bf16x2(p0, p1);
+                pk[c * 16 + (e >> 1)] = pkv;
+                if ((e >> 1) & 1) add_bf16x2_to_f32(ps[2], ps[3], pkv);
+                else add_bf16x2_to_f32(ps[0], ps[1], pkv);
+              }
+            if (fine) {
+#pragma unroll
+              for (int c = 0; c < 2; ++c) {
+                uint32_t rest[16];
+#pragma unroll
+                for (int f = 0; f < 16; ++f) {
+                  const float p0 = ex2_approx(fmaf(__uint_as_float(sr[c][2 * f]), p.c2, neg_m));
+                  const float p1 = ex2_approx(fmaf(__uint_as_float(sr[c][2 * f + 1]), p.c2, neg_m));
+                  const uint32_t hi = pk[c * 16 + f];
+                  rest[f] = pack_bf16x2(p0 - bf16lo_to_f32(hi), p1 - bf16hi_to_f32(hi));
+                  add_bf16x2_to_f32(ps[f & 2], ps[(f & 2) + 1], rest[f]);
+                }
+                tmem_st_32x32b_x16(s_addr + 32 + c * 16, rest);
+              }
             }
-            tmem_st_32x32b_x32(s_addr + 32, rest);
+            l_run = fmaf(l_run, alpha, (ps[0] + ps[1]) + (ps[2] + ps[3]));
           }
-          l_run = fmaf(l_run, alpha, (ps[0] + ps[1]) + (ps[2] + ps[3]));
+          tmem_st_32x32b_x32(s_addr, pk);
+          tmem_wait_st();
         }
-        tmem_st_32x32b_x32(s_addr, pk);
-        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->p_full[g & 1]);
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bars->p_full[buf]);
-    }
 
-    // ---------------- epilogue ----------------
-    if (nblk > 0 && ok && !mbar_wait(&bars->o_final, 0)) {
-      packed_timeout(p.status, 86);
-      ok = false;
-    }
-    tc_fence_after();
-    if (ok && !idle) {
-      if constexpr (KIND == kPackedPrefix) {
-        // Un-normalised rows and their (reference, sum), for the join with the requests' own keys.
-        const int64_t unit = (static_cast<int64_t>(tok) * p.Hkv + hkv) * p.G + head;
-        const int64_t at = static_cast<int64_t>(split) * p.B * p.Hkv * p.G + unit;
-        if (valid) p.part_ml[at] = make_float2(m_used, l_run);
-        float* dst = p.part_o + at * D;
+      // ---------------- epilogue ----------------
+      wait(&bars->o_final, i & 1, 86);
+      if (nblk > 1) ++twos;
+      tc_fence_after();
+      auto o_is_read = [&] {  // the next item's first PV may overwrite O
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars->o_empty);
+      };
+      const PackedItem& it = bars->item[i % kItemSlots];
+      const int row_tok = static_cast<int>(p.div_g.div(row));
+      const int head = row - row_tok * p.G;  // of the kv head's query heads
+      const bool sliced = KIND == kPackedPrefix || warp_uniform(it.part) >= 0;
+      // Rows of O: un-normalised with their (reference, sum) for the join, or the output (a row is D / 16 whole
+      // sectors of 32 bytes; one that saw no key is zeros).
+      const bool empty = l_run == 0.f;
+      const float inv = empty ? 0.f : 1.f / l_run;
+      float* part = nullptr;
+      __nv_bfloat16* dst = nullptr;
+      if (valid) {
+        if (!sliced) {
+          dst = p.out + static_cast<int64_t>(it.q_row + row_tok) * p.o_stride[0] +
+                static_cast<int64_t>(it.hkv * p.G + head) * p.o_stride[1];
+        } else {
+          int64_t at;
+          if constexpr (KIND == kPackedPrefix) {
+            at = static_cast<int64_t>(it.index) * p.B * p.Hkv * p.G +
+                 (static_cast<int64_t>(it.q_row + row_tok) * p.Hkv + it.hkv) * p.G + head;
+          } else {
+            at = (static_cast<int64_t>(it.part + it.index) * p.Hkv + it.hkv) * kPackedRows + row;
+          }
+          p.part_ml[at] = make_float2(m_used, l_run);
+          part = p.part_o + at * D;
+        }
+      }
 #pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t orr[32];
-          tmem_ld_32x32b_x32(o_addr + c * 32, orr);
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+        if (!idle) {
+          tmem_ld_32x32b_x32(o_addr + c, o);
           tmem_wait_ld();
+        }
+        if (c + 32 == D) {  // the next item's first PV may overwrite O
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&bars->o_empty);
+        }
+        if (sliced) {
           if (valid) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 8)
-              asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(
-                               dst + c * 32 + i),
-                           "r"(orr[i]), "r"(orr[i + 1]), "r"(orr[i + 2]), "r"(orr[i + 3]),
-                           "r"(orr[i + 4]), "r"(orr[i + 5]), "r"(orr[i + 6]), "r"(orr[i + 7])
-                           : "memory");
+            for (int e = 0; e < 32; e += 8) stg_32(part + c + e, &o[e]);
           }
-        }
-      } else {
-        // 32 columns of 32 rows at a time go through a swizzled 2 KB buffer of the warp, so that a store
-        // instruction writes eight 64-byte row segments. A row that saw no key is zeros.
-        const float inv = 1.f / l_run;
-        const bool empty = l_run == 0.f || nblk == 0;
-        unsigned char* stage = sStage + warp * 2048;
-        const int64_t row_off = valid ? static_cast<int64_t>(rq.q0 + tok) * p.o_stride[0] +
-                                            static_cast<int64_t>(hkv * p.G + head) * p.o_stride[1]
-                                      : -1;
-#pragma unroll 1
-        for (int c = 0; c < D / 32; ++c) {
-          uint32_t orr[32];
-          tmem_ld_32x32b_x32(o_addr + c * 32, orr);
-          tmem_wait_ld();
+        } else if (valid) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {  // piece q of row r sits at position q ^ ((r >> 1) & 3)
-            uint32_t w[4];
+          for (int e = 0; e < 32; e += 16) {
+            uint32_t w[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = empty ? 0u
-                           : pack_bf16x2(__uint_as_float(orr[8 * q + 2 * e]) * inv,
-                                         __uint_as_float(orr[8 * q + 2 * e + 1]) * inv);
-            *reinterpret_cast<uint4*>(stage + lane * 64 + ((q ^ ((lane >> 1) & 3)) << 4)) =
-                make_uint4(w[0], w[1], w[2], w[3]);
+            for (int f = 0; f < 8; ++f)
+              w[f] = empty ? 0u
+                           : pack_bf16x2(__uint_as_float(o[e + 2 * f]) * inv,
+                                         __uint_as_float(o[e + 2 * f + 1]) * inv);
+            if (p.out_sectors) {
+              stg_32(dst + c + e, w);
+            } else {
+              *reinterpret_cast<uint4*>(dst + c + e) = make_uint4(w[0], w[1], w[2], w[3]);
+              *reinterpret_cast<uint4*>(dst + c + e + 8) = make_uint4(w[4], w[5], w[6], w[7]);
+            }
           }
-          __syncwarp();
-#pragma unroll
-          for (int rr = 0; rr < 4; ++rr) {
-            const int r = rr * 8 + (lane >> 2), q = lane & 3;
-            const uint4 w = *reinterpret_cast<const uint4*>(stage + r * 64 + ((q ^ ((r >> 1) & 3)) << 4));
-            const int64_t o = __shfl_sync(0xffffffffu, row_off, r);
-            if (o >= 0) *reinterpret_cast<uint4*>(p.out + o + c * 32 + q * 8) = w;
-          }
-          __syncwarp();
         }
       }
+      if constexpr (KIND != kPackedPrefix) {
+        if (sliced) {
+          // The CTA that finishes the last slice of a tile joins them all, in order.
+          __threadfence();
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          if (threadIdx.x == 0)
+            bars->last_part = atomicAdd(&p.list[2 + it.counter * p.Hkv + it.hkv], 1u) + 1u ==
+                              static_cast<uint32_t>(it.n_parts);
+          asm volatile("bar.sync 1, 128;" ::: "memory");
+          const bool join = warp_uniform(bars->last_part) != 0;
+          asm volatile("bar.sync 1, 128;" ::: "memory");  // (the word is free again)
+          if (join && !idle) {
+            __threadfence();
+            join_slices<D>(p, it, warp, lane, rows);
+          }
+        }
+      }
+      free_item(i);
     }
   }
 
@@ -721,6 +958,7 @@ __device__ __forceinline__ void packed_tile(const CUtensorMap& tmap_q, const CUt
 struct PackedScore {
   bool softcap = false;
   float a = 1.f, c2 = 1.f;
+  float m_first = -INFINITY;
 };
 
 inline int packed_score(float scale, int n_mod, const int32_t* op, const float* arg, PackedScore* s) {
@@ -746,6 +984,9 @@ inline int packed_score(float scale, int n_mod, const int32_t* op, const float* 
   if (i < n_mod || !(s->c2 >= 0.f) || !(s->c2 < 1e30f) || !(fabsf(s->a) < 1e6f)) return LF_ERR_UNSUPPORTED;
   // (A factor of zero, or below the normal numbers, would turn masked scores into NaN.)
   s->c2 = fmaxf(s->c2 * kPackedLog2e, FLT_MIN);
+  // Capped logits lie within c2 of zero: up to 80, rows can begin with the reference 0 instead of looking
+  // for their first maximum (P from 2^-80; a row sum past 2^14 moves the reference as usual).
+  if (s->softcap && s->c2 <= 80.f) s->m_first = 0.f;
   return LF_OK;
 }
 

@@ -13,31 +13,38 @@ __global__ void __launch_bounds__(kPackedThreads, 2)
     packed_prefill_kernel(const __grid_constant__ CUtensorMap tmap_q,
                           const __grid_constant__ CUtensorMap tmap_k,
                           const __grid_constant__ CUtensorMap tmap_v, const PackedParams p) {
-  extern __shared__ unsigned char smem[];
   pdl_trigger();
-  pdl_wait();
-  packed_tile<D, KIND, SOFTCAP>(tmap_q, tmap_k, tmap_v, p, smem, blockIdx.x);
+  packed_tiles<D, KIND, SOFTCAP>(tmap_q, tmap_k, tmap_v, p, blockIdx.x);
 }
 
-// Order of the tiles of a batch that does not fit the machine at once: longest first, whosever they are
-// (counting sort by key blocks). With the requests one after the other the last one's longest tile would
-// start when the rest is nearly done. One CTA; among tiles of one length the order is arbitrary, and no
-// result depends on it.
+// The list of items of a batch: its tiles, longest first, whosever they are (counting sort by key blocks;
+// with the requests one after the other the last one's longest tile would start when the rest is nearly
+// done), and those that are long next to what a CTA has to do in all cut into slices of their keys (a
+// few new tokens behind a long context are a few tiles). One CTA; among items of one length the order is
+// arbitrary, and no result depends on it.
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderLevels = 1024;
 constexpr int kOrderRequests = 8192;  // in shared memory; larger batches keep the requests' order
+constexpr int kWholeBlocks = 32;      // tiles of up to 2048 keys are never cut: a prompt of that length has
+                                      // the same result in every batch
+constexpr int kSliceBlocks = 16;      // at least, since a slice costs the store and the join of its rows
 
 template <int KIND>
 __global__ void __launch_bounds__(kOrderThreads)
-    packed_order_kernel(const PackedParams p, int2* items, int32_t* n_items) {
+    packed_order_kernel(const PackedParams p, PackedItem* items, const int max_items, const int max_parts,
+                        const int n_slots) {
   extern __shared__ int32_t s_first[];  // [B + 1] first tile of each request
   __shared__ int32_t s_level[kOrderLevels];
   __shared__ int32_t s_warp[kOrderThreads / 32];
-  __shared__ int32_t s_longest;
+  __shared__ unsigned long long s_blocks;
+  __shared__ int32_t s_longest, s_parts, s_cut;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_trigger();
   s_level[tid] = 0;
-  if (tid == 0) s_longest = 0;
+  if (tid == 0) {
+    s_longest = s_parts = s_cut = 0;
+    s_blocks = 0;
+  }
   __syncthreads();
   pdl_wait();
   // Exclusive sums over the threads of the CTA; `all` gets the total.
@@ -51,6 +58,7 @@ __global__ void __launch_bounds__(kOrderThreads)
     if (lane == 31) s_warp[warp] = incl;
     __syncthreads();
     int before = 0, total = 0;
+#pragma unroll
     for (int w = 0; w < kOrderThreads / 32; ++w) {
       const int x = s_warp[w];
       if (w < warp) before += x;
@@ -60,55 +68,94 @@ __global__ void __launch_bounds__(kOrderThreads)
     *all = total;
     return before + incl - v;
   };
-  int base = 0, longest = 0;
+  int base = 0;
   for (int b0 = 0; b0 < p.B; b0 += kOrderThreads) {
     const int b = b0 + tid;
     int tiles = 0;
     if (b < p.B) {
       const PackedRequest r = packed_request<KIND>(p, b);
       tiles = (r.n + p.tq - 1) / p.tq;
-      longest = max(longest, r.m);
     }
     int all;
     const int first = scan(tiles, &all);
     if (b < p.B) s_first[b] = base + first;
     base += all;
   }
-  const int n = min(base, p.n_tiles);
-  atomicMax(&s_longest, longest);
   __syncthreads();
-  int shift = 0;
-  while ((((s_longest + kPackedKeys - 1) / kPackedKeys) >> shift) >= kOrderLevels) ++shift;
-
-  auto tile_of = [&](int e) {
+  const int n = min(base, p.n_tiles);
+  auto item_of = [&](int e) {
     int lo = 0, hi = p.B - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
       if (s_first[mid] <= e) lo = mid;
       else hi = mid - 1;
     }
-    return make_int2(lo, e - s_first[lo]);
+    return packed_item(p, packed_request<KIND>(p, lo), e - s_first[lo]);
   };
-  auto level_of = [&](int2 at) {  // longest first: level 0
-    const PackedRequest r = packed_request<KIND>(p, at.x);
-    const int t0 = at.y * p.tq, off = r.m - r.n;
-    int last = r.m, first = 0;
-    if (p.mask_kind != LF_MASK_NONE) last = min(last, min(t0 + p.tq, r.n) + off);
-    if (p.mask_kind == LF_MASK_CAUSAL_WINDOW) first = max(0, t0 + off - (p.window - 1));
-    const int blocks = last > first ? (last + kPackedKeys - 1) / kPackedKeys - first / kPackedKeys : 0;
+  // How much there is, and so how long a slice may be.
+  {
+    int longest = 0;
+    unsigned long long blocks = 0;
+    for (int e = tid; e < n; e += kOrderThreads) {
+      const PackedItem it = item_of(e);
+      longest = max(longest, it.hi - it.lo);
+      blocks += it.hi - it.lo;
+    }
+#pragma unroll
+    for (int d = 16; d >= 1; d >>= 1) {
+      longest = max(longest, __shfl_xor_sync(0xffffffffu, longest, d));
+      blocks += __shfl_xor_sync(0xffffffffu, blocks, d);
+    }
+    if (lane == 0) {
+      atomicMax(&s_longest, longest);
+      atomicAdd(&s_blocks, blocks);
+    }
+  }
+  __syncthreads();
+  // Slices of 0.6 of a CTA's share, so that the last ones to start do not stand out.
+  const long long share = (static_cast<long long>(s_blocks) * p.Hkv * 3 + 5ll * n_slots - 1) / (5ll * n_slots);
+  const int slice = static_cast<int>(min(max(share, static_cast<long long>(kSliceBlocks)), 1ll << 28));
+  const int whole = max(kWholeBlocks, slice + slice / 4);
+  auto parts_of = [&](int blocks) { return blocks > whole ? (blocks + slice - 1) / slice : 1; };
+  int shift = 0;
+  while ((s_longest >> shift) >= kOrderLevels) ++shift;
+  auto level_of = [&](int blocks) {  // longest first
     return kOrderLevels - 1 - min(blocks >> shift, kOrderLevels - 1);
   };
-  for (int e = tid; e < n; e += kOrderThreads) atomicAdd(&s_level[level_of(tile_of(e))], 1);
+  for (int e = tid; e < n; e += kOrderThreads) {
+    const PackedItem it = item_of(e);
+    const int blocks = it.hi - it.lo, parts = parts_of(blocks);
+    atomicAdd(&s_level[level_of((blocks + parts - 1) / parts)], parts);
+  }
   __syncthreads();
-  int all;
-  const int mine = scan(s_level[tid], &all);
+  int n_items;
+  const int mine = scan(s_level[tid], &n_items);
   s_level[tid] = mine;
   __syncthreads();
   for (int e = tid; e < n; e += kOrderThreads) {
-    const int2 at = tile_of(e);
-    items[atomicAdd(&s_level[level_of(at)], 1)] = at;
+    PackedItem it = item_of(e);
+    const int lo = it.lo, blocks = it.hi - it.lo, parts = parts_of(blocks);
+    const int at = atomicAdd(&s_level[level_of((blocks + parts - 1) / parts)], parts);
+    if (parts > 1) {
+      it.part = atomicAdd(&s_parts, parts);
+      it.counter = atomicAdd(&s_cut, 1);
+      it.n_parts = parts;
+    }
+    // (The host's room follows from the lengths of slices; see lf_packed_workspace_bytes.)
+    if (at + parts > max_items || (parts > 1 && it.part + parts > max_parts)) continue;
+    for (int s = 0; s < parts; ++s) {
+      it.index = s;
+      it.lo = lo + static_cast<int>(static_cast<long long>(blocks) * s / parts);
+      it.hi = lo + static_cast<int>(static_cast<long long>(blocks) * (s + 1) / parts);
+      items[at + s] = it;
+    }
+    if (parts > 1)
+      for (int h = 0; h < p.Hkv; ++h) p.list[2 + it.counter * p.Hkv + h] = 0;
   }
-  if (tid == 0) *n_items = n;
+  if (tid == 0) {
+    p.list[0] = min(n_items, max_items);
+    p.list[1] = 0;
+  }
 }
 
 static int sm_count() {
@@ -125,12 +172,41 @@ static int sm_count() {
 // Tiles of a kv head that a batch has at most: whatever the lengths, each request has one partly filled.
 static int64_t most_tiles(int32_t B, int32_t T, int32_t tq) { return T / tq + std::min(B, T); }
 
-// Batches of more tiles than two per SM are ordered; the others start all at once.
-static bool is_ordered(int64_t tiles, int32_t Hkv, int32_t B) {
-  return tiles * Hkv > 2ll * sm_count() && B <= kOrderRequests && B > 1;
+// Whether a batch gets a list, and the room that it needs: batches of more tiles than two per SM, and
+// those whose tiles can be long. `max_keys`: keys that a request has at most. The others start all at
+// once, and a launch ahead of them would cost more than an order brings.
+struct PackedList {
+  bool used = false;
+  int64_t max_items = 0, max_parts = 0;  // (of a kv head)
+  size_t head_bytes = 0, item_bytes = 0, part_bytes = 0;
+  size_t bytes() const { return used ? head_bytes + item_bytes + part_bytes : 0; }
+};
+static PackedList plan_list(int32_t B, int32_t T, int32_t Hq, int32_t Hkv, int32_t D, int64_t max_keys) {
+  PackedList l;
+  const int64_t sms = sm_count(), tiles = most_tiles(B, T, kPackedRows / (Hq / Hkv));
+  const bool cuts = max_keys > static_cast<int64_t>(kWholeBlocks) * kPackedKeys;
+  l.used = B <= kOrderRequests && (cuts || (tiles * Hkv > 2 * sms && B > 1));
+  if (!l.used) return l;
+  // Slices: a tile of n blocks has ceil(n / slice) with slice >= 0.6 of a CTA's share W / (2 sms) and n >
+  // 1.25 slice, so all heads' together are at most W / slice + W / (1.25 slice) = 6 sms.
+  l.max_parts = cuts ? (6 * sms + Hkv - 1) / Hkv + 1 : 0;
+  l.max_items = tiles + l.max_parts;
+  l.head_bytes = ((2 + static_cast<size_t>(l.max_parts) / 2 * Hkv) * 4 + 127) / 128 * 128;
+  l.item_bytes = (static_cast<size_t>(l.max_items) * sizeof(PackedItem) + 127) / 128 * 128;
+  l.part_bytes = static_cast<size_t>(l.max_parts) * Hkv * kPackedRows * (D + 2) * 4;
+  return l;
 }
 
-constexpr size_t kOrderHeader = 16;
+// Keys that a request has at most, and that all have together.
+static int64_t most_keys(const LfPackedArgs* a, int64_t* together) {
+  if (!a->block_table) {
+    *together = a->Tk;
+    return a->Tk;
+  }
+  const int64_t held = static_cast<int64_t>(a->bt_blocks) * a->page_size;
+  *together = std::min(held * a->B, static_cast<int64_t>(a->n_pages) * a->page_size);
+  return held;
+}
 
 template <int D, int KIND, bool SOFTCAP>
 static int launch_packed(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
@@ -147,9 +223,10 @@ static int launch_packed(const CUtensorMap& mq, const CUtensorMap& mk, const CUt
 }
 
 template <int KIND>
-static int launch_order(const PackedParams& p, int2* items, int32_t* n_items, cudaStream_t st) {
+static int launch_order(const PackedParams& p, PackedItem* items, const PackedList& l, cudaStream_t st) {
   const size_t smem = (static_cast<size_t>(p.B) + 1) * sizeof(int32_t);
-  launch_pdl(packed_order_kernel<KIND>, dim3(1), kOrderThreads, smem, st, p, items, n_items);
+  launch_pdl(packed_order_kernel<KIND>, dim3(1), kOrderThreads, smem, st, p, items,
+             static_cast<int>(l.max_items), static_cast<int>(l.max_parts), 2 * sm_count());
   return check_launch("packed_order_kernel");
 }
 
@@ -157,11 +234,13 @@ static int launch_order(const PackedParams& p, int2* items, int32_t* n_items, cu
 
 extern "C" {
 
-size_t lf_packed_workspace_bytes(int32_t B, int32_t T, int32_t Hq, int32_t Hkv) {
+size_t lf_packed_workspace_bytes(const LfPackedArgs* a) {
   using namespace lf;
-  if (B <= 0 || T <= 0 || Hkv <= 0 || Hq <= 0 || Hq % Hkv || Hq / Hkv > kPackedRows) return 0;
-  const int64_t tiles = most_tiles(B, T, kPackedRows / (Hq / Hkv));
-  return is_ordered(tiles, Hkv, B) ? kOrderHeader + static_cast<size_t>(tiles) * sizeof(int2) : 0;
+  if (!a || a->B <= 0 || a->T <= 0 || a->Hkv <= 0 || a->Hq <= 0 || a->Hq % a->Hkv ||
+      a->Hq / a->Hkv > kPackedRows)
+    return 0;
+  int64_t together;
+  return plan_list(a->B, a->T, a->Hq, a->Hkv, a->D, most_keys(a, &together)).bytes();
 }
 
 int lf_packed_prefill_bf16(const LfPackedArgs* a, void* stream) {
@@ -192,6 +271,7 @@ int lf_packed_prefill_bf16(const LfPackedArgs* a, void* stream) {
   p.out = static_cast<__nv_bfloat16*>(a->out);
   p.o_stride[0] = a->o_stride[0];
   p.o_stride[1] = a->o_stride[1];
+  p.out_sectors = reinterpret_cast<uintptr_t>(a->out) % 32 == 0 && a->o_stride[0] % 16 == 0 && a->o_stride[1] % 16 == 0;
   p.cu_q = a->cu_q;
   p.cu_k = a->cu_k;
   p.kv_lens = a->kv_lens;
@@ -207,6 +287,7 @@ int lf_packed_prefill_bf16(const LfPackedArgs* a, void* stream) {
   p.window = a->window;
   p.a = score.a;
   p.c2 = score.c2;
+  p.m_first = score.m_first;
   p.bt_blocks = a->bt_blocks;
   p.page_size = paged ? a->page_size : 1;
   p.page_shift = packed_page_shift(p.page_size);
@@ -227,41 +308,42 @@ int lf_packed_prefill_bf16(const LfPackedArgs* a, void* stream) {
   if (rc != LF_OK) return rc;
 
   const int64_t tiles = most_tiles(a->B, a->T, p.tq);
-  const bool ordered = is_ordered(tiles, a->Hkv, a->B);
+  int64_t keys;
+  const int64_t max_keys = most_keys(a, &keys);
+  const PackedList list = plan_list(a->B, a->T, a->Hq, a->Hkv, a->D, max_keys);
   // The heads of a chunk run together: as many as keep their K and V in half of L2, since the tiles that
   // read them do so at different times.
-  const int64_t keys = paged ? std::min<int64_t>(static_cast<int64_t>(a->n_pages) * a->page_size,
-                                                 static_cast<int64_t>(a->B) * a->bt_blocks * a->page_size)
-                             : a->Tk;
-  const int64_t fit = (64ll << 20) / std::max<int64_t>(1, keys * a->D * 4);
-  const int64_t chunks = (a->Hkv + std::max<int64_t>(fit, 1) - 1) / std::max<int64_t>(fit, 1);
+  const int64_t fit = std::max<int64_t>(1, (64ll << 20) / std::max<int64_t>(1, keys * a->D * 4));
+  const int64_t chunks = (a->Hkv + fit - 1) / fit;
   const int64_t per_chunk = (a->Hkv + chunks - 1) / chunks;
-  if (tiles * per_chunk * chunks > 0x7fffffff) return LF_ERR_TOO_LARGE;
+  if ((tiles + list.max_parts) * per_chunk * chunks > 0x7fffffff - 4096) return LF_ERR_TOO_LARGE;
   p.n_tiles = static_cast<int32_t>(tiles);
   p.div_chunk = FastDiv::make(static_cast<int32_t>(per_chunk));
   p.div_tiles = FastDiv::make(p.n_tiles);
   p.div_g = FastDiv::make(G);
-  const unsigned grid = static_cast<unsigned>(tiles * per_chunk * chunks);
+  int64_t grid = tiles * per_chunk * chunks;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (ordered) {
-    if (!a->workspace || a->workspace_bytes < lf_packed_workspace_bytes(a->B, a->T, a->Hq, a->Hkv))
-      return LF_ERR_WORKSPACE;
-    if (!packed_aligned(a->workspace)) return LF_ERR_ALIGNMENT;
-    int32_t* n_items = static_cast<int32_t*>(a->workspace);
-    int2* items = reinterpret_cast<int2*>(static_cast<char*>(a->workspace) + kOrderHeader);
-    rc = paged ? launch_order<kPackedPaged>(p, items, n_items, st)
-               : launch_order<kPackedDense>(p, items, n_items, st);
+  if (list.used) {
+    if (!a->workspace || a->workspace_bytes < list.bytes()) return LF_ERR_WORKSPACE;
+    if (reinterpret_cast<uintptr_t>(a->workspace) & 31u) return LF_ERR_ALIGNMENT;  // (32-byte stores)
+    char* ws = static_cast<char*>(a->workspace);
+    PackedItem* items = reinterpret_cast<PackedItem*>(ws + list.head_bytes);
+    p.list = reinterpret_cast<uint32_t*>(ws);
+    p.part_o = reinterpret_cast<float*>(ws + list.head_bytes + list.item_bytes);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + list.max_parts * a->Hkv * kPackedRows * a->D);
+    rc = paged ? launch_order<kPackedPaged>(p, items, list, st)
+               : launch_order<kPackedDense>(p, items, list, st);
     if (rc != LF_OK) return rc;
     p.items = items;
-    p.n_items = n_items;
+    grid = std::min<int64_t>(grid + list.max_parts * per_chunk * chunks, 2ll * sm_count());
   }
   auto with_d = [&](auto d) {
     constexpr int D = decltype(d)::value;
     if (paged)
-      return score.softcap ? launch_packed<D, kPackedPaged, true>(mq, mk, mv, p, grid, st)
-                           : launch_packed<D, kPackedPaged, false>(mq, mk, mv, p, grid, st);
-    return score.softcap ? launch_packed<D, kPackedDense, true>(mq, mk, mv, p, grid, st)
-                         : launch_packed<D, kPackedDense, false>(mq, mk, mv, p, grid, st);
+      return score.softcap ? launch_packed<D, kPackedPaged, true>(mq, mk, mv, p, static_cast<unsigned>(grid), st)
+                           : launch_packed<D, kPackedPaged, false>(mq, mk, mv, p, static_cast<unsigned>(grid), st);
+    return score.softcap ? launch_packed<D, kPackedDense, true>(mq, mk, mv, p, static_cast<unsigned>(grid), st)
+                         : launch_packed<D, kPackedDense, false>(mq, mk, mv, p, static_cast<unsigned>(grid), st);
   };
   return a->D == 128 ? with_d(std::integral_constant<int, 128>{}) : with_d(std::integral_constant<int, 64>{});
 }

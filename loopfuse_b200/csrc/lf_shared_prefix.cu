@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32, 2) own_kernel(const OwnParams 
   constexpr int NT = D / 8;
   constexpr int CPR = D / 8, RPI = 32 / CPR;
   constexpr int kRowBytes = D * 2, kStageBytes = 2 * kOwnGroup * kRowBytes;
-  extern __shared__ __align__(128) unsigned char smem[];
+  extern __shared__ __align__(1024) unsigned char smem[];
   pdl_trigger();
   pdl_wait();
   const int split = blockIdx.x;
@@ -380,10 +380,8 @@ template <int D, bool SOFTCAP>
 __global__ void __launch_bounds__(kPackedThreads, 2)
     prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
                   const __grid_constant__ CUtensorMap tmap_v, const PackedParams p) {
-  extern __shared__ unsigned char smem[];
   pdl_trigger();
-  pdl_wait();
-  packed_tile<D, kPackedPrefix, SOFTCAP>(tmap_q, tmap_k, tmap_v, p, smem, blockIdx.x);
+  packed_tiles<D, kPackedPrefix, SOFTCAP>(tmap_q, tmap_k, tmap_v, p, blockIdx.x);
 }
 
 // How a call is cut: slices of the prefix (a multiple of a key block each), and of the requests' own keys.
@@ -516,6 +514,7 @@ int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* a, void* stream) {
     pp.tq = kPackedRows / a->G;
     pp.a = score.a;
     pp.c2 = score.c2;
+    pp.m_first = score.m_first;
     pp.bt_blocks = a->bt_blocks;
     pp.page_size = a->page_size;
     pp.page_shift = page_shift;
@@ -523,7 +522,6 @@ int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* a, void* stream) {
     pp.box = packed_box(a->page_size);
     pp.prefix_len = prefix_len;
     pp.chunk = cut.prefix_chunk;
-    pp.splits = cut.prefix_splits;
     pp.part_o = part_o;
     pp.part_ml = part_ml;
     pp.status = a->status;

@@ -378,7 +378,7 @@ def test_packed_batch_of_many_tiles_is_ordered_and_the_same():
     T = sum(lens)
     q, k, v = normal(g, T, 16, D), normal(g, T, 16, D), normal(g, T, 16, D)
     cu = offsets(lens)
-    assert _workspace(len(lens), T, 16, 16) > 0
+    assert _workspace(len(lens), T, 16, 16, D) > 0
     ws = F.DecodeWorkspace()
     got = F.packed_prefill_attention(q, k, v, cu, scale=D ** -0.5, workspace=ws)
     assert torch.equal(got, F.packed_prefill_attention(q, k, v, cu, scale=D ** -0.5, workspace=ws))
@@ -389,9 +389,60 @@ def test_packed_batch_of_many_tiles_is_ordered_and_the_same():
         assert torch.equal(alone, got[one]), b
 
 
-def _workspace(B, T, Hq, Hkv):
+def _workspace(B, T, Hq, Hkv, D):
+    import ctypes
+
     from loopfuse_b200 import _native
-    return _native.load().lf_packed_workspace_bytes(B, T, Hq, Hkv)
+    a = _native.LfPackedArgs()
+    a.B, a.T, a.Tk, a.Hq, a.Hkv, a.D = B, T, T, Hq, Hkv, D
+    return _native.load().lf_packed_workspace_bytes(ctypes.byref(a))
+
+
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 4, 4), (128, 8, 2)])
+@pytest.mark.parametrize("paged", [False, True])
+def test_packed_few_tokens_behind_long_contexts(D, Hq, Hkv, paged):
+    """Long tiles are cut into slices of their keys, which the last one to finish joins."""
+    g = torch.Generator(device="cuda").manual_seed(14)
+    lens, keys, P = [3, 40, 1, 0, 200], [6000, 9001, 2049, 10, 3111], 16
+    q = normal(g, sum(lens), Hq, D) * 3
+    k, v = normal(g, sum(keys), Hkv, D), normal(g, sum(keys), Hkv, D)
+    ck = offsets(keys)
+    options = dict(cu_seqlens_k=ck)
+    kk, vv = k, v
+    if paged:
+        blocks = [-(-m // P) for m in keys]
+        ids = torch.randperm(sum(blocks), generator=g, device="cuda")
+        kk, vv = (torch.full((sum(blocks), P, Hkv, D), float("nan"), dtype=torch.bfloat16, device="cuda")
+                  for _ in "kv")
+        table = torch.zeros(len(keys), max(blocks), dtype=torch.int32, device="cuda")
+        for b, m in enumerate(keys):
+            mine = ids[sum(blocks[:b]):sum(blocks[:b + 1])]
+            table[b, :len(mine)] = mine.int()
+            j = torch.arange(m, device="cuda")
+            kk[mine[j // P], j % P], vv[mine[j // P], j % P] = k[ck[b]:ck[b + 1]], v[ck[b]:ck[b + 1]]
+        options = dict(block_table=table, seq_lens=ints(keys))
+    for cap, mask, window in ((0.0, S.MASK_CAUSAL, 0), (30.0, S.MASK_CAUSAL_WINDOW, 5000)):
+        st = F.new_status("cuda")
+        got = F.packed_prefill_attention(q, kk, vv, offsets(lens), scale=D ** -0.5, status=st,
+                                         mods=softcap(cap) if cap else (), mask_kind=mask, window=window, **options)
+        again = F.packed_prefill_attention(q, kk, vv, offsets(lens), scale=D ** -0.5,
+                                           mods=softcap(cap) if cap else (), mask_kind=mask, window=window, **options)
+        assert int(st.item()) == 0 and torch.equal(got, again)
+        check_packed(got, q, lambda b: (k[ck[b]:ck[b + 1]], v[ck[b]:ck[b + 1]]), lens, D ** -0.5, cap, mask, window)
+
+
+def test_packed_many_requests_without_keys():
+    """Tiles without a key block, more of them than a CTA keeps in hand at once, between ordinary ones."""
+    g = torch.Generator(device="cuda").manual_seed(15)
+    lens = [30] * 900
+    keys = [0 if b % 9 else 30 for b in range(900)]
+    q, k, v = normal(g, sum(lens), 4, 64), normal(g, sum(keys), 4, 64), normal(g, sum(keys), 4, 64)
+    got = F.packed_prefill_attention(q, k, v, offsets_fast(lens), cu_seqlens_k=offsets_fast(keys), scale=0.125)
+    got = got.view(900, 30, 4, 64)
+    assert (got[torch.tensor([b for b in range(900) if b % 9])] == 0).all()
+    want, bound = reference(q.view(900, 30, 4, 64)[::9].transpose(1, 2), k.view(100, 30, 4, 64).transpose(1, 2),
+                            v.view(100, 30, 4, 64).transpose(1, 2), 0.125, 0.0, seen_of(30, 30, S.MASK_CAUSAL, 0))
+    check(got[::9].transpose(1, 2), want, bound)
 
 
 def test_packed_batch_beyond_the_order_kernels_requests():
