@@ -81,6 +81,7 @@ struct PackedParams {
   float m_first;              // a row's first reference: -inf, or 0 where no logit is far from it
   int32_t bt_blocks, page_size, page_shift, n_pages;
   int32_t box;                // keys per copy of a paged operand: they lie in one page
+  int32_t page_groups;        // groups of 8 slots per page, where a copy can move several (see packed_pool_map)
   int32_t n_tiles;            // tiles of a kv head (no list: an upper bound)
   FastDiv div_chunk;          // heads of a chunk of kv heads (see the launch); prefix: kv heads
   FastDiv div_tiles;          // tiles (no list)
@@ -336,6 +337,10 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
   constexpr uint32_t kColO = 128;
   constexpr int kKWarp = 4, kQkWarp = 5, kVWarp = 6, kPvWarp = 7;
   constexpr bool kPages = KIND != kPackedDense;
+  // A K or V block in shared memory: 8-row groups of 64-column halves, [half][group] where one copy moves
+  // them all, [group][half] where a copy moves the groups of a page.
+  constexpr uint32_t kHalf = kPages ? 1024 : Shape::kKVBlockBytes;         // bytes between halves
+  constexpr uint32_t kGroup = kPages ? 1024 * kBlocksD : 1024;             // and between groups
 
   // (Aligned by declaration: every address is a constant then, and none of them takes registers.)
   extern __shared__ __align__(1024) unsigned char smem[];
@@ -495,62 +500,77 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
             mbar_arrive_expect_tx(&bars->q_full, static_cast<uint32_t>(p.tq * p.G) * 128 * kBlocksD);
 #pragma unroll
             for (int kb = 0; kb < kBlocksD; ++kb)
-              tma_load_4d(sQ + kb * Shape::kQBlockBytes, &tmap_q, &bars->q_full, kb * 64, 0, it.hkv, it.q_row);
+              tma_load_5d(sQ + kb * Shape::kQBlockBytes, &tmap_q, &bars->q_full, kb * 64, 0, it.hkv, it.q_row, 0);
           }
           hand_on(next, i + 1);
         }
+        // Table entries of the copies ("boxes"), 32 at a time, a box per lane; the next 32 are requested before
+        // these are used. (Block by block the look-up took 800 clocks of each.)
         const int32_t* table = p.table + static_cast<int64_t>(it.k_from) * p.bt_stride;
-        // Boxes of block j that hold a key (the rest of the last block is not fetched).
-        auto live_boxes = [&](int j) { return min(boxes, (it.m - j * kPackedKeys + p.box - 1) / p.box); };
-        // Table entries of a block's boxes, one or two per lane, requested a block ahead of their use.
-        int32_t entry[2] = {0, 0};
-        auto request = [&](int j) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int r = e * 32 + lane;
-            entry[e] = 0;
-            if (j < hi && r < live_boxes(j)) entry[e] = table[page_of(j * kPackedKeys + r * p.box)];
-          }
+        const int all_boxes = kPages ? (it.m + p.box - 1) / p.box : 0;  // that hold a key
+        int window = kPages ? lo * boxes / 32 : 0;
+        int32_t page = 0, page_next = 0;
+        auto request = [&](int w) -> int32_t {
+          const int n = w * 32 + lane;
+          return n < all_boxes && n < hi * boxes ? table[page_of(n * p.box)] : 0;
         };
-        if constexpr (kPages) request(lo);
+        auto checked = [&](int32_t pg) -> int32_t {
+          if (pg >= 0 && pg < p.n_pages) return pg;
+          if (p.status) atomicExch(p.status, LF_DEV_BAD_PAGE);
+          return 0;
+        };
+        if constexpr (kPages) {
+          page = request(window);
+          page_next = request(window + 1);
+          page = checked(page);
+        }
         for (int j = lo; j < hi; ++j, ++g) {
-          int32_t page[2];
-          if constexpr (kPages) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              page[e] = entry[e];
-              if (page[e] < 0 || page[e] >= p.n_pages) {
-                if (p.status) atomicExch(p.status, LF_DEV_BAD_PAGE);
-                page[e] = 0;
-              }
-            }
-            request(j + 1);
-          }
           const int stage = g % kStages;
           wait(&empty[stage], ((g / kStages) & 1) ^ 1, 81);
-          if (__any_sync(0xffffffffu, lost)) break;
+          __syncwarp();
+          const bool run = elected && !lost;
           unsigned char* dst = ring + stage * Shape::kTileBytes;
           if constexpr (!kPages) {
-            if (elected) {
+            // (Both 64-column halves in one copy: the third dimension of the map.)
+            if (run) {
               mbar_arrive_expect_tx(&full[stage], Shape::kTileBytes);
-#pragma unroll
-              for (int kb = 0; kb < kBlocksD; ++kb)
-                tma_load_4d(dst + kb * Shape::kKVBlockBytes, map, &full[stage], kb * 64,
-                            it.k_from + j * kPackedKeys, it.hkv, 0);
+              tma_load_5d(dst, map, &full[stage], 0, it.k_from + j * kPackedKeys, 0, it.hkv, 0);
             }
           } else {
-            const int live = live_boxes(j);
-            if (elected)
+            const int n0 = j * boxes;
+            const int live = min(boxes, all_boxes - n0);  // (the rest of the last block is not fetched)
+            if (run)
               mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(live * p.box) * 128 * kBlocksD);
-            for (int r = 0; r < live; ++r) {
-              const int pg = __shfl_sync(0xffffffffu, r < 32 ? page[0] : page[1], r & 31);
-              const int t = j * kPackedKeys + r * p.box;
-              const int slot = t - page_of(t) * p.page_size;
-              if (elected) {
+            // Four boxes at a time: places by shuffle, then the copies in one go. (They lie in one window: 32 is a
+            // multiple of them, or they of 32.)
+            for (int r0 = 0; r0 < live; r0 += 4) {
+              if ((n0 + r0) / 32 != window) {
+                ++window;
+                page = checked(page_next);
+                page_next = request(window + 1);
+              }
+              int pg[4], slot[4];
 #pragma unroll
-                for (int kb = 0; kb < kBlocksD; ++kb)
-                  tma_load_4d(dst + kb * Shape::kKVBlockBytes + r * p.box * 128, map, &full[stage], kb * 64,
-                              slot, it.hkv, pg);
+              for (int u = 0; u < 4; ++u) {
+                const int n = n0 + min(r0 + u, live - 1);
+                pg[u] = __shfl_sync(0xffffffffu, page, n & 31);
+                slot[u] = n * p.box - page_of(n * p.box) * p.page_size;
+              }
+              if (run) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                  const int row = (r0 + u) * p.box;
+                  if (r0 + u >= live) continue;
+                  if (p.page_groups > 0) {  // 8-row groups of the whole pool are evenly spaced
+                    tma_load_5d(dst + row * (128 * kBlocksD), map, &full[stage], 0, 0, 0, it.hkv,
+                                pg[u] * p.page_groups + (slot[u] >> 3));
+                  } else {
+#pragma unroll
+                    for (int kb = 0; kb < kBlocksD; ++kb)
+                      tma_load_5d(dst + (row >> 3) * (1024 * kBlocksD) + kb * 1024 + (row & 7) * 128, map,
+                                  &full[stage], kb * 64, slot[u], 0, it.hkv, pg[u]);
+                  }
+                }
               }
             }
           }
@@ -563,7 +583,7 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
     const bool elected = elect_one_sync();
     constexpr uint32_t kStageUnits = Shape::kTileBytes >> 4;
     const uint64_t qdesc = make_smem_desc_sw128(smem_u32(sQ), 16, 1024);
-    const uint64_t kdesc0 = make_smem_desc_sw128(smem_u32(sK), 16, 1024);
+    const uint64_t kdesc0 = make_smem_desc_sw128(smem_u32(sK), 16, kGroup);
     int g = 0;
     for (int i = 0;; ++i) {
       PackedItem it;
@@ -584,7 +604,7 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
         for (int ks = 0; ks < D / 16; ++ks)
           mma_ss_if(run, d,
                     qdesc + static_cast<uint64_t>((ks / 4) * (Shape::kQBlockBytes >> 4) + (ks % 4) * 2),
-                    kd + static_cast<uint64_t>((ks / 4) * (Shape::kKVBlockBytes >> 4) + (ks % 4) * 2),
+                    kd + static_cast<uint64_t>((ks / 4) * (kHalf >> 4) + (ks % 4) * 2),
                     kIdescQK, ks > 0 ? 1u : 0u);
         tc_commit_if(run, &bars->s_full[g & 1]);
         tc_commit_if(run, &bars->k_empty[stage]);
@@ -595,7 +615,7 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
     // ---------------- O += P V ----------------
     const bool elected = elect_one_sync();
     constexpr uint32_t kStageUnits = Shape::kTileBytes >> 4;
-    const uint64_t vdesc0 = make_smem_desc_sw128(smem_u32(sV), Shape::kKVBlockBytes, 1024);
+    const uint64_t vdesc0 = make_smem_desc_sw128(smem_u32(sV), kHalf, kGroup);
     const uint32_t o_col = tmem_base + kColO;
     int g = 0;
     for (int i = 0;; ++i) {
@@ -615,12 +635,12 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
         const uint32_t a = tmem_base + (g & 1) * 64;
 #pragma unroll
         for (int ks = 0; ks < kPackedKeys / 16; ++ks)
-          mma_ts_if(run, o_col, a + ks * 8, vd + static_cast<uint64_t>(ks * (2048 >> 4)), kIdescPV,
+          mma_ts_if(run, o_col, a + ks * 8, vd + static_cast<uint64_t>(ks * (2 * kGroup >> 4)), kIdescPV,
                     ks > 0 || j > it.lo ? 1u : 0u);
         if (fine) {
 #pragma unroll
           for (int ks = 0; ks < kPackedKeys / 16; ++ks)
-            mma_ts_if(run, o_col, a + 32 + ks * 8, vd + static_cast<uint64_t>(ks * (2048 >> 4)), kIdescPV, 1u);
+            mma_ts_if(run, o_col, a + 32 + ks * 8, vd + static_cast<uint64_t>(ks * (2 * kGroup >> 4)), kIdescPV, 1u);
         }
         tc_commit_if(run, &bars->s_free[g & 1]);
         tc_commit_if(run, &bars->v_empty[stage]);
@@ -692,7 +712,8 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
           for (int e = first * 8 + row; e < kPackedKeys * 8; e += 128)
 #pragma unroll
             for (int kb = 0; kb < kBlocksD; ++kb)
-              *reinterpret_cast<uint4*>(v + kb * Shape::kKVBlockBytes + e * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(v + kb * kHalf + (e >> 6) * kGroup + (e & 63) * 16) =
+                  make_uint4(0, 0, 0, 0);
           fence_proxy_async_smem();
         }
         if (!idle) {
@@ -1005,10 +1026,30 @@ inline int packed_page_shift(int page_size) {
   return -1;
 }
 
-// Map of a pool [n_pages, page_size, Hkv, D] with strides (page, slot, kv head) for boxes of `box` slots.
-inline int packed_pool_map(CUtensorMap* map, const void* pool, const int64_t* st, int n_pages, int page_size,
-                           int Hkv, int D, int box) {
-  return make_map_4d(map, TileMapSpec{pool, {D, page_size, Hkv, n_pages}, {st[1], st[2], st[0]}, {box, 1, 1}});
+// Maps of the pools [n_pages, page_size, Hkv, D] with strides (page, slot, kv head). Where both pools' groups
+// of 8 slots are evenly spaced through all pages, a copy moves the groups of p->box slots with all their
+// columns, by (column, slot of the group, half, kv head, group); else p->box slots of a group and 64 columns,
+// by (column, slot, -, kv head, page), and p->page_groups is 0.
+inline int packed_pool_maps(CUtensorMap* mk, CUtensorMap* mv, const void* k, const void* v,
+                            const int64_t* k_st, const int64_t* v_st, int n_pages, int page_size, int Hkv,
+                            int D, PackedParams* p) {
+  const int64_t groups = static_cast<int64_t>(n_pages) * (page_size / 8);
+  const bool even = page_size % 8 == 0 && groups < (1ll << 31) &&
+                    (n_pages == 1 || (k_st[0] == k_st[1] * page_size && v_st[0] == v_st[1] * page_size));
+  p->page_groups = even ? page_size / 8 : 0;
+  p->box = packed_box(page_size);
+  if (!even && p->box > 8) p->box = 8;
+  for (int i = 0; i < 2; ++i) {
+    const int64_t* st = i ? v_st : k_st;
+    TileMapSpec spec;
+    if (even)
+      spec = {i ? v : k, {64, 8, D / 64, Hkv, groups}, {st[1], 64, st[2], 8 * st[1]}, {8, D / 64, 1, p->box / 8}};
+    else
+      spec = {i ? v : k, {D, page_size, 1, Hkv, n_pages}, {st[1], 0, st[2], st[0]}, {p->box, 1, 1, 1}};
+    const int rc = make_map_5d(i ? mv : mk, spec);
+    if (rc != LF_OK) return rc;
+  }
+  return LF_OK;
 }
 
 template <class Kernel>

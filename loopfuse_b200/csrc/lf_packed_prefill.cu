@@ -292,18 +292,19 @@ int lf_packed_prefill_bf16(const LfPackedArgs* a, void* stream) {
   p.page_size = paged ? a->page_size : 1;
   p.page_shift = packed_page_shift(p.page_size);
   p.n_pages = a->n_pages;
-  p.box = packed_box(p.page_size);
   p.status = a->status;
 
   CUtensorMap mq, mk, mv;
-  rc = make_map_4d(&mq, TileMapSpec{a->q, {a->D, G, a->Hkv, a->T},
-                                    {a->q_stride[1], a->q_stride[1] * G, a->q_stride[0]}, {G, 1, p.tq}});
-  for (int i = 0; i < 2 && rc == LF_OK; ++i) {
-    CUtensorMap* map = i ? &mv : &mk;
+  rc = make_map_5d(&mq, TileMapSpec{a->q, {a->D, G, a->Hkv, a->T, 1},
+                                    {a->q_stride[1], a->q_stride[1] * G, a->q_stride[0], 0}, {G, 1, p.tq, 1}});
+  if (rc == LF_OK && paged)
+    rc = packed_pool_maps(&mk, &mv, kv[0], kv[1], a->k_stride, a->v_stride, a->n_pages, a->page_size, a->Hkv,
+                          a->D, &p);
+  for (int i = 0; i < 2 && rc == LF_OK && !paged; ++i) {
     const int64_t* st = i ? a->v_stride : a->k_stride;
-    rc = paged ? packed_pool_map(map, kv[i], st, a->n_pages, a->page_size, a->Hkv, a->D, p.box)
-               : make_map_4d(map, TileMapSpec{kv[i], {a->D, std::max(a->Tk, 1), a->Hkv, 1},
-                                              {st[0], st[1], 0}, {kPackedKeys, 1, 1}});
+    // (By column, token, half, kv head.)
+    rc = make_map_5d(i ? &mv : &mk, TileMapSpec{kv[i], {64, std::max(a->Tk, 1), a->D / 64, a->Hkv, 1},
+                                                {st[0], 64, st[1], 0}, {kPackedKeys, a->D / 64, 1, 1}});
   }
   if (rc != LF_OK) return rc;
 

@@ -4,12 +4,13 @@
 //   shared part  for a kv head, the B * G query rows against the prefix are one product with M = B * G:
 //                the tiles of lf_packed.cuh, each over a slice of the prefix. The prefix is read from
 //                HBM once for all requests, where a paged decode reads it B times.
-//   own part     own_kernel: a CTA per (request, kv head, slice of its own keys), as in decode: bound by
-//                HBM.
-//   join         join_kernel: out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the slices of both.
+//   own part     a unit is the own keys of a (request, kv head), in groups of 16; all units' groups in one
+//                row are dealt out to the warps in equal runs, as in decode: bound by HBM.
+//   join         join_kernel: out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the parts of both.
 #include "lf_packed.cuh"
 
 #include <algorithm>
+#include <stdlib.h>
 #include <type_traits>
 
 namespace lf {
@@ -27,12 +28,17 @@ struct OwnParams {
   const int32_t* table;
   int64_t bt_stride;
   const int32_t* seq_lens;
-  int32_t B, Hkv, G, head_groups;
-  int32_t prefix_len, max_len, chunk, first_split;  // first_split: slices of the prefix
+  int32_t B, G;
+  int32_t heads;       // units of a request: kv heads times groups of 8 query heads
+  FastDiv div_groups;  // groups of query heads
+  int32_t prefix_len, max_len;
   int32_t page_size, page_shift, n_pages;
   float a, c2;
+  // Part of warp w for unit u: at place w + u, which no other pair has, since both only grow along the row
+  // of groups; [place][8 query heads][D], (maximum, sum), and the warps that a unit's groups went to.
   float* part_o;
   float2* part_ml;
+  int2* warps;
   int32_t* status;
 };
 
@@ -44,76 +50,139 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+constexpr int kOwnRun = 2;  // groups of a warp, at least
+
 // Keys of request b that count, from its length: never more than the caller said or the table holds.
 __device__ __forceinline__ int own_end(const int32_t* seq_lens, int b, int max_len) {
   return min(max(seq_lens[b], 0), max_len);
 }
 
+// Sixteen tokens of a unit, as a warp has them in hand.
+struct OwnGroup {
+  int b, head;  // request; kv head and group of query heads. b < 0: no more
+  int t, end;   // first token, end of the unit
+};
+
+// The own keys, by warps 0..3 of a CTA, each for itself: all units' groups of 16 tokens in one row, of which
+// warp `w` of `n_warps` has an equal run, whatever the requests' lengths. A warp's groups follow each other
+// across units - the page of one is looked up while two are being copied and one is computed - so the start
+// of a unit costs no round trip to memory. (128 requests of 2048 own keys, a CTA per slice of 256 keys: 3.5
+// TB/s.)
+//
 // The layout of the products is that of decode_mma_kernel: the G query rows are rows 0..7 of the M
-// dimension of m16n8k16, K and V fragments come straight from the 16-byte pieces that were copied
-// (piece j of row r sits at piece j ^ (r & 7)), and P enters the second product as two bf16, its
-// rounding in rows g and what that leaves in rows 8 + g, at no extra MMA.
+// dimension of m16n8k16, K and V fragments come straight from the 16-byte pieces that were copied (piece j
+// of row r sits at piece j ^ (r & 7)), and P enters the second product as two bf16, its rounding in rows g
+// and what that leaves in rows 8 + g, at no extra MMA.
 template <int D, bool SOFTCAP>
-__global__ void __launch_bounds__(kOwnWarps * 32, 2) own_kernel(const OwnParams p) {
+__device__ __forceinline__ void own_part(const OwnParams& p, int w, int n_warps) {
   constexpr int KI = D / 32;  // 16-byte pieces of a K row per lane
   constexpr int VH = D / 64;
   constexpr int NT = D / 8;
   constexpr int CPR = D / 8, RPI = 32 / CPR;
   constexpr int kRowBytes = D * 2, kStageBytes = 2 * kOwnGroup * kRowBytes;
   extern __shared__ __align__(1024) unsigned char smem[];
-  pdl_trigger();
-  pdl_wait();
-  const int split = blockIdx.x;
-  const int kvh = blockIdx.y / p.head_groups;
-  const int g0 = (blockIdx.y - kvh * p.head_groups) * kOwnHeads;
-  const int b = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
-  const int n_heads = min(kOwnHeads, p.G - g0);
-  const int end = own_end(p.seq_lens, b, p.max_len);
-  const int t0 = p.prefix_len + split * p.chunk;
-  const int t1 = min(end, t0 + p.chunk);
-  if (t0 >= t1) return;
 
-  uint4 qr[KI];
-#pragma unroll
-  for (int i = 0; i < KI; ++i) {
-    qr[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (g < n_heads)
-      qr[i] = *reinterpret_cast<const uint4*>(p.q + b * p.q_stride[0] + kvh * p.q_stride[1] +
-                                              (g0 + g) * p.q_stride[2] + 8 * (4 * i + c));
+  // Groups of the requests [b0, b0 + 32), one per lane; those of a unit.
+  int b0 = 0, groups = 0;
+  auto load_groups = [&](int from) {
+    b0 = from;
+    const int own = b0 + lane < p.B ? own_end(p.seq_lens, b0 + lane, p.max_len) - p.prefix_len : 0;
+    groups = own > 0 ? (own + kOwnGroup - 1) / kOwnGroup : 0;
+  };
+  long long all = 0;
+  for (int from = 0; from < p.B; from += 32) {
+    load_groups(from);
+    all += groups;
   }
-  const __nv_bfloat16* kbase = p.k + kvh * p.k_stride[2];
-  const __nv_bfloat16* vbase = p.v + kvh * p.v_stride[2];
-  const int32_t* table = p.table + b * p.bt_stride;
+#pragma unroll
+  for (int d = 16; d >= 1; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
+  all *= p.heads;
+  const long long run = max((all + n_warps - 1) / n_warps, static_cast<long long>(kOwnRun));
+  long long left = min(all - w * run, run);  // groups of this warp
+  if (left <= 0) return;
+  OwnGroup now;
+  {
+    long long skip = w * run;  // of the requests ahead, then of the units ahead
+    long long incl = 0;
+    unsigned past = 0;
+    for (int from = 0; from < p.B && !past; from += 32) {
+      if (from) skip -= __shfl_sync(0xffffffffu, incl, 31);
+      load_groups(from);
+      incl = static_cast<long long>(groups) * p.heads;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long x = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += x;
+      }
+      past = __ballot_sync(0xffffffffu, incl > skip);
+    }
+    const int l = __ffs(past) - 1;
+    const int n = __shfl_sync(0xffffffffu, groups, l);
+    const long long into = skip - __shfl_sync(0xffffffffu, incl, l) + static_cast<long long>(n) * p.heads;
+    now.b = b0 + l;
+    now.head = static_cast<int>(into / n);
+    now.t = p.prefix_len + static_cast<int>(into - static_cast<long long>(now.head) * n) * kOwnGroup;
+    now.end = own_end(p.seq_lens, now.b, p.max_len);
+  }
+  // The group behind x, while this warp has any.
+  auto next_group = [&](const OwnGroup& x) {
+    OwnGroup y = x;
+    if (--left <= 0) {
+      y.b = -1;
+      return y;
+    }
+    y.t += kOwnGroup;
+    if (y.t < y.end) return y;
+    y.t = p.prefix_len;
+    if (++y.head < p.heads) return y;
+    y.head = 0;
+    for (;;) {  // the next request that has own keys
+      const unsigned some = __ballot_sync(0xffffffffu, groups > 0 && b0 + lane > y.b);
+      if (some) {
+        y.b = b0 + __ffs(some) - 1;
+        y.end = own_end(p.seq_lens, y.b, p.max_len);
+        return y;
+      }
+      load_groups(b0 + 32);
+    }
+  };
+  auto kv_head = [&](int head, int* g0) {
+    const int kvh = static_cast<int>(p.div_groups.div(head));
+    *g0 = (head - kvh * static_cast<int>(p.div_groups.d)) * kOwnHeads;
+    return kvh;
+  };
+
   auto page_of = [&](int t) { return p.page_shift >= 0 ? (t >> p.page_shift) : (t / p.page_size); };
-  const int t_last = t1 - 1;
-  // Page of this lane's row of the group at tg (rows past the end: the last token again), requested a
-  // group ahead of its use.
-  auto request = [&](int tg) {
-    return tg < t1 ? table[page_of(min(tg + (lane & 15), t_last))] : 0;
+  // Page of this lane's row of a group (rows past the end: the last token again).
+  auto look_up = [&](const OwnGroup& x) {
+    if (x.b < 0) return 0;
+    return p.table[x.b * p.bt_stride + page_of(min(x.t + (lane & 15), x.end - 1))];
   };
   unsigned char* ring = smem + warp * (kOwnStages * kStageBytes);
   const int r0 = lane / CPR, j0 = lane % CPR;
   const uint32_t ring_u32 = smem_u32(ring) + r0 * kRowBytes;
-  auto copy_group = [&](int tg, int stage, int page) {
-    if (tg < t1) {
+  auto copy_group = [&](const OwnGroup& x, int stage, int page) {
+    if (x.b >= 0) {
+      int g0;
+      const int kvh = kv_head(x.head, &g0);
+      const __nv_bfloat16* kbase = p.k + kvh * p.k_stride[2];
+      const __nv_bfloat16* vbase = p.v + kvh * p.v_stride[2];
       const uint32_t dst = ring_u32 + stage * kStageBytes;
-      const int t = min(tg + (lane & 15), t_last);
-      const int pg = page_of(t);
+      const int t = min(x.t + (lane & 15), x.end - 1);
       if (page < 0 || page >= p.n_pages) {
         if (p.status) atomicExch(p.status, LF_DEV_BAD_PAGE);
         page = 0;
       }
-      const int slot = t - pg * p.page_size;
-      if (tg + 15 <= t_last && page_of(tg) == page_of(tg + 15)) {
+      const int slot = t - page_of(t) * p.page_size;
+      if (x.t + kOwnGroup <= x.end && page_of(x.t) == page_of(x.t + 15)) {
         // A group inside one page: its rows are evenly spaced.
+        const int slot0 = __shfl_sync(0xffffffffu, slot, 0);
         const __nv_bfloat16* kp = kbase + static_cast<int64_t>(page) * p.k_stride[0] +
-                                  __shfl_sync(0xffffffffu, slot, 0) * p.k_stride[1] +
-                                  r0 * p.k_stride[1] + 8 * j0;
+                                  (slot0 + r0) * p.k_stride[1] + 8 * j0;
         const __nv_bfloat16* vp = vbase + static_cast<int64_t>(page) * p.v_stride[0] +
-                                  __shfl_sync(0xffffffffu, slot, 0) * p.v_stride[1] +
-                                  r0 * p.v_stride[1] + 8 * j0;
+                                  (slot0 + r0) * p.v_stride[1] + 8 * j0;
 #pragma unroll
         for (int q = 0; q < 16 / RPI; ++q) {
           const uint32_t to = dst + q * RPI * kRowBytes + ((j0 ^ ((r0 + q * RPI) & 7)) << 4);
@@ -136,6 +205,29 @@ __global__ void __launch_bounds__(kOwnWarps * 32, 2) own_kernel(const OwnParams 
     }
     cp_async_commit();
   };
+  uint4 qr[KI];
+  auto load_q = [&](const OwnGroup& x) {
+    int g0;
+    const int kvh = kv_head(x.head, &g0);
+#pragma unroll
+    for (int i = 0; i < KI; ++i) {
+      qr[i] = make_uint4(0u, 0u, 0u, 0u);
+      if (g0 + g < p.G)
+        qr[i] = *reinterpret_cast<const uint4*>(p.q + x.b * p.q_stride[0] + kvh * p.q_stride[1] +
+                                                (g0 + g) * p.q_stride[2] + 8 * (4 * i + c));
+    }
+  };
+
+  // now: computed; then, later: being copied; last: its page is being looked up.
+  static_assert(kOwnStages == 3, "two groups are copied while one is computed");
+  OwnGroup then = next_group(now), later = next_group(then);
+  load_q(now);
+  {
+    const int pg0 = look_up(now), pg1 = look_up(then);
+    copy_group(now, 0, pg0);
+    copy_group(then, 1, pg1);
+  }
+  int page = look_up(later);
 
   float m_run = -INFINITY, l_run = 0.f;
   float o[NT][4];
@@ -144,38 +236,25 @@ __global__ void __launch_bounds__(kOwnWarps * 32, 2) own_kernel(const OwnParams 
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
 
-  constexpr int kStep = kOwnGroup * kOwnWarps;
-  const int tg0 = t0 + warp * kOwnGroup;
-  int page = request(tg0);
-#pragma unroll
-  for (int st = 0; st < kOwnStages - 1; ++st) {
-    const int next = request(tg0 + (st + 1) * kStep);
-    copy_group(tg0 + st * kStep, st, page);
-    page = next;
-  }
-  int it = 0;
-  for (int tg = tg0; tg < t1; tg += kStep, ++it) {
-    const int next = request(tg + kOwnStages * kStep);
-    copy_group(tg + (kOwnStages - 1) * kStep, (it + kOwnStages - 1) % kOwnStages, page);
-    page = next;
+  for (int it = 0; now.b >= 0; it = it == 2 ? 0 : it + 1) {
+    copy_group(later, it == 0 ? 2 : it - 1, page);
+    const OwnGroup last = next_group(later);
+    page = look_up(last);
     cp_async_wait<kOwnStages - 1>();
     __syncwarp();
-    const unsigned char* stage = ring + (it % kOwnStages) * kStageBytes;
-    uint4 kr[2][KI];
-#pragma unroll
-    for (int s8 = 0; s8 < 2; ++s8)
-#pragma unroll
-      for (int i = 0; i < KI; ++i)
-        kr[s8][i] =
-            *reinterpret_cast<const uint4*>(stage + (8 * s8 + g) * kRowBytes + (((4 * i + c) ^ g) << 4));
+    const unsigned char* stage = ring + it * kStageBytes;
     float sc[2][2];
 #pragma unroll
     for (int s8 = 0; s8 < 2; ++s8) {
+      uint4 kr[KI];
+#pragma unroll
+      for (int i = 0; i < KI; ++i)
+        kr[i] = *reinterpret_cast<const uint4*>(stage + (8 * s8 + g) * kRowBytes + (((4 * i + c) ^ g) << 4));
       float x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < KI; ++i) {
-        mma_16816(x, qr[i].x, 0u, qr[i].y, 0u, kr[s8][i].x, kr[s8][i].y);
-        mma_16816(y, qr[i].z, 0u, qr[i].w, 0u, kr[s8][i].z, kr[s8][i].w);
+        mma_16816(x, qr[i].x, 0u, qr[i].y, 0u, kr[i].x, kr[i].y);
+        mma_16816(y, qr[i].z, 0u, qr[i].w, 0u, kr[i].z, kr[i].w);
       }
       sc[s8][0] = x[0] + y[0];
       sc[s8][1] = x[1] + y[1];
@@ -188,7 +267,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32, 2) own_kernel(const OwnParams 
         float s = sc[s8][e];
         if constexpr (SOFTCAP) s = tanh_approx(s * p.a);
         s *= p.c2;
-        if (tg + 8 * s8 + 2 * c + e >= t1) s = -INFINITY;
+        if (now.t + 8 * s8 + 2 * c + e >= now.end) s = -INFINITY;
         sc[s8][e] = s;
         mx = fmaxf(mx, s);
       }
@@ -213,7 +292,7 @@ __global__ void __launch_bounds__(kOwnWarps * 32, 2) own_kernel(const OwnParams 
         pr[s8][e] = ex2_approx(sc[s8][e] - m_safe);
         psum += pr[s8][e];
       }
-    l_run += psum;  // this lane's share; the quad is summed after the loop
+    l_run += psum;  // this lane's share; the quad is summed at the end of the unit
     const uint32_t pa0 = pack_bf16x2(pr[0][0], pr[0][1]);
     const uint32_t pa2 = pack_bf16x2(pr[1][0], pr[1][1]);
     const uint32_t pa1 = pack_bf16x2(pr[0][0] - bf16lo_to_f32(pa0), pr[0][1] - bf16hi_to_f32(pa0));
@@ -238,71 +317,66 @@ __global__ void __launch_bounds__(kOwnWarps * 32, 2) own_kernel(const OwnParams 
                   __byte_perm(w2[e >> 1], w3[e >> 1], sel));
       }
     }
-    __syncwarp();
+    const int unit = now.b * p.heads + now.head;
+    if (lane == 0) {  // where the join finds the unit's parts
+      if (now.t == p.prefix_len) p.warps[unit].x = w;
+      if (now.t + kOwnGroup >= now.end) p.warps[unit].y = w;
+    }
+    if (then.b != now.b || then.head != now.head) {
+      // This warp is done with the unit: its rows and their (maximum, sum) go to the join.
+      int g0;
+      kv_head(now.head, &g0);
+      l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
+      l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
+      if (g0 + g < p.G) {
+        const int64_t at = (static_cast<int64_t>(w) + unit) * kOwnHeads + g;
+        float* dst = p.part_o + at * D;
+#pragma unroll
+        for (int h = 0; h < VH; ++h)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {  // output column 2c + u of MMA (h, e): d = 64 h + 16 c + 8 u + e
+            uint32_t x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float y = o[h * 8 + e][u];
+              x[e] = __float_as_uint(fabsf(y) != INFINITY ? y + o[h * 8 + e][2 + u] : y);
+            }
+            stg_32(dst + 64 * h + 16 * c + 8 * u, x);
+          }
+        if (c == 0) p.part_ml[at] = make_float2(m_run, l_run);
+      }
+      m_run = -INFINITY;
+      l_run = 0.f;
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[j][e] = 0.f;
+      if (then.b >= 0) load_q(then);
+    }
+    __syncwarp();  // every lane is done with this stage before it is refilled
+    now = then;
+    then = later;
+    later = last;
   }
   cp_async_wait<0>();
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      if (fabsf(o[j][e]) != INFINITY) o[j][e] += o[j][2 + e];
-  l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
-  l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
-
-  // The warps' parts meet in shared memory (in the rings), [warp][head][D + 2].
-  constexpr int kStride = D + 2;
-  float* merge = reinterpret_cast<float*>(smem);
-  __syncthreads();
-  if (g < n_heads) {
-    float* dst = merge + (warp * n_heads + g) * kStride;
-#pragma unroll
-    for (int h = 0; h < VH; ++h)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        dst[64 * h + 16 * c + e] = o[h * 8 + e][0];
-        dst[64 * h + 16 * c + 8 + e] = o[h * 8 + e][1];
-      }
-    if (c == 0) {
-      dst[D] = m_run;
-      dst[D + 1] = l_run;
-    }
-  }
-  __syncthreads();
-  const int64_t row0 = (static_cast<int64_t>(b) * p.Hkv + kvh) * p.G + g0;
-  const int64_t rows = static_cast<int64_t>(p.B) * p.Hkv * p.G;
-  for (int idx = threadIdx.x; idx < n_heads * D; idx += kOwnWarps * 32) {
-    const int gg = idx / D, cc = idx - gg * D;
-    float m_all = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < kOwnWarps; ++w) m_all = fmaxf(m_all, merge[(w * n_heads + gg) * kStride + D]);
-    const float m_safe = m_all == -INFINITY ? 0.f : m_all;
-    float l_all = 0.f, acc = 0.f;
-#pragma unroll
-    for (int w = 0; w < kOwnWarps; ++w) {
-      const float* src = merge + (w * n_heads + gg) * kStride;
-      const float wt = ex2_approx(src[D] - m_safe);
-      l_all += src[D + 1] * wt;
-      acc += src[cc] * wt;
-    }
-    const int64_t at = (p.first_split + split) * rows + row0 + gg;
-    p.part_o[at * D + cc] = acc;
-    if (cc == 0) p.part_ml[at] = make_float2(m_all, l_all);
-  }
 }
 
 struct JoinParams {
-  const float* part_o;
-  const float2* part_ml;
+  const float* prefix_o;    // [split][row][D]
+  const float2* prefix_ml;  // [split][row]
+  const float* own_o;       // as OwnParams has them
+  const float2* own_ml;
+  const int2* warps;
   __nv_bfloat16* out;
   int64_t o_stride[3];  // (b, kv head, g)
   const int32_t* seq_lens;
-  int32_t prefix_len, max_len, chunk, prefix_splits;
+  int32_t prefix_len, max_len, prefix_splits;
   int64_t rows;
-  int32_t Hkv, G;
+  int32_t Hkv, G, groups;  // groups of 8 query heads
 };
 
-// One warp per output row. Lane s holds (reference, sum) of slice s; the rows of the slices stream in with
-// their weights broadcast. Slices that hold no key of the row have sum 0 and are left out (what their
+// One warp per output row. Lane s holds (reference, sum) of part s; the rows of the parts stream in with
+// their weights broadcast. Parts that hold no key of the row have sum 0 and are left out (what their
 // accumulators hold is of no value); a row without a key is zeros.
 template <int D>
 __global__ void __launch_bounds__(128) join_kernel(const JoinParams p) {
@@ -315,15 +389,27 @@ __global__ void __launch_bounds__(128) join_kernel(const JoinParams p) {
   const int64_t b = row / (p.Hkv * p.G);
   const int rest = static_cast<int>(row - b * (p.Hkv * p.G));
   const int kvh = rest / p.G, g = rest - kvh * p.G;
-  const int own = own_end(p.seq_lens, static_cast<int>(b), p.max_len) - p.prefix_len;
-  const int n = p.prefix_splits + (own > 0 ? (own + p.chunk - 1) / p.chunk : 0);
+  const int64_t unit = (b * p.Hkv + kvh) * p.groups + g / kOwnHeads;
+  int64_t own_at = 0;
+  int n = p.prefix_splits;
+  if (own_end(p.seq_lens, static_cast<int>(b), p.max_len) > p.prefix_len) {
+    const int2 w = p.warps[unit];
+    own_at = (w.x + unit) * kOwnHeads + g % kOwnHeads;
+    n += w.y - w.x + 1;
+  }
+  // Place of part s.
+  auto place = [&](int s) {
+    return s < p.prefix_splits ? s * p.rows + row
+                               : own_at + static_cast<int64_t>(s - p.prefix_splits) * kOwnHeads;
+  };
   float m_all = -INFINITY, l_all = 0.f;
   float o[EPL];
 #pragma unroll
   for (int e = 0; e < EPL; ++e) o[e] = 0.f;
   for (int s0 = 0; s0 < n; s0 += 32) {
     float2 ml = make_float2(-INFINITY, 0.f);
-    if (s0 + lane < n) ml = p.part_ml[(s0 + lane) * p.rows + row];
+    const int mine = s0 + lane;
+    if (mine < n) ml = (mine < p.prefix_splits ? p.prefix_ml : p.own_ml)[place(mine)];
     const bool live = ml.y != 0.f;
     float m_new = live ? ml.x : -INFINITY;
 #pragma unroll
@@ -341,16 +427,16 @@ __global__ void __launch_bounds__(128) join_kernel(const JoinParams p) {
     for (int e = 0; e < EPL; ++e) o[e] *= back;
     unsigned todo = __ballot_sync(0xffffffffu, live);
     while (todo) {
-      float x[4][EPL], wt[4];
+      float x[8][EPL], wt[8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < 8; ++u) {
         const int s = todo ? __ffs(todo) - 1 : 0;
         const float ws = __shfl_sync(0xffffffffu, w, s);
         wt[u] = todo ? ws : 0.f;
 #pragma unroll
         for (int e = 0; e < EPL; ++e) x[u][e] = 0.f;
         if (todo) {
-          const float* src = p.part_o + ((s0 + s) * p.rows + row) * D + lane * EPL;
+          const float* src = (s0 + s < p.prefix_splits ? p.prefix_o : p.own_o) + place(s0 + s) * D + lane * EPL;
           if constexpr (EPL == 4) {
             const float4 v = *reinterpret_cast<const float4*>(src);
             x[u][0] = v.x; x[u][1] = v.y; x[u][2] = v.z; x[u][3] = v.w;
@@ -362,7 +448,7 @@ __global__ void __launch_bounds__(128) join_kernel(const JoinParams p) {
         todo &= todo - 1;
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+      for (int u = 0; u < 8; ++u)
 #pragma unroll
         for (int e = 0; e < EPL; ++e) o[e] = fmaf(x[u][e], wt[u], o[e]);
     }
@@ -376,17 +462,36 @@ __global__ void __launch_bounds__(128) join_kernel(const JoinParams p) {
     *reinterpret_cast<uint32_t*>(op) = pack_bf16x2(o[0] * inv, o[1] * inv);
 }
 
+// Both parts in one launch: the slices of the prefix, which are long, come first and take two CTAs per
+// SM at most; those of the requests' own keys fill the places that are left, then the ones that get free.
 template <int D, bool SOFTCAP>
 __global__ void __launch_bounds__(kPackedThreads, 2)
-    prefix_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ CUtensorMap tmap_k,
-                  const __grid_constant__ CUtensorMap tmap_v, const PackedParams p) {
+    shared_prefix_kernel(const __grid_constant__ CUtensorMap tmap_q,
+                         const __grid_constant__ CUtensorMap tmap_k,
+                         const __grid_constant__ CUtensorMap tmap_v, const PackedParams p,
+                         const OwnParams own, const int prefix_ctas) {
   pdl_trigger();
-  packed_tiles<D, kPackedPrefix, SOFTCAP>(tmap_q, tmap_k, tmap_v, p, blockIdx.x);
+  const int cta = static_cast<int>(blockIdx.x);
+  if (cta < prefix_ctas) {
+    packed_tiles<D, kPackedPrefix, SOFTCAP>(tmap_q, tmap_k, tmap_v, p, cta);
+  } else if (threadIdx.x >= kOwnWarps * 32) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+    pdl_wait();
+    // (Runs go round the CTAs first, then their warps: few of them are spread over all SMs.)
+    const int ctas = static_cast<int>(gridDim.x) - prefix_ctas;
+    own_part<D, SOFTCAP>(own, (threadIdx.x >> 5) * ctas + cta - prefix_ctas, ctas * kOwnWarps);
+  }
 }
 
-// How a call is cut: slices of the prefix (a multiple of a key block each), and of the requests' own keys.
+// How a call is cut, and the room for its parts.
 struct PrefixCut {
-  int prefix_splits, prefix_chunk, own_splits, own_chunk;
+  int prefix_splits = 0, prefix_chunk = kPackedKeys;  // slices of the prefix, whole key blocks each
+  int own_ctas = 0, heads = 1;
+  int64_t units = 0;
+  size_t prefix_parts = 0, own_parts = 0;  // rows
+  size_t bytes(int D) const { return (prefix_parts + own_parts) * (D + 2) * sizeof(float) + units * sizeof(int2); }
 };
 
 static int shared_sm_count() {
@@ -400,61 +505,47 @@ static int shared_sm_count() {
   return cached > 0 ? cached : 148;
 }
 
+static int XP = getenv("XP") ? atoi(getenv("XP")) : 4, XO = getenv("XO") ? atoi(getenv("XO")) : 4, XB = getenv("XB") ? atoi(getenv("XB")) : 2;
 static PrefixCut cut_prefix(int B, int Hkv, int G, int prefix_len, int max_len) {
-  PrefixCut c = {0, kPackedKeys, 0, 256};
+  PrefixCut c;
   const int sms = shared_sm_count();
+  const int64_t rows = static_cast<int64_t>(B) * Hkv * G;
   if (prefix_len > 0) {
     const int tq = kPackedRows / G;
     const int64_t units = static_cast<int64_t>((B + tq - 1) / tq) * Hkv;
     const int blocks = (prefix_len + kPackedKeys - 1) / kPackedKeys;
-    // As many slices as one wave of two CTAs per SM takes, of four key blocks or more.
-    int64_t s = std::max<int64_t>(1, 2ll * sms / units);
-    s = std::min<int64_t>(s, (blocks + 3) / 4);
+    // As many slices as one wave of two CTAs per SM takes, of two key blocks or more.
+    int64_t s = std::max<int64_t>(1, static_cast<int64_t>(XP) * sms / 2 / units);
+    s = std::min<int64_t>(s, (blocks + XB - 1) / XB);
     const int per = static_cast<int>((blocks + s - 1) / s);
     c.prefix_chunk = per * kPackedKeys;
     c.prefix_splits = (blocks + per - 1) / per;
+    c.prefix_parts = static_cast<size_t>(c.prefix_splits) * rows;
   }
   const int own = std::max(0, max_len - prefix_len);
   if (own > 0) {
-    const int64_t units = static_cast<int64_t>(B) * Hkv * ((G + kOwnHeads - 1) / kOwnHeads);
-    if (units * ((own + 255) / 256) < 2 * sms) c.own_chunk = 128;
-    // (Slices of very long requests grow, so that there are never more than 256 of them.)
-    c.own_chunk = std::max(c.own_chunk, ((own + 255) / 256 + kOwnGroup - 1) / kOwnGroup * kOwnGroup);
-    c.own_splits = (own + c.own_chunk - 1) / c.own_chunk;
+    c.heads = Hkv * ((G + kOwnHeads - 1) / kOwnHeads);
+    c.units = static_cast<int64_t>(B) * c.heads;
+    const int64_t runs = (c.units * ((own + kOwnGroup - 1) / kOwnGroup) + kOwnRun - 1) / kOwnRun;
+    c.own_ctas = static_cast<int>(std::min<int64_t>(runs, static_cast<int64_t>(XO) * sms / 2));
+    c.own_parts = static_cast<size_t>(c.units + c.own_ctas * kOwnWarps) * kOwnHeads;
   }
   return c;
 }
 
-static size_t shared_workspace(const PrefixCut& c, int64_t rows, int D) {
-  return static_cast<size_t>(c.prefix_splits + c.own_splits) * rows * (D + 2) * sizeof(float);
-}
-
 template <int D, bool SOFTCAP>
 static int launch_shared(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
-                         const PackedParams& pp, unsigned grid, const OwnParams& po, const PrefixCut& cut,
+                         const PackedParams& pp, const OwnParams& po, int prefix_ctas, unsigned grid,
                          cudaStream_t st) {
   using Shape = PackedShape<D>;
-  if (cut.prefix_splits > 0) {
-    static thread_local int configured_dev = -1;
-    const auto kernel = prefix_kernel<D, SOFTCAP>;
-    int rc = packed_configure(kernel, Shape::kSmem, &configured_dev);
-    if (rc != LF_OK) return rc;
-    launch_pdl(kernel, dim3(grid), kPackedThreads, Shape::kSmem, st, mq, mk, mv, pp);
-    rc = check_launch("prefix_kernel");
-    if (rc != LF_OK) return rc;
-  }
-  if (cut.own_splits > 0) {
-    constexpr size_t smem = static_cast<size_t>(kOwnWarps) * kOwnStages * 2 * kOwnGroup * D * 2;
-    static_assert(static_cast<size_t>(kOwnWarps) * kOwnHeads * (D + 2) * 4 <= smem, "merge area in the rings");
-    static thread_local int configured_dev = -1;
-    const auto kernel = own_kernel<D, SOFTCAP>;
-    int rc = packed_configure(kernel, smem, &configured_dev);
-    if (rc != LF_OK) return rc;
-    launch_pdl(kernel, dim3(cut.own_splits, po.Hkv * po.head_groups, po.B), kOwnWarps * 32, smem, st, po);
-    rc = check_launch("own_kernel");
-    if (rc != LF_OK) return rc;
-  }
-  return LF_OK;
+  constexpr size_t ring = static_cast<size_t>(kOwnWarps) * kOwnStages * 2 * kOwnGroup * D * 2;
+  static_assert(ring <= Shape::kSmem, "the rings of the own part");
+  static thread_local int configured_dev = -1;
+  const auto kernel = shared_prefix_kernel<D, SOFTCAP>;
+  const int rc = packed_configure(kernel, Shape::kSmem, &configured_dev);
+  if (rc != LF_OK) return rc;
+  launch_pdl(kernel, dim3(grid), kPackedThreads, Shape::kSmem, st, mq, mk, mv, pp, po, prefix_ctas);
+  return check_launch("shared_prefix_kernel");
 }
 
 }  // namespace lf
@@ -465,8 +556,7 @@ size_t lf_shared_prefix_workspace_bytes(int32_t B, int32_t Hkv, int32_t G, int32
                                         int32_t max_seq_len) {
   using namespace lf;
   if (B <= 0 || Hkv <= 0 || G <= 0 || G > kPackedRows || D <= 0 || prefix_len < 0) return 0;
-  return shared_workspace(cut_prefix(B, Hkv, G, std::min(prefix_len, max_seq_len), max_seq_len),
-                          static_cast<int64_t>(B) * Hkv * G, D);
+  return cut_prefix(B, Hkv, G, std::min(prefix_len, max_seq_len), max_seq_len).bytes(D);
 }
 
 int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* a, void* stream) {
@@ -483,7 +573,7 @@ int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* a, void* stream) {
   int rc = packed_score(a->scale, a->n_mod, a->mod_op, a->mod_arg, &score);
   if (rc != LF_OK) return rc;
   const int head_groups = (a->G + kOwnHeads - 1) / kOwnHeads;
-  if (a->B > 65535 || static_cast<int64_t>(a->Hkv) * head_groups > 65535) return LF_ERR_TOO_LARGE;
+  if (a->B > 65535 || static_cast<int64_t>(a->B) * a->Hkv * head_groups > (1 << 26)) return LF_ERR_TOO_LARGE;
   if (!packed_aligned(a->q) || !packed_aligned(a->k) || !packed_aligned(a->v) || !packed_aligned(a->out))
     return LF_ERR_ALIGNMENT;
   for (int i = 0; i < 3; ++i)
@@ -492,17 +582,19 @@ int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* a, void* stream) {
   const int64_t rows = static_cast<int64_t>(a->B) * a->Hkv * a->G;
   const int prefix_len = std::min(a->prefix_len, a->max_seq_len);
   const PrefixCut cut = cut_prefix(a->B, a->Hkv, a->G, prefix_len, a->max_seq_len);
-  const size_t need = shared_workspace(cut, rows, a->D);
+  const size_t need = cut.bytes(a->D);
   if (need && (!a->workspace || a->workspace_bytes < need)) return LF_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(a->workspace) & 31u) return LF_ERR_ALIGNMENT;  // (32-byte stores)
   float* part_o = static_cast<float*>(a->workspace);
-  float2* part_ml =
-      reinterpret_cast<float2*>(part_o + static_cast<size_t>(cut.prefix_splits + cut.own_splits) * rows * a->D);
+  float* own_o = part_o + cut.prefix_parts * a->D;
+  float2* part_ml = reinterpret_cast<float2*>(own_o + cut.own_parts * a->D);
+  float2* own_ml = part_ml + cut.prefix_parts;
+  int2* warps = reinterpret_cast<int2*>(own_ml + cut.own_parts);
 
   PackedParams pp = {};
   OwnParams po = {};
   CUtensorMap mq = {}, mk = {}, mv = {};
-  unsigned grid = 0;
+  int64_t prefix_ctas = 0;
   const int page_shift = packed_page_shift(a->page_size);
   if (cut.prefix_splits > 0) {
     pp.kv_lens = a->seq_lens;
@@ -519,7 +611,6 @@ int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* a, void* stream) {
     pp.page_size = a->page_size;
     pp.page_shift = page_shift;
     pp.n_pages = a->n_pages;
-    pp.box = packed_box(a->page_size);
     pp.prefix_len = prefix_len;
     pp.chunk = cut.prefix_chunk;
     pp.part_o = part_o;
@@ -529,15 +620,12 @@ int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* a, void* stream) {
     pp.div_tiles = FastDiv::make(pp.n_tiles);
     pp.div_chunk = FastDiv::make(a->Hkv);
     pp.div_g = FastDiv::make(a->G);
-    const int64_t ctas = static_cast<int64_t>(pp.n_tiles) * a->Hkv * cut.prefix_splits;
-    if (ctas > 0x7fffffff) return LF_ERR_TOO_LARGE;
-    grid = static_cast<unsigned>(ctas);
-    rc = make_map_4d(&mq, TileMapSpec{a->q, {a->D, a->G, a->Hkv, a->B},
-                                      {a->q_stride[2], a->q_stride[1], a->q_stride[0]}, {a->G, 1, pp.tq}});
+    prefix_ctas = static_cast<int64_t>(pp.n_tiles) * a->Hkv * cut.prefix_splits;
+    rc = make_map_5d(&mq, TileMapSpec{a->q, {a->D, a->G, a->Hkv, a->B, 1},
+                                      {a->q_stride[2], a->q_stride[1], a->q_stride[0], 0}, {a->G, 1, pp.tq, 1}});
     if (rc == LF_OK)
-      rc = packed_pool_map(&mk, a->k, a->k_stride, a->n_pages, a->page_size, a->Hkv, a->D, pp.box);
-    if (rc == LF_OK)
-      rc = packed_pool_map(&mv, a->v, a->v_stride, a->n_pages, a->page_size, a->Hkv, a->D, pp.box);
+      rc = packed_pool_maps(&mk, &mv, a->k, a->v, a->k_stride, a->v_stride, a->n_pages, a->page_size, a->Hkv,
+                            a->D, &pp);
     if (rc != LF_OK) return rc;
   }
   po.q = static_cast<const __nv_bfloat16*>(a->q);
@@ -554,32 +642,41 @@ int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* a, void* stream) {
   po.bt_stride = a->bt_stride;
   po.seq_lens = pj.seq_lens = a->seq_lens;
   po.B = a->B;
-  po.Hkv = pj.Hkv = a->Hkv;
   po.G = pj.G = a->G;
-  po.head_groups = head_groups;
+  po.heads = a->Hkv * head_groups;
+  po.div_groups = FastDiv::make(head_groups);
   po.prefix_len = pj.prefix_len = prefix_len;
   po.max_len = pj.max_len = a->max_seq_len;
-  po.chunk = pj.chunk = cut.own_chunk;
-  po.first_split = pj.prefix_splits = cut.prefix_splits;
   po.page_size = a->page_size;
   po.page_shift = page_shift;
   po.n_pages = a->n_pages;
   po.a = score.a;
   po.c2 = score.c2;
-  po.part_o = part_o;
-  po.part_ml = part_ml;
+  po.part_o = own_o;
+  po.part_ml = own_ml;
+  po.warps = warps;
   po.status = a->status;
-  pj.part_o = part_o;
-  pj.part_ml = part_ml;
+  pj.prefix_o = part_o;
+  pj.prefix_ml = part_ml;
+  pj.own_o = own_o;
+  pj.own_ml = own_ml;
+  pj.warps = warps;
+  pj.prefix_splits = cut.prefix_splits;
+  pj.Hkv = a->Hkv;
+  pj.groups = head_groups;
   pj.out = static_cast<__nv_bfloat16*>(a->out);
   pj.rows = rows;
 
+  const int64_t grid = prefix_ctas + cut.own_ctas;
+  if (grid > 0x7fffffff) return LF_ERR_TOO_LARGE;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto with_d = [&](auto d) {
     constexpr int D = decltype(d)::value;
-    const int r = score.softcap ? launch_shared<D, true>(mq, mk, mv, pp, grid, po, cut, st)
-                                : launch_shared<D, false>(mq, mk, mv, pp, grid, po, cut, st);
-    if (r != LF_OK) return r;
+    if (grid > 0) {
+      const auto launch = score.softcap ? launch_shared<D, true> : launch_shared<D, false>;
+      const int r = launch(mq, mk, mv, pp, po, static_cast<int>(prefix_ctas), static_cast<unsigned>(grid), st);
+      if (r != LF_OK) return r;
+    }
     launch_pdl(join_kernel<D>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, st, pj);
     return check_launch("join_kernel");
   };

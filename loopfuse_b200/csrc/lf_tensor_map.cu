@@ -9,13 +9,13 @@
 
 namespace lf {
 
-static int encode_map_4d(CUtensorMap* map, const TileMapSpec& s) {
+static int encode_map_5d(CUtensorMap* map, const TileMapSpec& s) {
   const auto fn = get_encode_fn();
   if (!fn) return LF_ERR_CUDA;
-  cuuint64_t dims[4], strides[3];
-  cuuint32_t box[4] = {64, 0, 0, 0}, estr[4] = {1, 1, 1, 1};
-  for (int i = 0; i < 4; ++i) dims[i] = static_cast<cuuint64_t>(s.dim[i]);
-  for (int i = 0; i < 3; ++i) {
+  cuuint64_t dims[5], strides[4];
+  cuuint32_t box[5] = {64, 0, 0, 0, 0}, estr[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < 5; ++i) dims[i] = static_cast<cuuint64_t>(s.dim[i]);
+  for (int i = 0; i < 4; ++i) {
     box[i + 1] = static_cast<cuuint32_t>(s.box[i]);
     strides[i] = static_cast<cuuint64_t>(s.stride[i]) * 2;
     // (A dimension of extent 1 may carry any stride; keep it a valid multiple of 16 bytes.)
@@ -25,7 +25,7 @@ static int encode_map_4d(CUtensorMap* map, const TileMapSpec& s) {
     }
   }
   const CUresult r =
-      fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(s.base), dims, strides, box,
+      fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(s.base), dims, strides, box,
          estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
@@ -46,16 +46,16 @@ constexpr int kMapSlots = 256;
 static std::mutex g_map_mutex;
 static MapEntry g_maps[kMapSlots];
 
-int make_map_4d(CUtensorMap* map, const TileMapSpec& spec) {
+int make_map_5d(CUtensorMap* map, const TileMapSpec& spec) {
   TileMapSpec key;  // (with the padding zeroed: entries are compared as bytes)
   memset(&key, 0, sizeof(key));
   key.base = spec.base;
   uint64_t h = reinterpret_cast<uintptr_t>(spec.base) * 0x9E3779B97F4A7C15ull;
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 5; ++i) {
     key.dim[i] = spec.dim[i];
     h = (h ^ static_cast<uint64_t>(spec.dim[i])) * 0xC2B2AE3D27D4EB4Full;
   }
-  for (int i = 0; i < 3; ++i) {
+  for (int i = 0; i < 4; ++i) {
     key.stride[i] = spec.stride[i];
     key.box[i] = spec.box[i];
     h = (h ^ static_cast<uint64_t>(spec.stride[i]) ^ static_cast<uint64_t>(spec.box[i]) << 48) *
@@ -70,7 +70,7 @@ int make_map_4d(CUtensorMap* map, const TileMapSpec& spec) {
       return LF_OK;
     }
   }
-  const int rc = encode_map_4d(map, key);
+  const int rc = encode_map_5d(map, key);
   if (rc != LF_OK) return rc;
   std::lock_guard<std::mutex> lock(g_map_mutex);
   MapEntry& e = g_maps[slot];
