@@ -802,12 +802,14 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
                 pk[c * 16 + (e >> 1)] = pkv;
                 if ((e >> 1) & 1) add_bf16x2_to_f32(fs[2], fs[3], pkv);
                 else add_bf16x2_to_f32(fs[0], fs[1], pkv);
+                if (e == 30) tmem_st_32x32b_x16(s_addr + c * 16, pk + c * 16);
               }
             const float sum = (fs[0] + fs[1]) + (fs[2] + fs[3]);
             own_max = __any_sync(0xffffffffu, valid && !(sum <= 16384.f));
             if (!own_max) l_run += sum;
           }
           if (own_max) {
+            tmem_wait_st();
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int c = 0; c < 2; ++c)
@@ -862,8 +864,8 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
               }
             }
             l_run = fmaf(l_run, alpha, (ps[0] + ps[1]) + (ps[2] + ps[3]));
+            tmem_st_32x32b_x32(s_addr, pk);
           }
-          tmem_st_32x32b_x32(s_addr, pk);
           tmem_wait_st();
         }
         tc_fence_before();

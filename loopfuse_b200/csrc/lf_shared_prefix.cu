@@ -10,7 +10,6 @@
 #include "lf_packed.cuh"
 
 #include <algorithm>
-#include <stdlib.h>
 #include <type_traits>
 
 namespace lf {
@@ -92,6 +91,7 @@ __device__ __forceinline__ void own_part(const OwnParams& p, int w, int n_warps)
     groups = own > 0 ? (own + kOwnGroup - 1) / kOwnGroup : 0;
   };
   long long all = 0;
+#pragma unroll 4
   for (int from = 0; from < p.B; from += 32) {
     load_groups(from);
     all += groups;
@@ -218,7 +218,8 @@ __device__ __forceinline__ void own_part(const OwnParams& p, int w, int n_warps)
     }
   };
 
-  // now: computed; then, later: being copied; last: its page is being looked up.
+  // now: computed; then, later: being copied; ahead, last: their pages are being looked up. (One look-up
+  // ahead, a warp took a group of 8 KB per round trip to the table.)
   static_assert(kOwnStages == 3, "two groups are copied while one is computed");
   OwnGroup then = next_group(now), later = next_group(then);
   load_q(now);
@@ -227,7 +228,8 @@ __device__ __forceinline__ void own_part(const OwnParams& p, int w, int n_warps)
     copy_group(now, 0, pg0);
     copy_group(then, 1, pg1);
   }
-  int page = look_up(later);
+  OwnGroup ahead = next_group(later);
+  int page = look_up(later), page_ahead = look_up(ahead);
 
   float m_run = -INFINITY, l_run = 0.f;
   float o[NT][4];
@@ -238,8 +240,9 @@ __device__ __forceinline__ void own_part(const OwnParams& p, int w, int n_warps)
 
   for (int it = 0; now.b >= 0; it = it == 2 ? 0 : it + 1) {
     copy_group(later, it == 0 ? 2 : it - 1, page);
-    const OwnGroup last = next_group(later);
-    page = look_up(last);
+    const OwnGroup last = next_group(ahead);
+    page = page_ahead;
+    page_ahead = look_up(last);
     cp_async_wait<kOwnStages - 1>();
     __syncwarp();
     const unsigned char* stage = ring + it * kStageBytes;
@@ -356,7 +359,8 @@ __device__ __forceinline__ void own_part(const OwnParams& p, int w, int n_warps)
     __syncwarp();  // every lane is done with this stage before it is refilled
     now = then;
     then = later;
-    later = last;
+    later = ahead;
+    ahead = last;
   }
   cp_async_wait<0>();
 }
@@ -474,14 +478,20 @@ __global__ void __launch_bounds__(kPackedThreads, 2)
   const int cta = static_cast<int>(blockIdx.x);
   if (cta < prefix_ctas) {
     packed_tiles<D, kPackedPrefix, SOFTCAP>(tmap_q, tmap_k, tmap_v, p, cta);
-  } else if (threadIdx.x >= kOwnWarps * 32) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
-    pdl_wait();
-    // (Runs go round the CTAs first, then their warps: few of them are spread over all SMs.)
-    const int ctas = static_cast<int>(gridDim.x) - prefix_ctas;
-    own_part<D, SOFTCAP>(own, (threadIdx.x >> 5) * ctas + cta - prefix_ctas, ctas * kOwnWarps);
+    // (No tensor memory for these, but the right to ask for it has to be given up: until its CTA has done so, an
+    // SM takes no other one of this kernel.)
+    if (threadIdx.x >= kOwnWarps * 32) {
+      asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    } else {
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+      if (threadIdx.x < 32) tmem_relinquish();
+      pdl_wait();
+      // (Runs go round the CTAs first, then their warps: few of them are spread over all SMs.)
+      const int ctas = static_cast<int>(gridDim.x) - prefix_ctas;
+      own_part<D, SOFTCAP>(own, (threadIdx.x >> 5) * ctas + cta - prefix_ctas, ctas * kOwnWarps);
+    }
+    __syncthreads();
   }
 }
 
@@ -505,7 +515,6 @@ static int shared_sm_count() {
   return cached > 0 ? cached : 148;
 }
 
-static int XP = getenv("XP") ? atoi(getenv("XP")) : 4, XO = getenv("XO") ? atoi(getenv("XO")) : 4, XB = getenv("XB") ? atoi(getenv("XB")) : 2;
 static PrefixCut cut_prefix(int B, int Hkv, int G, int prefix_len, int max_len) {
   PrefixCut c;
   const int sms = shared_sm_count();
@@ -514,9 +523,12 @@ static PrefixCut cut_prefix(int B, int Hkv, int G, int prefix_len, int max_len) 
     const int tq = kPackedRows / G;
     const int64_t units = static_cast<int64_t>((B + tq - 1) / tq) * Hkv;
     const int blocks = (prefix_len + kPackedKeys - 1) / kPackedKeys;
-    // As many slices as one wave of two CTAs per SM takes, of two key blocks or more.
-    int64_t s = std::max<int64_t>(1, static_cast<int64_t>(XP) * sms / 2 / units);
-    s = std::min<int64_t>(s, (blocks + XB - 1) / XB);
+    // As many slices as one wave of two CTAs per SM takes, of four key blocks or more: a slice's rows are
+    // written and read again, 64 KB each way against 32 KB of K and V a block. (64 requests, 2048 shared keys: two
+    // blocks 25 us, four 20.) Few rows cost less: 4 requests of 4 heads, 512 shared keys, two blocks 9.9 us, four 11.1.
+    const int least = std::min(B, tq) * G > kPackedRows / 2 ? 4 : 2;
+    int64_t s = std::max<int64_t>(1, 2ll * sms / units);
+    s = std::min<int64_t>(s, (blocks + least - 1) / least);
     const int per = static_cast<int>((blocks + s - 1) / s);
     c.prefix_chunk = per * kPackedKeys;
     c.prefix_splits = (blocks + per - 1) / per;
@@ -527,7 +539,7 @@ static PrefixCut cut_prefix(int B, int Hkv, int G, int prefix_len, int max_len) 
     c.heads = Hkv * ((G + kOwnHeads - 1) / kOwnHeads);
     c.units = static_cast<int64_t>(B) * c.heads;
     const int64_t runs = (c.units * ((own + kOwnGroup - 1) / kOwnGroup) + kOwnRun - 1) / kOwnRun;
-    c.own_ctas = static_cast<int>(std::min<int64_t>(runs, static_cast<int64_t>(XO) * sms / 2));
+    c.own_ctas = static_cast<int>(std::min<int64_t>(runs, 2ll * sms));
     c.own_parts = static_cast<size_t>(c.units + c.own_ctas * kOwnWarps) * kOwnHeads;
   }
   return c;
