@@ -711,8 +711,16 @@ PagePlan run_plan_pages(const Tensor& kv_lens, const Tensor& new_lens, const Ten
   const int64_t T = narrow_i32(num_tokens, "num_tokens");
   // One allocation: slots, positions, offsets, lengths, count.
   const Tensor all = at::empty({2 * T + 2 * B + 2}, at::TensorOptions().dtype(at::kInt).device(dev));
-  PagePlan r{all.narrow(0, 2 * T, B + 1), all.narrow(0, 2 * T + B + 1, B), all.narrow(0, 0, T),
-             all.narrow(0, T, T), all.narrow(0, 2 * T + 2 * B + 1, 1)};
+  // (Tensors over the one storage, made without the dispatcher: five narrow() took 4 us of a call's 10.)
+  auto part = [&](int64_t from, int64_t n) {
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(all.storage()), all.key_set(),
+                                                        all.dtype());
+    t.unsafeGetTensorImpl()->set_storage_offset(from);
+    t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+    return t;
+  };
+  PagePlan r{part(2 * T, B + 1), part(2 * T + B + 1, B), part(0, T), part(T, T),
+             part(2 * T + 2 * B + 1, 1)};
   LfPagePlanArgs a;
   std::memset(&a, 0, sizeof(a));
   a.kv_lens = i32_ptr(kv_lens);

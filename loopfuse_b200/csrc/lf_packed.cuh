@@ -264,30 +264,30 @@ __device__ __forceinline__ void stg_32(void* p, const uint32_t* r) {
 }
 
 // Output rows of a tile from its slices, a warp for its 32 rows, lanes along the columns: o = sum_s o_s
-// 2^(m_s - m) / sum_s l_s 2^(m_s - m). Four rows at a time, so that their loads are in flight together.
+// 2^(m_s - m) / sum_s l_s 2^(m_s - m). Eight rows at a time, so that their loads are in flight together.
 template <int D>
 __device__ __forceinline__ void join_slices(const PackedParams& p, const PackedItem& it, int warp, int lane,
                                          int rows) {
-  constexpr int kCols = D / 32;
+  constexpr int kCols = D / 32, kRows = 8;
   const int n = it.n_parts, hkv = it.hkv, q_row = it.q_row;
   const int64_t part0 = (static_cast<int64_t>(it.part) * p.Hkv + hkv) * kPackedRows;
   const int64_t step = static_cast<int64_t>(p.Hkv) * kPackedRows;
   const int end = min(warp * 32 + 32, rows);
   #pragma unroll 1
-  for (int r0 = warp * 32; r0 < end; r0 += 4) {
-    float acc[4][kCols], l[4], m[4];
+  for (int r0 = warp * 32; r0 < end; r0 += kRows) {
+    float acc[kRows][kCols], l[kRows], m[kRows];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kRows; ++u) {
       m[u] = -INFINITY;
       l[u] = 0.f;
 #pragma unroll
       for (int c = 0; c < kCols; ++c) acc[u][c] = 0.f;
     }
     for (int s = 0; s < n; ++s) {
-      float2 ml[4];
-      float x[4][kCols];
+      float2 ml[kRows];
+      float x[kRows][kCols];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kRows; ++u) {
         const int64_t at = part0 + s * step + min(r0 + u, end - 1);
         ml[u] = __ldcg(&p.part_ml[at]);
         const float* src = p.part_o + at * D + lane * kCols;
@@ -300,7 +300,7 @@ __device__ __forceinline__ void join_slices(const PackedParams& p, const PackedI
         }
       }
 #pragma unroll
-      for (int u = 0; u < 4; ++u) {
+      for (int u = 0; u < kRows; ++u) {
         if (ml[u].y == 0.f) continue;  // (no key of this row: what its accumulator holds is of no value)
         const float top = fmaxf(m[u], ml[u].x);
         const float back = ex2_approx(m[u] - top), w = ex2_approx(ml[u].x - top);
@@ -311,7 +311,7 @@ __device__ __forceinline__ void join_slices(const PackedParams& p, const PackedI
       }
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kRows; ++u) {
       if (r0 + u >= end) break;
       const int tok = static_cast<int>(p.div_g.div(r0 + u));
       __nv_bfloat16* dst = p.out + static_cast<int64_t>(q_row + tok) * p.o_stride[0] +
