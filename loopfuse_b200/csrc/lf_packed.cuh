@@ -512,7 +512,9 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
         int32_t page = 0, page_next = 0;
         auto request = [&](int w) -> int32_t {
           const int n = w * 32 + lane;
-          return n < all_boxes && n < hi * boxes ? table[page_of(n * p.box)] : 0;
+          if (n >= all_boxes || n >= hi * boxes) return 0;
+          const int at = page_of(n * p.box);
+          return LF_BOUNDS(at >= 0 && at < p.bt_blocks, p.status, 70) ? table[at] : 0;
         };
         auto checked = [&](int32_t pg) -> int32_t {
           if (pg >= 0 && pg < p.n_pages) return pg;
@@ -694,7 +696,7 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
           if (p.mask_kind == LF_MASK_CAUSAL_WINDOW) c_lo = max(0, last - (p.window - 1));
         }
       }
-      const bool valid = row < rows;
+      bool valid = row < rows;
       const bool idle = warp_uniform(warp * 32) >= rows;  // no row of this warp is one of the tile's
       float m_used = p.m_first;  // reference that P and O are scaled by (log2 domain)
       float l_run = 0.f;
@@ -890,6 +892,10 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
       // sectors of 32 bytes; one that saw no key is zeros).
       const bool empty = l_run == 0.f;
       const float inv = empty ? 0.f : 1.f / l_run;
+      if (valid && !LF_BOUNDS(it.q_row >= 0 && it.q_row + row_tok < (KIND == kPackedPrefix ? p.B : p.T) &&
+                                  it.hkv >= 0 && it.hkv < p.Hkv && head < p.G,
+                              p.status, 71))
+        valid = false;
       float* part = nullptr;
       __nv_bfloat16* dst = nullptr;
       if (valid) {

@@ -135,6 +135,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
     int slot = -1, pos = 0;
     if (t < n_tokens) {
       const int b = owner(s_cu, t);
+      if (!LF_BOUNDS(t >= s_cu[b] && t < s_cu[b + 1], p.status, 74)) continue;
       const int held = min(max(p.kv_lens[b], 0), kMaxLength);
       pos = held + (t - s_cu[b]);
       const int blk = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
@@ -187,6 +188,7 @@ __global__ void __launch_bounds__(256) kv_append_packed_kernel(const AppendPacke
       if (p.status) atomicExch(p.status, LF_DEV_BAD_PAGE);
       continue;
     }
+    if (!LF_BOUNDS(t < p.total / p.div_token.d && h * p.div_head.d < p.div_token.d, p.status, 73)) continue;
     const int page = p.page_shift >= 0 ? slot >> p.page_shift : slot / p.page_size;
     const int at = slot - page * p.page_size;
     const uint4 kx = ldg_stream_16(p.k_new + t * p.kn_stride[0] + h * p.kn_stride[1] + c * 8);

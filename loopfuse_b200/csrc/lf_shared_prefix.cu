@@ -31,7 +31,7 @@ struct OwnParams {
   int32_t heads;       // units of a request: kv heads times groups of 8 query heads
   FastDiv div_groups;  // groups of query heads
   int32_t prefix_len, max_len;
-  int32_t page_size, page_shift, n_pages;
+  int32_t bt_blocks, page_size, page_shift, n_pages;
   float a, c2;
   // Part of warp w for unit u: at place w + u, which no other pair has, since both only grow along the row
   // of groups; [place][8 query heads][D], (maximum, sum), and the warps that a unit's groups went to.
@@ -158,7 +158,9 @@ __device__ __forceinline__ void own_part(const OwnParams& p, int w, int n_warps)
   // Page of this lane's row of a group (rows past the end: the last token again).
   auto look_up = [&](const OwnGroup& x) {
     if (x.b < 0) return 0;
-    return p.table[x.b * p.bt_stride + page_of(min(x.t + (lane & 15), x.end - 1))];
+    const int at = page_of(min(x.t + (lane & 15), x.end - 1));
+    if (!LF_BOUNDS(x.b < p.B && x.head < p.heads && at >= 0 && at < p.bt_blocks, p.status, 72)) return 0;
+    return p.table[x.b * p.bt_stride + at];
   };
   unsigned char* ring = smem + warp * (kOwnStages * kStageBytes);
   const int r0 = lane / CPR, j0 = lane % CPR;
@@ -659,6 +661,7 @@ int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* a, void* stream) {
   po.div_groups = FastDiv::make(head_groups);
   po.prefix_len = pj.prefix_len = prefix_len;
   po.max_len = pj.max_len = a->max_seq_len;
+  po.bt_blocks = a->bt_blocks;
   po.page_size = a->page_size;
   po.page_shift = page_shift;
   po.n_pages = a->n_pages;
