@@ -57,16 +57,16 @@ __global__ void __launch_bounds__(kOrderThreads)
     }
     if (lane == 31) s_warp[warp] = incl;
     __syncthreads();
-    int before = 0, total = 0;
+    int warps = s_warp[lane];  // (as many warps as lanes)
+    const int own = __shfl_sync(0xffffffffu, warps, warp);
 #pragma unroll
-    for (int w = 0; w < kOrderThreads / 32; ++w) {
-      const int x = s_warp[w];
-      if (w < warp) before += x;
-      total += x;
+    for (int d = 1; d < 32; d <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, warps, d);
+      if (lane >= d) warps += x;
     }
     __syncthreads();
-    *all = total;
-    return before + incl - v;
+    *all = __shfl_sync(0xffffffffu, warps, 31);
+    return __shfl_sync(0xffffffffu, warps, warp) - own + incl - v;
   };
   int base = 0;
   for (int b0 = 0; b0 < p.B; b0 += kOrderThreads) {
@@ -92,12 +92,16 @@ __global__ void __launch_bounds__(kOrderThreads)
     }
     return packed_item(p, packed_request<KIND>(p, lo), e - s_first[lo]);
   };
+  // (A thread's first tile is looked up once; most batches have no second.)
+  PackedItem mine_first = {};
+  if (tid < n) mine_first = item_of(tid);
+  auto item_at = [&](int e) { return e == tid ? mine_first : item_of(e); };
   // How much there is, and so how long a slice may be.
   {
     int longest = 0;
     unsigned long long blocks = 0;
     for (int e = tid; e < n; e += kOrderThreads) {
-      const PackedItem it = item_of(e);
+      const PackedItem it = item_at(e);
       longest = max(longest, it.hi - it.lo);
       blocks += it.hi - it.lo;
     }
@@ -124,7 +128,7 @@ __global__ void __launch_bounds__(kOrderThreads)
     return kOrderLevels - 1 - min(blocks >> shift, kOrderLevels - 1);
   };
   for (int e = tid; e < n; e += kOrderThreads) {
-    const PackedItem it = item_of(e);
+    const PackedItem it = item_at(e);
     const int blocks = it.hi - it.lo, parts = parts_of(blocks);
     atomicAdd(&s_level[level_of((blocks + parts - 1) / parts)], parts);
   }
@@ -134,7 +138,7 @@ __global__ void __launch_bounds__(kOrderThreads)
   s_level[tid] = mine;
   __syncthreads();
   for (int e = tid; e < n; e += kOrderThreads) {
-    PackedItem it = item_of(e);
+    PackedItem it = item_at(e);
     const int lo = it.lo, blocks = it.hi - it.lo, parts = parts_of(blocks);
     const int at = atomicAdd(&s_level[level_of((blocks + parts - 1) / parts)], parts);
     if (parts > 1) {
