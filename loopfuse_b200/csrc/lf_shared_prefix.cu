@@ -7,6 +7,11 @@
 //   own part     a unit is the own keys of a (request, kv head), in groups of 16; all units' groups in one
 //                row are dealt out to the warps in equal runs, as in decode: bound by HBM.
 //   join         join_kernel: out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the parts of both.
+//
+// The first two are CTAs of one launch, so the tensor pipe works on the shared part while the own keys stream
+// in. 64 requests, 2048 shared keys and up to 1024 own, 32 heads on 8: 38 us (bytes once at HBM's rate 12.6); 128
+// requests, 32768 shared and up to 2048 own: 138 us (53.6), where a paged decode of the same cache reads the
+// prefix 128 times.
 #include "lf_packed.cuh"
 
 #include <algorithm>
@@ -383,7 +388,8 @@ struct JoinParams {
 
 // One warp per output row. Lane s holds (reference, sum) of part s; the rows of the parts stream in with
 // their weights broadcast. Parts that hold no key of the row have sum 0 and are left out (what their
-// accumulators hold is of no value); a row without a key is zeros.
+// accumulators hold is of no value); a row without a key is zeros. Bound by the latency of its loads, 5 to 8
+// us for 2048 and 4096 rows.
 template <int D>
 __global__ void __launch_bounds__(128) join_kernel(const JoinParams p) {
   constexpr int EPL = D / 32;
@@ -580,6 +586,7 @@ int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* a, void* stream) {
   if (a->G > kPackedRows) return LF_ERR_UNSUPPORTED;
   const int64_t held = static_cast<int64_t>(a->bt_blocks) * a->page_size;
   if (a->prefix_len > held || a->max_seq_len > held) return LF_ERR_INVALID_ARG;
+  if (a->max_seq_len > kMostKeys) return LF_ERR_TOO_LARGE;
   PackedScore score;
   int rc = packed_score(a->scale, a->n_mod, a->mod_op, a->mod_arg, &score);
   if (rc != LF_OK) return rc;

@@ -9,6 +9,8 @@ and in the row sum. What fp32 scores, exp2 and sums add is below 2^-18 of the sa
 beyond 0.4 is the unit's (relative error 2^-11): it moves a logit s by |s| 2^-11 at most, and so every
 weight by that share, twice like the rounding.
 """
+import gc
+
 import pytest
 import torch
 
@@ -62,6 +64,14 @@ def offsets(lens):
 
 def ints(x):
     return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _no_garbage():
+    """Tensors that cycles keep (exceptions and their frames, modules) go with the module that made them, not
+    in the middle of a later test that counts allocated bytes."""
+    yield
+    gc.collect()
 
 
 @pytest.fixture(autouse=True)
@@ -160,6 +170,12 @@ def test_plan_pages_cuts_lengths_that_make_no_sense():
     plan = F.plan_pages(ints([0, 0]), ints([5, 2 ** 30]), ints([1, 2, 3]), table[:2], page_size=4,
                         num_tokens=8, status=st)
     assert plan.cu_seqlens.tolist() == [0, 5, 8] and int(st.item()) != 0
+    st.zero_()
+    table.fill_(-1)
+    plan = F.plan_pages(ints([0, 0, 0]), ints([2 ** 30] * 3), ints([7]), table, page_size=1, num_tokens=8, status=st)
+    assert plan.cu_seqlens.tolist() == [0, 8, 8, 8] and plan.pages_used.tolist() == [2 ** 31 - 1]
+    assert plan.slots.tolist() == [7] + [-1] * 7 and int(st.item()) != 0
+    assert table[0].tolist() == [7, -1, -1, -1] and (table[1:] == -1).all()
     with pytest.raises(RuntimeError, match="length"):
         F.check_status(ints([4]))
 

@@ -1,12 +1,21 @@
 """The serving example: page plans, appends, packed prefill and shared-prefix decode as one loop, its last
 step against the paged decode of the same cache. Both round their output to bf16 and one of them its
 weights too: for outputs of at most 4 (values are projections of N(0, 1) rows) that is within 2e-2."""
+import gc
 import importlib.util
 from pathlib import Path
 
 import pytest
 
 PATH = Path(__file__).resolve().parents[1] / "examples" / "serve_shared_prefix.py"
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _no_garbage():
+    """Tensors that cycles keep (exceptions and their frames, modules) go with the module that made them, not
+    in the middle of a later test that counts allocated bytes."""
+    yield
+    gc.collect()
 
 
 def example():

@@ -1,6 +1,7 @@
 """What the entry points for requests of different lengths refuse, without a GPU: the C ABI by status
 before any CUDA work, the tensor functions by exception."""
 import ctypes as C
+import gc
 
 import pytest
 import torch
@@ -9,6 +10,14 @@ from loopfuse_b200 import _native
 from loopfuse_b200 import functional as F
 
 INVALID, UNSUPPORTED, ALIGNMENT, WORKSPACE, TOO_LARGE = -1, -2, -3, -4, -7
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _no_garbage():
+    """Tensors that cycles keep (exceptions and their frames, modules) go with the module that made them, not
+    in the middle of a later test that counts allocated bytes."""
+    yield
+    gc.collect()
 
 
 def test_plan_pages_refusals(native_lib):
@@ -76,6 +85,7 @@ def test_packed_prefill_refusals(native_lib):
     refused(INVALID, mask_kind=2, window=0)
     refused(INVALID, cu_k=None)
     refused(INVALID, block_table=0x1000)           # a table without its page geometry
+    refused(TOO_LARGE, Tk=(1 << 30) + 1)
     refused(ALIGNMENT, q=0x1008)
     refused(ALIGNMENT, out=0x1004)
     refused(UNSUPPORTED, scale=-1.0)               # scores times a negative factor
