@@ -26,8 +26,8 @@
 // What bounds it: with a head dim of 128 the products of a block are 512 clocks of the tensor pipe, and two
 // CTAs of 128 rows keep it busy half of the time; the rest is the chain score -> exp2 -> P of each CTA
 // and the load of a row's scores and store of its weights (the load of S 160 clocks, the arithmetic some
-// 1200, the hand-over of P and the wait for the next S 700). 8 prompts up to 8192 tokens, 32 heads on 8: 700 us
-// for 664 GFLOP (0.95 PFLOP/s); 24 up to 2048 with a window of 256 and a softcap: 132 us.
+// 1200, the hand-over of P and the wait for the next S 700). 8 prompts up to 8192 tokens, 32 heads on 8: 662 us
+// for 664 GFLOP (1.0 PFLOP/s); 24 up to 2048 with a window of 256 and a softcap: 129 us.
 //
 // What a packed batch adds to the tiles of the prefill kernels: the last key block of a request holds
 // rows of the next one (or, in a page, of whoever had it before). Their scores are masked; their V rows
@@ -453,14 +453,15 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
     auto page_of = [&](int t) { return p.page_shift >= 0 ? (t >> p.page_shift) : (t / p.page_size); };
     const int boxes = kPages ? kPackedKeys / p.box : 1;
 
-    // K warp: the item behind the present one goes to the others as soon as Q of this one is on its way.
+    // K warp: takes the place of the next item as the last blocks of the present one are on their way. (Earlier, at
+    // the start of the item, it is another CTA's that could start it sooner: 256 slices of 36 blocks were two each
+    // for 50 of the CTAs. The blocks that are still to be computed hide the look-ups.)
     uint32_t n_list = 0, at = cta;
     auto read_item = [&](bool first) {
       PackedItem x;
       x.count = 0;
       if (p.items) {
         if (n_list > 0) x = listed_item(p, at, n_list);
-        at = take_place();
       } else if (first) {
         x = own_item<KIND>(p, cta);
       }
@@ -476,6 +477,7 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
                                     static_cast<int64_t>(x.hkv * p.G + r - t * p.G) * p.o_stride[1] +
                                     (e % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
         }
+        at = take_place();
         x = read_item(false);
       }
       wait(&bars->item_empty[i % kItemSlots], ((i / kItemSlots) & 1) ^ 1, 87);
@@ -499,7 +501,6 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
       const int lo = it.lo, hi = it.hi;
       {
         if (is_k) {
-          const PackedItem next = read_item(false);
           if (i > 0) wait(&bars->q_empty, (i - 1) & 1, 81);
           __syncwarp();
           if (elected) {
@@ -509,7 +510,6 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
             for (int kb = 0; kb < kBlocksD; ++kb)
               tma_load_5d(sQ + kb * Shape::kQBlockBytes, &tmap_q, &bars->q_full, kb * 64, 0, it.hkv, it.q_row, 0);
           }
-          hand_on(next, i + 1);
         }
         // Table entries of the copies ("boxes"), 32 at a time, a box per lane; the next 32 are requested before
         // these are used. (Block by block the look-up took 800 clocks of each.)
@@ -583,7 +583,9 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
               }
             }
           }
+          if (is_k && j == max(lo, hi - 2)) at = take_place();
         }
+        if (is_k) hand_on(read_item(false), i + 1);
       }
     }
   } else if (warp == kQkWarp) {

@@ -21,14 +21,16 @@ __global__ void __launch_bounds__(kPackedThreads, 2)
 // with the requests one after the other the last one's longest tile would start when the rest is nearly
 // done), and those that are long next to what a CTA has to do in all cut into slices of their keys (a
 // few new tokens behind a long context are a few tiles). One CTA; among items of one length the order is
-// arbitrary, and no result depends on it. About 7 us, which the tiles wait for: 32 chunks of up to 512 tokens
-// behind up to 4096 take 113 us with it.
+// arbitrary, and no result depends on it. 6 us, 9 where slices are compared, which the tiles wait for: 32 chunks of up
+// to 512 tokens behind up to 4096 take 88 us with it.
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderLevels = 1024;
 constexpr int kOrderRequests = 8192;  // in shared memory; larger batches keep the requests' order
 constexpr int kWholeBlocks = 32;      // tiles of up to 2048 keys are never cut: a prompt of that length has
                                       // the same result in every batch
 constexpr int kSliceBlocks = 16;      // at least, since a slice costs the store and the join of its rows
+constexpr int kItemBlocks = 8;        // about what the start, the store and the join of a slice take, in blocks
+constexpr int kOrderChoices = 8;      // lengths of slices that are compared
 
 template <int KIND>
 __global__ void __launch_bounds__(kOrderThreads)
@@ -39,6 +41,8 @@ __global__ void __launch_bounds__(kOrderThreads)
   __shared__ int32_t s_warp[kOrderThreads / 32];
   __shared__ unsigned long long s_blocks;
   __shared__ int32_t s_longest, s_parts, s_cut;
+  __shared__ int32_t s_slice[kOrderChoices], s_long[kOrderChoices], s_long_blocks[kOrderChoices];
+  __shared__ long long s_cost[kOrderChoices];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_trigger();
   s_level[tid] = 0;
@@ -117,11 +121,53 @@ __global__ void __launch_bounds__(kOrderThreads)
     }
   }
   __syncthreads();
-  // Slices of 0.8 of a CTA's share, so that the last ones to start do not stand out. (28 chunks of 128 to 512
-  // tokens behind up to 4096: 0.5 and 0.6 201 us, 0.8 166, 1.0 167.)
-  const long long share = (static_cast<long long>(s_blocks) * p.Hkv * 4 + 5ll * n_slots - 1) / (5ll * n_slots);
-  const int slice = static_cast<int>(min(max(share, static_cast<long long>(kSliceBlocks)), 1ll << 28));
-  const int whole = max(kWholeBlocks, slice + slice / 4);
+  // Slices of 0.8 to 1.5 of a CTA's share: as long as makes the whole shortest, if that is either what there
+  // is over all CTAs or the rounds that the long items take on them, whichever is more. (Shorter ones are more
+  // items than they bring balance. With 0.8 always, the 128 tiles of 512 tokens behind 4096 are 384 items for 296
+  // CTAs: 99 us, and 68 now.)
+  if (tid < kOrderChoices) {
+    const long long share = (static_cast<long long>(s_blocks) * p.Hkv * (8 + tid) + 10ll * n_slots - 1) / (10ll * n_slots);
+    s_slice[tid] = static_cast<int>(min(max(share, static_cast<long long>(kSliceBlocks)), 1ll << 28));
+    s_long[tid] = s_long_blocks[tid] = 0;
+  }
+  __syncthreads();
+  auto whole_of = [&](int slice) { return max(kWholeBlocks, slice + slice / 4); };
+  int choice = 0;
+  if (s_longest > whole_of(s_slice[0])) {
+    int items_of[kOrderChoices] = {}, blocks_of[kOrderChoices] = {};  // long items, and the longest's blocks
+    for (int e = tid; e < n; e += kOrderThreads) {
+      const PackedItem it = item_at(e);
+      const int blocks = it.hi - it.lo;
+      if (blocks <= kWholeBlocks) continue;
+#pragma unroll
+      for (int c = 0; c < kOrderChoices; ++c) {
+        const int slice = s_slice[c], parts = blocks > whole_of(slice) ? (blocks + slice - 1) / slice : 1;
+        items_of[c] += parts;
+        blocks_of[c] = max(blocks_of[c], (blocks + parts - 1) / parts);
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < kOrderChoices; ++c) {
+      const int items = __reduce_add_sync(0xffffffffu, items_of[c]);
+      const int blocks = __reduce_max_sync(0xffffffffu, blocks_of[c]);
+      if (lane == 0 && items) {
+        atomicAdd(&s_long[c], items);
+        atomicMax(&s_long_blocks[c], blocks);
+      }
+    }
+    __syncthreads();
+    if (tid < kOrderChoices) {
+      const long long items = static_cast<long long>(s_long[tid]) * p.Hkv;
+      const long long rounds = (items + n_slots - 1) / n_slots;
+      const long long spread = static_cast<long long>(s_blocks) * p.Hkv + items * kItemBlocks;
+      s_cost[tid] = max(spread, rounds * (s_long_blocks[tid] + kItemBlocks) * n_slots);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int c = 1; c < kOrderChoices; ++c)
+      if (s_cost[c] < s_cost[choice]) choice = c;
+  }
+  const int slice = s_slice[choice], whole = whole_of(slice);
   auto parts_of = [&](int blocks) { return blocks > whole ? (blocks + slice - 1) / slice : 1; };
   int shift = 0;
   while ((s_longest >> shift) >= kOrderLevels) ++shift;
