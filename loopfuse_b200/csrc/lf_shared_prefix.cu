@@ -10,7 +10,7 @@
 //
 // The first two are CTAs of one launch, so the tensor pipe works on the shared part while the own keys stream
 // in. 64 requests, 2048 shared keys and up to 1024 own, 32 heads on 8: 38 us (bytes once at HBM's rate 12.6); 128
-// requests, 32768 shared and up to 2048 own: 138 us (53.6), where a paged decode of the same cache reads the
+// requests, 32768 shared and up to 2048 own: 136 us (53.6), where a paged decode of the same cache reads the
 // prefix 128 times.
 #include "lf_packed.cuh"
 
