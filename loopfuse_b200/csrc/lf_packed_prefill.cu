@@ -337,7 +337,9 @@ int lf_packed_prefill_bf16(const LfPackedArgs* a, void* stream) {
   p.G = G;
   p.tq = kPackedRows / G;
   p.mask_kind = a->mask_kind;
-  p.window = a->window;
+  // (No request has more keys, and the first key of a query, `pos - (window - 1)` with pos from -2^30 up, stays
+  // within 32 bits.)
+  p.window = std::min(a->window, kMostKeys);
   p.a = score.a;
   p.c2 = score.c2;
   p.m_first = score.m_first;
