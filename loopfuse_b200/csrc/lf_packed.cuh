@@ -735,7 +735,17 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
 
           if constexpr (SOFTCAP) {
             // tanh(x), x = raw * a: x (1 - x^2 / 3) up to |x| = 0.125 (error below 4.1e-6), its series to
-            // x^7 up to 0.4 (below 6e-6), the unit's approximation beyond.
+            // x^7 up to 0.4 (below 6e-6), the unit's approximation beyond. The warp takes the form that its largest
+            // score asks for; columns past the last key (other requests' rows, or whatever was in the stage) have
+            // no say in it, nor have rows that see no key.
+            if (c0 + kPackedKeys > m) {
+#pragma unroll
+              for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if (c * 32 + e >= m - c0) sr[c][e] = 0u;
+            }
+            const bool sees = valid && c_hi >= 0;
             float mx[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int c = 0; c < 2; ++c)
@@ -749,7 +759,7 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
             const float bound = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * fabsf(p.a);
             const float a2 = p.a * p.a;
             const float b1 = a2 * (-1.f / 3.f);
-            if (!__any_sync(0xffffffffu, valid && !(bound <= 0.125f))) {
+            if (!__any_sync(0xffffffffu, sees && !(bound <= 0.125f))) {
               const uint64_t a_2 = pack2(p.a, p.a), b_2 = pack2(b1 * p.a, b1 * p.a);
 #pragma unroll
               for (int c = 0; c < 2; ++c)
@@ -761,7 +771,7 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
                   sr[c][e] = __float_as_uint(t0);
                   sr[c][e + 1] = __float_as_uint(t1);
                 }
-            } else if (!__any_sync(0xffffffffu, valid && !(bound <= 0.4f))) {
+            } else if (!__any_sync(0xffffffffu, sees && !(bound <= 0.4f))) {
               const float b2 = a2 * a2 * (2.f / 15.f);
               const float b3 = a2 * a2 * a2 * (-17.f / 315.f);
 #pragma unroll

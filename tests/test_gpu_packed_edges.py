@@ -80,3 +80,74 @@ def test_a_window_that_holds_every_key_is_the_causal_mask(window, pages):
     got = F.packed_prefill_attention(q, k, v, offsets(lens), scale=0.125, mask_kind=S.MASK_CAUSAL_WINDOW, window=window,
                                      **options)
     assert want[3:13].abs().amax() > 0 and torch.equal(got, want)
+
+
+# -- what may not change a capped result ----------------------------------------------------------------
+STRANGERS = [float("nan"), float("inf"), -float("inf"), 3e38, 1e4]
+
+
+@pytest.mark.parametrize("bad", STRANGERS)
+def test_capped_results_do_not_depend_on_neighbours(bad):
+    """Logits of |x| < 0.125 of the cap, where the form of tanh that large ones take would show."""
+    g = torch.Generator(device="cuda").manual_seed(2)
+    lens, D = [70, 33, 130, 20], 128
+    T = sum(lens)
+    q, k, v = normal(g, T + 40, 4, D), normal(g, T + 40, 2, D), normal(g, T + 40, 2, D)
+    cu, options = offsets(lens), dict(scale=D ** -0.5, mods=softcap(50.0))
+    want = F.packed_prefill_attention(q, k, v, cu, **options)
+    for b in (1, 3):
+        q2, k2, v2 = q.clone(), k.clone(), v.clone()
+        for x in (q2, k2, v2):
+            x[cu[b]:cu[b + 1]] = bad
+            x[T:] = bad
+        got = F.packed_prefill_attention(q2, k2, v2, cu, **options)
+        for o in range(4):
+            if o != b:
+                assert torch.equal(got[cu[o]:cu[o + 1]], want[cu[o]:cu[o + 1]]), (b, o)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("pages", [False, True])
+def test_capped_results_are_those_of_the_request_alone(D, pages):
+    """Requests with large keys between small ones, several per CTA: what they leave in shared memory changes
+    nothing."""
+    g = torch.Generator(device="cuda").manual_seed(D)
+    B = 700
+    lens = [70 + b % 50 if b % 2 else 200 for b in range(B)]
+    T = sum(lens)
+    q, k, v = normal(g, T, 4, D), normal(g, T, 2, D), normal(g, T, 2, D)
+    cu = offsets(lens)
+    for b in range(0, B, 2):
+        k[cu[b]:cu[b + 1]] *= 200.0
+    kk, vv, options = k, v, dict(scale=D ** -0.5, mods=softcap(50.0))
+    if pages:
+        kk, vv, table = paged(g, k, v, lens, 16)
+        options.update(block_table=table, seq_lens=ints(lens))
+    got = F.packed_prefill_attention(q, kk, vv, cu, **options)
+    for _ in range(3):
+        assert torch.equal(got, F.packed_prefill_attention(q, kk, vv, cu, **options))
+    for b in range(1, B, 24):
+        one = slice(int(cu[b]), int(cu[b + 1]))
+        alone = F.packed_prefill_attention(q[one], k[one], v[one], ints([0, lens[b]]), scale=D ** -0.5, mods=softcap(50.0))
+        assert torch.equal(got[one], alone), b
+
+
+@pytest.mark.parametrize("bad", STRANGERS)
+def test_capped_decode_does_not_depend_on_rows_without_a_request(bad):
+    """Padding rows of the batch (length 0), and what the prefix's last page holds behind the prefix."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    D, P, prefix, lens = 128, 16, 200, [230, 0, 201, 200, 0, 260]
+    q, kp, vp = normal(g, 6, 2, 4, D), normal(g, 80, P, 2, D), normal(g, 80, P, 2, D)
+    table = torch.randperm(79, generator=g, device="cuda").int()[:60].view(6, 10).repeat(1, 2)[:, :17] + 1
+    table[:, :prefix // P] = table[0, :prefix // P].clone()
+    table[0, prefix // P] = 0                 # a page of row 0 alone: its first half is shared
+    options = dict(scale=D ** -0.5, mods=softcap(50.0), max_seq_len=270)
+    want = F.shared_prefix_decode_attention(q, kp, vp, table, ints(lens), prefix, **options)
+    q2, k2 = q.clone(), kp.clone()
+    q2[1] = q2[4] = bad
+    got = F.shared_prefix_decode_attention(q2, kp, vp, table, ints(lens), prefix, **options)
+    assert torch.equal(got, want)
+    k2[0, prefix % P:] = bad
+    got = F.shared_prefix_decode_attention(q, k2, vp, table, ints([200] + lens[1:]), prefix, **options)
+    want = F.shared_prefix_decode_attention(q, kp, vp, table, ints([200] + lens[1:]), prefix, **options)
+    assert torch.equal(got, want)
