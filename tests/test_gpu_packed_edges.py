@@ -151,3 +151,30 @@ def test_capped_decode_does_not_depend_on_rows_without_a_request(bad):
     got = F.shared_prefix_decode_attention(q, k2, vp, table, ints([200] + lens[1:]), prefix, **options)
     want = F.shared_prefix_decode_attention(q, kp, vp, table, ints([200] + lens[1:]), prefix, **options)
     assert torch.equal(got, want)
+
+
+# -- pages behind the window ----------------------------------------------------------------------------
+@pytest.mark.parametrize("P", [1, 4, 16, 24, 64, 128])
+@pytest.mark.parametrize("D,Hq,Hkv", [(64, 4, 4), (128, 8, 2)])
+@pytest.mark.parametrize("cap", [0.0, 50.0])
+def test_pages_behind_the_window_need_not_be_there(P, D, Hq, Hkv, cap):
+    """A cache that has given the pages back that no query sees any more: their entries are -1, and page 0 holds
+    NaN. Short tiles, several tiles, tiles that are cut into slices."""
+    g = torch.Generator(device="cuda").manual_seed(P)
+    lens, keys = [1, 40, 3, 150, 1, 2], [700, 2100, 64, 900, 129, 6000]
+    q = normal(g, sum(lens), Hq, D)
+    k, v = normal(g, sum(keys), Hkv, D), normal(g, sum(keys), Hkv, D)
+    kp, vp, table = paged(g, k, v, keys, P, spare=float("nan"))
+    for window in (1, 63, 64, 100, 2500):
+        options = dict(scale=D ** -0.5, mask_kind=S.MASK_CAUSAL_WINDOW, window=window, mods=softcap(cap) if cap else (),
+                       seq_lens=ints(keys))
+        want = F.packed_prefill_attention(q, k, v, offsets(lens), cu_seqlens_k=offsets(keys),
+                                          **{n: x for n, x in options.items() if n != "seq_lens"})
+        evicted = table.clone()
+        for b, (n, m) in enumerate(zip(lens, keys)):
+            first = max(0, m - n - (window - 1))      # that the request's first query sees
+            evicted[b, :first // P] = -1
+        st = F.new_status("cuda")
+        got = F.packed_prefill_attention(q, kp, vp, offsets(lens), block_table=evicted, status=st, **options)
+        assert int(st.item()) == 0, window
+        assert torch.equal(got, want), window
