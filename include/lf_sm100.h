@@ -65,8 +65,9 @@ typedef enum {
 #define LF_DEV_BOUNDS 3         /* debug-bounds build only: an index left its range; bits 8..
                                    say where. The access was skipped or clamped.            */
 
-#define LF_DEV_BAD_LENGTHS 4    /* a request's length is negative or the batch has more tokens than
-                                   the caller's buffers; lengths are cut to what fits          */
+#define LF_DEV_BAD_LENGTHS 4    /* a request's length is negative or above the caller's bound, or the
+                                   batch has more tokens than the caller's buffers; lengths are cut
+                                   to what fits                                                 */
 
 /* Mask kinds (what the capture layer deduces from loopfuse::causal_mask / sliding_mask). */
 #define LF_MASK_NONE 0
@@ -286,7 +287,8 @@ typedef struct {
   int64_t bt_stride;
   int32_t bt_blocks, page_size, n_pages;
   int32_t prefix_len;     /* keys below it are read through row 0 of the table, for all requests */
-  int32_t max_seq_len;    /* no request is longer (one that is, is cut); sizes the workspace */
+  int32_t max_seq_len;    /* no request is longer (one that is, is cut to it, and reported as
+                             LF_DEV_BAD_LENGTHS like a negative length); sizes the workspace */
   float scale;
   int32_t n_mod;
   int32_t mod_op[LF_MAX_MODS];

@@ -384,6 +384,7 @@ struct JoinParams {
   int32_t prefix_len, max_len, prefix_splits;
   int64_t rows;
   int32_t Hkv, G, groups;  // groups of 8 query heads
+  int32_t* status;
 };
 
 // One warp per output row. Lane s holds (reference, sum) of part s; the rows of the parts stream in with
@@ -402,6 +403,10 @@ __global__ void __launch_bounds__(128) join_kernel(const JoinParams p) {
   const int rest = static_cast<int>(row - b * (p.Hkv * p.G));
   const int kvh = rest / p.G, g = rest - kvh * p.G;
   const int64_t unit = (b * p.Hkv + kvh) * p.groups + g / kOwnHeads;
+  if (p.status && rest == 0 && lane == 0) {  // (what is cut is reported once, by the request's first row)
+    const int len = p.seq_lens[b];
+    if (len < 0 || len > p.max_len) atomicCAS(p.status, 0, LF_DEV_BAD_LENGTHS);
+  }
   int64_t own_at = 0;
   int n = p.prefix_splits;
   if (own_end(p.seq_lens, static_cast<int>(b), p.max_len) > p.prefix_len) {
@@ -685,6 +690,7 @@ int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* a, void* stream) {
   pj.groups = head_groups;
   pj.out = static_cast<__nv_bfloat16*>(a->out);
   pj.rows = rows;
+  pj.status = a->status;
 
   const int64_t grid = prefix_ctas + cut.own_ctas;
   if (grid > 0x7fffffff) return LF_ERR_TOO_LARGE;

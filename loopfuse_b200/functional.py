@@ -58,8 +58,8 @@ def check_status(status: torch.Tensor, what: str = "kernel") -> None:
     if (code & 0xFF) == _DEV_BAD_PAGE:
         raise RuntimeError(f"{what}: block_table holds a page id outside the pool")
     if (code & 0xFF) == _DEV_BAD_LENGTHS:
-        raise RuntimeError(f"{what}: a request's length is negative, or the batch has more tokens "
-                           "than num_tokens")
+        raise RuntimeError(f"{what}: a request's length is negative or above max_seq_len, or the batch "
+                           "has more tokens than num_tokens")
     raise RuntimeError(f"{what}: device status {code}")
 
 
@@ -380,7 +380,8 @@ def shared_prefix_decode_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool
     other tokens through its own row. A request of length 0 (a row of a padded batch) gets zeros.
 
     ``max_seq_len`` is a bound on the lengths that the host knows (default: all that the table
-    holds); the closer it is, the better the work is cut. ``mods`` as for
+    holds); the closer it is, the better the work is cut. A longer request is cut to it and reported
+    in ``status``: a step recorded in a graph needs a bound that holds for every replay. ``mods`` as for
     ``packed_prefill_attention``."""
     return _native.host().shared_prefix_decode(q, k_pool, v_pool, block_table, seq_lens, prefix_len,
                                                max_seq_len, out, workspace, status, scale, mods)

@@ -178,3 +178,19 @@ def test_pages_behind_the_window_need_not_be_there(P, D, Hq, Hkv, cap):
         got = F.packed_prefill_attention(q, kp, vp, offsets(lens), block_table=evicted, status=st, **options)
         assert int(st.item()) == 0, window
         assert torch.equal(got, want), window
+
+
+# -- lengths that are cut -------------------------------------------------------------------------------
+def test_shared_prefix_reports_lengths_that_it_cuts():
+    """A step recorded with a bound on the lengths that they have outgrown would lose the newest keys."""
+    g = torch.Generator(device="cuda").manual_seed(4)
+    kp, q = normal(g, 6, 16, 2, 64), normal(g, 2, 2, 2, 64)
+    table = ints([[0, 1, 2], [0, 3, 4]])
+    for lens, bound, prefix, bad in (([40, 48], 48, 16, False), ([40, 48], None, 16, False), ([40, 49], None, 16, True),
+                                     ([40, 33], 32, 16, True), ([17, 0], 16, 16, True), ([16, 0], 16, 16, False),
+                                     ([9, 3], 8, 16, True), ([-1, 40], 48, 16, True), ([5, 0], 0, 0, True)):
+        st = F.new_status("cuda")
+        F.shared_prefix_decode_attention(q, kp, kp, table, ints(lens), prefix, max_seq_len=bound, status=st)
+        assert int(st.item()) == (BAD_LENGTHS if bad else 0), (lens, bound)
+    with pytest.raises(RuntimeError, match="max_seq_len"):
+        F.check_status(ints([BAD_LENGTHS]))
