@@ -709,7 +709,7 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
         const int tok = row < rows ? static_cast<int>(p.div_g.div(row)) : 0;
         c_lo = 0, c_hi = m - 1;
         if constexpr (KIND == kPackedPrefix) {
-          if (row < rows) c_hi = min(c_hi, p.kv_lens[it.q_row + tok] - 1);
+          if (row < rows) c_hi = min(c_hi, max(p.kv_lens[it.q_row + tok], 0) - 1);
         } else {
           const int last = it.pos + tok;
           if (p.mask_kind != LF_MASK_NONE) c_hi = min(c_hi, last);

@@ -194,3 +194,12 @@ def test_shared_prefix_reports_lengths_that_it_cuts():
         assert int(st.item()) == (BAD_LENGTHS if bad else 0), (lens, bound)
     with pytest.raises(RuntimeError, match="max_seq_len"):
         F.check_status(ints([BAD_LENGTHS]))
+
+
+def test_shared_prefix_takes_the_smallest_length_for_none():
+    g = torch.Generator(device="cuda").manual_seed(5)
+    kp, q = normal(g, 8, 16, 2, 64), normal(g, 2, 2, 2, 64)
+    table = ints([[0, 1, 2, 3, 4, 5], [0, 1, 2, 3, 6, 7]])
+    for least in (-1, -2 ** 31, -2 ** 31 + 70):
+        got = F.shared_prefix_decode_attention(q, kp, kp, table, ints([70, least]), 64)
+        assert (got[1] == 0).all() and got[0].abs().amax() > 0, least
