@@ -225,7 +225,8 @@ typedef struct {
   int32_t* slots;             /* out [num_tokens]: page * page_size + slot of each row; -1 past the
                                  last token and where no page was left                          */
   int32_t* positions;         /* out [num_tokens]: position in its request; 0 past the last token */
-  int32_t* pages_used;        /* out [1]: pages the step needs (may be more than n_free)         */
+  int32_t* pages_used;        /* out [1]: pages taken; where n_free is too few for the step, how many
+                                 the lengths ask for, which is more than n_free                  */
   int64_t bt_stride;          /* elements between rows of block_table                           */
   int32_t B, n_free, bt_blocks, page_size;
   int32_t num_tokens;         /* rows of the packed batch, padding included                     */
@@ -440,8 +441,8 @@ int lf_kv_append_bf16(const LfKvAppendArgs* args, void* stream);
  * page_size) pages, named by its row of the table, and gets
  * ceil((kv_lens[b] + new_lens[b]) / page_size) less those from the free list, requests in order.
  * Too few free pages, a table that is too narrow or an old entry that is negative: LF_DEV_BAD_PAGE in
- * `status`, entry and slot -1. A negative length counts as 0, tokens past num_tokens are dropped
- * (LF_DEV_BAD_LENGTHS). The outputs must not overlap the inputs. */
+ * `status`, entry and slot -1. A negative length counts as 0; tokens past num_tokens are dropped, and take
+ * no page (LF_DEV_BAD_LENGTHS). The outputs must not overlap the inputs. */
 int lf_plan_pages(const LfPagePlanArgs* args, void* stream);
 
 /* The store that goes with it: row t of k_new / v_new to slot slots[t] of the pools (bit-exact). A

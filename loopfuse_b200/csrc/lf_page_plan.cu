@@ -53,59 +53,67 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
     if (n < 0 || n > most) s_bad = 1;
     return min(max(n, 0), most);
   };
-  // Sums in 64 bits: lengths that make no sense add up to more than any buffer holds, and are cut there.
-  long long tokens_before = 0, pages_before = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
-    const int b = b0 + tid;
-    int held = 0, fresh = 0;
-    if (b < p.B) {
-      held = clamp_len(p.kv_lens[b], kMaxLength);
-      fresh = clamp_len(p.new_lens[b], kMaxLength - 1);
-    }
-    long long tok = fresh, pg = pages_of(held + fresh) - pages_of(held);
-    const long long my_tok = tok, my_pg = pg;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const long long a = __shfl_up_sync(0xffffffffu, tok, d);
-      const long long c = __shfl_up_sync(0xffffffffu, pg, d);
-      if (lane >= d) {
-        tok += a;
-        pg += c;
+  // Sums in 64 bits: lengths that make no sense add up to more than any buffer holds. Tokens past num_tokens are
+  // dropped; where there are some, a second pass takes pages for the tokens that are left.
+  long long tokens_before, pages_before, pages_asked = 0;
+  for (bool cut = false;; cut = true) {
+    tokens_before = pages_before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kPlanThreads) {
+      const int b = b0 + tid;
+      int held = 0, fresh = 0;
+      if (b < p.B) {
+        held = clamp_len(p.kv_lens[b], kMaxLength);
+        fresh = cut ? s_cu[b + 1] - s_cu[b] : clamp_len(p.new_lens[b], kMaxLength - 1);
       }
+      long long tok = fresh, pg = pages_of(held + fresh) - pages_of(held);
+      const long long my_tok = tok, my_pg = pg;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const long long a = __shfl_up_sync(0xffffffffu, tok, d);
+        const long long c = __shfl_up_sync(0xffffffffu, pg, d);
+        if (lane >= d) {
+          tok += a;
+          pg += c;
+        }
+      }
+      if (lane == 31) {
+        s_warp[0][warp] = tok;
+        s_warp[1][warp] = pg;
+      }
+      __syncthreads();
+      long long wt = 0, wp = 0, all_t = 0, all_p = 0;
+#pragma unroll
+      for (int w = 0; w < kPlanThreads / 32; ++w) {
+        if (w < warp) {
+          wt += s_warp[0][w];
+          wp += s_warp[1][w];
+        }
+        all_t += s_warp[0][w];
+        all_p += s_warp[1][w];
+      }
+      if (b < p.B) {
+        const long long t0 = tokens_before + wt + tok - my_tok;
+        s_cu[b] = static_cast<int32_t>(min(t0, static_cast<long long>(p.num_tokens)));
+        s_page[b] = static_cast<int32_t>(min(pages_before + wp + pg - my_pg, 0x7fffffffll));
+      }
+      tokens_before += all_t;
+      pages_before += all_p;
+      __syncthreads();
     }
-    if (lane == 31) {
-      s_warp[0][warp] = tok;
-      s_warp[1][warp] = pg;
+    if (tid == 0) {
+      s_cu[p.B] = static_cast<int32_t>(min(tokens_before, static_cast<long long>(p.num_tokens)));
+      s_page[p.B] = static_cast<int32_t>(min(pages_before, 0x7fffffffll));
     }
     __syncthreads();
-    long long wt = 0, wp = 0, all_t = 0, all_p = 0;
-#pragma unroll
-    for (int w = 0; w < kPlanThreads / 32; ++w) {
-      if (w < warp) {
-        wt += s_warp[0][w];
-        wp += s_warp[1][w];
-      }
-      all_t += s_warp[0][w];
-      all_p += s_warp[1][w];
-    }
-    if (b < p.B) {
-      const long long t0 = tokens_before + wt + tok - my_tok;
-      s_cu[b] = static_cast<int32_t>(min(t0, static_cast<long long>(p.num_tokens)));
-      s_page[b] = static_cast<int32_t>(min(pages_before + wp + pg - my_pg, 0x7fffffffll));
-    }
-    tokens_before += all_t;
-    pages_before += all_p;
-    __syncthreads();
+    if (!cut) pages_asked = pages_before;
+    if (cut || tokens_before <= p.num_tokens) break;
+    if (tid == 0) s_bad = 1;
   }
-  if (tid == 0) {
-    s_cu[p.B] = static_cast<int32_t>(min(tokens_before, static_cast<long long>(p.num_tokens)));
-    s_page[p.B] = static_cast<int32_t>(min(pages_before, 0x7fffffffll));
-  }
-  __syncthreads();
   const int n_tokens = s_cu[p.B], n_pages = s_page[p.B];
   if (tid == 0 && blockIdx.x == 0) {
-    *p.pages_used = n_pages;
-    if (p.status && (s_bad || tokens_before > p.num_tokens)) atomicCAS(p.status, 0, LF_DEV_BAD_LENGTHS);
+    // (Where pages run out: what the lengths ask for, dropped tokens included.)
+    *p.pages_used = n_pages > p.n_free ? static_cast<int32_t>(min(pages_asked, 0x7fffffffll)) : n_pages;
+    if (p.status && s_bad) atomicCAS(p.status, 0, LF_DEV_BAD_LENGTHS);
     if (p.status && n_pages > p.n_free) atomicCAS(p.status, 0, LF_DEV_BAD_PAGE);
   }
 
@@ -126,8 +134,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(const PlanPara
     if (b < p.B)
       p.seq_lens[b] = min(max(p.kv_lens[b], 0), kMaxLength) + (s_cu[b + 1] - s_cu[b]);
   }
-  for (int64_t at = start; at < n_pages; at += step) {  // (nonsense lengths: up to 2^31 - 1)
-    const int e = static_cast<int>(at);
+  for (int e = start; e < n_pages; e += step) {  // (no more than tokens: 2^30)
     const int b = owner(s_page, e);
     const int c = pages_of(min(max(p.kv_lens[b], 0), kMaxLength)) + (e - s_page[b]);
     if (c < p.bt_blocks) p.table[b * p.bt_stride + c] = e < p.n_free ? p.free_pages[e] : -1;

@@ -325,8 +325,9 @@ def plan_pages(kv_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.
     ``free_pages``, requests in order, and are written into its row in place. A row may begin with
     pages that other requests hold too (a shared prefix), as long as the last one is full.
     ``num_tokens`` is the number of rows of the packed batch: rows past the last token get slot -1
-    and position 0. If pages run out, ``pages_used`` says how many were needed, and what got none
-    has entry and slot -1 (reported in ``status``)."""
+    and position 0. If pages run out, ``pages_used`` says how many the lengths ask for, and what got
+    none has entry and slot -1 (reported in ``status``). Tokens past ``num_tokens`` are dropped and
+    take no page: ``cu_seqlens`` and ``seq_lens`` count the others (reported too)."""
     return PagePlan(*_native.host().plan_pages(kv_lens, new_lens, free_pages, block_table, page_size,
                                                num_tokens, status))
 

@@ -203,3 +203,37 @@ def test_shared_prefix_takes_the_smallest_length_for_none():
     for least in (-1, -2 ** 31, -2 ** 31 + 70):
         got = F.shared_prefix_decode_attention(q, kp, kp, table, ints([70, least]), 64)
         assert (got[1] == 0).all() and got[0].abs().amax() > 0, least
+
+
+# -- page plans of more tokens than the batch has rows ------------------------------------------------------
+@pytest.mark.parametrize("kv,new,num_tokens,P", [
+    ([0, 0], [5, 20], 8, 4), ([3, 6, 0], [9, 30, 7], 20, 4), ([0, 5, 1], [16, 40, 3], 16, 16), ([7], [100], 0, 8),
+    ([i % 9 for i in range(1300)], [i % 7 for i in range(1300)], 1000, 4),
+])
+def test_plan_pages_takes_pages_for_the_tokens_that_fit(kv, new, num_tokens, P):
+    """Tokens past num_tokens are dropped, and with them their pages: the free list, the table and the lengths tell
+    the same story."""
+    kept, left = [], num_tokens
+    for n in new:
+        kept.append(min(n, left))
+        left -= kept[-1]
+    table = torch.full((len(kv), 40), -1, dtype=torch.int32, device="cuda")
+    pages, at = list(range(1000, 1000 + sum(new) + len(kv))), 0
+    want = [[-1] * 40 for _ in kv]
+    for b, h in enumerate(kv):
+        have = -(-h // P)
+        table[b, :have] = torch.arange(have, device="cuda").int()
+        want[b][:have] = range(have)
+    free = pages[:]
+    for b, (h, n) in enumerate(zip(kv, kept)):
+        for c in range(-(-h // P), -(-(h + n) // P)):
+            want[b][c] = free[at]
+            at += 1
+    st = F.new_status("cuda")
+    plan = F.plan_pages(ints(kv), ints(new), ints(free), table, page_size=P, num_tokens=num_tokens, status=st)
+    assert int(st.item()) == BAD_LENGTHS
+    assert plan.seq_lens.tolist() == [h + n for h, n in zip(kv, kept)]
+    assert plan.cu_seqlens.tolist() == [sum(kept[:b]) for b in range(len(kv) + 1)]
+    assert plan.pages_used.tolist() == [at]
+    assert table.tolist() == want
+    assert (plan.slots >= 0).all()
