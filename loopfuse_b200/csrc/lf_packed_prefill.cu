@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(kOrderThreads)
                         const int n_slots) {
   extern __shared__ int32_t s_first[];  // [B + 1] first tile of each request
   __shared__ int32_t s_level[kOrderLevels];
-  __shared__ int32_t s_warp[kOrderThreads / 32];
+  __shared__ long long s_warp[kOrderThreads / 32];
   __shared__ unsigned long long s_blocks;
   __shared__ int32_t s_longest, s_parts, s_cut;
   __shared__ int32_t s_slice[kOrderChoices], s_long[kOrderChoices], s_long_blocks[kOrderChoices];
@@ -52,28 +52,30 @@ __global__ void __launch_bounds__(kOrderThreads)
   }
   __syncthreads();
   pdl_wait();
-  // Exclusive sums over the threads of the CTA; `all` gets the total.
-  auto scan = [&](int v, int* all) {
-    int incl = v;
+  // Exclusive sums over the threads of the CTA; `all` gets the total. (In 64 bits: offsets out of order can let
+  // every request hold the whole batch.)
+  auto scan = [&](int v, long long* all) {
+    long long incl = v;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, incl, d);
+      const long long x = __shfl_up_sync(0xffffffffu, incl, d);
       if (lane >= d) incl += x;
     }
     if (lane == 31) s_warp[warp] = incl;
     __syncthreads();
-    int warps = s_warp[lane];  // (as many warps as lanes)
-    const int own = __shfl_sync(0xffffffffu, warps, warp);
+    long long warps = s_warp[lane];  // (as many warps as lanes)
+    const long long own = __shfl_sync(0xffffffffu, warps, warp);
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, warps, d);
+      const long long x = __shfl_up_sync(0xffffffffu, warps, d);
       if (lane >= d) warps += x;
     }
     __syncthreads();
     *all = __shfl_sync(0xffffffffu, warps, 31);
     return __shfl_sync(0xffffffffu, warps, warp) - own + incl - v;
   };
-  int base = 0;
+  // (Tiles past n_tiles, which requests in order do not have, are left out.)
+  long long base = 0;
   for (int b0 = 0; b0 < p.B; b0 += kOrderThreads) {
     const int b = b0 + tid;
     int tiles = 0;
@@ -81,13 +83,13 @@ __global__ void __launch_bounds__(kOrderThreads)
       const PackedRequest r = packed_request<KIND>(p, b);
       tiles = (r.n + p.tq - 1) / p.tq;
     }
-    int all;
-    const int first = scan(tiles, &all);
-    if (b < p.B) s_first[b] = base + first;
+    long long all;
+    const long long first = scan(tiles, &all);
+    if (b < p.B) s_first[b] = static_cast<int32_t>(min(base + first, static_cast<long long>(p.n_tiles)));
     base += all;
   }
   __syncthreads();
-  const int n = min(base, p.n_tiles);
+  const int n = static_cast<int>(min(base, static_cast<long long>(p.n_tiles)));
   auto item_of = [&](int e) {
     int lo = 0, hi = p.B - 1;
     while (lo < hi) {
@@ -180,8 +182,8 @@ __global__ void __launch_bounds__(kOrderThreads)
     atomicAdd(&s_level[level_of((blocks + parts - 1) / parts)], parts);
   }
   __syncthreads();
-  int n_items;
-  const int mine = scan(s_level[tid], &n_items);
+  long long n_items;
+  const int mine = static_cast<int>(scan(s_level[tid], &n_items));
   s_level[tid] = mine;
   __syncthreads();
   for (int e = tid; e < n; e += kOrderThreads) {
@@ -205,7 +207,7 @@ __global__ void __launch_bounds__(kOrderThreads)
       for (int h = 0; h < p.Hkv; ++h) p.list[2 + it.counter * p.Hkv + h] = 0;
   }
   if (tid == 0) {
-    p.list[0] = min(n_items, max_items);
+    p.list[0] = static_cast<uint32_t>(min(n_items, static_cast<long long>(max_items)));
     p.list[1] = 0;
   }
 }

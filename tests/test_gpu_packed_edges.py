@@ -237,3 +237,19 @@ def test_plan_pages_takes_pages_for_the_tokens_that_fit(kv, new, num_tokens, P):
     assert plan.pages_used.tolist() == [at]
     assert table.tolist() == want
     assert (plan.slots >= 0).all()
+
+
+# -- offsets out of order --------------------------------------------------------------------------------
+def test_offsets_out_of_order_in_a_large_batch():
+    """4096 requests that each claim all 524289 tokens: their tiles together pass 31 bits. No key anywhere, so every row
+    that a tile holds is written as zeros. (Rows of q and out overlap: nothing reads the one, and zeros on zeros are
+    zeros.)"""
+    T, G, D = 524289, 128, 64
+    flat = torch.full((8 * (T - 1) + G * D,), 7.0, dtype=torch.bfloat16, device="cuda")
+    out = flat.as_strided((T, G, D), (8, D, 1))
+    q = torch.zeros_like(flat).as_strided((T, G, D), (8, D, 1))
+    k = torch.empty(0, 1, D, dtype=torch.bfloat16, device="cuda")
+    cu = ints([0, T] * 4096 + [0])
+    got = F.packed_prefill_attention(q, k, k, cu, cu_seqlens_k=torch.zeros_like(cu), out=out)
+    assert got.data_ptr() == out.data_ptr()
+    assert (flat == 0).all()
