@@ -253,3 +253,53 @@ def test_offsets_out_of_order_in_a_large_batch():
     got = F.packed_prefill_attention(q, k, k, cu, cu_seqlens_k=torch.zeros_like(cu), out=out)
     assert got.data_ptr() == out.data_ptr()
     assert (flat == 0).all()
+
+
+# -- pools whose pages are not evenly spaced ---------------------------------------------------------------
+def pool_pair(layout, n, P, Hkv, D):
+    """K and V pools as views [n, P, Hkv, D]: halves of each page of one tensor, heads in front of the slots, rows of a
+    wider tensor, or pages with a gap between them."""
+    if layout == "halves":
+        both = torch.zeros(n, 2, P, Hkv, D, dtype=torch.bfloat16, device="cuda")
+        return both[:, 0], both[:, 1]
+    if layout == "heads first":
+        return [torch.zeros(n, Hkv, P, D, dtype=torch.bfloat16, device="cuda").transpose(1, 2) for _ in "kv"]
+    if layout == "one row":
+        both = torch.zeros(n, P, 2 * Hkv, D, dtype=torch.bfloat16, device="cuda")
+        return both[:, :, :Hkv], both[:, :, Hkv:]
+    return [torch.zeros(n, P + 3, Hkv, D, dtype=torch.bfloat16, device="cuda")[:, :P] for _ in "kv"]
+
+
+@pytest.mark.parametrize("layout", ["halves", "heads first", "one row", "gap"])
+@pytest.mark.parametrize("P", [1, 4, 12, 16, 24, 64, 128])
+@pytest.mark.parametrize("D", [64, 128])
+def test_pools_of_any_strides_hold_the_same(layout, P, D):
+    """Append, packed prefill and shared-prefix decode on them are those on contiguous pools, to the bit."""
+    g = torch.Generator(device="cuda").manual_seed(P)
+    Hkv, G, lens, keys = 2, 3, [40, 1, 150], [300, 129, 150]
+    prefix = 128 // P * P
+    blocks = [-(-m // P) for m in keys]
+    n = sum(blocks) + 2
+    table = torch.zeros(3, max(blocks), dtype=torch.int32, device="cuda")
+    ids = torch.randperm(n, generator=g, device="cuda").int()
+    for b, m in enumerate(blocks):
+        table[b, :m] = ids[sum(blocks[:b]):sum(blocks[:b + 1])]
+    T = n * P
+    k, v = normal(g, T, Hkv, D), normal(g, T, Hkv, D)
+    slots = torch.randperm(T, generator=g, device="cuda").int()
+    q, q1 = normal(g, sum(lens), Hkv * G, D), normal(g, 3, Hkv, G, D)
+    results = []
+    for pools in ([torch.zeros(n, P, Hkv, D, dtype=torch.bfloat16, device="cuda") for _ in "kv"],
+                  pool_pair(layout, n, P, Hkv, D)):
+        st = F.new_status("cuda")
+        F.kv_append_packed(k, v, *pools, slots, status=st)
+        a = F.packed_prefill_attention(q, *pools, offsets(lens), block_table=table, seq_lens=ints(keys), scale=0.125,
+                                       status=st)
+        b = F.packed_prefill_attention(q, *pools, offsets(lens), block_table=table, seq_lens=ints(keys), scale=0.125,
+                                       mask_kind=S.MASK_CAUSAL_WINDOW, window=70, mods=softcap(30.0), status=st)
+        shared = table.clone()
+        shared[:, :prefix // P] = shared[0, :prefix // P]
+        c = F.shared_prefix_decode_attention(q1, *pools, shared, ints(keys), prefix, scale=0.125, status=st)
+        assert int(st.item()) == 0
+        results.append([x.contiguous() for x in pools] + [a, b, c])
+    assert all(torch.equal(x, y) for x, y in zip(*results))
