@@ -61,7 +61,8 @@ typedef enum {
 /* Codes the kernels write to the `status` device word (0 = nothing happened). */
 #define LF_DEV_OK 0
 #define LF_DEV_TIMEOUT 1        /* a bounded mbarrier wait gave up; low bits say which      */
-#define LF_DEV_BAD_PAGE 2       /* block_table entry outside [0, n_pages)                   */
+#define LF_DEV_BAD_PAGE 2       /* block_table entry or slot outside the pool, a position that the
+                                   table has no entry for, or no free page left             */
 #define LF_DEV_BOUNDS 3         /* debug-bounds build only: an index left its range; bits 8..
                                    say where. The access was skipped or clamped.            */
 

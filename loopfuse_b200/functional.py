@@ -56,7 +56,8 @@ def check_status(status: torch.Tensor, what: str = "kernel") -> None:
     if (code & 0xFF) == _DEV_TIMEOUT:
         raise RuntimeError(f"{what}: a bounded device-side wait ran out (site {code >> 8})")
     if (code & 0xFF) == _DEV_BAD_PAGE:
-        raise RuntimeError(f"{what}: block_table holds a page id outside the pool")
+        raise RuntimeError(f"{what}: block_table holds a page id outside the pool or has no entry for a "
+                           "position, or the free pages ran out")
     if (code & 0xFF) == _DEV_BAD_LENGTHS:
         raise RuntimeError(f"{what}: a request's length is negative or above max_seq_len, or the batch "
                            "has more tokens than num_tokens")

@@ -303,3 +303,13 @@ def test_pools_of_any_strides_hold_the_same(layout, P, D):
         assert int(st.item()) == 0
         results.append([x.contiguous() for x in pools] + [a, b, c])
     assert all(torch.equal(x, y) for x, y in zip(*results))
+
+
+# -- errors ---------------------------------------------------------------------------------------------
+def test_a_pool_that_runs_out_is_named_as_one():
+    st = F.new_status("cuda")
+    table = torch.full((1, 4), -1, dtype=torch.int32, device="cuda")
+    plan = F.plan_pages(ints([0]), ints([9]), ints([5, 6]), table, page_size=4, num_tokens=9, status=st)
+    assert plan.pages_used.tolist() == [3] and table.tolist() == [[5, 6, -1, -1]]
+    with pytest.raises(RuntimeError, match="plan_pages: .*page id.*ran out"):
+        F.check_status(st, "plan_pages")
