@@ -87,7 +87,7 @@ struct PackedParams {
   float c2;                   // logit in the log2 domain = score * c2; > 0
   float m_first;              // a row's first reference: -inf, or 0 where no logit is far from it
   int32_t bt_blocks, page_size, page_shift, n_pages;
-  int32_t box;                // keys per copy of a paged operand: they lie in one page
+  int32_t box, box_shift;     // keys per copy of a paged operand, a power of two: they lie in one page
   int32_t page_groups;        // groups of 8 slots per page, where a copy can move several (see packed_pool_map)
   int32_t n_tiles;            // tiles of a kv head (no list: an upper bound)
   FastDiv div_chunk;          // heads of a chunk of kv heads (see the launch); prefix: kv heads
@@ -163,13 +163,9 @@ __device__ __forceinline__ PackedRequest packed_request(const PackedParams& p, i
   return r;
 }
 
-// First key that any row of an item sees, and of the boxes (runs of keys in one page, fetched by one copy) the first
-// that holds such a key. The pages in front of it may be anybody's by now: their entries are not looked at.
+// First key that any row of an item sees.
 __device__ __forceinline__ int first_key(const PackedParams& p, const PackedItem& it) {
   return p.mask_kind == LF_MASK_CAUSAL_WINDOW ? max(0, it.pos - (p.window - 1)) : 0;
-}
-__device__ __forceinline__ int first_box(const PackedParams& p, const PackedItem& it) {
-  return max(it.lo * (kPackedKeys / p.box), first_key(p, it) / p.box);
 }
 
 // Tile `tile` of request r as one item.
@@ -523,17 +519,20 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
         // Table entries of the copies ("boxes"), 32 at a time, a box per lane; the next 32 are requested before
         // these are used. (Block by block the look-up took 800 clocks of each.)
         const int32_t* table = p.table + static_cast<int64_t>(it.k_from) * p.bt_stride;
-        const int all_boxes = kPages ? (it.m + p.box - 1) / p.box : 0;  // that hold a key
-        const int box0 = KIND == kPackedPaged ? first_box(p, it) : lo * boxes;  // the first that is fetched
-        int window = kPages ? box0 / 32 : 0;
+        const int box_end = kPages ? min((it.m + p.box - 1) >> p.box_shift, hi * boxes) : 0;  // that hold a key
+        int window = kPages ? lo * boxes / 32 : 0;
         int32_t page = 0, page_next = 0;
+        // Boxes in front of all keys that a row sees (the first block may have some): their pages may be anybody's by
+        // now, so their entries are not looked at, and the copy reads past the last page, which is zeros.
+        const int box0 = KIND == kPackedPaged ? first_key(p, it) >> p.box_shift : 0;
         auto request = [&](int w) -> int32_t {
           const int n = w * 32 + lane;
-          if (n < box0 || n >= all_boxes || n >= hi * boxes) return 0;
+          if (n < box0 || n >= box_end) return 0;
           const int at = page_of(n * p.box);
           return LF_BOUNDS(at >= 0 && at < p.bt_blocks, p.status, 70) ? table[at] : 0;
         };
-        auto checked = [&](int32_t pg) -> int32_t {
+        auto checked = [&](int32_t pg, int w) -> int32_t {
+          if (KIND == kPackedPaged && w * 32 + lane < box0) return p.n_pages;
           if (pg >= 0 && pg < p.n_pages) return pg;
           if (p.status) atomicExch(p.status, LF_DEV_BAD_PAGE);
           return 0;
@@ -541,7 +540,7 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
         if constexpr (kPages) {
           page = request(window);
           page_next = request(window + 1);
-          page = checked(page);
+          page = checked(page, window);
         }
         for (int j = lo; j < hi; ++j, ++g) {
           const int stage = g % kStages;
@@ -556,17 +555,16 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
               tma_load_5d(dst, map, &full[stage], 0, it.k_from + j * kPackedKeys, 0, it.hkv, 0);
             }
           } else {
-            // (What a window leaves out of the first block, and the rest of the last one, is not fetched.)
             const int n0 = j * boxes;
-            const int dead = max(box0 - n0, 0), live = min(boxes, all_boxes - n0);
+            const int live = min(boxes, box_end - n0);  // (the rest of the last block is not fetched)
             if (run)
-              mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>((live - dead) * p.box) * 128 * kBlocksD);
+              mbar_arrive_expect_tx(&full[stage], static_cast<uint32_t>(live * p.box) * 128 * kBlocksD);
             // Four boxes at a time: places by shuffle, then the copies in one go. (They lie in one window: 32 is a
             // multiple of them, or they of 32.)
-            for (int r0 = dead & ~3; r0 < live; r0 += 4) {
+            for (int r0 = 0; r0 < live; r0 += 4) {
               if ((n0 + r0) / 32 != window) {
                 ++window;
-                page = checked(page_next);
+                page = checked(page_next, window);
                 page_next = request(window + 1);
               }
               int pg[4], slot[4];
@@ -580,7 +578,7 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                   const int row = (r0 + u) * p.box;
-                  if (r0 + u < dead || r0 + u >= live) continue;
+                  if (r0 + u >= live) continue;
                   if (p.page_groups > 0) {  // 8-row groups of the whole pool are evenly spaced
                     tma_load_5d(dst + row * (128 * kBlocksD), map, &full[stage], 0, 0, 0, it.hkv,
                                 pg[u] * p.page_groups + (slot[u] >> 3));
@@ -725,27 +723,17 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
         const uint32_t s_addr = s_base + (g & 1) * 64;
         wait(&bars->s_full[g & 1], (g >> 1) & 1, 83);
         tc_fence_after();
-        // Columns of the block that were not fetched, in front of an item's first box.
-        int dead = 0;
-        if constexpr (KIND == kPackedPaged) {
-          if (k == 0 && p.mask_kind == LF_MASK_CAUSAL_WINDOW)
-            dead = warp_uniform(first_box(p, bars->item[i % kItemSlots]) * p.box - c0);
-        }
-        if (c0 + kPackedKeys > m || dead > 0) {
-          // V rows past the last key, and those that were not fetched, become zeros (the stage's next fill waits for
-          // this block's PV).
+        if (c0 + kPackedKeys > m) {
+          // V rows past the last key become zeros (the stage's next fill waits for this block's PV).
           const int stage = g % kStages;
           wait(&bars->v_full[stage], (g / kStages) & 1, 84);
           unsigned char* v = sV + stage * Shape::kTileBytes;
-          auto clear = [&](int from, int to) {
-            for (int e = from * 8 + row; e < to * 8; e += 128)
+          const int first = m - c0;  // (0 < first < 64)
+          for (int e = first * 8 + row; e < kPackedKeys * 8; e += 128)
 #pragma unroll
-              for (int kb = 0; kb < kBlocksD; ++kb)
-                *reinterpret_cast<uint4*>(v + kb * kHalf + (e >> 6) * kGroup + (e & 63) * 16) =
-                    make_uint4(0, 0, 0, 0);
-          };
-          clear(min(m - c0, kPackedKeys), kPackedKeys);  // (m > c0)
-          clear(0, dead);
+            for (int kb = 0; kb < kBlocksD; ++kb)
+              *reinterpret_cast<uint4*>(v + kb * kHalf + (e >> 6) * kGroup + (e & 63) * 16) =
+                  make_uint4(0, 0, 0, 0);
           fence_proxy_async_smem();
         }
         if (!idle) {
@@ -757,14 +745,14 @@ __device__ __forceinline__ void packed_tiles(const CUtensorMap& tmap_q, const CU
           if constexpr (SOFTCAP) {
             // tanh(x), x = raw * a: x (1 - x^2 / 3) up to |x| = 0.125 (error below 4.1e-6), its series to
             // x^7 up to 0.4 (below 6e-6), the unit's approximation beyond. The warp takes the form that its largest
-            // score asks for; columns past the last key or not fetched (other requests' rows, or whatever was in
-            // the stage) have no say in it, nor have rows that see no key.
-            if (c0 + kPackedKeys > m || dead > 0) {
+            // score asks for; columns past the last key (other requests' rows, or whatever was in the stage) have
+            // no say in it, nor have rows that see no key.
+            if (c0 + kPackedKeys > m) {
 #pragma unroll
               for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int e = 0; e < 32; ++e)
-                  if (c * 32 + e >= m - c0 || c * 32 + e < dead) sr[c][e] = 0u;
+                  if (c * 32 + e >= m - c0) sr[c][e] = 0u;
             }
             const bool sees = valid && c_hi >= 0;
             float mx[4] = {0.f, 0.f, 0.f, 0.f};
@@ -1087,6 +1075,7 @@ inline int packed_pool_maps(CUtensorMap* mk, CUtensorMap* mv, const void* k, con
   p->page_groups = even ? page_size / 8 : 0;
   p->box = packed_box(page_size);
   if (!even && p->box > 8) p->box = 8;
+  p->box_shift = packed_page_shift(p->box);
   for (int i = 0; i < 2; ++i) {
     const int64_t* st = i ? v_st : k_st;
     TileMapSpec spec;
