@@ -447,28 +447,34 @@ int lf_kv_append_bf16(const LfKvAppendArgs* args, void* stream);
 int lf_plan_pages(const LfPagePlanArgs* args, void* stream);
 
 /* The store that goes with it: row t of k_new / v_new to slot slots[t] of the pools (bit-exact). A
- * slot outside the pool is reported as LF_DEV_BAD_PAGE and not written. Of rows with the same slot
- * one wins. */
+ * slot outside the pool is reported as LF_DEV_BAD_PAGE and not written. Slots must differ: rows with
+ * the same one may end up mixed, in pieces of 16 bytes. */
 int lf_kv_append_packed_bf16(const LfKvAppendPackedArgs* args, void* stream);
 
 /* Attention of packed requests of different lengths, one launch (or two: batches of many or long tiles
  * are ordered by length first, and long tiles cut, which takes the workspace; requests of up to 2048
  * keys are never cut, and have the same result in every batch). The mask is per request and
  * aligned at its end; a row that sees no key is zeros (lf_prefill_bf16 gives NaN there). Offsets that
- * are out of order or outside the tensors are cut to them; rows that no request holds are not written.
+ * are out of order or outside the tensors are cut to them, kv_lens to what a row of the table holds, neither
+ * with a report; rows that no request holds are not written. Table entries are read, and have to name
+ * pages, from the first key that a request's queries see to its last. Batches of more than 8192 requests
+ * are neither ordered nor cut, and slow.
  * The mod chain may hold multipliers, or the softcap form (MUL|DIV)* TANH (MUL|DIV)*, with a product of
  * scale and multipliers that is not negative; anything else is LF_ERR_UNSUPPORTED. Keys and values of
  * other requests, or of a page's unused slots, never reach a result, whatever they hold; within a
- * request, a value row that a query does not see must be finite (its weight is zero). */
+ * request, a value row that a query does not see must be finite (its weight is zero). Weights enter the
+ * product with the values as one bf16 each, as two where a tile's first row sees fewer than 16 keys. */
 int lf_packed_prefill_bf16(const LfPackedArgs* args, void* stream);
 /* Workspace of a call with these sizes on the current device; 0 = none. */
 size_t lf_packed_workspace_bytes(const LfPackedArgs* args);
 
 /* Decode attention of requests that share their first prefix_len tokens, with the pages of the shared
  * ones read once for the whole batch: equal to lf_decode_paged_bf16 on each request with a table whose
- * first entries are those of row 0, up to rounding. Score functions as for lf_packed_prefill_bf16. A
- * request of length 0 gets zeros. The page that holds key prefix_len may hold shared keys too: they are
- * read through row 0, the others through the request's own row. */
+ * first entries are those of row 0, up to rounding (weights of shared keys are one bf16, which that call,
+ * and the requests' own keys here, keep as two); the last bits may change with the batch. Score functions
+ * as for lf_packed_prefill_bf16. A request of length 0 gets zeros. Values of shared keys must be finite.
+ * The page that holds key prefix_len may hold shared keys too: they are read through row 0, the others
+ * through the request's own row. B up to 65535. */
 int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* args, void* stream);
 size_t lf_shared_prefix_workspace_bytes(int32_t B, int32_t Hkv, int32_t G, int32_t D, int32_t prefix_len,
                                         int32_t max_seq_len);

@@ -21,11 +21,12 @@ __global__ void __launch_bounds__(kPackedThreads, 2)
 // with the requests one after the other the last one's longest tile would start when the rest is nearly
 // done), and those that are long next to what a CTA has to do in all cut into slices of their keys (a
 // few new tokens behind a long context are a few tiles). One CTA; among items of one length the order is
-// arbitrary, and no result depends on it. 6 us, 9 where slices are compared, which the tiles wait for: 32 chunks of up
-// to 512 tokens behind up to 4096 take 88 us with it.
+// arbitrary, and no result depends on it. 7 us, 9 where slices are compared, which the tiles wait for: 32 chunks of up
+// to 512 tokens behind up to 4096 take 90 us with it.
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderLevels = 1024;
-constexpr int kOrderRequests = 8192;  // in shared memory; larger batches keep the requests' order
+constexpr int kOrderRequests = 8192;  // in shared memory; larger batches keep the requests' order, are not cut, and
+                                      // each CTA looks its tile up in the offsets, 32 requests at a time
 constexpr int kWholeBlocks = 32;      // tiles of up to 2048 keys are never cut: a prompt of that length has
                                       // the same result in every batch
 constexpr int kSliceBlocks = 16;      // at least, since a slice costs the store and the join of its rows

@@ -8,10 +8,11 @@
 //                row are dealt out to the warps in equal runs, as in decode: bound by HBM.
 //   join         join_kernel: out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the parts of both.
 //
-// The first two are CTAs of one launch, so the tensor pipe works on the shared part while the own keys stream
-// in. 64 requests, 2048 shared keys and up to 1024 own, 32 heads on 8: 38 us (bytes once at HBM's rate 12.6); 128
-// requests, 32768 shared and up to 2048 own: 136 us (53.6), where a paged decode of the same cache reads the
-// prefix 128 times.
+// The first two are CTAs of one launch: where the slices of the prefix leave places, the own keys stream in beside
+// them, and otherwise as they end. 64 requests, 2048 shared keys and up to 1024 own, 32 heads on 8: 128 prefix CTAs
+// on 148 SMs, 38 us (bytes once at HBM's rate 12.6). 128 requests, 32768 shared and up to 2048 own: 288 prefix CTAs
+// take nearly every place, and the own keys follow them; 136 us (53.6), where a paged decode of the same cache reads
+// the prefix 128 times.
 #include "lf_packed.cuh"
 
 #include <algorithm>
@@ -275,7 +276,7 @@ __device__ __forceinline__ void own_part(const OwnParams& p, int w, int n_warps)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float s = sc[s8][e];
-        if constexpr (SOFTCAP) s = tanh_approx(s * p.a);
+        if constexpr (SOFTCAP) s = tanh_approx(s * p.a);  // (the unit's, within 2^-11, as in decode)
         s *= p.c2;
         if (now.t + 8 * s8 + 2 * c + e >= now.end) s = -INFINITY;
         sc[s8][e] = s;
@@ -389,8 +390,8 @@ struct JoinParams {
 
 // One warp per output row. Lane s holds (reference, sum) of part s; the rows of the parts stream in with
 // their weights broadcast. Parts that hold no key of the row have sum 0 and are left out (what their
-// accumulators hold is of no value); a row without a key is zeros. Bound by the latency of its loads, 5 to 8
-// us for 2048 and 4096 rows.
+// accumulators hold is of no value); a row without a key is zeros. Bound by the latency of its loads, with cold caches
+// 5 us for 128 rows and 8 for 2048 and 4096.
 template <int D>
 __global__ void __launch_bounds__(128) join_kernel(const JoinParams p) {
   constexpr int EPL = D / 32;

@@ -337,8 +337,8 @@ def kv_append_packed(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Ten
                      v_pool: torch.Tensor, slots: torch.Tensor, *,
                      status: Optional[torch.Tensor] = None) -> None:
     """Write the K/V rows ``[T, Hkv, D]`` of a packed batch into a paged cache, in place: row ``t``
-    goes to ``pool[slots[t] // page_size, slots[t] % page_size]``; a negative slot is skipped. The
-    ``slots`` of ``plan_pages`` put every token where ``packed_prefill_attention`` and the paged
+    goes to ``pool[slots[t] // page_size, slots[t] % page_size]``; a negative slot is skipped, the others
+    must differ. The ``slots`` of ``plan_pages`` put every token where ``packed_prefill_attention`` and the paged
     decodes read it."""
     _native.host().kv_append_packed(k_new, v_new, k_pool, v_pool, slots, status)
 
@@ -363,8 +363,11 @@ def packed_prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
     The mask is per request and aligned at its end: query ``i`` of ``n`` sees key ``j`` of ``m`` up
     to ``i + m - n``, with ``MASK_CAUSAL_WINDOW`` the last ``window`` of those. A query that sees no
-    key gets zeros. ``mods`` may hold multipliers or a softcap chain (multipliers around one
-    tanh). No length is read by the host."""
+    key gets zeros; rows that no request holds (the padding of a batch) are not written, so in an
+    ``out`` that the call allocates they hold anything. ``mods`` may hold multipliers or a softcap
+    chain (multipliers around one tanh). No length is read by the host; one that the block table does
+    not hold is cut to what it holds. Pages that lie in front of every query's window may have been
+    given back."""
     return _native.host().packed_prefill(q, k, v, cu_seqlens, cu_seqlens_k, block_table, seq_lens, out,
                                          workspace, status, scale, mods, mask_kind, window)
 
