@@ -103,8 +103,7 @@ struct PackedParams {
 template <int D>
 struct PackedShape {
   static constexpr int kStages = D == 64 ? 4 : 2;  // of K, and of V: blocks in flight
-  // Behind the rings: a CTA has to stay above a third of the SM's shared memory, so that a third one does
-  // not wait for tensor memory.
+  // Behind the rings, unused: see packed_keeps_tensor_memory.
   static constexpr uint32_t kRest = 13 * 1024;
   static constexpr uint32_t kTmemColumns = 256;
   static constexpr uint32_t kQBlockBytes = kPackedRows * 128;  // [128][64] bf16
@@ -113,6 +112,16 @@ struct PackedShape {
   static constexpr size_t kSmem = 1024 /*barriers*/ + kRest +
                                   kQBlockBytes * (D / 64) + kStages * 2 * kTileBytes;
 };
+
+// An SM's 512 columns, by shared memory (of 228 KB): two of these CTAs, never three, and never one beside a CTA of
+// prefill_kernel that takes all the columns, whose smallest leaves less than 96256 bytes. (A CTA may wait for the
+// kernel before its own with its columns taken.)
+template <int D>
+constexpr bool packed_keeps_tensor_memory() {
+  constexpr size_t smem = PackedShape<D>::kSmem;
+  return smem >= 96256 && 2 * (smem + 1024) <= 233472 && 3 * (smem + 1024) > 233472;
+}
+static_assert(packed_keeps_tensor_memory<64>() && packed_keeps_tensor_memory<128>(), "tensor memory runs out on an SM");
 
 constexpr int kItemSlots = 4;
 

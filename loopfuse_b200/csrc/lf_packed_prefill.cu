@@ -267,8 +267,6 @@ template <int D, int KIND, bool SOFTCAP>
 static int launch_packed(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv,
                          const PackedParams& p, unsigned grid, cudaStream_t st) {
   using Shape = PackedShape<D>;
-  static_assert(2 * (Shape::kSmem + 1024) <= 233472 && 3 * (Shape::kSmem + 1024) > 233472,
-                "two CTAs per SM, for its 512 columns of tensor memory");
   static thread_local int configured_dev = -1;
   const auto kernel = packed_prefill_kernel<D, KIND, SOFTCAP>;
   const int rc = packed_configure(kernel, Shape::kSmem, &configured_dev);
