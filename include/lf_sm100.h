@@ -69,6 +69,8 @@ typedef enum {
 #define LF_DEV_BAD_LENGTHS 4    /* a request's length is negative or above the caller's bound, or the
                                    batch has more tokens than the caller's buffers; lengths are cut
                                    to what fits                                                 */
+#define LF_DEV_BAD_POSITION 5   /* a position that the rotation table has no row for: the nearest row
+                                   is taken                                                      */
 
 /* Mask kinds (what the capture layer deduces from loopfuse::causal_mask / sliding_mask). */
 #define LF_MASK_NONE 0
@@ -300,6 +302,89 @@ typedef struct {
   int32_t* status;
 } LfSharedPrefixArgs;
 
+/* 4-bit caches. A row of D columns (D in {64, 128}) of one kv head is a record of D / 2 + D / 8 bytes:
+ *   bytes 0 .. D/2        codes c in 0..15, two to a byte, in the order below
+ *   then D/32 bf16        a scale s for each group of 32 columns
+ *   then D/32 bf16        a midpoint z for each group
+ * and column d stands for z + s * (c - 8), z and s those of group d / 32. A row x is stored as
+ *   s = bf16((max - min) * (1/15)), z = bf16(min + 8 s), c = clamp(rint((x - z) * (1/s)) + 8, 0, 15),
+ * each step rounded once in fp32 (s = 0: c = 8), so that every column is at most 0.51 s + |z| 2^-8 away.
+ * Groups with a NaN or infinity, or a range above the largest fp32, stand for NaN or infinities.
+ * Order of the codes: those of a key's columns 32 g + 8 i .. + 7 are the 32-bit word g of piece i (of four,
+ * D/8 bytes each), those of a value's columns 32 g + 4 i .. + 3 the 16-bit word g of piece i (of eight, D/16
+ * bytes each), the first column in the lowest bits: a lane of a matrix instruction then finds its columns of
+ * all groups in one piece. Pools are [n_pages, page_size, Hkv, record] bytes; any strides that are
+ * multiples of 16 (D = 128) or 8 (D = 64) bytes, as the addresses are. */
+#define LF_RECORD4_BYTES(D) ((D) / 2 + (D) / 8)
+
+typedef struct {
+  const void* q;          /* bf16 [T, Hq, D], innermost stride 1; NULL = no queries */
+  const void* k;          /* bf16 [T, Hkv, D] */
+  const void* v;          /* bf16 [T, Hkv, D]: with pools only */
+  void* q_out;            /* bf16 [T, Hq, D]; may be q itself */
+  void* k_out;            /* bf16 [T, Hkv, D]; may be k itself. NULL with pools */
+  void* k_pool;           /* NULL = k_out. bits 16: bf16 [n_pages, page_size, Hkv, D]; bits 4: records */
+  void* v_pool;
+  const int32_t* slots;      /* with pools: [T] page * page_size + slot; negative = not stored */
+  const int32_t* positions;  /* [T] */
+  const float* table;        /* [n_positions, rot]: rot / 2 cosines, then rot / 2 sines of each position */
+  const void* q_weight;      /* [D] of the norm of each query head, bf16 or fp32; NULL = no norm */
+  const void* k_weight;
+  int32_t T, Hq, Hkv, D;     /* D in {64, 128} */
+  int32_t rot;               /* columns that are turned: a multiple of 16, up to D */
+  int32_t n_positions;
+  int32_t interleaved;       /* 0: column i turns with i + rot / 2. 1: column 2 i with 2 i + 1 */
+  int32_t q_weight_f32, k_weight_f32;
+  int32_t bits;              /* of the pools' values: 16 or 4 */
+  float eps;
+  int32_t page_size, n_pages;
+  int64_t table_stride;      /* elements between rows of the table, a multiple of 4 */
+  int64_t q_stride[2], k_stride[2], v_stride[2];  /* elements, of (token, head), multiples of 8 */
+  int64_t qo_stride[2], ko_stride[2];
+  int64_t kp_stride[3], vp_stride[3];  /* of (page, slot, kv head): elements, or bytes of 4-bit pools */
+  int32_t* status;
+} LfRotaryArgs;
+
+typedef struct {
+  const void* k_pool;     /* records [n_pages, page_size, Hkv, record] */
+  const void* v_pool;
+  void* k_out;            /* bf16 [T, Hkv, D], innermost stride 1 */
+  void* v_out;
+  const int32_t* block_table;  /* [B, bt_blocks] */
+  const int32_t* cu_k;         /* [B + 1]: rows [cu_k[b], cu_k[b + 1]) are the keys 0, 1, ... of request b */
+  int32_t B, T, Hkv, D;
+  int32_t page_size, n_pages, bt_blocks;
+  int64_t bt_stride;
+  int64_t kp_stride[3], vp_stride[3];  /* bytes, of (page, slot, kv head) */
+  int64_t ko_stride[2], vo_stride[2];  /* elements, of (token, kv head), multiples of 8 */
+  int32_t* status;
+} LfGather4Args;
+
+typedef struct {
+  const void* q;          /* bf16 [B, Hkv, G, D]: the G query heads that share a kv head */
+  const void* k;          /* records [n_pages, page_size, Hkv, record] */
+  const void* v;
+  void* out;              /* bf16 [B, Hkv, G, D] */
+  const int32_t* block_table;  /* [B, bt_blocks] */
+  const int32_t* seq_lens;     /* [B]: keys of each request; 0 = none */
+  int32_t B, Hkv, G, D;   /* D in {64, 128}; G <= 128 */
+  int64_t q_stride[3];    /* elements, of (b, kv head, g), multiples of 8 */
+  int64_t o_stride[3];    /* multiples of 4 */
+  int64_t k_stride[3];    /* bytes, of (page, slot, kv head) */
+  int64_t v_stride[3];
+  int64_t bt_stride;
+  int32_t bt_blocks, page_size, n_pages;
+  int32_t window;         /* only the last `window` keys of a request; 0 = all */
+  int32_t max_seq_len;    /* as in LfSharedPrefixArgs */
+  float scale;
+  int32_t n_mod;
+  int32_t mod_op[LF_MAX_MODS];
+  float mod_arg[LF_MAX_MODS];
+  void* workspace;        /* device, >= lf_decode_4bit_workspace_bytes(...), 16-byte aligned */
+  size_t workspace_bytes;
+  int32_t* status;
+} LfDecode4Args;
+
 typedef struct {
   int32_t abi_version;
   int32_t device;         /* current CUDA device ordinal */
@@ -478,6 +563,33 @@ size_t lf_packed_workspace_bytes(const LfPackedArgs* args);
 int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* args, void* stream);
 size_t lf_shared_prefix_workspace_bytes(int32_t B, int32_t Hkv, int32_t G, int32_t D, int32_t prefix_len,
                                         int32_t max_seq_len);
+
+/* Norm of each head of q and k, then the rotation of its position, in one pass; and, with pools, the append of
+ * the rotated keys and of the values:
+ *   x' = x * rsqrt(mean(x^2) + eps) * weight          (where a weight is given)
+ *   y_i = x'_i cos_i - x'_j sin_i,  y_j = x'_j cos_i + x'_i sin_i    (i, j: see `interleaved`; i < rot / 2)
+ * in fp32, with one rounding to bf16 or to 4 bits at the end; columns from `rot` on are not turned. Without a
+ * norm each product and sum of the rotation is rounded once in fp32, so that the stored bits are defined. A
+ * position outside the table is reported as LF_DEV_BAD_POSITION and takes the nearest row, a slot outside
+ * the pool as LF_DEV_BAD_PAGE and is not written; slots must differ. q_out may be q and k_out k (same strides);
+ * apart from that outputs must not overlap inputs. */
+int lf_rotary_bf16(const LfRotaryArgs* args, void* stream);
+
+/* Keys and values of requests from a 4-bit cache as packed bf16 rows: what lf_packed_prefill_bf16 takes as
+ * dense keys with the same cu_k. Row cu_k[b] + j is z + s (c - 8) of key j of request b, rounded once. Rows
+ * that no request has are not written; cu_k is cut to 0..T. A table entry that is missing or names no page is
+ * reported as LF_DEV_BAD_PAGE, and the row is zeros. */
+int lf_kv_gather_4bit(const LfGather4Args* args, void* stream);
+
+/* Decode attention of requests of different lengths over a 4-bit paged cache, one token per request: what
+ * lf_decode_paged_bf16 gives on the values that the records stand for, up to rounding (the weight of a key
+ * times its scale is rounded to bf16 once per group of columns). Score functions as for
+ * lf_packed_prefill_bf16. A request of length 0 gets zeros. With a window, table entries in front of its first
+ * key are not read. Values of keys that a request sees must be finite. B up to 65535. The last bits
+ * may change with the batch, never between two calls of the same one. */
+int lf_decode_4bit(const LfDecode4Args* args, void* stream);
+size_t lf_decode_4bit_workspace_bytes(int32_t B, int32_t Hkv, int32_t G, int32_t D, int32_t window,
+                                      int32_t max_seq_len);
 
 /* 1 when the library was built with -DLF_DEBUG_BOUNDS (python -m loopfuse_b200.build
  * --debug-bounds -> liblf_sm100_dbg.so): every index that a kernel forms for a plain global

@@ -22,6 +22,7 @@ EXPORTS = [
     "lf_prefill_row_bias_bf16", "lf_prefill_form",
     "lf_plan_pages", "lf_kv_append_packed_bf16", "lf_packed_prefill_bf16",
     "lf_packed_workspace_bytes", "lf_shared_prefix_decode_bf16", "lf_shared_prefix_workspace_bytes",
+    "lf_rotary_bf16", "lf_kv_gather_4bit", "lf_decode_4bit", "lf_decode_4bit_workspace_bytes",
 ]
 
 LF_STATIC_SCRATCH_BYTES = 8 << 20
@@ -130,6 +131,48 @@ class LfSharedPrefixArgs(C.Structure):
     ]
 
 
+class LfRotaryArgs(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p),
+        ("k_out", C.c_void_p), ("k_pool", C.c_void_p), ("v_pool", C.c_void_p), ("slots", C.c_void_p),
+        ("positions", C.c_void_p), ("table", C.c_void_p), ("q_weight", C.c_void_p),
+        ("k_weight", C.c_void_p),
+        ("T", C.c_int32), ("Hq", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32),
+        ("rot", C.c_int32), ("n_positions", C.c_int32), ("interleaved", C.c_int32),
+        ("q_weight_f32", C.c_int32), ("k_weight_f32", C.c_int32), ("bits", C.c_int32),
+        ("eps", C.c_float), ("page_size", C.c_int32), ("n_pages", C.c_int32),
+        ("table_stride", C.c_int64), ("q_stride", C.c_int64 * 2), ("k_stride", C.c_int64 * 2),
+        ("v_stride", C.c_int64 * 2), ("qo_stride", C.c_int64 * 2), ("ko_stride", C.c_int64 * 2),
+        ("kp_stride", C.c_int64 * 3), ("vp_stride", C.c_int64 * 3), ("status", C.c_void_p),
+    ]
+
+
+class LfGather4Args(C.Structure):
+    _fields_ = [
+        ("k_pool", C.c_void_p), ("v_pool", C.c_void_p), ("k_out", C.c_void_p), ("v_out", C.c_void_p),
+        ("block_table", C.c_void_p), ("cu_k", C.c_void_p),
+        ("B", C.c_int32), ("T", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32),
+        ("page_size", C.c_int32), ("n_pages", C.c_int32), ("bt_blocks", C.c_int32),
+        ("bt_stride", C.c_int64), ("kp_stride", C.c_int64 * 3), ("vp_stride", C.c_int64 * 3),
+        ("ko_stride", C.c_int64 * 2), ("vo_stride", C.c_int64 * 2), ("status", C.c_void_p),
+    ]
+
+
+class LfDecode4Args(C.Structure):
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("out", C.c_void_p),
+        ("block_table", C.c_void_p), ("seq_lens", C.c_void_p),
+        ("B", C.c_int32), ("Hkv", C.c_int32), ("G", C.c_int32), ("D", C.c_int32),
+        ("q_stride", C.c_int64 * 3), ("o_stride", C.c_int64 * 3), ("k_stride", C.c_int64 * 3),
+        ("v_stride", C.c_int64 * 3), ("bt_stride", C.c_int64),
+        ("bt_blocks", C.c_int32), ("page_size", C.c_int32), ("n_pages", C.c_int32),
+        ("window", C.c_int32), ("max_seq_len", C.c_int32),
+        ("scale", C.c_float), ("n_mod", C.c_int32),
+        ("mod_op", C.c_int32 * LF_MAX_MODS), ("mod_arg", C.c_float * LF_MAX_MODS),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("status", C.c_void_p),
+    ]
+
+
 class LfDeviceInfo(C.Structure):
     _fields_ = [
         ("abi_version", C.c_int32), ("device", C.c_int32), ("cc_major", C.c_int32),
@@ -206,7 +249,9 @@ def load() -> C.CDLL:
     for name, args in (("lf_plan_pages", LfPagePlanArgs),
                        ("lf_kv_append_packed_bf16", LfKvAppendPackedArgs),
                        ("lf_packed_prefill_bf16", LfPackedArgs),
-                       ("lf_shared_prefix_decode_bf16", LfSharedPrefixArgs)):
+                       ("lf_shared_prefix_decode_bf16", LfSharedPrefixArgs),
+                       ("lf_rotary_bf16", LfRotaryArgs), ("lf_kv_gather_4bit", LfGather4Args),
+                       ("lf_decode_4bit", LfDecode4Args)):
         fn = getattr(lib, name)
         fn.argtypes = [C.POINTER(args), C.c_void_p]
         fn.restype = C.c_int
@@ -214,6 +259,8 @@ def load() -> C.CDLL:
     lib.lf_packed_workspace_bytes.restype = C.c_size_t
     lib.lf_shared_prefix_workspace_bytes.argtypes = [C.c_int32] * 6
     lib.lf_shared_prefix_workspace_bytes.restype = C.c_size_t
+    lib.lf_decode_4bit_workspace_bytes.argtypes = [C.c_int32] * 6
+    lib.lf_decode_4bit_workspace_bytes.restype = C.c_size_t
     _lib = lib
     return lib
 

@@ -84,6 +84,10 @@ struct Lib {
   size_t (*packed_workspace)(const LfPackedArgs*) = nullptr;
   int (*shared_prefix)(const LfSharedPrefixArgs*, void*) = nullptr;
   size_t (*shared_prefix_workspace)(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) = nullptr;
+  int (*rotary)(const LfRotaryArgs*, void*) = nullptr;
+  int (*kv_gather4)(const LfGather4Args*, void*) = nullptr;
+  int (*decode4)(const LfDecode4Args*, void*) = nullptr;
+  size_t (*decode4_workspace)(int32_t, int32_t, int32_t, int32_t, int32_t, int32_t) = nullptr;
   PyObject* check = nullptr;  // _native.check(rc, what): raises LfError
 } lib;
 
@@ -927,6 +931,277 @@ Tensor run_shared_prefix(const Tensor& q, const Tensor& k_pool, const Tensor& v_
 }
 
 // ---------------------------------------------------------------------------------------
+// Norm, rotation and append; the 4-bit cache
+// ---------------------------------------------------------------------------------------
+// First and last byte of a tensor's elements (strides are not negative).
+std::pair<const char*, const char*> extent(const Tensor& t) {
+  int64_t last = 0;
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    if (t.size(i) == 0) return {nullptr, nullptr};
+    last += (t.size(i) - 1) * t.stride(i);
+  }
+  const char* p = static_cast<const char*>(t.data_ptr());
+  return {p, p + (last + 1) * t.element_size()};
+}
+
+// An output of `like`'s shape: made here, or the caller's, which may be `like` itself but not lie across it.
+Tensor out_like(Tensor out, const Tensor& like, const c10::Device& dev, const char* name) {
+  if (!out.defined()) return new_bf16(like.sizes(), dev);
+  require_cuda(out, dev);
+  check_bf16(out, name);
+  if (out.sizes() != like.sizes()) value_error(std::string(name) + " must have the shape of its input");
+  for (int64_t i = 0; i + 1 < out.dim(); ++i)
+    if (out.size(i) > 1 && out.stride(i) < out.size(-1))
+      value_error(std::string(name) + " has rows that overlap");
+  const auto x = extent(out), y = extent(like);
+  if (x.first < y.second && y.first < x.second &&
+      (out.data_ptr() != like.data_ptr() || out.strides() != like.strides()))
+    value_error(std::string(name) + " must be its input itself or lie apart from it");
+  return out;
+}
+
+// A cache of 4-bit records [pages, page_size, Hkv, D / 2 + D / 8] (uint8).
+void check_pool4(const Tensor& t, const c10::Device& dev, int64_t heads, int64_t D, const char* name) {
+  require_cuda(t, dev);
+  if (t.scalar_type() != at::kByte) type_error(std::string(name) + " must be uint8 (a 4-bit cache)");
+  if (t.dim() != 4 || t.size(2) != heads || t.size(3) != LF_RECORD4_BYTES(D) || t.stride(3) != 1)
+    value_error(std::string(name) + " must be [pages, page_size, " + std::to_string(heads) + ", " +
+                std::to_string(LF_RECORD4_BYTES(D)) + "] for head dim " + std::to_string(D) + ", got " +
+                shape_text(t.sizes()));
+}
+
+struct RotaryOptions {
+  double eps = 0.0;
+  bool interleaved = false;
+};
+
+const void* norm_weight(const Tensor* w, const c10::Device& dev, int64_t D, int32_t* f32, const char* name) {
+  if (!w) return nullptr;
+  require_cuda(*w, dev);
+  if (w->scalar_type() != at::kBFloat16 && w->scalar_type() != at::kFloat)
+    type_error(std::string(name) + " must be bfloat16 or float32");
+  if (w->dim() != 1 || w->size(0) != D || w->stride(0) != 1)
+    value_error(std::string(name) + " must be a contiguous vector of the head dim, got " + shape_text(w->sizes()));
+  *f32 = w->scalar_type() == at::kFloat;
+  return w->data_ptr();
+}
+
+// What qk_norm_rotary and kv_append_rotary have in common; `q` may be missing.
+void fill_rotary(LfRotaryArgs& a, const Tensor* q, const Tensor& k, const Tensor& positions, const Tensor& table,
+                 const Tensor* q_weight, const Tensor* k_weight, const RotaryOptions& o, Tensor& q_out,
+                 const Tensor* status) {
+  const c10::Device dev = k.device();
+  require_cuda(k, dev);
+  check_bf16(k, "k");
+  if (k.dim() != 3) value_error("k must be [T, Hkv, D], got " + shape_text(k.sizes()));
+  const int64_t T = k.size(0), D = k.size(2);
+  check_i32(positions, dev, "positions", -1);
+  if (positions.size(0) < T) value_error("positions must have an entry for each row");
+  require_cuda(table, dev);
+  if (table.scalar_type() != at::kFloat) type_error("table must be float32");
+  if (table.dim() != 2 || table.size(0) == 0 || (table.size(1) > 1 && table.stride(1) != 1))
+    value_error("table must be [positions, turned columns] with contiguous rows, got " + shape_text(table.sizes()));
+  std::memset(&a, 0, sizeof(a));
+  if (q) {
+    require_cuda(*q, dev);
+    check_bf16(*q, "q");
+    if (q->dim() != 3 || q->size(0) != T || q->size(2) != D || q->size(1) == 0)
+      value_error("q must be [T, Hq, D] with the rows of k, got " + shape_text(q->sizes()) + " and " +
+                  shape_text(k.sizes()));
+    q_out = out_like(std::move(q_out), *q, dev, "q_out");
+    a.q = q->data_ptr();
+    a.q_out = q_out.data_ptr();
+    a.Hq = narrow_i32(q->size(1), "Hq");
+    for (int i = 0; i < 2; ++i) {
+      a.q_stride[i] = q->stride(i);
+      a.qo_stride[i] = q_out.stride(i);
+    }
+    a.q_weight = norm_weight(q_weight, dev, D, &a.q_weight_f32, "q_weight");
+  } else if (q_weight || q_out.defined()) {
+    value_error("q_weight and q_out go with q");
+  }
+  a.k = k.data_ptr();
+  a.k_weight = norm_weight(k_weight, dev, D, &a.k_weight_f32, "k_weight");
+  a.positions = i32_ptr(positions);
+  a.table = static_cast<const float*>(table.data_ptr());
+  a.table_stride = table.stride(0);
+  a.n_positions = narrow_i32(table.size(0), "positions");
+  a.rot = narrow_i32(table.size(1), "turned columns");
+  a.T = narrow_i32(T, "T");
+  a.Hkv = narrow_i32(k.size(1), "Hkv");
+  a.D = narrow_i32(D, "D");
+  a.interleaved = o.interleaved;
+  a.eps = static_cast<float>(o.eps);
+  for (int i = 0; i < 2; ++i) a.k_stride[i] = k.stride(i);
+  a.status = status_ptr(status);
+}
+
+std::pair<Tensor, Tensor> run_qk_norm_rotary(const Tensor& q, const Tensor& k, const Tensor& positions,
+                                             const Tensor& table, const Tensor* q_weight, const Tensor* k_weight,
+                                             Tensor q_out, Tensor k_out, const Tensor* status,
+                                             const RotaryOptions& o) {
+  const c10::Device dev = k.device();
+  LfRotaryArgs a;
+  fill_rotary(a, &q, k, positions, table, q_weight, k_weight, o, q_out, status);
+  k_out = out_like(std::move(k_out), k, dev, "k_out");
+  a.k_out = k_out.data_ptr();
+  for (int i = 0; i < 2; ++i) a.ko_stride[i] = k_out.stride(i);
+  check_rc(launch(dev, [&](void* st) { return lib.rotary(&a, st); }), "lf_rotary_bf16");
+  return {q_out, k_out};
+}
+
+Tensor run_kv_append_rotary(const Tensor& k, const Tensor& v, const Tensor& k_pool, const Tensor& v_pool,
+                            const Tensor& slots, const Tensor& positions, const Tensor& table, const Tensor* q,
+                            const Tensor* q_weight, const Tensor* k_weight, Tensor q_out, const Tensor* status,
+                            const RotaryOptions& o) {
+  const c10::Device dev = k.device();
+  LfRotaryArgs a;
+  fill_rotary(a, q, k, positions, table, q_weight, k_weight, o, q_out, status);
+  require_cuda(v, dev);
+  check_bf16(v, "v_new");
+  if (v.sizes() != k.sizes())
+    value_error("k_new and v_new must be [T, Hkv, D], got " + shape_text(k.sizes()) + " and " +
+                shape_text(v.sizes()));
+  check_i32(slots, dev, "slots", -1);
+  if (slots.size(0) < k.size(0)) value_error("slots must have an entry for each new row");
+  require_cuda(k_pool, dev);
+  require_cuda(v_pool, dev);
+  Tensor kp = k_pool, vp = v_pool;
+  if (k_pool.scalar_type() == at::kByte) {
+    a.bits = 4;
+    check_pool4(kp, dev, a.Hkv, a.D, "k_pool");
+    check_pool4(vp, dev, a.Hkv, a.D, "v_pool");
+  } else {
+    a.bits = 16;
+    kp = pool_view(k_pool, "k_pool");
+    vp = pool_view(v_pool, "v_pool");
+    if (kp.size(2) != k.size(1) || kp.size(3) != k.size(2))
+      value_error("pool shape mismatch: new " + shape_text(k.sizes()) + " pool " + shape_text(kp.sizes()));
+  }
+  if (vp.sizes() != kp.sizes())
+    value_error("pool shape mismatch: k_pool " + shape_text(kp.sizes()) + " v_pool " + shape_text(vp.sizes()));
+  a.v = v.data_ptr();
+  a.k_pool = kp.data_ptr();
+  a.v_pool = vp.data_ptr();
+  a.slots = i32_ptr(slots);
+  a.page_size = narrow_i32(kp.size(1), "page_size");
+  a.n_pages = narrow_i32(kp.size(0), "pages");
+  for (int i = 0; i < 2; ++i) a.v_stride[i] = v.stride(i);
+  strides3(a.kp_stride, kp);
+  strides3(a.vp_stride, vp);
+  check_rc(launch(dev, [&](void* st) { return lib.rotary(&a, st); }), "lf_rotary_bf16");
+  return q_out;
+}
+
+std::pair<Tensor, Tensor> run_kv_gather4(const Tensor& k_pool, const Tensor& v_pool, const Tensor& table,
+                                         const Tensor& cu_k, int64_t num_tokens, Tensor k_out, Tensor v_out,
+                                         const Tensor* status) {
+  const c10::Device dev = k_pool.device();
+  require_cuda(k_pool, dev);
+  require_cuda(v_pool, dev);
+  if (k_pool.dim() != 4) value_error("k_pool must be [pages, page_size, Hkv, record], got " + shape_text(k_pool.sizes()));
+  const int64_t Hkv = k_pool.size(2), D = k_pool.size(3) * 8 / 5;
+  check_pool4(k_pool, dev, Hkv, D, "k_pool");
+  check_pool4(v_pool, dev, Hkv, D, "v_pool");
+  if (v_pool.sizes() != k_pool.sizes())
+    value_error("pool shape mismatch: k_pool " + shape_text(k_pool.sizes()) + " v_pool " + shape_text(v_pool.sizes()));
+  require_cuda(table, dev);
+  const Tensor bt = table_i32(table);
+  check_i32(cu_k, dev, "cu_seqlens_k", bt.size(0) + 1);
+  const int64_t T = narrow_i32(num_tokens, "num_tokens");
+  for (Tensor* t : {&k_out, &v_out}) {
+    if (!t->defined()) {
+      *t = new_bf16({T, Hkv, D}, dev);
+      continue;
+    }
+    require_cuda(*t, dev);
+    check_bf16(*t, "k_out and v_out");
+    if (t->dim() != 3 || t->size(0) != T || t->size(1) != Hkv || t->size(2) != D)
+      value_error("k_out and v_out must be [num_tokens, Hkv, D], got " + shape_text(t->sizes()));
+  }
+  LfGather4Args a;
+  std::memset(&a, 0, sizeof(a));
+  a.k_pool = k_pool.data_ptr();
+  a.v_pool = v_pool.data_ptr();
+  a.k_out = k_out.data_ptr();
+  a.v_out = v_out.data_ptr();
+  a.block_table = i32_ptr(bt);
+  a.cu_k = i32_ptr(cu_k);
+  a.B = narrow_i32(bt.size(0), "batch");
+  a.T = i32(T);
+  a.Hkv = narrow_i32(Hkv, "Hkv");
+  a.D = narrow_i32(D, "D");
+  a.page_size = narrow_i32(k_pool.size(1), "page_size");
+  a.n_pages = narrow_i32(k_pool.size(0), "pages");
+  a.bt_blocks = narrow_i32(bt.size(1), "blocks");
+  a.bt_stride = bt.stride(0);
+  strides3(a.kp_stride, k_pool);
+  strides3(a.vp_stride, v_pool);
+  for (int i = 0; i < 2; ++i) {
+    a.ko_stride[i] = k_out.stride(i);
+    a.vo_stride[i] = v_out.stride(i);
+  }
+  a.status = status_ptr(status);
+  check_rc(launch(dev, [&](void* st) { return lib.kv_gather4(&a, st); }), "lf_kv_gather_4bit");
+  return {k_out, v_out};
+}
+
+Tensor run_decode4(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& table, const Tensor& seq_lens,
+                   int64_t window, int64_t max_len, Tensor out, PyObject* workspace, const Tensor* status,
+                   double scale, const Mods& mods) {
+  const c10::Device dev = q.device();
+  for (const Tensor* t : {&q, &k, &v, &table}) require_cuda(*t, dev);
+  check_bf16(q, "q");
+  if (q.dim() != 4) value_error("q must be [B, Hkv, G, D], got " + shape_text(q.sizes()));
+  const int64_t B = q.size(0);
+  check_pool4(k, dev, q.size(1), q.size(3), "k_pool");
+  check_pool4(v, dev, q.size(1), q.size(3), "v_pool");
+  if (v.sizes() != k.sizes())
+    value_error("pool shape mismatch: k_pool " + shape_text(k.sizes()) + " v_pool " + shape_text(v.sizes()));
+  const Tensor bt = table_i32(table);
+  if (bt.size(0) != B) value_error("block_table batch mismatch");
+  check_i32(seq_lens, dev, "seq_lens", B);
+  const int64_t held = bt.size(1) * k.size(1);
+  if (max_len < 0) max_len = held;
+  if (max_len > held)
+    value_error("max_seq_len must lie in what the block table holds (" + std::to_string(held) + " tokens)");
+  if (!out.defined()) {
+    out = new_bf16(q.sizes(), dev);
+  } else {
+    require_cuda(out, dev);
+    check_bf16(out, "out");
+    if (out.sizes() != q.sizes()) value_error("out must have the shape of q");
+  }
+  LfDecode4Args a;
+  std::memset(&a, 0, sizeof(a));
+  a.q = q.data_ptr();
+  a.k = k.data_ptr();
+  a.v = v.data_ptr();
+  a.out = out.data_ptr();
+  a.block_table = i32_ptr(bt);
+  a.seq_lens = i32_ptr(seq_lens);
+  a.B = narrow_i32(B, "batch"), a.Hkv = i32(q.size(1)), a.G = i32(q.size(2)), a.D = i32(q.size(3));
+  strides3(a.q_stride, q);
+  strides3(a.o_stride, out);
+  strides3(a.k_stride, k);
+  strides3(a.v_stride, v);
+  a.bt_stride = bt.stride(0);
+  a.bt_blocks = narrow_i32(bt.size(1), "blocks");
+  a.page_size = narrow_i32(k.size(1), "page_size");
+  a.n_pages = narrow_i32(k.size(0), "pages");
+  a.window = narrow_i32(window, "window");
+  a.max_seq_len = narrow_i32(max_len, "max_seq_len");
+  fill_mods(a, scale, mods);
+  a.status = status_ptr(status);
+  const c10::cuda::CUDAGuard guard(dev);
+  a.workspace_bytes = lib.decode4_workspace(a.B, a.Hkv, a.G, a.D, a.window, a.max_seq_len);
+  Scratch scratch;
+  a.workspace = scratch.get(a.workspace_bytes, workspace, q);
+  check_rc(launch(dev, [&](void* st) { return lib.decode4(&a, st); }), "lf_decode_4bit");
+  return out;
+}
+
+// ---------------------------------------------------------------------------------------
 // Python functions (positional arguments only; functional.py has the keyword forms)
 // ---------------------------------------------------------------------------------------
 void want_args(Py_ssize_t n, Py_ssize_t want) {
@@ -1086,6 +1361,65 @@ PyObject* py_shared_prefix_decode(PyObject*, PyObject* const* a, Py_ssize_t n) {
         tensor_arg(a[0], "q"), tensor_arg(a[1], "k_pool"), tensor_arg(a[2], "v_pool"),
         tensor_arg(a[3], "block_table"), tensor_arg(a[4], "seq_lens"), int_arg(a[5]), max_len,
         out_arg(a[7]), a[8], optional_tensor(a[9], "status"), float_arg(a[10]), mods_arg(a[11])));
+  });
+}
+
+RotaryOptions rotary_options(PyObject* eps, PyObject* interleaved) {
+  RotaryOptions o;
+  o.eps = float_arg(eps);
+  const int yes = PyObject_IsTrue(interleaved);
+  if (yes < 0) throw PyErrorSet{};
+  o.interleaved = yes;
+  return o;
+}
+
+// q, k, positions, table, q_weight, k_weight, eps, interleaved, q_out, k_out, status
+PyObject* py_qk_norm_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    want_args(n, 11);
+    const auto r = run_qk_norm_rotary(
+        tensor_arg(a[0], "q"), tensor_arg(a[1], "k"), tensor_arg(a[2], "positions"), tensor_arg(a[3], "table"),
+        optional_tensor(a[4], "q_weight"), optional_tensor(a[5], "k_weight"), out_arg(a[8]), out_arg(a[9]),
+        optional_tensor(a[10], "status"), rotary_options(a[6], a[7]));
+    return Py_BuildValue("(NN)", THPVariable_Wrap(r.first), THPVariable_Wrap(r.second));
+  });
+}
+
+// k_new, v_new, k_pool, v_pool, slots, positions, table, q, q_weight, k_weight, eps, interleaved, q_out, status
+PyObject* py_kv_append_rotary(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    want_args(n, 14);
+    const Tensor q = run_kv_append_rotary(
+        tensor_arg(a[0], "k_new"), tensor_arg(a[1], "v_new"), tensor_arg(a[2], "k_pool"),
+        tensor_arg(a[3], "v_pool"), tensor_arg(a[4], "slots"), tensor_arg(a[5], "positions"),
+        tensor_arg(a[6], "table"), optional_tensor(a[7], "q"), optional_tensor(a[8], "q_weight"),
+        optional_tensor(a[9], "k_weight"), out_arg(a[12]), optional_tensor(a[13], "status"),
+        rotary_options(a[10], a[11]));
+    if (!q.defined()) Py_RETURN_NONE;
+    return THPVariable_Wrap(q);
+  });
+}
+
+// k_pool, v_pool, block_table, cu_seqlens_k, num_tokens, k_out, v_out, status
+PyObject* py_kv_gather_4bit(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&]() -> PyObject* {
+    want_args(n, 8);
+    const auto r = run_kv_gather4(tensor_arg(a[0], "k_pool"), tensor_arg(a[1], "v_pool"),
+                                  tensor_arg(a[2], "block_table"), tensor_arg(a[3], "cu_seqlens_k"), int_arg(a[4]),
+                                  out_arg(a[5]), out_arg(a[6]), optional_tensor(a[7], "status"));
+    return Py_BuildValue("(NN)", THPVariable_Wrap(r.first), THPVariable_Wrap(r.second));
+  });
+}
+
+// q, k_pool, v_pool, block_table, seq_lens, window, max_seq_len, out, workspace, status, scale, mods
+PyObject* py_decode_4bit(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded([&] {
+    want_args(n, 12);
+    const int64_t max_len = a[6] == Py_None ? -1 : narrow_i32(int_arg(a[6]), "max_seq_len");
+    return THPVariable_Wrap(run_decode4(tensor_arg(a[0], "q"), tensor_arg(a[1], "k_pool"), tensor_arg(a[2], "v_pool"),
+                                        tensor_arg(a[3], "block_table"), tensor_arg(a[4], "seq_lens"), int_arg(a[5]),
+                                        max_len, out_arg(a[7]), a[8], optional_tensor(a[9], "status"),
+                                        float_arg(a[10]), mods_arg(a[11])));
   });
 }
 
@@ -1402,6 +1736,10 @@ PyObject* py_bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
     get("lf_packed_workspace_bytes", lib.packed_workspace);
     get("lf_shared_prefix_decode_bf16", lib.shared_prefix);
     get("lf_shared_prefix_workspace_bytes", lib.shared_prefix_workspace);
+    get("lf_rotary_bf16", lib.rotary);
+    get("lf_kv_gather_4bit", lib.kv_gather4);
+    get("lf_decode_4bit", lib.decode4);
+    get("lf_decode_4bit_workspace_bytes", lib.decode4_workspace);
     Py_INCREF(a[1]);
     Py_XSETREF(lib.check, a[1]);
     Py_RETURN_NONE;
@@ -1421,6 +1759,10 @@ PyMethodDef methods[] = {
     {"kv_append_packed", LF_FAST(py_kv_append_packed), "launch lf_kv_append_packed_bf16"},
     {"packed_prefill", LF_FAST(py_packed_prefill), "launch lf_packed_prefill_bf16"},
     {"shared_prefix_decode", LF_FAST(py_shared_prefix_decode), "launch lf_shared_prefix_decode_bf16"},
+    {"qk_norm_rotary", LF_FAST(py_qk_norm_rotary), "launch lf_rotary_bf16"},
+    {"kv_append_rotary", LF_FAST(py_kv_append_rotary), "launch lf_rotary_bf16 with pools"},
+    {"kv_gather_4bit", LF_FAST(py_kv_gather_4bit), "launch lf_kv_gather_4bit"},
+    {"decode_4bit", LF_FAST(py_decode_4bit), "launch lf_decode_4bit"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_host",

@@ -19,6 +19,7 @@ from .spec import MASK_CAUSAL, MASK_NONE, ScoreMod
 _DEV_TIMEOUT = 1
 _DEV_BAD_PAGE = 2
 _DEV_BAD_LENGTHS = 4
+_DEV_BAD_POSITION = 5
 
 
 def _require_cuda(*tensors: torch.Tensor) -> torch.device:
@@ -61,6 +62,8 @@ def check_status(status: torch.Tensor, what: str = "kernel") -> None:
     if (code & 0xFF) == _DEV_BAD_LENGTHS:
         raise RuntimeError(f"{what}: a request's length is negative or above max_seq_len, or the batch "
                            "has more tokens than num_tokens")
+    if (code & 0xFF) == _DEV_BAD_POSITION:
+        raise RuntimeError(f"{what}: a position has no row in the rotation table")
     raise RuntimeError(f"{what}: device status {code}")
 
 
@@ -390,3 +393,78 @@ def shared_prefix_decode_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool
     ``packed_prefill_attention``."""
     return _native.host().shared_prefix_decode(q, k_pool, v_pool, block_table, seq_lens, prefix_len,
                                                max_seq_len, out, workspace, status, scale, mods)
+
+
+def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, *,
+                   q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                   eps: float = 1e-6, interleaved: bool = False, q_out: Optional[torch.Tensor] = None,
+                   k_out: Optional[torch.Tensor] = None,
+                   status: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Norm of every head of ``q`` ``[T, Hq, D]`` and ``k`` ``[T, Hkv, D]``, then the rotation of row t's
+    ``positions[t]`` (int32), in one pass; what prompt and decode attention take.
+
+    ``table`` (float32 ``[positions, rot]``) holds rot / 2 cosines, then rot / 2 sines of each position; rot, a
+    multiple of 16, columns are turned: column i with i + rot / 2, or with ``interleaved`` column 2 i with 2 i + 1.
+    The others stay as they are. ``q_weight`` / ``k_weight`` (``[D]``, bfloat16 or float32):
+    ``x * rsqrt(mean(x^2) + eps) * weight`` in front of it; without one that tensor's rows are only turned.
+    All in float32, rounded once. ``q_out`` may be ``q`` and ``k_out`` ``k``; apart from that the outputs must not
+    overlap the inputs. A position that the table has no row for takes the nearest (reported in ``status``)."""
+    return _native.host().qk_norm_rotary(q, k, positions, table, q_weight, k_weight, eps, interleaved, q_out,
+                                         k_out, status)
+
+
+def kv_append_rotary(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                     slots: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, *,
+                     q: Optional[torch.Tensor] = None, q_weight: Optional[torch.Tensor] = None,
+                     k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False,
+                     q_out: Optional[torch.Tensor] = None,
+                     status: Optional[torch.Tensor] = None) -> Optional[torch.Tensor]:
+    """``kv_append_packed`` with the norm and rotation of ``qk_norm_rotary`` on the way: row t of ``k_new``
+    (normed, turned) and of ``v_new`` (as it is), both ``[T, Hkv, D]``, go to slot ``slots[t]`` of the pools,
+    which hold bfloat16 ``[pages, page_size, Hkv, D]`` or 4 bits (``kv_cache_4bit``). A negative slot is skipped,
+    the others must differ. ``slots`` and ``positions`` are those of ``plan_pages``.
+
+    With ``q`` ``[T, Hq, D]``, its normed and turned rows are returned (in ``q_out``, which may be ``q``): all that
+    a step does between its projections and its attention, in one launch."""
+    return _native.host().kv_append_rotary(k_new, v_new, k_pool, v_pool, slots, positions, table, q, q_weight,
+                                           k_weight, eps, interleaved, q_out, status)
+
+
+def kv_cache_4bit(pages: int, page_size: int, kv_heads: int, head_dim: int,
+                  device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
+    """Key and value pool of a 4-bit paged cache, zeroed: uint8 ``[pages, page_size, kv_heads, record]``, a
+    record of ``head_dim / 2 + head_dim / 8`` bytes per row and head (codes, then a scale and a midpoint per 32
+    columns; ``include/lf_sm100.h`` has the format). The rows of a page and head lie next to each other in memory,
+    which is how the kernels read them; pools of other strides work too."""
+    if head_dim not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
+    shape = (pages, kv_heads, page_size, head_dim // 2 + head_dim // 8)
+    k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).transpose(1, 2) for _ in range(2))
+    return k, v
+
+
+def kv_gather_4bit(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torch.Tensor,
+                   cu_seqlens_k: torch.Tensor, num_tokens: int, *, k_out: Optional[torch.Tensor] = None,
+                   v_out: Optional[torch.Tensor] = None,
+                   status: Optional[torch.Tensor] = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Keys and values of requests from a 4-bit cache as packed bfloat16 ``[num_tokens, Hkv, D]``: key j of
+    request b, ``cu_seqlens_k[b + 1] - cu_seqlens_k[b]`` of them, is row ``cu_seqlens_k[b] + j``. With the same
+    ``cu_seqlens_k`` they are the keys of ``packed_prefill_attention``: chunks of prompts over a 4-bit cache. Rows
+    that no request has are not written. A page that the table does not name reads as zeros (reported)."""
+    return _native.host().kv_gather_4bit(k_pool, v_pool, block_table, cu_seqlens_k, num_tokens, k_out, v_out,
+                                         status)
+
+
+def decode_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                          block_table: torch.Tensor, seq_lens: torch.Tensor, *, window: int = 0,
+                          max_seq_len: Optional[int] = None, scale: float = 1.0,
+                          mods: Sequence[ScoreMod] = (), out: Optional[torch.Tensor] = None,
+                          workspace: Optional[DecodeWorkspace] = None,
+                          status: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Decode attention over a 4-bit paged cache, one token per request: ``q`` ``[B, Hkv, G, D]``, any G up to
+    128; request b sees its ``seq_lens[b]`` keys (int32 ``[B]``, its new one among them), with ``window`` the last
+    ``window`` of those. A request of length 0 (a row of a padded batch) gets zeros.
+
+    ``max_seq_len`` and ``mods`` as for ``shared_prefix_decode_attention``."""
+    return _native.host().decode_4bit(q, k_pool, v_pool, block_table, seq_lens, window, max_seq_len, out,
+                                      workspace, status, scale, mods)
