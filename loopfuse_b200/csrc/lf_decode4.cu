@@ -3,15 +3,17 @@
 // With codes c, scales s and midpoints z of the groups g of 32 columns (include/lf_sm100.h has the format),
 //   score_j = sum_g sK_jg (q_g . (cK_jg - 8)) + sum_g zK_jg sum(q_g)
 //   o       = sum_g sum_j (p_j sV_jg) (cV_jg - 8) + sum_g sum_j p_j zV_jg,    p_j = 2^(score_j - m),
-// so a cache row is never unpacked to its values: the codes become bf16 by setting an exponent above them
-// (128 + c, or 16 + c three bits up), which a matrix instruction takes as they are; scales are applied to the
-// scores of a group and to the weights, and what the exponents added comes off where it was added: a group's scores
-// start at minus that times the sums of q, and the weights meet the same constants, negative, in a product of their own.
+// so a cache row is never unpacked to its values. A code in bits 0..3 (4..7) of a bf16 whose other bits are zero is the
+// subnormal number c 2^-133 (16 c 2^-133: the first normal binade carries on where the subnormals end), which a matrix
+// instruction multiplies exactly: one AND makes two operands of codes, and with the other factor times 2^64 the
+// products are ordinary fp32 numbers. Scales are applied to the scores of a group and to the weights; the 8 comes off where it was added: a
+// group's scores start at -8 sum(q), and the weights meet a constant -8 in a product of their own.
 //
-// Bound by HBM, 5/8 byte per value: an SM has to take some 40 values a clock, so the instructions per value count
-// (a quarter of one per lane and key value, as much per value of V).
+// Bound by HBM, 5/8 byte per value, if the integer pipe keeps up: an SM has to take some 40 values a clock, and that
+// pipe does 64 operations. (Codes with an exponent set above them, 128 + c and 16 + c three bits up, took 7 operations for
+// 8 codes where this takes 5, and long sums lost their last bits to the offsets: 65536 keys, against fp64, 0.015 with
+// one correction at the end.)
 #include "lf_cache4.cuh"
-#include "lf_join.cuh"
 #include "lf_packed.cuh"
 
 #include <algorithm>
@@ -20,16 +22,22 @@
 namespace lf {
 
 constexpr int kD4Warps = 4;
-constexpr int kD4Stages = 3;   // groups of a warp's ring: two are copied while one is computed
+constexpr int kD4Stages = 2;  // groups of a warp's ring: one is copied while one is computed
 constexpr int kD4Group = 32;   // tokens that a warp takes at a time
 constexpr int kD4Run = 1;      // groups of a warp, at least
-constexpr int kD4Ctas = 3;     // of an SM
+// CTAs of an SM: as many as fit without spilled registers (D = 128, four: 83 us for 32 x 8192 keys, three 78; D = 64,
+// three: 63, four 52).
+constexpr int d4_ctas(int D) { return D == 128 ? 3 : 4; }
+
+constexpr int kD4Heads = 8;     // query heads that a warp computes together: the columns of a matrix instruction
+constexpr int kD4Scan = 128;    // up to so many requests, the join adds their lengths up itself
 
 struct Decode4Params {
   const __nv_bfloat16* q;
   const char* k;
   const char* v;
   int64_t q_stride[3], k_stride[3], v_stride[3];  // (b, kv head, g); bytes of (page, slot, kv head)
+  int32_t even_stride[4];  // EVEN: page and kv head of keys, then of values
   const int32_t* table;
   int64_t bt_stride;
   const int32_t* seq_lens;
@@ -44,15 +52,38 @@ struct Decode4Params {
   float* part_o;
   float2* part_ml;
   int2* warps;
+  uint32_t n_warps;
+  __nv_bfloat16* out;
+  int64_t o_stride[3];
   int32_t* status;
+
+  // Keys of a request that count: never more than the caller said.
+  __device__ __forceinline__ int length(int b) const { return min(max(seq_lens[b], 0), max_len); }
+  // Of those, the first that the groups begin with: that of the window, or of the sixteen it lies in (pages of 16 and more
+  // then hold whole halves of a group).
+  __device__ __forceinline__ int first_token(int end) const {
+    return window > 0 && end > window ? (end - window) & ~15 : 0;
+  }
+  __device__ __forceinline__ int groups_of(int end) const {
+    return end > 0 ? (end - first_token(end) + kD4Group - 1) / kD4Group : 0;
+  }
+  // Groups of a warp, when all units have `all` (the host sees to it that they are fewer than 2^31).
+  __device__ __forceinline__ uint32_t run(uint32_t all) const {
+    return max((all + n_warps - 1) / n_warps, static_cast<uint32_t>(kD4Run));
+  }
 };
 
-__device__ __forceinline__ void mma_bf16(float& d0, float& d1, float& d2, float& d3, uint32_t a0, uint32_t a1,
-                                         uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+struct Acc {
+  float x[4];
+};
+__device__ __forceinline__ Acc mma_bf16(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                        const Acc& c) {
+  Acc d;
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
-      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d0), "+f"(d1), "+f"(d2), "+f"(d3)
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d.x[0]), "=f"(d.x[1]), "=f"(d.x[2]), "=f"(d.x[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x[0]), "f"(c.x[1]), "f"(c.x[2]), "f"(c.x[3]));
+  return d;
 }
 
 // Transpose of an 8 x 8 matrix of 16-bit values held by a warp, two neighbours of a row per lane.
@@ -62,10 +93,14 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   return y;
 }
 
-// Codes at bits 0..3 of both halves of a word -> 128 + c as bf16; at bits 3..6 -> 16 + c.
-__device__ __forceinline__ uint32_t code_128(uint32_t w) { return (w & 0x000f000fu) | 0x43004300u; }
-__device__ __forceinline__ uint32_t code_16(uint32_t w) { return (w & 0x00780078u) | 0x41804180u; }
-constexpr float kOff128 = 136.f, kOff16 = 24.f;  // what has to come off, so that c - 8 is left
+// The codes of both halves of a word as bf16: nibbles 0 and 4 in units of 2^-133, 1 and 5 in units of 2^-129.
+__device__ __forceinline__ uint32_t codes_even(uint32_t w) { return w & 0x000f000fu; }
+__device__ __forceinline__ uint32_t codes_odd(uint32_t w) { return w & 0x00f000f0u; }
+constexpr uint32_t kMinus8Even = 0x80088008u, kMinus8Odd = 0x80808080u;  // -8 in either unit
+constexpr float kUp = 0x1p64f;           // of the other factor
+constexpr float kProduct = 0x1p-69f;     // of a product with even codes; with odd ones, 2^-65
+constexpr float kEven = 0x1p69f, kOdd = 0x1p65f;
+constexpr float kRise = 8.f;             // weights may reach 2^8 before the reference moves
 
 template <int BYTES>
 __device__ __forceinline__ void cp_async_piece(uint32_t dst, const void* src) {
@@ -75,16 +110,45 @@ __device__ __forceinline__ void cp_async_piece(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
 
-// The first key of a unit's groups: that of the window, or of the sixteen it lies in (pages of 16 and more then
-// hold whole halves of a group).
-__device__ __forceinline__ int first_token(int end, int window) {
-  return window > 0 && end > window ? (end - window) & ~15 : 0;
+template <int N>
+__device__ __forceinline__ void lds_words(const unsigned char* p, uint32_t (&x)[N]) {
+  if constexpr (N == 4) {
+    const uint4 r = *reinterpret_cast<const uint4*>(p);
+    x[0] = r.x, x[1] = r.y, x[2] = r.z, x[3] = r.w;
+  } else if constexpr (N == 2) {
+    const uint2 r = *reinterpret_cast<const uint2*>(p);
+    x[0] = r.x, x[1] = r.y;
+  } else {
+    x[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
 }
 
-// Thirty-two tokens of a unit, as a warp has them in hand.
-struct D4Group {
-  int b, head;  // request; kv head and group of query heads. b < 0: no more
-  int t, end;   // first token, end of the unit
+// A place in the row of all units' groups: a group of 32 tokens of a unit.
+struct D4Walk {
+  int b, head;  // request; kv head and group of query heads
+  int t, end;   // first token of the group, end of the unit
+
+  // The unit behind this one; there has to be one.
+  __device__ __forceinline__ void next_unit(const Decode4Params& p, int lane) {
+    t = p.first_token(end);
+    if (++head < p.heads) return;
+    head = 0;
+    for (++b;; b += 32) {  // the next request that has keys
+      const int n = b + lane < p.B ? p.length(b + lane) : 0;
+      const unsigned some = __ballot_sync(0xffffffffu, n > 0);
+      if (some) {
+        const int l = __ffs(some) - 1;
+        b += l;
+        end = __shfl_sync(0xffffffffu, n, l);
+        t = p.first_token(end);
+        return;
+      }
+      if (b + 32 >= p.B) {  // (lengths that change under the call end here)
+        b = p.B - 1;
+        return;
+      }
+    }
+  }
 };
 
 // All units' groups of 32 tokens are one row, of which warp `w` of `n_warps` has an equal run, whatever the
@@ -97,8 +161,11 @@ struct D4Group {
 //   output  rows: 16 columns of V, inner dimension: 16 keys. Lane (g, c) reads piece g of keys 2c, 2c + 1, 2c + 8,
 //           2c + 9 and pairs halfwords of two keys. The weights, times the scale of a column group and rounded to
 //           bf16, get from the first product's layout to the second's by two 8 x 8 transposes.
-template <int D, bool SOFTCAP>
-__global__ void __launch_bounds__(kD4Warps * 32, kD4Ctas) decode4_kernel(const Decode4Params p) {
+//
+// EVEN: pages of a power of two of slots, 16 or more, whose rows lie next to each other: half a group is then one run
+// of bytes, and its place takes few operations (a lane's own row for each piece took 60 of a group's 820).
+template <int D, bool SOFTCAP, bool EVEN>
+__global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(const Decode4Params p) {
   using R = Record4<D>;
   constexpr int NG = R::kGroups;
   constexpr int kHalf = kD4Group * R::kBytes;  // keys, then values
@@ -106,160 +173,159 @@ __global__ void __launch_bounds__(kD4Warps * 32, kD4Ctas) decode4_kernel(const D
   constexpr int kPieces = R::kBytes / R::kAlign;  // of a record: 5
   static_assert(kPieces * kD4Group % 32 == 0, "a group's pieces are dealt out evenly");
   extern __shared__ __align__(1024) unsigned char smem[];
-  pdl_trigger();
   pdl_wait();
+  pdl_trigger();  // (behind the wait: the join reads lengths before its own)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, c = lane & 3;
   // (Runs go round the CTAs first, then their warps: few of them are spread over all SMs.)
-  const int w = warp * static_cast<int>(gridDim.x) + static_cast<int>(blockIdx.x);
-  const int n_warps = static_cast<int>(gridDim.x) * kD4Warps;
+  const uint32_t w = warp * gridDim.x + blockIdx.x;
 
-  // Groups of the requests [b0, b0 + 32), one per lane; those of a unit.
-  int b0 = 0, groups = 0;
-  auto load_groups = [&](int from) {
-    b0 = from;
-    const int end = b0 + lane < p.B ? own_end(p.seq_lens, b0 + lane, p.max_len) : 0;
-    groups = end > 0 ? (end - first_token(end, p.window) + kD4Group - 1) / kD4Group : 0;
-  };
-  long long all = 0;
+  D4Walk at;  // what is computed
+  // Groups of the requests [b, b + 32), one per lane.
+  auto groups_at = [&](int b) { return b + lane < p.B ? static_cast<uint32_t>(p.groups_of(p.length(b + lane))) : 0u; };
+  uint32_t all = 0, groups = 0;
 #pragma unroll 4
-  for (int from = 0; from < p.B; from += 32) {
-    load_groups(from);
+  for (int b = 0; b < p.B; b += 32) {
+    groups = groups_at(b);
     all += groups;
   }
-#pragma unroll
-  for (int d = 16; d >= 1; d >>= 1) all += __shfl_xor_sync(0xffffffffu, all, d);
-  all *= p.heads;
-  const long long run = max((all + n_warps - 1) / n_warps, static_cast<long long>(kD4Run));
-  long long left = min(all - w * run, run);  // groups of this warp
-  if (left <= 0) return;
-  D4Group now;
+  all = __reduce_add_sync(0xffffffffu, all) * p.heads;
+  const uint32_t run = p.run(all);
+  if (all <= w * run) return;  // (run times the warps is below 2^31 and 2^31 more)
+  int left = static_cast<int>(min(all - w * run, run));  // groups of this warp
   {
-    long long skip = w * run;  // of the requests ahead, then of the units ahead
-    long long incl = 0;
+    uint32_t skip = w * run;  // of the requests ahead, then of the units ahead
+    uint32_t incl = 0;
     unsigned past = 0;
-    for (int from = 0; from < p.B && !past; from += 32) {
-      if (from) skip -= __shfl_sync(0xffffffffu, incl, 31);
-      load_groups(from);
-      incl = static_cast<long long>(groups) * p.heads;
+    int from = 0;
+    for (int b = 0; b < p.B && !past; b += 32) {
+      if (b) skip -= __shfl_sync(0xffffffffu, incl, 31);
+      if (p.B > 32) groups = groups_at(b);
+      from = b;
+      incl = groups * p.heads;
 #pragma unroll
       for (int d = 1; d < 32; d <<= 1) {
-        const long long x = __shfl_up_sync(0xffffffffu, incl, d);
+        const uint32_t x = __shfl_up_sync(0xffffffffu, incl, d);
         if (lane >= d) incl += x;
       }
       past = __ballot_sync(0xffffffffu, incl > skip);
     }
     const int l = __ffs(past) - 1;
-    const int n = __shfl_sync(0xffffffffu, groups, l);
-    const long long into = skip - __shfl_sync(0xffffffffu, incl, l) + static_cast<long long>(n) * p.heads;
-    now.b = b0 + l;
-    now.head = static_cast<int>(into / n);
-    now.end = own_end(p.seq_lens, now.b, p.max_len);
-    now.t = first_token(now.end, p.window) + static_cast<int>(into - static_cast<long long>(now.head) * n) * kD4Group;
+    const uint32_t n = __shfl_sync(0xffffffffu, groups, l);
+    const uint32_t into = skip - __shfl_sync(0xffffffffu, incl, l) + n * p.heads;
+    at.b = from + l;
+    at.head = static_cast<int>(into / n);
+    at.end = p.length(at.b);
+    at.t = p.first_token(at.end) + static_cast<int>(into - at.head * n) * kD4Group;
   }
-  // The group behind x, while this warp has any.
-  auto next_group = [&](const D4Group& x) {
-    D4Group y = x;
-    if (--left <= 0) {
-      y.b = -1;
-      return y;
-    }
-    y.t += kD4Group;
-    if (y.t < y.end) return y;
-    y.t = first_token(y.end, p.window);
-    if (++y.head < p.heads) return y;
-    y.head = 0;
-    for (;;) {  // the next request that has keys
-      const unsigned some = __ballot_sync(0xffffffffu, groups > 0 && b0 + lane > y.b);
-      if (some) {
-        y.b = b0 + __ffs(some) - 1;
-        y.end = own_end(p.seq_lens, y.b, p.max_len);
-        y.t = first_token(y.end, p.window);
-        return y;
-      }
-      load_groups(b0 + 32);
-    }
-  };
   auto kv_head = [&](int head, int* g0) {
     const int kvh = static_cast<int>(p.div_groups.div(head));
-    *g0 = (head - kvh * static_cast<int>(p.div_groups.d)) * kOwnHeads;
+    *g0 = (head - kvh * static_cast<int>(p.div_groups.d)) * kD4Heads;
     return kvh;
   };
 
-  auto page_of = [&](int t) { return p.page_shift >= 0 ? (t >> p.page_shift) : (t / p.page_size); };
-  // The token that this lane finds for a group: rows past the end repeat the last, rows in front of the window
-  // its first.
-  auto token_of = [&](const D4Group& x) {
-    const int from = p.window > 0 ? max(x.end - p.window, 0) : 0;
-    return max(min(x.t + lane, x.end - 1), from);
+  // Where a group lies. EVEN: the pages of its halves and the first row of each (of a half past the end, rows that are
+  // there). Else this lane's row: rows past the end repeat the last, rows in front of the window its first.
+  struct Place {
+    int page[2], slot[2], kvh;
   };
-  auto look_up = [&](const D4Group& x) {
-    if (x.b < 0) return 0;
-    const int at = page_of(token_of(x));
-    if (!LF_BOUNDS(x.b < p.B && x.head < p.heads && at >= 0 && at < p.bt_blocks, p.status, 75)) return 0;
-    return p.table[x.b * p.bt_stride + at];
+  D4Walk ahead = at;  // what is looked up
+  int unseen = left, ignored;
+  int kvh_ahead = kv_head(ahead.head, &ignored);
+  auto look_up = [&] {
+    Place x = {{0, 0}, {0, 0}, kvh_ahead};
+    if (unseen <= 0) return x;
+    const int32_t* row = p.table + ahead.b * p.bt_stride;
+    if constexpr (EVEN) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int t = min(ahead.t + 16 * h, ahead.end - 1), block = t >> p.page_shift;
+        x.slot[h] = (t & (p.page_size - 1)) & ~15;
+        if (LF_BOUNDS(ahead.b < p.B && ahead.head < p.heads && t >= 0 && block < p.bt_blocks, p.status, 75))
+          x.page[h] = row[block];
+      }
+    } else {
+      const int t = max(min(ahead.t + lane, ahead.end - 1), p.window > 0 ? ahead.end - p.window : 0);
+      const int block = p.page_shift >= 0 ? t >> p.page_shift : t / p.page_size;
+      x.slot[0] = t - block * p.page_size;
+      if (LF_BOUNDS(ahead.b < p.B && ahead.head < p.heads && t >= 0 && block < p.bt_blocks, p.status, 76))
+        x.page[0] = row[block];
+    }
+    --unseen;
+    ahead.t += kD4Group;
+    if (ahead.t >= ahead.end && unseen > 0) {
+      ahead.next_unit(p, lane);
+      kvh_ahead = kv_head(ahead.head, &ignored);
+    }
+    return x;
   };
   unsigned char* ring = smem + warp * (kD4Stages * kStageBytes);
   const uint32_t ring_u32 = smem_u32(ring);
-  auto copy_group = [&](const D4Group& x, int stage, int page) {
-    if (x.b >= 0) {
-      int g0;
-      const int kvh = kv_head(x.head, &g0);
-      const int t = token_of(x);
-      if (page < 0 || page >= p.n_pages) {
-        if (p.status) atomicExch(p.status, LF_DEV_BAD_PAGE);
-        page = 0;
-      }
-      int slot = t - page_of(t) * p.page_size;
-      if (!LF_BOUNDS(slot >= 0 && slot < p.page_size && stage >= 0 && stage < kD4Stages, p.status, 76)) slot = 0;
-      const char* krow = p.k + kvh * p.k_stride[2] + page * p.k_stride[0] + slot * p.k_stride[1];
-      const char* vrow = p.v + kvh * p.v_stride[2] + page * p.v_stride[0] + slot * p.v_stride[1];
-      const uint32_t dst = ring_u32 + stage * kStageBytes;
+  int uncopied = left;
+  auto copy_group = [&](Place x, int stage) {
+    if (uncopied > 0) {
+      --uncopied;
 #pragma unroll
-      for (int i = 0; i < kPieces * kD4Group / 32; ++i) {
-        const int id = lane + 32 * i, row = id / kPieces, piece = id - row * kPieces;
-        const char* kp = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(krow), row));
-        const char* vp = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(vrow), row));
-        cp_async_piece<R::kAlign>(dst + id * R::kAlign, kp + piece * R::kAlign);
-        cp_async_piece<R::kAlign>(dst + kHalf + id * R::kAlign, vp + piece * R::kAlign);
+      for (int h = 0; h < (EVEN ? 2 : 1); ++h)
+        if (static_cast<uint32_t>(x.page[h]) >= static_cast<uint32_t>(p.n_pages)) {
+          if (p.status) atomicExch(p.status, LF_DEV_BAD_PAGE);
+          x.page[h] = 0;
+        }
+      const uint32_t dst = ring_u32 + stage * kStageBytes + lane * R::kAlign;
+      if constexpr (EVEN) {
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) {
+          const char* base = (kv ? p.v : p.k) + static_cast<int64_t>(x.kvh) * p.even_stride[2 * kv + 1] + lane * R::kAlign;
+          const char* lo = base + static_cast<int64_t>(x.page[0]) * p.even_stride[2 * kv] + x.slot[0] * R::kBytes;
+          const char* hi = base + static_cast<int64_t>(x.page[1]) * p.even_stride[2 * kv] + (x.slot[1] - 16) * R::kBytes;
+          const char* mid = lane < 16 ? lo : hi;  // (a half is 2.5 pieces of each lane)
+#pragma unroll
+          for (int i = 0; i < 5; ++i)
+            cp_async_piece<R::kAlign>(dst + kv * kHalf + 32 * i * R::kAlign,
+                                      (i < 2 ? lo : i == 2 ? mid : hi) + 32 * i * R::kAlign);
+        }
+      } else {
+        const int64_t kr = x.kvh * p.k_stride[2] + x.page[0] * p.k_stride[0] + x.slot[0] * p.k_stride[1];
+        const int64_t vr = x.kvh * p.v_stride[2] + x.page[0] * p.v_stride[0] + x.slot[0] * p.v_stride[1];
+#pragma unroll
+        for (int i = 0; i < kPieces * kD4Group / 32; ++i) {
+          const int id = lane + 32 * i, row = id / kPieces, from = (id - row * kPieces) * R::kAlign;
+          cp_async_piece<R::kAlign>(dst + 32 * i * R::kAlign, p.k + __shfl_sync(0xffffffffu, kr, row) + from);
+          cp_async_piece<R::kAlign>(dst + kHalf + 32 * i * R::kAlign, p.v + __shfl_sync(0xffffffffu, vr, row) + from);
+        }
       }
     }
     cp_async_commit();
   };
 
-  // The query heads of a unit: columns of the first product, in the order that the codes have; what the
-  // accumulators of a column group start at (heads 2c, 2c + 1); and the sums of the columns, which go with the
-  // midpoints, as three bf16 each.
+  // The query heads of a unit: columns of the first product, in the order that the codes have; and the sums of the
+  // columns, which go with the midpoints (sum_z) and, times -8, with the scales (sum_s), as two or three bf16 each.
+  // Scores are in units of 2^-69 until they are scaled.
   uint32_t qf[NG][4];
-  float start[NG][2];
-  uint32_t sum_b0 = 0, sum_b1 = 0;
-  auto load_q = [&](const D4Group& x) {
+  uint32_t sum_z, sum_s;
+  auto load_q = [&] {
     int g0;
-    const int kvh = kv_head(x.head, &g0);
+    const int kvh = kv_head(at.head, &g0);
     float sum[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
       uint4 r = make_uint4(0u, 0u, 0u, 0u);
       if (g0 + g < p.G)
-        r = *reinterpret_cast<const uint4*>(p.q + x.b * p.q_stride[0] + kvh * p.q_stride[1] +
+        r = *reinterpret_cast<const uint4*>(p.q + at.b * p.q_stride[0] + kvh * p.q_stride[1] +
                                             (g0 + g) * p.q_stride[2] + 32 * n + 8 * c);
-      qf[n][0] = __byte_perm(r.x, r.z, 0x5410);  // columns 0 and 4 of the eight
-      qf[n][1] = __byte_perm(r.x, r.z, 0x7632);  // 1, 5
-      qf[n][2] = __byte_perm(r.y, r.w, 0x5410);  // 2, 6
-      qf[n][3] = __byte_perm(r.y, r.w, 0x7632);  // 3, 7
-      float even = bf16lo_to_f32(r.x) + bf16lo_to_f32(r.y) + bf16lo_to_f32(r.z) + bf16lo_to_f32(r.w);
-      float odd = bf16hi_to_f32(r.x) + bf16hi_to_f32(r.y) + bf16hi_to_f32(r.z) + bf16hi_to_f32(r.w);
+      // (Times a power of two, exact; odd codes come times 16.)
+      const float x0 = bf16lo_to_f32(r.x), x1 = bf16hi_to_f32(r.x), x2 = bf16lo_to_f32(r.y), x3 = bf16hi_to_f32(r.y);
+      const float x4 = bf16lo_to_f32(r.z), x5 = bf16hi_to_f32(r.z), x6 = bf16lo_to_f32(r.w), x7 = bf16hi_to_f32(r.w);
+      qf[n][0] = pack_bf16x2(x0 * kUp, x4 * kUp);
+      qf[n][1] = pack_bf16x2(x1 * (kUp / 16), x5 * (kUp / 16));
+      qf[n][2] = pack_bf16x2(x2 * kUp, x6 * kUp);
+      qf[n][3] = pack_bf16x2(x3 * (kUp / 16), x7 * (kUp / 16));
+      float all_q = ((x0 + x1) + (x2 + x3)) + ((x4 + x5) + (x6 + x7));
 #pragma unroll
-      for (int d = 1; d <= 2; d <<= 1) {
-        even += __shfl_xor_sync(0xffffffffu, even, d);
-        odd += __shfl_xor_sync(0xffffffffu, odd, d);
-      }
-      sum[n] = even + odd;
-      const float off = -(kOff128 * even + kOff16 * odd);
-      start[n][0] = __shfl_sync(0xffffffffu, off, 8 * c);
-      start[n][1] = __shfl_sync(0xffffffffu, off, 8 * c + 4);
+      for (int d = 1; d <= 2; d <<= 1) all_q += __shfl_xor_sync(0xffffffffu, all_q, d);
+      sum[n] = all_q * kProduct;
     }
-    // Inner index 2c, 2c + 1 (and 8 more) of the midpoints' product: a pair of column groups, and a part of the sums.
+    // Inner index 2c, 2c + 1 of the product of both: a pair of column groups, and a part of the sums.
     uint32_t part[3][NG / 2];
 #pragma unroll
     for (int n = 0; n < NG / 2; ++n) {
@@ -271,235 +337,332 @@ __global__ void __launch_bounds__(kD4Warps * 32, kD4Ctas) decode4_kernel(const D
         x1 -= bf16hi_to_f32(part[i][n]);
       }
     }
-    if constexpr (NG == 4) {
-      sum_b0 = c == 0 ? part[0][0] : c == 1 ? part[0][1] : c == 2 ? part[1][0] : part[1][1];
-      sum_b1 = c == 0 ? part[2][0] : c == 1 ? part[2][1] : 0u;
-    } else {
-      sum_b0 = c == 0 ? part[0][0] : c == 1 ? part[1][0] : c == 2 ? part[2][0] : 0u;
-      sum_b1 = 0u;
-    }
+    if constexpr (NG == 4)
+      sum_z = c == 0 ? part[0][0] : c == 1 ? part[0][1] : c == 2 ? part[1][0] : part[1][1];
+    else
+      sum_z = c == 0 ? part[0][0] : c == 1 ? part[1][0] : c == 2 ? part[2][0] : 0u;
+    sum_s = pack_bf16x2(-8.f * bf16lo_to_f32(sum_z), -8.f * bf16hi_to_f32(sum_z));  // (exact)
   };
 
-  // now: computed; then, later: being copied; ahead, last: their pages are being looked up.
-  static_assert(kD4Stages == 3, "two groups are copied while one is computed");
-  D4Group then = next_group(now), later = next_group(then);
-  load_q(now);
-  {
-    const int pg0 = look_up(now), pg1 = look_up(then);
-    copy_group(now, 0, pg0);
-    copy_group(then, 1, pg1);
-  }
-  D4Group ahead = next_group(later);
-  int page = look_up(later), page_ahead = look_up(ahead);
-
-  // Query heads 2c, 2c + 1.
-  float m_run[2], l_run[2], mids[NG][2];
-  float o[2 * NG][4];  // rows of instruction 2n + h: columns 32 n + 4 g + 2 h, then + 1; each for both heads
+  // Query heads 2c, 2c + 1. Pairs: of the sums over keys g and g + 8 (of every sixteen).
+  float m_run[2];
+  uint64_t l_run[2], mids[NG][2];
+  Acc o[2 * NG];  // rows of instruction 2n + h: columns 32 n + 4 g + 2 h, then + 1; each for both heads
   auto clear = [&] {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       m_run[r] = -INFINITY;
-      l_run[r] = 0.f;
+      l_run[r] = 0;
 #pragma unroll
-      for (int n = 0; n < NG; ++n) mids[n][r] = 0.f;
+      for (int n = 0; n < NG; ++n) mids[n][r] = 0;
     }
 #pragma unroll
     for (int n = 0; n < 2 * NG; ++n)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o[n][e] = 0.f;
+      for (int e = 0; e < 4; ++e) o[n].x[e] = 0.f;
   };
-  clear();
 
-  for (int it = 0; now.b >= 0; it = it == 2 ? 0 : it + 1) {
-    copy_group(later, it == 0 ? 2 : it - 1, page);
-    const D4Group last = next_group(ahead);
-    page = page_ahead;
-    page_ahead = look_up(last);
-    cp_async_wait<kD4Stages - 1>();
-    __syncwarp();
-    const unsigned char* stage = ring + it * kStageBytes;
-
+  // The products of the group at.t, which lies in `stage`. EDGE: not all of its keys are seen, but [from, at.end).
+  int from = 0;
+  auto compute = [&](const unsigned char* stage, auto edge) {
+    constexpr bool EDGE = decltype(edge)::value;
+    auto hidden = [&](int i) { return at.t + i < from || at.t + i >= at.end; };
     float sc[2][4];  // [half of the group]: key g (two heads), key g + 8
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const unsigned char* k0 = stage + (16 * h + g) * R::kBytes;
       const unsigned char* k1 = k0 + 8 * R::kBytes;
       uint32_t w0[NG], w1[NG], s0[NG / 2], s1[NG / 2];
-      if constexpr (NG == 4) {
-        const uint4 x = *reinterpret_cast<const uint4*>(k0 + 16 * c), y = *reinterpret_cast<const uint4*>(k1 + 16 * c);
-        w0[0] = x.x, w0[1] = x.y, w0[2] = x.z, w0[3] = x.w;
-        w1[0] = y.x, w1[1] = y.y, w1[2] = y.z, w1[3] = y.w;
-        const uint2 u = *reinterpret_cast<const uint2*>(k0 + R::kScales), v = *reinterpret_cast<const uint2*>(k1 + R::kScales);
-        s0[0] = u.x, s0[1] = u.y, s1[0] = v.x, s1[1] = v.y;
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(k0 + 8 * c), y = *reinterpret_cast<const uint2*>(k1 + 8 * c);
-        w0[0] = x.x, w0[1] = x.y;
-        w1[0] = y.x, w1[1] = y.y;
-        s0[0] = *reinterpret_cast<const uint32_t*>(k0 + R::kScales);
-        s1[0] = *reinterpret_cast<const uint32_t*>(k1 + R::kScales);
-      }
+      lds_words<NG>(k0 + 4 * NG * c, w0);
+      lds_words<NG>(k1 + 4 * NG * c, w1);
+      lds_words<NG / 2>(k0 + R::kScales, s0);
+      lds_words<NG / 2>(k1 + R::kScales, s1);
       const int pair = NG == 4 ? 4 * (c & 1) : 0;
-      const uint32_t z0 = *reinterpret_cast<const uint32_t*>(k0 + R::kMids + pair);
-      const uint32_t z1 = *reinterpret_cast<const uint32_t*>(k1 + R::kMids + pair);
-      float x0 = 0.f, x1 = 0.f, x2 = 0.f, x3 = 0.f;
-      mma_bf16(x0, x1, x2, x3, z0, z1, z0, z1, sum_b0, sum_b1);
+      auto word = [&](const unsigned char* at) { return *reinterpret_cast<const uint32_t*>(at + pair); };
+      constexpr Acc kZero = {{0.f, 0.f, 0.f, 0.f}};
+      Acc x = mma_bf16(word(k0 + R::kMids), word(k1 + R::kMids), word(k0 + R::kScales), word(k1 + R::kScales), sum_z,
+                       sum_s, kZero);
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
-        float y0 = start[n][0], y1 = start[n][1], y2 = start[n][0], y3 = start[n][1];
-        mma_bf16(y0, y1, y2, y3, code_128(w0[n]), code_128(w1[n]), code_16(w0[n] >> 1), code_16(w1[n] >> 1),
-                 qf[n][0], qf[n][1]);
-        mma_bf16(y0, y1, y2, y3, code_128(w0[n] >> 8), code_128(w1[n] >> 8), code_16(w0[n] >> 9),
-                 code_16(w1[n] >> 9), qf[n][2], qf[n][3]);
+        const uint32_t u0 = w0[n] >> 8, u1 = w1[n] >> 8;
+        Acc y = mma_bf16(codes_even(w0[n]), codes_even(w1[n]), codes_odd(w0[n]), codes_odd(w1[n]), qf[n][0], qf[n][1],
+                         kZero);
+        y = mma_bf16(codes_even(u0), codes_even(u1), codes_odd(u0), codes_odd(u1), qf[n][2], qf[n][3], y);
         const float a = n & 1 ? bf16hi_to_f32(s0[n / 2]) : bf16lo_to_f32(s0[n / 2]);
         const float b = n & 1 ? bf16hi_to_f32(s1[n / 2]) : bf16lo_to_f32(s1[n / 2]);
-        x0 = fmaf(a, y0, x0);
-        x1 = fmaf(a, y1, x1);
-        x2 = fmaf(b, y2, x2);
-        x3 = fmaf(b, y3, x3);
+        x.x[0] = fmaf(a, y.x[0], x.x[0]);
+        x.x[1] = fmaf(a, y.x[1], x.x[1]);
+        x.x[2] = fmaf(b, y.x[2], x.x[2]);
+        x.x[3] = fmaf(b, y.x[3], x.x[3]);
       }
-      sc[h][0] = x0, sc[h][1] = x1, sc[h][2] = x2, sc[h][3] = x3;
-    }
-
-    const int from = p.window > 0 ? now.end - p.window : 0;
-    const bool edge = now.t < from || now.t + kD4Group > now.end;
-    float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        float s = sc[h][e];
+        float s = x.x[e];
         if constexpr (SOFTCAP) s = tanh_approx(s * p.a);  // (the unit's, within 2^-11, as in decode)
-        s *= p.c2;
-        if (edge) {
-          const int t = now.t + 16 * h + g + 8 * (e >> 1);
-          if (t < from || t >= now.end) s = -INFINITY;
-        }
+        if (EDGE && hidden(16 * h + g + 8 * (e >> 1))) s = -INFINITY;
         sc[h][e] = s;
-        mx[e & 1] = fmaxf(mx[e & 1], s);
       }
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-#pragma unroll
-      for (int d = 4; d <= 16; d <<= 1) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], d));
-      mx[r] = fmaxf(mx[r], m_run[r]);
     }
-    const float m_safe[2] = {mx[0] == -INFINITY ? 0.f : mx[0], mx[1] == -INFINITY ? 0.f : mx[1]};
-    if (__any_sync(0xffffffffu, mx[0] > m_run[0] || mx[1] > m_run[1])) {
+    // The reference of a row moves when a score rises more than kRise above it, not with every maximum: the lanes of
+    // a row look at each other's scores only then.
+    float mx[2];
+    mx[0] = fmaxf(max3(sc[0][0], sc[0][2], sc[1][0]), sc[1][2]) * p.c2;
+    mx[1] = fmaxf(max3(sc[0][1], sc[0][3], sc[1][1]), sc[1][3]) * p.c2;
+    if (__any_sync(0xffffffffu, mx[0] > m_run[0] + kRise || mx[1] > m_run[1] + kRise)) {
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        const float alpha = ex2_approx(m_run[r] - m_safe[r]);
-        m_run[r] = mx[r];
-        l_run[r] *= alpha;
 #pragma unroll
-        for (int n = 0; n < NG; ++n) mids[n][r] *= alpha;
+        for (int d = 4; d <= 16; d <<= 1) mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], d));
+        mx[r] = fmaxf(mx[r], m_run[r]);
+        const float alpha = mx[r] == -INFINITY ? 0.f : ex2_approx(m_run[r] - mx[r]);
+        m_run[r] = mx[r];
+        const uint64_t alpha2 = pack2(alpha, alpha);
+        l_run[r] = mul2(l_run[r], alpha2);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) mids[n][r] = mul2(mids[n][r], alpha2);
 #pragma unroll
         for (int n = 0; n < 2 * NG; ++n) {
-          o[n][r] *= alpha;
-          o[n][2 + r] *= alpha;
+          o[n].x[r] *= alpha;
+          o[n].x[2 + r] *= alpha;
         }
       }
+    }
+    // (Weights come times 2^64: the other factor of the codes.)
+    uint64_t up[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float x = m_run[r] == -INFINITY ? 0.f : 64.f - m_run[r];
+      up[r] = pack2(x, x);
     }
 
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float pr[4];
+      uint64_t pr[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        pr[e] = ex2_approx(sc[h][e] - m_safe[e & 1]);
-        l_run[e & 1] += pr[e];  // this lane's share; the keys are summed at the end of the unit
+      for (int r = 0; r < 2; ++r) {
+        float x, y;
+        unpack2(fma2(pack2(sc[h][r], sc[h][2 + r]), pack2(p.c2, p.c2), up[r]), x, y);
+        pr[r] = pack2(ex2_approx(x), ex2_approx(y));
+        l_run[r] = add2(l_run[r], pr[r]);  // this lane's share; the keys are summed at the end of the unit
       }
       const unsigned char* v = stage + kHalf + 16 * h * R::kBytes;
-      const unsigned char* m0 = v + g * R::kBytes + R::kScales;
-      const unsigned char* m1 = m0 + 8 * R::kBytes;
       uint32_t s0[NG], s1[NG];  // scales, then midpoints, of keys g and g + 8
-      if constexpr (NG == 4) {
-        const uint4 x = *reinterpret_cast<const uint4*>(m0), y = *reinterpret_cast<const uint4*>(m1);
-        s0[0] = x.x, s0[1] = x.y, s0[2] = x.z, s0[3] = x.w;
-        s1[0] = y.x, s1[1] = y.y, s1[2] = y.z, s1[3] = y.w;
-      } else {
-        const uint2 x = *reinterpret_cast<const uint2*>(m0), y = *reinterpret_cast<const uint2*>(m1);
-        s0[0] = x.x, s0[1] = x.y;
-        s1[0] = y.x, s1[1] = y.y;
+      lds_words<NG>(v + g * R::kBytes + R::kScales, s0);
+      lds_words<NG>(v + (g + 8) * R::kBytes + R::kScales, s1);
+      if constexpr (EDGE) {  // (what lies in rows that are not seen may be NaN)
+        const bool no0 = hidden(16 * h + g), no1 = hidden(16 * h + g + 8);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          s0[n] = no0 ? 0u : s0[n];
+          s1[n] = no1 ? 0u : s1[n];
+        }
       }
       // Codes of keys 2c, 2c + 1, 2c + 8, 2c + 9: [key][pair of column groups].
       uint32_t cv[4][NG / 2];
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const unsigned char* at = v + (2 * c + (r & 1) + 8 * (r >> 1)) * R::kBytes + g * R::kValuePiece;
-        if constexpr (NG == 4) {
-          const uint2 x = *reinterpret_cast<const uint2*>(at);
-          cv[r][0] = x.x, cv[r][1] = x.y;
-        } else {
-          cv[r][0] = *reinterpret_cast<const uint32_t*>(at);
-        }
-      }
+      for (int r = 0; r < 4; ++r)
+        lds_words<NG / 2>(v + (2 * c + (r & 1) + 8 * (r >> 1)) * R::kBytes + g * R::kValuePiece, cv[r]);
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         const float a = n & 1 ? bf16hi_to_f32(s0[n / 2]) : bf16lo_to_f32(s0[n / 2]);
         const float b = n & 1 ? bf16hi_to_f32(s1[n / 2]) : bf16lo_to_f32(s1[n / 2]);
         const float za = n & 1 ? bf16hi_to_f32(s0[NG / 2 + n / 2]) : bf16lo_to_f32(s0[NG / 2 + n / 2]);
         const float zb = n & 1 ? bf16hi_to_f32(s1[NG / 2 + n / 2]) : bf16lo_to_f32(s1[NG / 2 + n / 2]);
+        float x0, y0, x1, y1;
+        unpack2(mul2(pr[0], pack2(a, b)), x0, y0);
+        unpack2(mul2(pr[1], pack2(a, b)), x1, y1);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) mids[n][r] = fmaf(pr[r], za, fmaf(pr[2 + r], zb, mids[n][r]));
-        const uint32_t pb0 = transpose_8x8(pack_bf16x2(pr[0] * a, pr[1] * a));
-        const uint32_t pb1 = transpose_8x8(pack_bf16x2(pr[2] * b, pr[3] * b));
+        for (int r = 0; r < 2; ++r) mids[n][r] = fma2(pr[r], pack2(za, zb), mids[n][r]);
+        const uint32_t pb0 = transpose_8x8(pack_bf16x2(x0, x1));
+        const uint32_t pb1 = transpose_8x8(pack_bf16x2(y0, y1));
         const uint32_t sel = n & 1 ? 0x7632u : 0x5410u;
         const uint32_t x = __byte_perm(cv[0][n / 2], cv[1][n / 2], sel);
         const uint32_t y = __byte_perm(cv[2][n / 2], cv[3][n / 2], sel);
-        // (What the exponents added comes off step by step: over a long run the sum of the weights, times 136, would
-        // leave few bits for what is left. 65536 keys, against fp64: 0.015 with one correction at the end, 0.0022.)
-        constexpr uint32_t kMinus128 = 0xc308c308u, kMinus16 = 0xc1c0c1c0u;  // -136, -24
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float(&d)[4] = o[2 * n + e];
-          mma_bf16(d[0], d[1], d[2], d[3], kMinus128, kMinus16, kMinus128, kMinus16, pb0, pb1);
-          mma_bf16(d[0], d[1], d[2], d[3], code_128(x >> 8 * e), code_16(x >> (8 * e + 1)), code_128(y >> 8 * e),
-                   code_16(y >> (8 * e + 1)), pb0, pb1);
+          const uint32_t ux = e ? x >> 8 : x, uy = e ? y >> 8 : y;
+          Acc& d = o[2 * n + e];
+          d = mma_bf16(kMinus8Even, kMinus8Odd, kMinus8Even, kMinus8Odd, pb0, pb1, d);
+          d = mma_bf16(codes_even(ux), codes_odd(ux), codes_even(uy), codes_odd(uy), pb0, pb1, d);
         }
       }
+    }
+  };
+
+  // A group is looked up while the one before it is copied, and that while the one before that is computed.
+  copy_group(look_up(), 0);
+  Place next = look_up();
+  int it = 0;
+  while (left > 0) {
+    // A unit, or the part of one that is this warp's.
+    load_q();
+    clear();
+    const int unit = at.b * p.heads + at.head, first = p.first_token(at.end);
+    if (lane == 0 && at.t == first) p.warps[unit].x = static_cast<int>(w);  // where the join finds the unit's parts
+    from = p.window > 0 ? at.end - p.window : 0;
+    int here = min(left, (at.end - at.t + kD4Group - 1) / kD4Group);
+    left -= here;
+    for (; here > 0; --here, at.t += kD4Group) {
+      copy_group(next, it ^ 1);
+      next = look_up();
+      cp_async_wait<1>();
+      __syncwarp();
+      const unsigned char* stage = ring + it * kStageBytes;
+      if (at.t < from || at.t + kD4Group > at.end)
+        compute(stage, std::true_type{});
+      else
+        compute(stage, std::false_type{});
+      __syncwarp();  // every lane is done with this stage before it is refilled
+      it ^= 1;
     }
 
-    const int unit = now.b * p.heads + now.head;
-    if (lane == 0) {  // where the join finds the unit's parts
-      if (now.t == first_token(now.end, p.window)) p.warps[unit].x = w;
-      if (now.t + kD4Group >= now.end) p.warps[unit].y = w;
-    }
-    if (then.b != now.b || then.head != now.head) {
-      // This warp is done with the unit: its rows and their (maximum, sum) go to the join.
-      int g0;
-      kv_head(now.head, &g0);
+    // This warp is done with the unit: its rows and their (maximum, sum) go to the join.
+    int g0;
+    kv_head(at.head, &g0);
+    const bool done = at.t >= at.end;
+    if (left > 0) at.next_unit(p, lane);
+    if (lane == 0 && done) p.warps[unit].y = static_cast<int>(w);
+    auto over_keys = [](uint64_t pair) {
+      float x, y;
+      unpack2(pair, x, y);
+      x += y;
 #pragma unroll
-      for (int r = 0; r < 2; ++r)
+      for (int d = 4; d <= 16; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+      return x * (1.f / kUp);
+    };
 #pragma unroll
-        for (int d = 4; d <= 16; d <<= 1) {
-          l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], d);
+    for (int r = 0; r < 2; ++r) {
+      const float l = over_keys(l_run[r]);
+      float z[NG];
 #pragma unroll
-          for (int n = 0; n < NG; ++n) mids[n][r] += __shfl_xor_sync(0xffffffffu, mids[n][r], d);
+      for (int n = 0; n < NG; ++n) z[n] = over_keys(mids[n][r]);
+      if (g0 + 2 * c + r < p.G) {
+        const int64_t place = (static_cast<int64_t>(w) + unit) * kD4Heads + 2 * c + r;
+        float* dst = p.part_o + place * D + 4 * g;
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+          *reinterpret_cast<float4*>(dst + 32 * n) =
+              make_float4(fmaf(o[2 * n].x[r], kEven, z[n]), fmaf(o[2 * n].x[2 + r], kOdd, z[n]),
+                          fmaf(o[2 * n + 1].x[r], kEven, z[n]), fmaf(o[2 * n + 1].x[2 + r], kOdd, z[n]));
         }
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        if (g0 + 2 * c + r < p.G) {
-          const int64_t at = (static_cast<int64_t>(w) + unit) * kOwnHeads + 2 * c + r;
-          float* dst = p.part_o + at * D + 4 * g;
-#pragma unroll
-          for (int n = 0; n < NG; ++n) {
-            const float z = mids[n][r];
-            *reinterpret_cast<float4*>(dst + 32 * n) =
-                make_float4(o[2 * n][r] + z, o[2 * n][2 + r] + z, o[2 * n + 1][r] + z, o[2 * n + 1][2 + r] + z);
-          }
-          if (g == 0) p.part_ml[at] = make_float2(m_run[r], l_run[r]);
-        }
+        if (g == 0) p.part_ml[place] = make_float2(m_run[r], l);
       }
-      clear();
-      if (then.b >= 0) load_q(then);
     }
-    __syncwarp();  // every lane is done with this stage before it is refilled
-    now = then;
-    then = later;
-    later = ahead;
-    ahead = last;
   }
   cp_async_wait<0>();
+}
+
+// out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the parts of a row's unit, which WARPS warps share. Bound by the
+// latency of its loads: which parts there are follows from the lengths, which it adds up while the products still run,
+// so that behind them there is one round trip to memory. Up to some eight parts a row, one warp each; four where there
+// are more (one request of 32768 keys: 1776 parts for 32 rows).
+template <int D, int WARPS>
+__global__ void __launch_bounds__(128) decode4_join_kernel(const Decode4Params p) {
+  constexpr int EPL = D / 32;
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % WARPS;
+  const uint32_t row = blockIdx.x * (4 / WARPS) + (threadIdx.x >> 5) / WARPS;
+  const uint32_t kv_heads = p.heads / p.div_groups.d;
+  const uint32_t bh = row / p.G, head = row - bh * p.G;
+  const uint32_t b = bh / kv_heads, kvh = bh - b * kv_heads;
+  const bool here = b < static_cast<uint32_t>(p.B);
+  const uint32_t of_b = kvh * p.div_groups.d + head / kD4Heads;  // units of the request ahead of the row's
+  const int64_t unit = static_cast<int64_t>(b) * p.heads + of_b;
+  const uint32_t groups = here ? p.groups_of(p.length(b)) : 0;
+  uint32_t first = 0, n = 0;
+  if (p.B <= kD4Scan) {
+    uint32_t all = 0, before = 0;
+#pragma unroll
+    for (int i = 0; i < kD4Scan; i += 32) {
+      const uint32_t x = i + lane < p.B ? p.groups_of(p.length(i + lane)) : 0;
+      all += x;
+      before += i + lane < static_cast<int>(b) ? x : 0;
+    }
+    const uint32_t run = p.run(__reduce_add_sync(0xffffffffu, all) * p.heads);
+    const uint32_t from = __reduce_add_sync(0xffffffffu, before) * p.heads + of_b * groups;
+    first = from / run;
+    n = groups > 0 ? (from + groups - 1) / run - first + 1 : 0;
+  }
+  pdl_wait();
+  if (p.status && here && kvh == 0 && head == 0 && warp == 0 && lane == 0) {  // (what is cut is reported once)
+    const int len = p.seq_lens[b];
+    if (len < 0 || len > p.max_len) atomicCAS(p.status, 0, LF_DEV_BAD_LENGTHS);
+  }
+  if (p.B > kD4Scan && groups > 0) {
+    const int2 w = p.warps[unit];
+    first = w.x;
+    n = w.y - w.x + 1;
+  }
+  const int64_t at = (first + unit) * kD4Heads + head % kD4Heads;  // its parts: kD4Heads rows apart
+  float m_all = -INFINITY, l_all = 0.f, o[EPL] = {};
+  for (uint32_t s0 = warp; s0 < n; s0 += 8 * WARPS) {  // eight parts of this warp
+    float x[8][EPL];
+    float2 ml = make_float2(-INFINITY, 0.f);
+    if (s0 + WARPS * (lane & 7) < n) ml = p.part_ml[at + static_cast<int64_t>(s0 + WARPS * (lane & 7)) * kD4Heads];
+#pragma unroll
+    for (uint32_t u = 0; u < 8; ++u) {
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) x[u][e] = 0.f;
+      if (s0 + WARPS * u < n) {
+        const float* src = p.part_o + (at + static_cast<int64_t>(s0 + WARPS * u) * kD4Heads) * D + lane * EPL;
+        if constexpr (EPL == 4) {
+          const float4 v = *reinterpret_cast<const float4*>(src);
+          x[u][0] = v.x, x[u][1] = v.y, x[u][2] = v.z, x[u][3] = v.w;
+        } else {
+          const float2 v = *reinterpret_cast<const float2*>(src);
+          x[u][0] = v.x, x[u][1] = v.y;
+        }
+      }
+    }
+    float m_new = fmaxf(ml.x, m_all);
+#pragma unroll
+    for (int d = 4; d >= 1; d >>= 1) m_new = fmaxf(m_new, __shfl_xor_sync(0xffffffffu, m_new, d));
+    const float m_safe = m_new == -INFINITY ? 0.f : m_new;
+    const float back = ex2_approx(m_all - m_safe), wt = ex2_approx(ml.x - m_safe);
+    float l = ml.y * wt;
+#pragma unroll
+    for (int d = 4; d >= 1; d >>= 1) l += __shfl_xor_sync(0xffffffffu, l, d);
+    l_all = fmaf(l_all, back, l);
+    m_all = m_new;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) o[e] *= back;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const float wu = __shfl_sync(0xffffffffu, wt, u);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) o[e] = fmaf(x[u][e], wu, o[e]);
+    }
+  }
+  if constexpr (WARPS > 1) {  // (the whole CTA has one row)
+    __shared__ float s_o[WARPS][D];
+    __shared__ float2 s_ml[WARPS];
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) s_o[warp][lane * EPL + e] = o[e];
+    if (lane == 0) s_ml[warp] = make_float2(m_all, l_all);
+    __syncthreads();
+    if (warp > 0) return;
+    m_all = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) m_all = fmaxf(m_all, s_ml[i].x);
+    const float m_safe = m_all == -INFINITY ? 0.f : m_all;
+    l_all = 0.f;
+#pragma unroll
+    for (int e = 0; e < EPL; ++e) o[e] = 0.f;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) {
+      const float wt = ex2_approx(s_ml[i].x - m_safe);
+      l_all = fmaf(s_ml[i].y, wt, l_all);
+#pragma unroll
+      for (int e = 0; e < EPL; ++e) o[e] = fmaf(s_o[i][lane * EPL + e], wt, o[e]);
+    }
+  }
+  if (!here) return;
+  const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+  __nv_bfloat16* dst = p.out + b * p.o_stride[0] + kvh * p.o_stride[1] + head * p.o_stride[2] + lane * EPL;
+  if constexpr (EPL == 4)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
+  else
+    *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(o[0] * inv, o[1] * inv);
 }
 
 // How a call is cut, and the room for its parts.
@@ -510,7 +673,7 @@ struct Decode4Cut {
   size_t bytes(int D) const { return parts * (D + 2) * sizeof(float) + units * sizeof(int2); }
 };
 
-static Decode4Cut cut_decode4(int B, int Hkv, int G, int window, int max_len) {
+static Decode4Cut cut_decode4(int B, int Hkv, int G, int D, int window, int max_len) {
   static thread_local int cached_dev = -1, cached = 148;
   int dev = 0;
   if (cudaGetDevice(&dev) == cudaSuccess && dev != cached_dev) {
@@ -519,20 +682,20 @@ static Decode4Cut cut_decode4(int B, int Hkv, int G, int window, int max_len) {
   }
   Decode4Cut c;
   if (max_len <= 0) return c;
-  c.heads = Hkv * ((G + kOwnHeads - 1) / kOwnHeads);
+  c.heads = Hkv * ((G + kD4Heads - 1) / kD4Heads);
   c.units = static_cast<int64_t>(B) * c.heads;
   const int64_t seen = window > 0 ? std::min<int64_t>(max_len, static_cast<int64_t>(window) + 15) : max_len;
   const int64_t runs = (c.units * ((seen + kD4Group - 1) / kD4Group) + kD4Run - 1) / kD4Run;
-  c.ctas = static_cast<int>(std::min<int64_t>(runs, static_cast<int64_t>(kD4Ctas) * cached));
-  c.parts = static_cast<size_t>(c.units + c.ctas * kD4Warps) * kOwnHeads;
+  c.ctas = static_cast<int>(std::min<int64_t>(runs, static_cast<int64_t>(d4_ctas(D)) * cached));
+  c.parts = static_cast<size_t>(c.units + c.ctas * kD4Warps) * kD4Heads;
   return c;
 }
 
-template <int D, bool SOFTCAP>
+template <int D, bool SOFTCAP, bool EVEN>
 static int launch_decode4(const Decode4Params& p, unsigned grid, cudaStream_t st) {
   constexpr size_t smem = static_cast<size_t>(kD4Warps) * kD4Stages * 2 * kD4Group * Record4<D>::kBytes;
   static thread_local int configured_dev = -1;
-  const auto kernel = decode4_kernel<D, SOFTCAP>;
+  const auto kernel = decode4_kernel<D, SOFTCAP, EVEN>;
   const int rc = packed_configure(kernel, smem, &configured_dev);
   if (rc != LF_OK) return rc;
   launch_pdl(kernel, dim3(grid), kD4Warps * 32, smem, st, p);
@@ -547,7 +710,7 @@ size_t lf_decode_4bit_workspace_bytes(int32_t B, int32_t Hkv, int32_t G, int32_t
                                       int32_t max_seq_len) {
   using namespace lf;
   if (B <= 0 || Hkv <= 0 || G <= 0 || G > kPackedRows || D <= 0 || window < 0 || max_seq_len < 0) return 0;
-  return cut_decode4(B, Hkv, G, window, max_seq_len).bytes(D);
+  return cut_decode4(B, Hkv, G, D, window, max_seq_len).bytes(D);
 }
 
 int lf_decode_4bit(const LfDecode4Args* a, void* stream) {
@@ -563,20 +726,22 @@ int lf_decode_4bit(const LfDecode4Args* a, void* stream) {
   PackedScore score;
   const int rc = packed_score(a->scale, a->n_mod, a->mod_op, a->mod_arg, &score);
   if (rc != LF_OK) return rc;
-  const int head_groups = (a->G + kOwnHeads - 1) / kOwnHeads;
-  if (a->B > 65535 || static_cast<int64_t>(a->B) * a->Hkv * head_groups > (1 << 26)) return LF_ERR_TOO_LARGE;
+  if (!score.softcap && !(score.c2 <= 1e15f)) return LF_ERR_UNSUPPORTED;  // (in the units of the scores, below 2^127)
+  const int head_groups = (a->G + kD4Heads - 1) / kD4Heads;
+  const int64_t units = static_cast<int64_t>(a->B) * a->Hkv * head_groups;
+  if (a->B > 65535 || units > (1 << 26)) return LF_ERR_TOO_LARGE;
+  if (units * ((static_cast<int64_t>(a->max_seq_len) + kD4Group - 1) / kD4Group) > 0x7fffffff) return LF_ERR_TOO_LARGE;
   if (!packed_aligned(a->q) || !packed_aligned(a->out) || !record4_aligned(a->k, a->k_stride, a->D) ||
       !record4_aligned(a->v, a->v_stride, a->D))
     return LF_ERR_ALIGNMENT;
   for (int i = 0; i < 3; ++i)
     if (a->q_stride[i] % 8 || a->o_stride[i] % 4) return LF_ERR_ALIGNMENT;
-  const Decode4Cut cut = cut_decode4(a->B, a->Hkv, a->G, a->window, a->max_seq_len);
+  const Decode4Cut cut = cut_decode4(a->B, a->Hkv, a->G, a->D, a->window, a->max_seq_len);
   const size_t need = cut.bytes(a->D);
   if (need && (!a->workspace || a->workspace_bytes < need)) return LF_ERR_WORKSPACE;
   if (!packed_aligned(a->workspace)) return LF_ERR_ALIGNMENT;
 
   Decode4Params p = {};
-  JoinParams pj = {};
   p.part_o = static_cast<float*>(a->workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + cut.parts * a->D);
   p.warps = reinterpret_cast<int2*>(p.part_ml + cut.parts);
@@ -587,41 +752,48 @@ int lf_decode_4bit(const LfDecode4Args* a, void* stream) {
     p.q_stride[i] = a->q_stride[i];
     p.k_stride[i] = a->k_stride[i];
     p.v_stride[i] = a->v_stride[i];
-    pj.o_stride[i] = a->o_stride[i];
+    p.o_stride[i] = a->o_stride[i];
   }
   p.table = a->block_table;
   p.bt_stride = a->bt_stride;
-  p.seq_lens = pj.seq_lens = a->seq_lens;
+  p.seq_lens = a->seq_lens;
   p.B = a->B;
-  p.G = pj.G = a->G;
+  p.G = a->G;
   p.heads = a->Hkv * head_groups;
   p.div_groups = FastDiv::make(head_groups);
   p.window = a->window;
-  p.max_len = pj.max_len = a->max_seq_len;
+  p.max_len = a->max_seq_len;
   p.bt_blocks = a->bt_blocks;
   p.page_size = a->page_size;
   p.page_shift = cache_page_shift(a->page_size);
   p.n_pages = a->n_pages;
-  p.a = score.a;
-  p.c2 = score.c2;
-  p.status = pj.status = a->status;
-  pj.own_o = p.part_o;
-  pj.own_ml = p.part_ml;
-  pj.warps = p.warps;
-  pj.Hkv = a->Hkv;
-  pj.groups = head_groups;
-  pj.out = static_cast<__nv_bfloat16*>(a->out);
-  pj.rows = static_cast<int64_t>(a->B) * a->Hkv * a->G;
+  // (Scores come in units of 2^-69.)
+  p.a = score.a * kEven;
+  p.c2 = score.softcap ? score.c2 : score.c2 * kEven;
+  p.status = a->status;
+  p.n_warps = std::max(cut.ctas, 1) * kD4Warps;
+  p.out = static_cast<__nv_bfloat16*>(a->out);
+  const int64_t rows = static_cast<int64_t>(a->B) * a->Hkv * a->G;
+  bool even = p.page_shift >= 4 && a->k_stride[1] == LF_RECORD4_BYTES(a->D) && a->v_stride[1] == LF_RECORD4_BYTES(a->D);
+  const int64_t strides[4] = {a->k_stride[0], a->k_stride[2], a->v_stride[0], a->v_stride[2]};
+  for (int i = 0; i < 4; ++i) {
+    even = even && strides[i] >= 0 && strides[i] <= 0x7fffffff;
+    p.even_stride[i] = static_cast<int32_t>(strides[i]);
+  }
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto with_d = [&](auto d) {
     constexpr int D = decltype(d)::value;
     if (cut.ctas > 0) {
-      const int r = (score.softcap ? launch_decode4<D, true> : launch_decode4<D, false>)(
-          p, static_cast<unsigned>(cut.ctas), st);
+      const auto run = score.softcap ? (even ? launch_decode4<D, true, true> : launch_decode4<D, true, false>)
+                                     : (even ? launch_decode4<D, false, true> : launch_decode4<D, false, false>);
+      const int r = run(p, static_cast<unsigned>(cut.ctas), st);
       if (r != LF_OK) return r;
     }
-    launch_pdl(join_kernel<D>, dim3(static_cast<unsigned>((pj.rows + 3) / 4)), 128, 0, st, pj);
-    return check_launch("join_kernel");
+    if (p.n_warps > 6 * units)
+      launch_pdl(decode4_join_kernel<D, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, st, p);
+    else
+      launch_pdl(decode4_join_kernel<D, 1>, dim3(static_cast<unsigned>((rows + 3) / 4)), 128, 0, st, p);
+    return check_launch("decode4_join_kernel");
   };
   return a->D == 128 ? with_d(std::integral_constant<int, 128>{}) : with_d(std::integral_constant<int, 64>{});
 }
