@@ -8,6 +8,8 @@
 // Bound by HBM: every row is read once and written once; the arithmetic is some twenty operations per value.
 #include "lf_cache4.cuh"
 
+#include <type_traits>
+
 namespace lf {
 
 struct RotaryParams {
@@ -77,36 +79,66 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   return d;
 }
 
-// The eight columns of a lane as codes of 4 bits, the first in the lowest bits; scale and midpoint of the group,
-// which four neighbouring lanes share. Each step is rounded once (no fused product, no approximate
-// division), so that a row has one encoding.
-__device__ __forceinline__ uint32_t encode8(const float (&y)[8], uint16_t* scale, uint16_t* mid) {
-  float lo = y[0], hi = y[0];
-#pragma unroll
-  for (int e = 1; e < 8; ++e) {
-    lo = min_nan(lo, y[e]);
-    hi = max_nan(hi, y[e]);
-  }
-#pragma unroll
-  for (int d = 1; d <= 2; d <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-    hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-  }
+// Scale and midpoint of a group from its smallest and largest value. Each step is rounded once (no fused product, no
+// approximate division), so that a row has one encoding.
+struct Group4 {
+  uint16_t scale, mid;
+  float z, inv;
+};
+__device__ __forceinline__ Group4 group_of(float lo, float hi) {
+  Group4 g;
   const __nv_bfloat16 sb = __float2bfloat16_rn(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f));
   const float s = __bfloat162float(sb);
   const __nv_bfloat16 zb = __float2bfloat16_rn(__fadd_rn(lo, __fmul_rn(8.f, s)));
-  const float z = __bfloat162float(zb);
-  const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
-  uint32_t w = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float t = __fadd_rn(rintf(__fmul_rn(__fsub_rn(y[e], z), inv)), 8.f);
-    w |= static_cast<uint32_t>(fminf(fmaxf(t, 0.f), 15.f)) << (4 * e);  // (a NaN becomes 0: its group has a NaN scale)
-  }
-  *scale = __bfloat16_as_ushort(sb);
-  *mid = __bfloat16_as_ushort(zb);
-  return w;
+  g.z = __bfloat162float(zb);
+  g.inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+  g.scale = __bfloat16_as_ushort(sb);
+  g.mid = __bfloat16_as_ushort(zb);
+  return g;
 }
+
+__device__ __forceinline__ void range8(const float (&y)[8], float& lo, float& hi) {
+  auto min3_nan = [](float a, float b, float c) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+  };
+  auto max3_nan = [](float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+  };
+  lo = min_nan(min3_nan(min3_nan(y[0], y[1], y[2]), y[3], y[4]), min3_nan(y[5], y[6], y[7]));
+  hi = max_nan(max3_nan(max3_nan(y[0], y[1], y[2]), y[3], y[4]), max3_nan(y[5], y[6], y[7]));
+}
+
+// Eight columns as codes of 4 bits, the first in the lowest bits. A number in -8..7 plus 1.5 2^23 + 8 has its nearest
+// whole number, plus 8, in its last bits (ties to even, as rint), above constant ones that the sum takes off. (A NaN
+// becomes 0: its group has a NaN scale.)
+__device__ __forceinline__ uint32_t codes8(const float (&y)[8], const Group4& g) {
+  const uint64_t z2 = pack2(-g.z, -g.z), inv2 = pack2(g.inv, g.inv), magic = pack2(12582920.f, 12582920.f);
+  uint32_t u[8];
+#pragma unroll
+  for (int e = 0; e < 8; e += 2) {
+    float a, b;
+    unpack2(mul2(add2(pack2(y[e], y[e + 1]), z2), inv2), a, b);
+    a = fminf(fmaxf(a, -8.f), 7.f);
+    b = fminf(fmaxf(b, -8.f), 7.f);
+    unpack2(add2(pack2(a, b), magic), a, b);
+    u[e] = __float_as_uint(a);
+    u[e + 1] = __float_as_uint(b);
+  }
+  uint32_t w = u[7];
+#pragma unroll
+  for (int e = 6; e >= 0; --e) w = w * 16u + u[e];
+  return w - 0x4b400000u * 0x11111111u;
+}
+
+// Heads of an item of rows that are turned in full, and CTAs of an SM, with a norm and without: 21 thousand rows of 40
+// heads with a norm, four heads and three CTAs 78 us, two and four 80; the append of 33 thousand rows, two and four 124,
+// four and three 126.
+constexpr int full_heads(bool norm) { return norm ? 4 : 2; }
+constexpr int full_ctas(bool norm) { return norm ? 3 : 4; }
 
 enum RotaryStore { kStoreRows = 0, kStorePool16 = 1, kStorePool4 = 2 };
 
@@ -223,8 +255,15 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
     const bool store = stored && h < heads;
     if constexpr (STORE == kStorePool4) {
       using R = Record4<D>;
-      uint16_t scale, mid;
-      const uint32_t w = encode8(y, &scale, &mid);
+      float lo, hi;
+      range8(y, lo, hi);
+#pragma unroll
+      for (int d = 1; d <= 2; d <<= 1) {  // (four lanes a group)
+        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+      }
+      const Group4 group = group_of(lo, hi);
+      const uint32_t w = codes8(y, group);
       const int g = sub >> 2, i = sub & 3;
       // (A value's two halfwords lie in different pieces: lanes of neighbouring groups trade one for one, and each
       // stores a word.)
@@ -238,7 +277,7 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
         } else {
           *reinterpret_cast<uint32_t*>(rec + i * R::kKeyPiece + 4 * g) = w;
         }
-        if (i < 2) *reinterpret_cast<uint16_t*>(rec + (i ? R::kMids : R::kScales) + 2 * g) = i ? mid : scale;
+        if (i < 2) *reinterpret_cast<uint16_t*>(rec + (i ? R::kMids : R::kScales) + 2 * g) = i ? group.mid : group.scale;
       }
       if (is_q && store)
         *reinterpret_cast<uint4*>(p.q_out + t * p.qo_stride[0] + h * p.qo_stride[1] + 8 * sub) = pack8(y);
@@ -257,16 +296,177 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   }
 }
 
+// The same for rows that are turned in full, column i with i + D / 2: a lane has eight columns of either half, so that
+// what is turned together is in one lane, sums and ranges take fewer steps between lanes, and products go in pairs. (21
+// thousand rows of 40 heads, D = 128, with the norm: 108 us in the layout above, 78 in this one; bytes once at HBM's rate 67.)
+template <int D, int HEADS, int STORE, bool NORM>
+__global__ void __launch_bounds__(256, full_ctas(NORM)) rotary_full_kernel(const RotaryParams p) {
+  constexpr int LPR = D / 16, H = D / 2;  // lanes of a row
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, sub = lane % LPR;
+  const uint32_t index = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;
+  const bool here = index < p.items;  // (the others compute along: rows exchange values across lanes)
+  const uint32_t item = here ? index : p.items - 1;
+  const uint32_t t = p.div_parts.div(item);
+  const int part = static_cast<int>(item - t * p.div_parts.d);
+  const bool is_q = part < p.q_parts;
+  const bool is_v = STORE != kStoreRows && part >= p.q_parts + p.k_parts;
+  const int heads = is_q ? p.Hq : p.Hkv;
+  const int h0 = (is_q ? part : is_v ? part - p.q_parts - p.k_parts : part - p.q_parts) * HEADS;
+  const __nv_bfloat16* src = is_q ? p.q + t * p.q_stride[0] : is_v ? p.v + t * p.v_stride[0]
+                                                                  : p.k + t * p.k_stride[0];
+  const int64_t src_head = is_q ? p.q_stride[1] : is_v ? p.v_stride[1] : p.k_stride[1];
+  src += h0 * src_head + 8 * sub;
+  uint4 raw[HEADS][2];
+#pragma unroll
+  for (int u = 0; u < HEADS; ++u) {
+    raw[u][0] = raw[u][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (here && h0 + u < heads) {
+      raw[u][0] = ld_stream_16(src + u * src_head);
+      raw[u][1] = ld_stream_16(src + u * src_head + H);
+    }
+  }
+  float cs[8] = {}, sn[8] = {};
+  if (!is_v) {
+    int pos = p.positions[t];
+    if (pos < 0 || pos >= p.n_positions) {
+      if (p.status && here) atomicCAS(p.status, 0, LF_DEV_BAD_POSITION);
+      pos = min(max(pos, 0), p.n_positions - 1);
+    }
+    const float* row = p.table + pos * p.table_stride + 8 * sub;
+    load8(row, cs);
+    load8(row + H, sn);
+  }
+  const void* wp = !NORM || is_v ? nullptr : is_q ? p.q_weight : p.k_weight;
+  const bool f32 = is_q ? p.q_weight_f32 : p.k_weight_f32;
+  auto weights_of = [&](int at, float (&w)[8]) {
+    if (f32)
+      load8(static_cast<const float*>(wp) + at, w);
+    else
+      unpack8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(wp) + at), w);
+  };
+  // Where the rows go.
+  bool stored = here;
+  char* dst;
+  int64_t dst_head;
+  if (is_q || STORE == kStoreRows) {
+    dst = reinterpret_cast<char*>(is_q ? p.q_out + t * p.qo_stride[0] : p.k_out + t * p.ko_stride[0]);
+    dst_head = 2 * (is_q ? p.qo_stride[1] : p.ko_stride[1]);
+  } else {
+    const int at = p.slots[t];
+    stored = here && at >= 0 && at < p.n_slots;  // (negative: a row of the padding)
+    if (here && at >= p.n_slots && p.status) atomicCAS(p.status, 0, LF_DEV_BAD_PAGE);
+    const int safe = stored ? at : 0;
+    const int page = p.page_shift >= 0 ? safe >> p.page_shift : safe / p.page_size;
+    const int slot = safe - page * p.page_size;
+    dst = is_v ? p.v_pool + page * p.vp_stride[0] + slot * p.vp_stride[1]
+               : p.k_pool + page * p.kp_stride[0] + slot * p.kp_stride[1];
+    dst_head = is_v ? p.vp_stride[2] : p.kp_stride[2];
+  }
+  dst += h0 * dst_head;
+
+#pragma unroll
+  for (int u = 0; u < HEADS; ++u) {
+    float x[8], y[8];
+    unpack8(raw[u][0], x);
+    unpack8(raw[u][1], y);
+    if constexpr (NORM) {
+      uint64_t sum2 = 0;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const uint64_t a = pack2(x[e], x[e + 1]), b = pack2(y[e], y[e + 1]);
+        sum2 = fma2(b, b, fma2(a, a, sum2));
+      }
+      float ss, odd;
+      unpack2(sum2, ss, odd);
+      ss += odd;
+#pragma unroll
+      for (int d = 1; d < LPR; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+      if (wp) {
+        const float r = rsqrtf(ss * (1.f / D) + p.eps);
+        const uint64_t r2 = pack2(r, r);
+        auto scale = [&](float (&v)[8], const float (&by)[8]) {
+#pragma unroll
+          for (int e = 0; e < 8; e += 2)
+            unpack2(mul2(mul2(pack2(v[e], v[e + 1]), r2), pack2(by[e], by[e + 1])), v[e], v[e + 1]);
+        };
+        float weight[8];  // (read again for each head: in registers all along they cost more than that)
+        weights_of(8 * sub, weight);
+        scale(x, weight);
+        weights_of(8 * sub + H, weight);
+        scale(y, weight);
+      }
+    }
+    if (!is_v) {  // (each product and sum rounded once: pairs of products would be fused with the sums)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const uint64_t ac = pack2(__fmul_rn(x[e], cs[e]), __fmul_rn(x[e + 1], cs[e + 1]));
+        const uint64_t bs = pack2(__fmul_rn(y[e], -sn[e]), __fmul_rn(y[e + 1], -sn[e + 1]));
+        const uint64_t bc = pack2(__fmul_rn(y[e], cs[e]), __fmul_rn(y[e + 1], cs[e + 1]));
+        const uint64_t as = pack2(__fmul_rn(x[e], sn[e]), __fmul_rn(x[e + 1], sn[e + 1]));
+        unpack2(add2(ac, bs), x[e], x[e + 1]);
+        unpack2(add2(bc, as), y[e], y[e + 1]);
+      }
+    }
+    const bool store = stored && h0 + u < heads;
+    char* to = dst + u * dst_head;
+    if (STORE == kStorePool4) {
+      using R = Record4<D>;
+      // Group sub / 4 of the 32 columns of either half, four lanes each.
+      float lo[2], hi[2];
+      range8(x, lo[0], hi[0]);
+      range8(y, lo[1], hi[1]);
+#pragma unroll
+      for (int d = 1; d <= 2; d <<= 1)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          lo[i] = min_nan(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], d));
+          hi[i] = max_nan(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], d));
+        }
+      if (!is_q) {
+        const Group4 gx = group_of(lo[0], hi[0]), gy = group_of(lo[1], hi[1]);
+        const uint32_t wx = codes8(x, gx), wy = codes8(y, gy);
+        const int g = sub >> 2, i = sub & 3;
+        constexpr int kSecond = R::kGroups / 2;  // groups of a half
+        if (store) {
+          if (is_v) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              char* piece = to + (2 * i + j) * R::kValuePiece + 2 * g;
+              *reinterpret_cast<uint16_t*>(piece) = static_cast<uint16_t>(wx >> (16 * j));
+              *reinterpret_cast<uint16_t*>(piece + 2 * kSecond) = static_cast<uint16_t>(wy >> (16 * j));
+            }
+          } else {
+            *reinterpret_cast<uint32_t*>(to + i * R::kKeyPiece + 4 * g) = wx;
+            *reinterpret_cast<uint32_t*>(to + i * R::kKeyPiece + 4 * (g + kSecond)) = wy;
+          }
+          const Group4& mine = i & 2 ? gy : gx;  // (a lane each for the scales and midpoints of both)
+          *reinterpret_cast<uint16_t*>(to + (i & 1 ? R::kMids : R::kScales) + 2 * (g + (i & 2 ? kSecond : 0))) =
+              i & 1 ? mine.mid : mine.scale;
+        }
+        continue;
+      }
+    }
+    if (store) {
+      *reinterpret_cast<uint4*>(to + 16 * sub) = pack8(x);
+      *reinterpret_cast<uint4*>(to + 16 * sub + 2 * H) = pack8(y);
+    }
+  }
+}
+
 static bool rotary_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <int D, int HEADS>
-static void launch_rotary(const RotaryParams& p, int store, unsigned grid, cudaStream_t st) {
-  if (store == kStoreRows)
-    launch_pdl(rotary_kernel<D, HEADS, kStoreRows>, dim3(grid), 256, 0, st, p);
-  else if (store == kStorePool16)
-    launch_pdl(rotary_kernel<D, HEADS, kStorePool16>, dim3(grid), 256, 0, st, p);
+template <int D, int STORE>
+static void launch_rotary(const RotaryParams& p, bool full, bool few, unsigned grid, cudaStream_t st) {
+  if (full && (p.q_weight || p.k_weight))
+    launch_pdl(few ? rotary_full_kernel<D, 1, STORE, true> : rotary_full_kernel<D, full_heads(true), STORE, true>, dim3(grid), 256, 0,
+               st, p);
+  else if (full)
+    launch_pdl(few ? rotary_full_kernel<D, 1, STORE, false> : rotary_full_kernel<D, full_heads(false), STORE, false>, dim3(grid), 256,
+               0, st, p);
   else
-    launch_pdl(rotary_kernel<D, HEADS, kStorePool4>, dim3(grid), 256, 0, st, p);
+    launch_pdl(few ? rotary_kernel<D, 1, STORE> : rotary_kernel<D, 4, STORE>, dim3(grid), 256, 0, st, p);
 }
 
 }  // namespace lf
@@ -345,22 +545,29 @@ extern "C" int lf_rotary_bf16(const LfRotaryArgs* a, void* stream) {
   }
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  // Four heads an item; one where that leaves threads without work.
+  // Several heads an item: what is read for the token serves them all. One where that leaves threads without work.
+  const bool full = a->rot == a->D && !a->interleaved;
+  const int lanes = a->D / (full ? 16 : 8);
   const int64_t rows = static_cast<int64_t>(a->T) * (p.Hq + (pools ? 2 : 1) * p.Hkv);
-  const int heads = rows * (a->D / 8) <= 2048ll * sms ? 1 : 4;
+  const bool few = rows * lanes <= 2048ll * sms;
+  const int heads = few ? 1 : full ? full_heads(p.q_weight || p.k_weight) : 4;
   p.q_parts = (p.Hq + heads - 1) / heads;
   p.k_parts = (p.Hkv + heads - 1) / heads;
   const int64_t parts = p.q_parts + static_cast<int64_t>(pools ? 2 : 1) * p.k_parts;
   if (parts * a->T > 0x7fffffff) return LF_ERR_TOO_LARGE;
   p.div_parts = FastDiv::make(static_cast<int32_t>(parts));
   p.items = static_cast<uint32_t>(parts * a->T);
-  const unsigned per_cta = 256u / (a->D / 8);
+  const unsigned per_cta = 256u / lanes;
   const unsigned grid = (p.items + per_cta - 1) / per_cta;
-  const int store = !pools ? kStoreRows : four ? kStorePool4 : kStorePool16;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto run = [&](auto d) {
+    constexpr int D = decltype(d)::value;
+    (!pools ? launch_rotary<D, kStoreRows> : four ? launch_rotary<D, kStorePool4> : launch_rotary<D, kStorePool16>)(
+        p, full, few, grid, st);
+  };
   if (a->D == 128)
-    (heads == 1 ? launch_rotary<128, 1> : launch_rotary<128, 4>)(p, store, grid, st);
+    run(std::integral_constant<int, 128>{});
   else
-    (heads == 1 ? launch_rotary<64, 1> : launch_rotary<64, 4>)(p, store, grid, st);
+    run(std::integral_constant<int, 64>{});
   return check_launch("rotary_kernel");
 }
