@@ -583,7 +583,8 @@ int lf_kv_gather_4bit(const LfGather4Args* args, void* stream);
 
 /* Decode attention of requests of different lengths over a 4-bit paged cache, one token per request: what
  * lf_decode_paged_bf16 gives on the values that the records stand for, up to rounding (the weight of a key
- * times its scale is rounded to bf16 once per group of columns). Score functions as for
+ * times its scale is rounded to fp16 once per group of columns; weights below 2^-33 of the largest are lost, and
+ * columns of q below 2^-24 of the row's largest). Score functions as for
  * lf_packed_prefill_bf16. A request of length 0 gets zeros. With a window, table entries in front of its first
  * key are not read. Values of keys that a request sees must be finite. B up to 65535. The last bits
  * may change with the batch, never between two calls of the same one. */

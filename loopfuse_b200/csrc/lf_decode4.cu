@@ -3,18 +3,22 @@
 // With codes c, scales s and midpoints z of the groups g of 32 columns (include/lf_sm100.h has the format),
 //   score_j = sum_g sK_jg (q_g . (cK_jg - 8)) + sum_g zK_jg sum(q_g)
 //   o       = sum_g sum_j (p_j sV_jg) (cV_jg - 8) + sum_g sum_j p_j zV_jg,    p_j = 2^(score_j - m),
-// so a cache row is never unpacked to its values. A code in bits 0..3 (4..7) of a bf16 whose other bits are zero is the
-// subnormal number c 2^-133 (16 c 2^-133: the first normal binade carries on where the subnormals end), which a matrix
-// instruction multiplies exactly: one AND makes two operands of codes, and with the other factor times 2^64 the
-// products are ordinary fp32 numbers. Scales are applied to the scores of a group and to the weights; the 8 comes off where it was added: a
-// group's scores start at -8 sum(q), and the weights meet a constant -8 in a product of their own.
+// so a cache row is never unpacked to its values. A code in bits 0..3 (4..7) of an fp16 whose other bits are zero is the
+// subnormal number c 2^-24 (16 c 2^-24), which a matrix instruction multiplies exactly: one AND makes two operands of
+// codes, and the products, in fp32, are ordinary numbers again. Query rows, times a power of two that brings them into fp16's
+// range, are exact as well. Scales are applied to the scores of a group and to the weights; the 8 comes off where it was
+// added: scores get -8 sum(q) with each scale, and weights meet a constant -8 in a product of their own.
 //
-// Bound by HBM, 5/8 byte per value, if the integer pipe keeps up: an SM has to take some 40 values a clock, and that
-// pipe does 64 operations. (Codes with an exponent set above them, 128 + c and 16 + c three bits up, took 7 operations for
-// 8 codes where this takes 5, and long sums lost their last bits to the offsets: 65536 keys, against fp64, 0.015 with
-// one correction at the end.)
+// Bound by HBM, 5/8 byte per value, if the instructions keep up: an SM has to take some 40 values a clock, its integer pipe
+// does 64 operations and its matrix instructions, 50 for 32 keys, 2 clocks each. 16 requests of up to 65536 keys, 32 heads on
+// 8, D = 128: 155 us, 4.7 TB/s (bytes once at HBM's rate 112); 64 of up to 4096 39 (19).
+// Built before, at 16 x 35700 keys: codes with an exponent set above them, 128 + c and 16 + c three bits up, 187 us (7
+// operations for 8 codes where this takes 5, and offsets that cost long sums their last bits: an error of 0.015 for 65536
+// keys); codes as subnormal bf16 161, with an error of 0.0024 from the weights' rounding where this has 0.0017.
 #include "lf_cache4.cuh"
 #include "lf_packed.cuh"
+
+#include <float.h>
 
 #include <algorithm>
 #include <type_traits>
@@ -25,8 +29,8 @@ constexpr int kD4Warps = 4;
 constexpr int kD4Stages = 2;  // groups of a warp's ring: one is copied while one is computed
 constexpr int kD4Group = 32;   // tokens that a warp takes at a time
 constexpr int kD4Run = 1;      // groups of a warp, at least
-// CTAs of an SM: as many as fit without spilled registers (D = 128, four: 83 us for 32 x 8192 keys, three 78; D = 64,
-// three: 63, four 52).
+// CTAs of an SM: as many as fit without spilled registers (D = 128, 16 requests of up to 65536 keys: four 157 us, three
+// 149; D = 64, 32 of 8192: three 63, four 52).
 constexpr int d4_ctas(int D) { return D == 128 ? 3 : 4; }
 
 constexpr int kD4Heads = 8;     // query heads that a warp computes together: the columns of a matrix instruction
@@ -76,6 +80,7 @@ struct Decode4Params {
 struct Acc {
   float x[4];
 };
+// Products of bf16 and of fp16.
 __device__ __forceinline__ Acc mma_bf16(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
                                         const Acc& c) {
   Acc d;
@@ -86,6 +91,26 @@ __device__ __forceinline__ Acc mma_bf16(uint32_t a0, uint32_t a1, uint32_t a2, u
   return d;
 }
 
+__device__ __forceinline__ Acc mma_f16(uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                       const Acc& c) {
+  Acc d;
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 "
+      "{%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+      : "=f"(d.x[0]), "=f"(d.x[1]), "=f"(d.x[2]), "=f"(d.x[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c.x[0]), "f"(c.x[1]), "f"(c.x[2]), "f"(c.x[3]));
+  return d;
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// 2^(field - 127), field in 1..254; 1 / x for such an x.
+__device__ __forceinline__ float power(int field) { return __int_as_float(field << 23); }
+__device__ __forceinline__ float over(float x) { return __int_as_float(0x7f000000 - __float_as_int(x)); }
+
 // Transpose of an 8 x 8 matrix of 16-bit values held by a warp, two neighbours of a row per lane.
 __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   uint32_t y;
@@ -93,14 +118,14 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
   return y;
 }
 
-// The codes of both halves of a word as bf16: nibbles 0 and 4 in units of 2^-133, 1 and 5 in units of 2^-129.
+// The codes of both halves of a word as fp16: nibbles 0 and 4 in units of 2^-24, 1 and 5 in units of 2^-20.
 __device__ __forceinline__ uint32_t codes_even(uint32_t w) { return w & 0x000f000fu; }
 __device__ __forceinline__ uint32_t codes_odd(uint32_t w) { return w & 0x00f000f0u; }
 constexpr uint32_t kMinus8Even = 0x80088008u, kMinus8Odd = 0x80808080u;  // -8 in either unit
-constexpr float kUp = 0x1p64f;           // of the other factor
-constexpr float kProduct = 0x1p-69f;     // of a product with even codes; with odd ones, 2^-65
-constexpr float kEven = 0x1p69f, kOdd = 0x1p65f;
-constexpr float kRise = 8.f;             // weights may reach 2^8 before the reference moves
+// Weights are at most 2^4 (the reference of a row moves when a score rises further above it), a scale times its column
+// group's factor at most 2^11, so that their product is an fp16; weights below 2^-33 of the largest are lost.
+constexpr float kRise = 4.f;
+constexpr int kFactor = 11;
 
 template <int BYTES>
 __device__ __forceinline__ void cp_async_piece(uint32_t dst, const void* src) {
@@ -298,32 +323,63 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
     cp_async_commit();
   };
 
-  // The query heads of a unit: columns of the first product, in the order that the codes have; and the sums of the
-  // columns, which go with the midpoints (sum_z) and, times -8, with the scales (sum_s), as two or three bf16 each.
-  // Scores are in units of 2^-69 until they are scaled.
-  uint32_t qf[NG][4];
+  // The query heads of a unit: columns of the first product, in the order that the codes have (in shared memory: registers
+  // are what bounds the warps of an SM); and the sums of the columns, which go with the midpoints (sum_z) and, times -8, with the scales (sum_s), as two or three bf16 each.
+  // Scores are in units of a power of two of each row until they are scaled.
+  uint4* qf = reinterpret_cast<uint4*>(smem + kD4Warps * kD4Stages * kStageBytes) + warp * (32 * NG) + lane;
   uint32_t sum_z, sum_s;
+  float row_a[2], row_c2[2];  // query heads 2c, 2c + 1: score = row_c2 x, or row_c2 tanh(row_a x)
+  struct Query {
+    uint4 x[NG];
+  };
   auto load_q = [&] {
     int g0;
     const int kvh = kv_head(at.head, &g0);
+    Query r;
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      r.x[n] = make_uint4(0u, 0u, 0u, 0u);
+      if (g0 + g < p.G)
+        r.x[n] = *reinterpret_cast<const uint4*>(p.q + at.b * p.q_stride[0] + kvh * p.q_stride[1] +
+                                                 (g0 + g) * p.q_stride[2] + 32 * n + 8 * c);
+    }
+    return r;
+  };
+  auto take_q = [&](const Query& raw) {
+    // The row times 2^(14 - E), E the exponent of its largest column (0 or not a number: any). Products with even codes are
+    // in units of 2^(E - 14 - 24).
+    uint32_t top = 0;  // (numbers without their signs compare like whole ones)
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const uint32_t words[4] = {raw.x[n].x, raw.x[n].y, raw.x[n].z, raw.x[n].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) top = __vmaxu2(top, words[e] & 0x7fff7fffu);
+    }
+#pragma unroll
+    for (int d = 1; d <= 2; d <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d));
+    const int field = min(max(static_cast<int>(max(top >> 16, top & 0xffffu) >> 7), 30), 220);
+    const float up = power(268 - field), unit = power(field + 10);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      const float of_row = __shfl_sync(0xffffffffu, unit, 8 * c + 4 * r);
+      row_a[r] = p.a * of_row;
+      // (Neither zero nor infinite: with a masked score, or a score of zero, either would be NaN.)
+      row_c2[r] = SOFTCAP ? p.c2 : fminf(fmaxf(p.c2 * of_row, FLT_MIN), FLT_MAX);
+    }
     float sum[NG];
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
-      uint4 r = make_uint4(0u, 0u, 0u, 0u);
-      if (g0 + g < p.G)
-        r = *reinterpret_cast<const uint4*>(p.q + at.b * p.q_stride[0] + kvh * p.q_stride[1] +
-                                            (g0 + g) * p.q_stride[2] + 32 * n + 8 * c);
-      // (Times a power of two, exact; odd codes come times 16.)
-      const float x0 = bf16lo_to_f32(r.x), x1 = bf16hi_to_f32(r.x), x2 = bf16lo_to_f32(r.y), x3 = bf16hi_to_f32(r.y);
-      const float x4 = bf16lo_to_f32(r.z), x5 = bf16hi_to_f32(r.z), x6 = bf16lo_to_f32(r.w), x7 = bf16hi_to_f32(r.w);
-      qf[n][0] = pack_bf16x2(x0 * kUp, x4 * kUp);
-      qf[n][1] = pack_bf16x2(x1 * (kUp / 16), x5 * (kUp / 16));
-      qf[n][2] = pack_bf16x2(x2 * kUp, x6 * kUp);
-      qf[n][3] = pack_bf16x2(x3 * (kUp / 16), x7 * (kUp / 16));
+      const uint4 r = raw.x[n];
+      // (Exact, but for columns below 2^-24 of the largest; odd codes come times 16.)
+      const float x0 = bf16lo_to_f32(r.x) * up, x1 = bf16hi_to_f32(r.x) * up, x2 = bf16lo_to_f32(r.y) * up,
+                  x3 = bf16hi_to_f32(r.y) * up, x4 = bf16lo_to_f32(r.z) * up, x5 = bf16hi_to_f32(r.z) * up,
+                  x6 = bf16lo_to_f32(r.w) * up, x7 = bf16hi_to_f32(r.w) * up;
+      qf[32 * n] = make_uint4(pack_f16x2(x0, x4), pack_f16x2(x1 * 0.0625f, x5 * 0.0625f), pack_f16x2(x2, x6),
+                              pack_f16x2(x3 * 0.0625f, x7 * 0.0625f));
       float all_q = ((x0 + x1) + (x2 + x3)) + ((x4 + x5) + (x6 + x7));
 #pragma unroll
       for (int d = 1; d <= 2; d <<= 1) all_q += __shfl_xor_sync(0xffffffffu, all_q, d);
-      sum[n] = all_q * kProduct;
+      sum[n] = all_q * 0x1p-24f;
     }
     // Inner index 2c, 2c + 1 of the product of both: a pair of column groups, and a part of the sums.
     uint32_t part[3][NG / 2];
@@ -344,9 +400,13 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
     sum_s = pack_bf16x2(-8.f * bf16lo_to_f32(sum_z), -8.f * bf16hi_to_f32(sum_z));  // (exact)
   };
 
-  // Query heads 2c, 2c + 1. Pairs: of the sums over keys g and g + 8 (of every sixteen).
+  // Query heads 2c, 2c + 1; this lane's keys, until the end of the unit. A pair: keys g, and g + 8, of every sixteen.
   float m_run[2];
-  uint64_t l_run[2], mids[NG][2];
+  uint64_t l_run[2];
+  float mids[NG][2];
+  // Of a column group of V: 2^11 over a power of two that no scale so far is above; those powers, as bf16.
+  float factor[NG];
+  uint32_t most[NG / 2];
   Acc o[2 * NG];  // rows of instruction 2n + h: columns 32 n + 4 g + 2 h, then + 1; each for both heads
   auto clear = [&] {
 #pragma unroll
@@ -355,6 +415,11 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
       l_run[r] = 0;
 #pragma unroll
       for (int n = 0; n < NG; ++n) mids[n][r] = 0;
+    }
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      factor[n] = 1.f;
+      most[n / 2] = 0u;
     }
 #pragma unroll
     for (int n = 0; n < 2 * NG; ++n)
@@ -385,9 +450,9 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
 #pragma unroll
       for (int n = 0; n < NG; ++n) {
         const uint32_t u0 = w0[n] >> 8, u1 = w1[n] >> 8;
-        Acc y = mma_bf16(codes_even(w0[n]), codes_even(w1[n]), codes_odd(w0[n]), codes_odd(w1[n]), qf[n][0], qf[n][1],
-                         kZero);
-        y = mma_bf16(codes_even(u0), codes_even(u1), codes_odd(u0), codes_odd(u1), qf[n][2], qf[n][3], y);
+        const uint4 q = qf[32 * n];
+        Acc y = mma_f16(codes_even(w0[n]), codes_even(w1[n]), codes_odd(w0[n]), codes_odd(w1[n]), q.x, q.y, kZero);
+        y = mma_f16(codes_even(u0), codes_even(u1), codes_odd(u0), codes_odd(u1), q.z, q.w, y);
         const float a = n & 1 ? bf16hi_to_f32(s0[n / 2]) : bf16lo_to_f32(s0[n / 2]);
         const float b = n & 1 ? bf16hi_to_f32(s1[n / 2]) : bf16lo_to_f32(s1[n / 2]);
         x.x[0] = fmaf(a, y.x[0], x.x[0]);
@@ -398,7 +463,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float s = x.x[e];
-        if constexpr (SOFTCAP) s = tanh_approx(s * p.a);  // (the unit's, within 2^-11, as in decode)
+        if constexpr (SOFTCAP) s = tanh_approx(s * row_a[e & 1]);  // (the unit's, within 2^-11, as in decode)
         if (EDGE && hidden(16 * h + g + 8 * (e >> 1))) s = -INFINITY;
         sc[h][e] = s;
       }
@@ -406,9 +471,50 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
     // The reference of a row moves when a score rises more than kRise above it, not with every maximum: the lanes of
     // a row look at each other's scores only then.
     float mx[2];
-    mx[0] = fmaxf(max3(sc[0][0], sc[0][2], sc[1][0]), sc[1][2]) * p.c2;
-    mx[1] = fmaxf(max3(sc[0][1], sc[0][3], sc[1][1]), sc[1][3]) * p.c2;
-    if (__any_sync(0xffffffffu, mx[0] > m_run[0] + kRise || mx[1] > m_run[1] + kRise)) {
+    mx[0] = fmaxf(max3(sc[0][0], sc[0][2], sc[1][0]), sc[1][2]) * row_c2[0];
+    mx[1] = fmaxf(max3(sc[0][1], sc[0][3], sc[1][1]), sc[1][3]) * row_c2[1];
+    // Likewise the factor of a column group, when a scale is above all before it.
+    uint32_t top[NG / 2];
+    bool moves = mx[0] > m_run[0] + kRise || mx[1] > m_run[1] + kRise;
+    uint32_t meta[4][NG];  // scales, then midpoints, of keys g + 8 i
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      lds_words<NG>(stage + kHalf + (g + 8 * i) * R::kBytes + R::kScales, meta[i]);
+      if constexpr (EDGE) {  // (what lies in rows that are not seen may be NaN)
+        const bool no = hidden(g + 8 * i);
+#pragma unroll
+        for (int n = 0; n < NG; ++n) meta[i][n] = no ? 0u : meta[i][n];
+      }
+#pragma unroll
+      for (int n = 0; n < NG / 2; ++n) top[n] = __vmaxu2(i ? top[n] : most[n], meta[i][n]);
+    }
+#pragma unroll
+    for (int n = 0; n < NG / 2; ++n) moves = moves || top[n] != most[n];
+    if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+      for (int n = 0; n < NG / 2; ++n) {
+#pragma unroll
+        for (int d = 4; d <= 16; d <<= 1) top[n] = __vmaxu2(top[n], __shfl_xor_sync(0xffffffffu, top[n], d));
+        if (top[n] == most[n]) continue;
+        uint32_t now = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint32_t of = (top[n] >> (16 * i)) & 0xffffu, before = (most[n] >> (16 * i)) & 0xffffu;
+          // (Up to four times as large, none moves it again. From 2^-114 to 2^127; what is beyond is zero or not a number.)
+          const uint32_t field = of > before ? min(max(max(((of & 0x7fffu) >> 7) + 3u, before >> 7), 13u), 254u) : before >> 7;
+          now |= (field << 7) << (16 * i);
+          if (of > before) {
+            const float f = power(254 + kFactor - static_cast<int>(field)), by = f * over(factor[2 * n + i]);
+            factor[2 * n + i] = f;
+            if (before)
+#pragma unroll
+              for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[4 * n + 2 * i + t].x[e] *= by;
+          }
+        }
+        most[n] = now;
+      }
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
 #pragma unroll
@@ -419,7 +525,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
         const uint64_t alpha2 = pack2(alpha, alpha);
         l_run[r] = mul2(l_run[r], alpha2);
 #pragma unroll
-        for (int n = 0; n < NG; ++n) mids[n][r] = mul2(mids[n][r], alpha2);
+        for (int n = 0; n < NG; ++n) mids[n][r] *= alpha;
 #pragma unroll
         for (int n = 0; n < 2 * NG; ++n) {
           o[n].x[r] *= alpha;
@@ -427,11 +533,10 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
         }
       }
     }
-    // (Weights come times 2^64: the other factor of the codes.)
     uint64_t up[2];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float x = m_run[r] == -INFINITY ? 0.f : 64.f - m_run[r];
+      const float x = m_run[r] == -INFINITY ? 0.f : -m_run[r];
       up[r] = pack2(x, x);
     }
 
@@ -441,22 +546,13 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         float x, y;
-        unpack2(fma2(pack2(sc[h][r], sc[h][2 + r]), pack2(p.c2, p.c2), up[r]), x, y);
+        unpack2(fma2(pack2(sc[h][r], sc[h][2 + r]), pack2(row_c2[r], row_c2[r]), up[r]), x, y);
         pr[r] = pack2(ex2_approx(x), ex2_approx(y));
         l_run[r] = add2(l_run[r], pr[r]);  // this lane's share; the keys are summed at the end of the unit
       }
       const unsigned char* v = stage + kHalf + 16 * h * R::kBytes;
-      uint32_t s0[NG], s1[NG];  // scales, then midpoints, of keys g and g + 8
-      lds_words<NG>(v + g * R::kBytes + R::kScales, s0);
-      lds_words<NG>(v + (g + 8) * R::kBytes + R::kScales, s1);
-      if constexpr (EDGE) {  // (what lies in rows that are not seen may be NaN)
-        const bool no0 = hidden(16 * h + g), no1 = hidden(16 * h + g + 8);
-#pragma unroll
-        for (int n = 0; n < NG; ++n) {
-          s0[n] = no0 ? 0u : s0[n];
-          s1[n] = no1 ? 0u : s1[n];
-        }
-      }
+      const uint32_t(&s0)[NG] = meta[2 * h];
+      const uint32_t(&s1)[NG] = meta[2 * h + 1];
       // Codes of keys 2c, 2c + 1, 2c + 8, 2c + 9: [key][pair of column groups].
       uint32_t cv[4][NG / 2];
 #pragma unroll
@@ -469,12 +565,17 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
         const float za = n & 1 ? bf16hi_to_f32(s0[NG / 2 + n / 2]) : bf16lo_to_f32(s0[NG / 2 + n / 2]);
         const float zb = n & 1 ? bf16hi_to_f32(s1[NG / 2 + n / 2]) : bf16lo_to_f32(s1[NG / 2 + n / 2]);
         float x0, y0, x1, y1;
-        unpack2(mul2(pr[0], pack2(a, b)), x0, y0);
-        unpack2(mul2(pr[1], pack2(a, b)), x1, y1);
+        const uint64_t scaled = mul2(pack2(a, b), pack2(factor[n], factor[n]));
+        unpack2(mul2(pr[0], scaled), x0, y0);
+        unpack2(mul2(pr[1], scaled), x1, y1);
 #pragma unroll
-        for (int r = 0; r < 2; ++r) mids[n][r] = fma2(pr[r], pack2(za, zb), mids[n][r]);
-        const uint32_t pb0 = transpose_8x8(pack_bf16x2(x0, x1));
-        const uint32_t pb1 = transpose_8x8(pack_bf16x2(y0, y1));
+        for (int r = 0; r < 2; ++r) {
+          float pa, pb;
+          unpack2(pr[r], pa, pb);
+          mids[n][r] = fmaf(pa, za, fmaf(pb, zb, mids[n][r]));
+        }
+        const uint32_t pb0 = transpose_8x8(pack_f16x2(x0, x1));
+        const uint32_t pb1 = transpose_8x8(pack_f16x2(y0, y1));
         const uint32_t sel = n & 1 ? 0x7632u : 0x5410u;
         const uint32_t x = __byte_perm(cv[0][n / 2], cv[1][n / 2], sel);
         const uint32_t y = __byte_perm(cv[2][n / 2], cv[3][n / 2], sel);
@@ -482,20 +583,21 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
         for (int e = 0; e < 2; ++e) {
           const uint32_t ux = e ? x >> 8 : x, uy = e ? y >> 8 : y;
           Acc& d = o[2 * n + e];
-          d = mma_bf16(kMinus8Even, kMinus8Odd, kMinus8Even, kMinus8Odd, pb0, pb1, d);
-          d = mma_bf16(codes_even(ux), codes_odd(ux), codes_even(uy), codes_odd(uy), pb0, pb1, d);
+          d = mma_f16(kMinus8Even, kMinus8Odd, kMinus8Even, kMinus8Odd, pb0, pb1, d);
+          d = mma_f16(codes_even(ux), codes_odd(ux), codes_even(uy), codes_odd(uy), pb0, pb1, d);
         }
       }
     }
   };
 
   // A group is looked up while the one before it is copied, and that while the one before that is computed.
+  Query query = load_q();
   copy_group(look_up(), 0);
   Place next = look_up();
   int it = 0;
   while (left > 0) {
     // A unit, or the part of one that is this warp's.
-    load_q();
+    take_q(query);
     clear();
     const int unit = at.b * p.heads + at.head, first = p.first_token(at.end);
     if (lane == 0 && at.t == first) p.warps[unit].x = static_cast<int>(w);  // where the join finds the unit's parts
@@ -520,19 +622,21 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
     int g0;
     kv_head(at.head, &g0);
     const bool done = at.t >= at.end;
-    if (left > 0) at.next_unit(p, lane);
+    if (left > 0) {  // (the next one's queries come in under what is left to do: 64 requests of 1500 keys 39 -> 36.5 us)
+      at.next_unit(p, lane);
+      query = load_q();
+    }
     if (lane == 0 && done) p.warps[unit].y = static_cast<int>(w);
-    auto over_keys = [](uint64_t pair) {
-      float x, y;
-      unpack2(pair, x, y);
-      x += y;
+    auto over_keys = [](float x) {
 #pragma unroll
       for (int d = 4; d <= 16; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-      return x * (1.f / kUp);
+      return x;
     };
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float l = over_keys(l_run[r]);
+      float la, lb;
+      unpack2(l_run[r], la, lb);
+      const float l = over_keys(la + lb);
       float z[NG];
 #pragma unroll
       for (int n = 0; n < NG; ++n) z[n] = over_keys(mids[n][r]);
@@ -541,9 +645,10 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
         float* dst = p.part_o + place * D + 4 * g;
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
+          const float back = over(factor[n]), even = 0x1p24f * back, odd = 0x1p20f * back;
           *reinterpret_cast<float4*>(dst + 32 * n) =
-              make_float4(fmaf(o[2 * n].x[r], kEven, z[n]), fmaf(o[2 * n].x[2 + r], kOdd, z[n]),
-                          fmaf(o[2 * n + 1].x[r], kEven, z[n]), fmaf(o[2 * n + 1].x[2 + r], kOdd, z[n]));
+              make_float4(fmaf(o[2 * n].x[r], even, z[n]), fmaf(o[2 * n].x[2 + r], odd, z[n]),
+                          fmaf(o[2 * n + 1].x[r], even, z[n]), fmaf(o[2 * n + 1].x[2 + r], odd, z[n]));
         }
         if (g == 0) p.part_ml[place] = make_float2(m_run[r], l);
       }
@@ -593,6 +698,7 @@ __global__ void __launch_bounds__(128) decode4_join_kernel(const Decode4Params p
     first = w.x;
     n = w.y - w.x + 1;
   }
+  if (!LF_BOUNDS(n == 0 || first + n <= p.n_warps, p.status, 77)) n = 0;
   const int64_t at = (first + unit) * kD4Heads + head % kD4Heads;  // its parts: kD4Heads rows apart
   float m_all = -INFINITY, l_all = 0.f, o[EPL] = {};
   for (uint32_t s0 = warp; s0 < n; s0 += 8 * WARPS) {  // eight parts of this warp
@@ -673,6 +779,12 @@ struct Decode4Cut {
   size_t bytes(int D) const { return parts * (D + 2) * sizeof(float) + units * sizeof(int2); }
 };
 
+// Groups of the longest unit.
+static int64_t most_groups(int window, int max_len) {
+  const int64_t seen = window > 0 ? std::min<int64_t>(max_len, static_cast<int64_t>(window) + 15) : max_len;
+  return (seen + kD4Group - 1) / kD4Group;
+}
+
 static Decode4Cut cut_decode4(int B, int Hkv, int G, int D, int window, int max_len) {
   static thread_local int cached_dev = -1, cached = 148;
   int dev = 0;
@@ -684,8 +796,7 @@ static Decode4Cut cut_decode4(int B, int Hkv, int G, int D, int window, int max_
   if (max_len <= 0) return c;
   c.heads = Hkv * ((G + kD4Heads - 1) / kD4Heads);
   c.units = static_cast<int64_t>(B) * c.heads;
-  const int64_t seen = window > 0 ? std::min<int64_t>(max_len, static_cast<int64_t>(window) + 15) : max_len;
-  const int64_t runs = (c.units * ((seen + kD4Group - 1) / kD4Group) + kD4Run - 1) / kD4Run;
+  const int64_t runs = (c.units * most_groups(window, max_len) + kD4Run - 1) / kD4Run;
   c.ctas = static_cast<int>(std::min<int64_t>(runs, static_cast<int64_t>(d4_ctas(D)) * cached));
   c.parts = static_cast<size_t>(c.units + c.ctas * kD4Warps) * kD4Heads;
   return c;
@@ -693,7 +804,7 @@ static Decode4Cut cut_decode4(int B, int Hkv, int G, int D, int window, int max_
 
 template <int D, bool SOFTCAP, bool EVEN>
 static int launch_decode4(const Decode4Params& p, unsigned grid, cudaStream_t st) {
-  constexpr size_t smem = static_cast<size_t>(kD4Warps) * kD4Stages * 2 * kD4Group * Record4<D>::kBytes;
+  constexpr size_t smem = static_cast<size_t>(kD4Warps) * (kD4Stages * 2 * kD4Group * Record4<D>::kBytes + 16 * D);
   static thread_local int configured_dev = -1;
   const auto kernel = decode4_kernel<D, SOFTCAP, EVEN>;
   const int rc = packed_configure(kernel, smem, &configured_dev);
@@ -726,11 +837,10 @@ int lf_decode_4bit(const LfDecode4Args* a, void* stream) {
   PackedScore score;
   const int rc = packed_score(a->scale, a->n_mod, a->mod_op, a->mod_arg, &score);
   if (rc != LF_OK) return rc;
-  if (!score.softcap && !(score.c2 <= 1e15f)) return LF_ERR_UNSUPPORTED;  // (in the units of the scores, below 2^127)
   const int head_groups = (a->G + kD4Heads - 1) / kD4Heads;
   const int64_t units = static_cast<int64_t>(a->B) * a->Hkv * head_groups;
-  if (a->B > 65535 || units > (1 << 26)) return LF_ERR_TOO_LARGE;
-  if (units * ((static_cast<int64_t>(a->max_seq_len) + kD4Group - 1) / kD4Group) > 0x7fffffff) return LF_ERR_TOO_LARGE;
+  if (a->B > 65535 || units > (1 << 26) || units * most_groups(a->window, a->max_seq_len) > 0x7fffffff)
+    return LF_ERR_TOO_LARGE;
   if (!packed_aligned(a->q) || !packed_aligned(a->out) || !record4_aligned(a->k, a->k_stride, a->D) ||
       !record4_aligned(a->v, a->v_stride, a->D))
     return LF_ERR_ALIGNMENT;
@@ -767,9 +877,8 @@ int lf_decode_4bit(const LfDecode4Args* a, void* stream) {
   p.page_size = a->page_size;
   p.page_shift = cache_page_shift(a->page_size);
   p.n_pages = a->n_pages;
-  // (Scores come in units of 2^-69.)
-  p.a = score.a * kEven;
-  p.c2 = score.softcap ? score.c2 : score.c2 * kEven;
+  p.a = score.a;
+  p.c2 = score.c2;
   p.status = a->status;
   p.n_warps = std::max(cut.ctas, 1) * kD4Warps;
   p.out = static_cast<__nv_bfloat16*>(a->out);

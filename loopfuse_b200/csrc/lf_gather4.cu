@@ -85,6 +85,7 @@ __global__ void __launch_bounds__(256, kGatherCtas) gather4_kernel(const Gather4
       if (open && from <= t && t < end) {
         const int at = t - from, block = p.page_shift >= 0 ? at >> p.page_shift : at / p.page_size;
         slot = at - block * p.page_size;
+        if (!LF_BOUNDS(b >= 0 && at >= 0 && slot >= 0 && slot < p.page_size, p.status, 79)) slot = 0;
         page = block < p.bt_blocks ? p.table[b * p.bt_stride + block] : -1;
         if (page < 0 || page >= p.n_pages) {
           if (p.status) atomicCAS(p.status, 0, LF_DEV_BAD_PAGE);

@@ -944,15 +944,19 @@ std::pair<const char*, const char*> extent(const Tensor& t) {
   return {p, p + (last + 1) * t.element_size()};
 }
 
+void check_rows_apart(const Tensor& out, const char* name) {
+  for (int64_t i = 0; i + 1 < out.dim(); ++i)
+    if (out.size(i) > 1 && out.stride(i) < out.size(-1))
+      value_error(std::string(name) + " has rows that overlap");
+}
+
 // An output of `like`'s shape: made here, or the caller's, which may be `like` itself but not lie across it.
 Tensor out_like(Tensor out, const Tensor& like, const c10::Device& dev, const char* name) {
   if (!out.defined()) return new_bf16(like.sizes(), dev);
   require_cuda(out, dev);
   check_bf16(out, name);
   if (out.sizes() != like.sizes()) value_error(std::string(name) + " must have the shape of its input");
-  for (int64_t i = 0; i + 1 < out.dim(); ++i)
-    if (out.size(i) > 1 && out.stride(i) < out.size(-1))
-      value_error(std::string(name) + " has rows that overlap");
+  check_rows_apart(out, name);
   const auto x = extent(out), y = extent(like);
   if (x.first < y.second && y.first < x.second &&
       (out.data_ptr() != like.data_ptr() || out.strides() != like.strides()))
@@ -1118,7 +1122,9 @@ std::pair<Tensor, Tensor> run_kv_gather4(const Tensor& k_pool, const Tensor& v_p
     check_bf16(*t, "k_out and v_out");
     if (t->dim() != 3 || t->size(0) != T || t->size(1) != Hkv || t->size(2) != D)
       value_error("k_out and v_out must be [num_tokens, Hkv, D], got " + shape_text(t->sizes()));
+    check_rows_apart(*t, "k_out or v_out");
   }
+  if (T > 0 && k_out.data_ptr() == v_out.data_ptr()) value_error("k_out and v_out must not be the same rows");
   LfGather4Args a;
   std::memset(&a, 0, sizeof(a));
   a.k_pool = k_pool.data_ptr();

@@ -31,7 +31,7 @@ struct RotaryParams {
   FastDiv div_parts;                   // parts of a token: runs of heads of q, then of k, then of v
   uint32_t items;                      // tokens times parts
   int32_t q_parts, k_parts;
-  int32_t Hq, Hkv, rot, n_positions, interleaved, q_weight_f32, k_weight_f32;
+  int32_t Hq, Hkv, rot, n_positions, q_weight_f32, k_weight_f32;
   int32_t n_slots, page_size, page_shift;
   float eps;
   int32_t* status;
@@ -61,10 +61,13 @@ __device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
                     pack_bf16x2(x[6], x[7]));
 }
 
-__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+__device__ __forceinline__ void load4(const float* p, float* x) {
+  const float4 a = *reinterpret_cast<const float4*>(p);
   x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
-  x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  load4(p, x);
+  load4(p + 4, x + 4);
 }
 
 // Largest and smallest that let a NaN through, so that it reaches the group's scale.
@@ -134,19 +137,27 @@ __device__ __forceinline__ uint32_t codes8(const float (&y)[8], const Group4& g)
   return w - 0x4b400000u * 0x11111111u;
 }
 
-// Heads of an item of rows that are turned in full, and CTAs of an SM, with a norm and without: 21 thousand rows of 40
-// heads with a norm, four heads and three CTAs 78 us, two and four 80; the append of 33 thousand rows, two and four 124,
-// four and three 126.
-constexpr int full_heads(bool norm) { return norm ? 4 : 2; }
-constexpr int full_ctas(bool norm) { return norm ? 3 : 4; }
+// Heads of an item, and CTAs of an SM, with a norm and without: 21 thousand rows of 40 heads with a norm, four heads and
+// three CTAs 78 us, two and four 80; the append of 33 thousand rows, two and four 124, four and three 126.
+constexpr int rotary_heads(bool norm) { return norm ? 4 : 2; }
+constexpr int rotary_ctas(bool norm) { return norm ? 3 : 4; }
 
-enum RotaryStore { kStoreRows = 0, kStorePool16 = 1, kStorePool4 = 2 };
+enum RotaryStore { kStoreRows = 0, kStorePool16 = 1, kStorePool4 = 2 };  // where keys go
 
-// An item is a token and HEADS neighbouring heads of q, k or v, for D / 8 lanes with eight columns each: what a
-// position needs of the table is read once for the heads, and their loads are in flight together.
-template <int D, int HEADS, int STORE>
-__global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
-  constexpr int LPR = D / 8;  // lanes of a row
+// An item is a token and HEADS neighbouring heads of q, k or v, for D / 16 lanes with two pieces of eight columns each:
+// what a position needs of the table is read once for the heads, and their loads are in flight together. The pieces are
+// such that what is turned together is in one lane, so that products go in pairs and nothing is traded between lanes:
+//   kWhole, i with i + D / 2      pieces 8 l and D / 2 + 8 l, as for values
+//   kPart, i with i + rot / 2     pieces 8 l and rot / 2 + 8 l; columns that are not turned: two neighbours
+//   kPairs, 2 i with 2 i + 1      pieces 8 l and D / 2 + 8 l
+// For 4 bits, a group of 32 columns is one piece of four lanes, or both pieces of two. (kWhole is kPart with rot = D, where
+// known places save registers: 21 thousand rows of 40 heads with a norm 78 us instead of 82, a 4-bit append and gather of
+// 22 thousand 56 instead of 62.)
+enum RotaryLayout { kWhole = 0, kPart = 1, kPairs = 2 };
+template <int D, int HEADS, int STORE, bool NORM, int LAYOUT>
+__global__ void __launch_bounds__(256, rotary_ctas(NORM)) rotary_kernel(const RotaryParams p) {
+  constexpr int LPR = D / 16;  // lanes of a row
+  constexpr bool PAIRS = LAYOUT == kPairs;
   pdl_trigger();
   pdl_wait();
   const int lane = threadIdx.x & 31, sub = lane % LPR;
@@ -159,184 +170,49 @@ __global__ void __launch_bounds__(256) rotary_kernel(const RotaryParams p) {
   const bool is_v = STORE != kStoreRows && part >= p.q_parts + p.k_parts;
   const int heads = is_q ? p.Hq : p.Hkv;
   const int h0 = (is_q ? part : is_v ? part - p.q_parts - p.k_parts : part - p.q_parts) * HEADS;
+  // First columns of the pieces; whether they are turned; whether a piece is a part of a group, or both are.
+  const int half = LAYOUT == kWhole ? D / 2 : p.rot / 2;
+  const bool split = LAYOUT != kPart || is_v;
+  int ca = 8 * sub, cb = D / 2 + 8 * sub;
+  const bool turned = !is_v && (LAYOUT == kWhole || ca < (PAIRS ? p.rot : half));
+  [[maybe_unused]] const bool turned_b = PAIRS && !is_v && cb < p.rot;
+  if (!split) {
+    ca = turned ? 8 * sub : p.rot + 16 * (sub - half / 8);
+    cb = turned ? half + 8 * sub : ca + 8;
+  }
+  [[maybe_unused]] const bool piece = split || (turned && half % 32 == 0);
   const __nv_bfloat16* src = is_q ? p.q + t * p.q_stride[0] : is_v ? p.v + t * p.v_stride[0]
                                                                   : p.k + t * p.k_stride[0];
   const int64_t src_head = is_q ? p.q_stride[1] : is_v ? p.v_stride[1] : p.k_stride[1];
-  uint4 raw[HEADS];
+  src += h0 * src_head;
+  uint4 raw[HEADS][2];
 #pragma unroll
   for (int u = 0; u < HEADS; ++u) {
-    raw[u] = make_uint4(0u, 0u, 0u, 0u);
-    if (here && h0 + u < heads) raw[u] = ld_stream_16(src + (h0 + u) * src_head + 8 * sub);
+    raw[u][0] = raw[u][1] = make_uint4(0u, 0u, 0u, 0u);
+    if (here && h0 + u < heads) {
+      raw[u][0] = ld_stream_16(src + u * src_head + ca);
+      raw[u][1] = ld_stream_16(src + u * src_head + cb);
+    }
   }
-
-  // Cosines and sines of this lane's columns.
-  const int half = p.rot / 2;
-  const bool turned = !is_v && 8 * sub < p.rot;
+  // Cosines and sines of columns that are turned together; PAIRS: four of each piece.
   float cs[8], sn[8];
-  int partner = lane;
-  float sign = 1.f;
-  if (turned) {
+  if (turned || turned_b) {
     int pos = p.positions[t];
     if (pos < 0 || pos >= p.n_positions) {
       if (p.status && here) atomicCAS(p.status, 0, LF_DEV_BAD_POSITION);
       pos = min(max(pos, 0), p.n_positions - 1);
     }
     const float* row = p.table + pos * p.table_stride;
-    if (p.interleaved) {
-      const float4 c4 = *reinterpret_cast<const float4*>(row + 4 * sub);
-      const float4 s4 = *reinterpret_cast<const float4*>(row + half + 4 * sub);
-      cs[0] = cs[1] = c4.x, cs[2] = cs[3] = c4.y, cs[4] = cs[5] = c4.z, cs[6] = cs[7] = c4.w;
-      sn[0] = sn[1] = s4.x, sn[2] = sn[3] = s4.y, sn[4] = sn[5] = s4.z, sn[6] = sn[7] = s4.w;
+    if constexpr (PAIRS) {
+      const int ia = ca / 2, ib = turned_b ? cb / 2 : ia;
+      load4(row + ia, cs);
+      load4(row + ib, cs + 4);
+      load4(row + half + ia, sn);
+      load4(row + half + ib, sn + 4);
     } else {
-      const bool first = 8 * sub < half;
-      const int i = first ? 8 * sub : 8 * sub - half;
-      load8(row + i, cs);
-      load8(row + half + i, sn);
-      partner = first ? lane + half / 8 : lane - half / 8;
-      sign = first ? -1.f : 1.f;
+      load8(row + ca, cs);
+      load8(row + half + ca, sn);
     }
-  }
-  float weight[8];
-  const void* wp = is_q ? p.q_weight : is_v ? nullptr : p.k_weight;
-  if (wp) {
-    if (is_q ? p.q_weight_f32 : p.k_weight_f32) {
-      load8(static_cast<const float*>(wp) + 8 * sub, weight);
-    } else {
-      unpack8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(wp) + 8 * sub), weight);
-    }
-  }
-  // Where a cache row goes.
-  bool stored = here;
-  int64_t page = 0;
-  int slot = 0;
-  if constexpr (STORE != kStoreRows) {
-    if (!is_q) {
-      const int at = p.slots[t];
-      stored = here && at >= 0 && at < p.n_slots;  // (negative: a row of the padding)
-      if (stored) {
-        page = p.page_shift >= 0 ? at >> p.page_shift : at / p.page_size;
-        slot = at - static_cast<int>(page) * p.page_size;
-      } else if (here && at >= 0 && p.status) {
-        atomicCAS(p.status, 0, LF_DEV_BAD_PAGE);
-      }
-    }
-  }
-
-#pragma unroll
-  for (int u = 0; u < HEADS; ++u) {
-    float x[8], y[8];
-    unpack8(raw[u], x);
-    if (p.q_weight || p.k_weight) {  // (the same for all lanes)
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-      for (int d = 1; d < LPR; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
-      if (wp) {
-        const float r = rsqrtf(ss * (1.f / D) + p.eps);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = x[e] * r * weight[e];
-      }
-    }
-    if (p.interleaved) {
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        y[e] = turned ? __fsub_rn(__fmul_rn(x[e], cs[e]), __fmul_rn(x[e + 1], sn[e])) : x[e];
-        y[e + 1] = turned ? __fadd_rn(__fmul_rn(x[e + 1], cs[e]), __fmul_rn(x[e], sn[e])) : x[e + 1];
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float other = __shfl_sync(0xffffffffu, x[e], partner);
-        y[e] = turned ? __fadd_rn(__fmul_rn(x[e], cs[e]), __fmul_rn(sign * other, sn[e])) : x[e];
-      }
-    }
-    const int h = h0 + u;
-    const bool store = stored && h < heads;
-    if constexpr (STORE == kStorePool4) {
-      using R = Record4<D>;
-      float lo, hi;
-      range8(y, lo, hi);
-#pragma unroll
-      for (int d = 1; d <= 2; d <<= 1) {  // (four lanes a group)
-        lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
-        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
-      }
-      const Group4 group = group_of(lo, hi);
-      const uint32_t w = codes8(y, group);
-      const int g = sub >> 2, i = sub & 3;
-      // (A value's two halfwords lie in different pieces: lanes of neighbouring groups trade one for one, and each
-      // stores a word.)
-      const uint32_t traded = __shfl_xor_sync(0xffffffffu, (g & 1) ? w & 0xffffu : w >> 16, 4);
-      if (!is_q && store) {
-        const int64_t* st = is_v ? p.vp_stride : p.kp_stride;
-        char* rec = (is_v ? p.v_pool : p.k_pool) + page * st[0] + slot * st[1] + h * st[2];
-        if (is_v) {
-          const uint32_t both = (g & 1) ? traded | (w & 0xffff0000u) : (w & 0xffffu) | traded << 16;
-          *reinterpret_cast<uint32_t*>(rec + (2 * i + (g & 1)) * R::kValuePiece + 4 * (g >> 1)) = both;
-        } else {
-          *reinterpret_cast<uint32_t*>(rec + i * R::kKeyPiece + 4 * g) = w;
-        }
-        if (i < 2) *reinterpret_cast<uint16_t*>(rec + (i ? R::kMids : R::kScales) + 2 * g) = i ? group.mid : group.scale;
-      }
-      if (is_q && store)
-        *reinterpret_cast<uint4*>(p.q_out + t * p.qo_stride[0] + h * p.qo_stride[1] + 8 * sub) = pack8(y);
-    } else if (store) {
-      char* dst;
-      if (is_q)
-        dst = reinterpret_cast<char*>(p.q_out + t * p.qo_stride[0] + h * p.qo_stride[1]);
-      else if constexpr (STORE == kStoreRows)
-        dst = reinterpret_cast<char*>(p.k_out + t * p.ko_stride[0] + h * p.ko_stride[1]);
-      else if (is_v)
-        dst = p.v_pool + page * p.vp_stride[0] + slot * p.vp_stride[1] + h * p.vp_stride[2];
-      else
-        dst = p.k_pool + page * p.kp_stride[0] + slot * p.kp_stride[1] + h * p.kp_stride[2];
-      *reinterpret_cast<uint4*>(dst + 16 * sub) = pack8(y);
-    }
-  }
-}
-
-// The same for rows that are turned in full, column i with i + D / 2: a lane has eight columns of either half, so that
-// what is turned together is in one lane, sums and ranges take fewer steps between lanes, and products go in pairs. (21
-// thousand rows of 40 heads, D = 128, with the norm: 108 us in the layout above, 78 in this one; bytes once at HBM's rate 67.)
-template <int D, int HEADS, int STORE, bool NORM>
-__global__ void __launch_bounds__(256, full_ctas(NORM)) rotary_full_kernel(const RotaryParams p) {
-  constexpr int LPR = D / 16, H = D / 2;  // lanes of a row
-  pdl_trigger();
-  pdl_wait();
-  const int lane = threadIdx.x & 31, sub = lane % LPR;
-  const uint32_t index = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;
-  const bool here = index < p.items;  // (the others compute along: rows exchange values across lanes)
-  const uint32_t item = here ? index : p.items - 1;
-  const uint32_t t = p.div_parts.div(item);
-  const int part = static_cast<int>(item - t * p.div_parts.d);
-  const bool is_q = part < p.q_parts;
-  const bool is_v = STORE != kStoreRows && part >= p.q_parts + p.k_parts;
-  const int heads = is_q ? p.Hq : p.Hkv;
-  const int h0 = (is_q ? part : is_v ? part - p.q_parts - p.k_parts : part - p.q_parts) * HEADS;
-  const __nv_bfloat16* src = is_q ? p.q + t * p.q_stride[0] : is_v ? p.v + t * p.v_stride[0]
-                                                                  : p.k + t * p.k_stride[0];
-  const int64_t src_head = is_q ? p.q_stride[1] : is_v ? p.v_stride[1] : p.k_stride[1];
-  src += h0 * src_head + 8 * sub;
-  uint4 raw[HEADS][2];
-#pragma unroll
-  for (int u = 0; u < HEADS; ++u) {
-    raw[u][0] = raw[u][1] = make_uint4(0u, 0u, 0u, 0u);
-    if (here && h0 + u < heads) {
-      raw[u][0] = ld_stream_16(src + u * src_head);
-      raw[u][1] = ld_stream_16(src + u * src_head + H);
-    }
-  }
-  float cs[8] = {}, sn[8] = {};
-  if (!is_v) {
-    int pos = p.positions[t];
-    if (pos < 0 || pos >= p.n_positions) {
-      if (p.status && here) atomicCAS(p.status, 0, LF_DEV_BAD_POSITION);
-      pos = min(max(pos, 0), p.n_positions - 1);
-    }
-    const float* row = p.table + pos * p.table_stride + 8 * sub;
-    load8(row, cs);
-    load8(row + H, sn);
   }
   const void* wp = !NORM || is_v ? nullptr : is_q ? p.q_weight : p.k_weight;
   const bool f32 = is_q ? p.q_weight_f32 : p.k_weight_f32;
@@ -365,6 +241,7 @@ __global__ void __launch_bounds__(256, full_ctas(NORM)) rotary_full_kernel(const
     dst_head = is_v ? p.vp_stride[2] : p.kp_stride[2];
   }
   dst += h0 * dst_head;
+  if (!LF_BOUNDS(t < p.items / p.div_parts.d && h0 < heads && ca + 8 <= D && cb + 8 <= D, p.status, 78)) stored = false;
 
 #pragma unroll
   for (int u = 0; u < HEADS; ++u) {
@@ -392,13 +269,25 @@ __global__ void __launch_bounds__(256, full_ctas(NORM)) rotary_full_kernel(const
             unpack2(mul2(mul2(pack2(v[e], v[e + 1]), r2), pack2(by[e], by[e + 1])), v[e], v[e + 1]);
         };
         float weight[8];  // (read again for each head: in registers all along they cost more than that)
-        weights_of(8 * sub, weight);
+        weights_of(ca, weight);
         scale(x, weight);
-        weights_of(8 * sub + H, weight);
+        weights_of(cb, weight);
         scale(y, weight);
       }
     }
-    if (!is_v) {  // (each product and sum rounded once: pairs of products would be fused with the sums)
+    // (Each product and sum rounded once: pairs of products would be fused with the sums.)
+    if constexpr (PAIRS) {
+      auto turn = [](float (&v)[8], const float* c, const float* s) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float a = v[2 * e], b = v[2 * e + 1];
+          v[2 * e] = __fsub_rn(__fmul_rn(a, c[e]), __fmul_rn(b, s[e]));
+          v[2 * e + 1] = __fadd_rn(__fmul_rn(b, c[e]), __fmul_rn(a, s[e]));
+        }
+      };
+      if (turned) turn(x, cs, sn);
+      if (turned_b) turn(y, cs + 4, sn + 4);
+    } else if (turned) {
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         const uint64_t ac = pack2(__fmul_rn(x[e], cs[e]), __fmul_rn(x[e + 1], cs[e + 1]));
@@ -413,60 +302,187 @@ __global__ void __launch_bounds__(256, full_ctas(NORM)) rotary_full_kernel(const
     char* to = dst + u * dst_head;
     if (STORE == kStorePool4) {
       using R = Record4<D>;
-      // Group sub / 4 of the 32 columns of either half, four lanes each.
       float lo[2], hi[2];
       range8(x, lo[0], hi[0]);
       range8(y, lo[1], hi[1]);
+      if (!piece) {
+        lo[0] = lo[1] = min_nan(lo[0], lo[1]);
+        hi[0] = hi[1] = max_nan(hi[0], hi[1]);
+      }
 #pragma unroll
       for (int d = 1; d <= 2; d <<= 1)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          lo[i] = min_nan(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], d));
-          hi[i] = max_nan(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], d));
+          const float a = __shfl_xor_sync(0xffffffffu, lo[i], d), b = __shfl_xor_sync(0xffffffffu, hi[i], d);
+          if (d == 1 || piece) {
+            lo[i] = min_nan(lo[i], a);
+            hi[i] = max_nan(hi[i], b);
+          }
         }
       if (!is_q) {
-        const Group4 gx = group_of(lo[0], hi[0]), gy = group_of(lo[1], hi[1]);
+        const Group4 gx = group_of(lo[0], hi[0]), gy = piece ? group_of(lo[1], hi[1]) : gx;
         const uint32_t wx = codes8(x, gx), wy = codes8(y, gy);
-        const int g = sub >> 2, i = sub & 3;
-        constexpr int kSecond = R::kGroups / 2;  // groups of a half
+        const int ga = ca / 32, ia = ca / 8 % 4, gb = cb / 32, ib = cb / 8 % 4;
         if (store) {
           if (is_v) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              char* piece = to + (2 * i + j) * R::kValuePiece + 2 * g;
-              *reinterpret_cast<uint16_t*>(piece) = static_cast<uint16_t>(wx >> (16 * j));
-              *reinterpret_cast<uint16_t*>(piece + 2 * kSecond) = static_cast<uint16_t>(wy >> (16 * j));
+              *reinterpret_cast<uint16_t*>(to + (2 * ia + j) * R::kValuePiece + 2 * ga) = static_cast<uint16_t>(wx >> (16 * j));
+              *reinterpret_cast<uint16_t*>(to + (2 * ib + j) * R::kValuePiece + 2 * gb) = static_cast<uint16_t>(wy >> (16 * j));
             }
           } else {
-            *reinterpret_cast<uint32_t*>(to + i * R::kKeyPiece + 4 * g) = wx;
-            *reinterpret_cast<uint32_t*>(to + i * R::kKeyPiece + 4 * (g + kSecond)) = wy;
+            *reinterpret_cast<uint32_t*>(to + ia * R::kKeyPiece + 4 * ga) = wx;
+            *reinterpret_cast<uint32_t*>(to + ib * R::kKeyPiece + 4 * gb) = wy;
           }
-          const Group4& mine = i & 2 ? gy : gx;  // (a lane each for the scales and midpoints of both)
-          *reinterpret_cast<uint16_t*>(to + (i & 1 ? R::kMids : R::kScales) + 2 * (g + (i & 2 ? kSecond : 0))) =
-              i & 1 ? mine.mid : mine.scale;
+          // (A lane each for the scale and the midpoint of a group.)
+          const bool second = piece && (sub & 2);
+          const Group4& mine = second ? gy : gx;
+          *reinterpret_cast<uint16_t*>(to + (sub & 1 ? R::kMids : R::kScales) + 2 * (second ? gb : ga)) =
+              sub & 1 ? mine.mid : mine.scale;
         }
         continue;
       }
     }
     if (store) {
-      *reinterpret_cast<uint4*>(to + 16 * sub) = pack8(x);
-      *reinterpret_cast<uint4*>(to + 16 * sub + 2 * H) = pack8(y);
+      *reinterpret_cast<uint4*>(to + 2 * ca) = pack8(x);
+      *reinterpret_cast<uint4*>(to + 2 * cb) = pack8(y);
     }
+  }
+}
+
+// The same for keys of 4 bits of which a part is turned whose halves are neither whole groups of 32 columns nor lie in one:
+// a lane has eight neighbouring columns, four lanes are a group, and what is turned together is traded between lanes.
+// (21 thousand rows of 40 heads, D = 128, to bf16 with the norm: 108 us in this layout, 78 in the other.)
+template <int D>
+__global__ void __launch_bounds__(256) rotary_odd_kernel(const RotaryParams p) {
+  constexpr int HEADS = 4;
+  constexpr int LPR = D / 8;  // lanes of a row
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, sub = lane % LPR;
+  const uint32_t index = blockIdx.x * (256u / LPR) + threadIdx.x / LPR;
+  const bool here = index < p.items;  // (the others compute along: rows exchange values across lanes)
+  const uint32_t item = here ? index : p.items - 1;
+  const uint32_t t = p.div_parts.div(item);
+  const int part = static_cast<int>(item - t * p.div_parts.d);
+  const bool is_q = part < p.q_parts;
+  const bool is_v = part >= p.q_parts + p.k_parts;
+  const int heads = is_q ? p.Hq : p.Hkv;
+  const int h0 = (is_q ? part : is_v ? part - p.q_parts - p.k_parts : part - p.q_parts) * HEADS;
+  const __nv_bfloat16* src = is_q ? p.q + t * p.q_stride[0] : is_v ? p.v + t * p.v_stride[0]
+                                                                  : p.k + t * p.k_stride[0];
+  const int64_t src_head = is_q ? p.q_stride[1] : is_v ? p.v_stride[1] : p.k_stride[1];
+  uint4 raw[HEADS];
+#pragma unroll
+  for (int u = 0; u < HEADS; ++u) {
+    raw[u] = make_uint4(0u, 0u, 0u, 0u);
+    if (here && h0 + u < heads) raw[u] = ld_stream_16(src + (h0 + u) * src_head + 8 * sub);
+  }
+
+  // Cosines and sines of this lane's columns.
+  const int half = p.rot / 2;
+  const bool turned = !is_v && 8 * sub < p.rot;
+  float cs[8], sn[8];
+  int partner = lane;
+  float sign = 1.f;
+  if (turned) {
+    int pos = p.positions[t];
+    if (pos < 0 || pos >= p.n_positions) {
+      if (p.status && here) atomicCAS(p.status, 0, LF_DEV_BAD_POSITION);
+      pos = min(max(pos, 0), p.n_positions - 1);
+    }
+    const float* row = p.table + pos * p.table_stride;
+    const bool first = 8 * sub < half;
+    const int i = first ? 8 * sub : 8 * sub - half;
+    load8(row + i, cs);
+    load8(row + half + i, sn);
+    partner = first ? lane + half / 8 : lane - half / 8;
+    sign = first ? -1.f : 1.f;
+  }
+  float weight[8];
+  const void* wp = is_q ? p.q_weight : is_v ? nullptr : p.k_weight;
+  if (wp) {
+    if (is_q ? p.q_weight_f32 : p.k_weight_f32) {
+      load8(static_cast<const float*>(wp) + 8 * sub, weight);
+    } else {
+      unpack8(*reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(wp) + 8 * sub), weight);
+    }
+  }
+  // Where a cache row goes.
+  bool stored = here;
+  int64_t page = 0;
+  int slot = 0;
+  if (!is_q) {
+    const int at = p.slots[t];
+    stored = here && at >= 0 && at < p.n_slots;  // (negative: a row of the padding)
+    if (stored) {
+      page = p.page_shift >= 0 ? at >> p.page_shift : at / p.page_size;
+      slot = at - static_cast<int>(page) * p.page_size;
+    } else if (here && at >= 0 && p.status) {
+      atomicCAS(p.status, 0, LF_DEV_BAD_PAGE);
+    }
+  }
+
+#pragma unroll
+  for (int u = 0; u < HEADS; ++u) {
+    float x[8], y[8];
+    unpack8(raw[u], x);
+    if (p.q_weight || p.k_weight) {  // (the same for all lanes)
+      float ss = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+      for (int d = 1; d < LPR; d <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+      if (wp) {
+        const float r = rsqrtf(ss * (1.f / D) + p.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = x[e] * r * weight[e];
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float other = __shfl_sync(0xffffffffu, x[e], partner);
+      y[e] = turned ? __fadd_rn(__fmul_rn(x[e], cs[e]), __fmul_rn(sign * other, sn[e])) : x[e];
+    }
+    const int h = h0 + u;
+    const bool store = stored && h < heads;
+    using R = Record4<D>;
+    float lo, hi;
+    range8(y, lo, hi);
+#pragma unroll
+    for (int d = 1; d <= 2; d <<= 1) {  // (four lanes a group)
+      lo = min_nan(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+      hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+    }
+    const Group4 group = group_of(lo, hi);
+    const uint32_t w = codes8(y, group);
+    const int g = sub >> 2, i = sub & 3;
+    // (A value's two halfwords lie in different pieces: lanes of neighbouring groups trade one for one, and each
+    // stores a word.)
+    const uint32_t traded = __shfl_xor_sync(0xffffffffu, (g & 1) ? w & 0xffffu : w >> 16, 4);
+    if (!is_q && store) {
+      const int64_t* st = is_v ? p.vp_stride : p.kp_stride;
+      char* rec = (is_v ? p.v_pool : p.k_pool) + page * st[0] + slot * st[1] + h * st[2];
+      if (is_v) {
+        const uint32_t both = (g & 1) ? traded | (w & 0xffff0000u) : (w & 0xffffu) | traded << 16;
+        *reinterpret_cast<uint32_t*>(rec + (2 * i + (g & 1)) * R::kValuePiece + 4 * (g >> 1)) = both;
+      } else {
+        *reinterpret_cast<uint32_t*>(rec + i * R::kKeyPiece + 4 * g) = w;
+      }
+      if (i < 2) *reinterpret_cast<uint16_t*>(rec + (i ? R::kMids : R::kScales) + 2 * g) = i ? group.mid : group.scale;
+    }
+    if (is_q && store)
+      *reinterpret_cast<uint4*>(p.q_out + t * p.qo_stride[0] + h * p.qo_stride[1] + 8 * sub) = pack8(y);
   }
 }
 
 static bool rotary_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <int D, int STORE>
-static void launch_rotary(const RotaryParams& p, bool full, bool few, unsigned grid, cudaStream_t st) {
-  if (full && (p.q_weight || p.k_weight))
-    launch_pdl(few ? rotary_full_kernel<D, 1, STORE, true> : rotary_full_kernel<D, full_heads(true), STORE, true>, dim3(grid), 256, 0,
-               st, p);
-  else if (full)
-    launch_pdl(few ? rotary_full_kernel<D, 1, STORE, false> : rotary_full_kernel<D, full_heads(false), STORE, false>, dim3(grid), 256,
-               0, st, p);
-  else
-    launch_pdl(few ? rotary_kernel<D, 1, STORE> : rotary_kernel<D, 4, STORE>, dim3(grid), 256, 0, st, p);
+template <int D, int STORE, int LAYOUT>
+static void launch_rotary(const RotaryParams& p, bool few, unsigned grid, cudaStream_t st) {
+  const auto normed = few ? rotary_kernel<D, 1, STORE, true, LAYOUT> : rotary_kernel<D, rotary_heads(true), STORE, true, LAYOUT>;
+  const auto plain = few ? rotary_kernel<D, 1, STORE, false, LAYOUT> : rotary_kernel<D, rotary_heads(false), STORE, false, LAYOUT>;
+  launch_pdl(p.q_weight || p.k_weight ? normed : plain, dim3(grid), 256, 0, st, p);
 }
 
 }  // namespace lf
@@ -533,7 +549,6 @@ extern "C" int lf_rotary_bf16(const LfRotaryArgs* a, void* stream) {
   p.Hkv = a->Hkv;
   p.rot = a->rot;
   p.n_positions = a->n_positions;
-  p.interleaved = a->interleaved;
   p.q_weight_f32 = a->q_weight_f32;
   p.k_weight_f32 = a->k_weight_f32;
   p.eps = a->eps;
@@ -546,11 +561,13 @@ extern "C" int lf_rotary_bf16(const LfRotaryArgs* a, void* stream) {
   int dev = 0, sms = 148;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   // Several heads an item: what is read for the token serves them all. One where that leaves threads without work.
-  const bool full = a->rot == a->D && !a->interleaved;
-  const int lanes = a->D / (full ? 16 : 8);
+  const int store = !pools ? kStoreRows : four ? kStorePool4 : kStorePool16;
+  const bool norm = p.q_weight || p.k_weight;
+  const bool odd = four && !a->interleaved && a->rot > 32 && a->rot % 64 != 0;
+  const int lanes = a->D / (odd ? 8 : 16);
   const int64_t rows = static_cast<int64_t>(a->T) * (p.Hq + (pools ? 2 : 1) * p.Hkv);
   const bool few = rows * lanes <= 2048ll * sms;
-  const int heads = few ? 1 : full ? full_heads(p.q_weight || p.k_weight) : 4;
+  const int heads = odd ? 4 : few ? 1 : rotary_heads(norm);
   p.q_parts = (p.Hq + heads - 1) / heads;
   p.k_parts = (p.Hkv + heads - 1) / heads;
   const int64_t parts = p.q_parts + static_cast<int64_t>(pools ? 2 : 1) * p.k_parts;
@@ -560,14 +577,26 @@ extern "C" int lf_rotary_bf16(const LfRotaryArgs* a, void* stream) {
   const unsigned per_cta = 256u / lanes;
   const unsigned grid = (p.items + per_cta - 1) / per_cta;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto run = [&](auto d) {
-    constexpr int D = decltype(d)::value;
-    (!pools ? launch_rotary<D, kStoreRows> : four ? launch_rotary<D, kStorePool4> : launch_rotary<D, kStorePool16>)(
-        p, full, few, grid, st);
+  auto pick = [&](auto d, auto to) {
+    constexpr int D = decltype(d)::value, STORE = decltype(to)::value;
+    const auto run = a->interleaved ? launch_rotary<D, STORE, kPairs>
+                     : a->rot == D  ? launch_rotary<D, STORE, kWhole>
+                                    : launch_rotary<D, STORE, kPart>;
+    run(p, few, grid, st);
+  };
+  auto with_d = [&](auto d) {
+    if (odd)
+      launch_pdl(rotary_odd_kernel<decltype(d)::value>, dim3(grid), 256, 0, st, p);
+    else if (store == kStoreRows)
+      pick(d, std::integral_constant<int, kStoreRows>{});
+    else if (store == kStorePool16)
+      pick(d, std::integral_constant<int, kStorePool16>{});
+    else
+      pick(d, std::integral_constant<int, kStorePool4>{});
   };
   if (a->D == 128)
-    run(std::integral_constant<int, 128>{});
+    with_d(std::integral_constant<int, 128>{});
   else
-    run(std::integral_constant<int, 64>{});
+    with_d(std::integral_constant<int, 64>{});
   return check_launch("rotary_kernel");
 }

@@ -1,9 +1,10 @@
 """Decode attention over a 4-bit cache against float64 on the values that its records stand for.
 
-Tolerance of an output column: its own rounding, 2^-8 |o|; the rounding of each key's weight times its scale,
-2^-8 sum_j w_j s_j |c_j - 8|; and what an error d of the scores does to the weights, 2 d sum_j w_j |v_j|. d: sums in
-float32 of products of up to 143 |q| (codes with the exponent that was set above them) for each group's scale, and
-of the midpoints, 2^-20 of their sizes; with a softcap 2^-10 of the largest score (the unit's tanh is within 2^-11)."""
+Tolerance of an output column: its own rounding, 2^-8 |o|; the rounding of each key's weight times its scale to
+fp16, 2^-11 sum_j w_j s_j |c_j - 8|, or where that is subnormal 2^-33 of the largest scale, eight times, for each of n
+keys; and what an error d of the scores does to the weights, 2 d sum_j w_j |v_j|. d: the sums of the query row enter with
+16 bits, 2^-16 of 8 |sum q| s and of |sum q| |z|, and sums in float32 are within 2^-20 of products of up to 15 |q| s;
+with a softcap 2^-10 of the largest score (the unit's tanh is within 2^-11)."""
 import math
 
 import pytest
@@ -54,7 +55,8 @@ class Batch:
             cv, sv, zv = (x.transpose(0, 1) for x in cache4.parts(self.pools[1][at], self.D, True))
             qd = q[b].double()                          # Hkv, G, D; the others Hkv, n, D
             s = qd @ (zk + sk * ck).transpose(1, 2) * self.scale
-            d = 2 ** -20 * (143 * (qd.abs() @ sk.transpose(1, 2)) + qd.abs() @ zk.abs().transpose(1, 2)) * self.scale
+            d = (2 ** -13 + 15 * 2 ** -20) * (qd.abs() @ sk.transpose(1, 2))
+            d = (d + 2 ** -16 * (qd.abs() @ zk.abs().transpose(1, 2))) * self.scale
             d = d.amax(-1, keepdim=True)
             if cap:
                 s = cap * torch.tanh(s / cap)
@@ -62,7 +64,8 @@ class Batch:
             w = torch.softmax(s, -1)
             v = zv + sv * cv
             want = w @ v
-            tol = 2 ** -8 * want.abs() + 2 ** -8 * (w @ (sv * cv).abs()) + (2 * d + 2 ** -19) * (w @ v.abs())
+            tol = 2 ** -8 * want.abs() + 2 ** -11 * (w @ (sv * cv).abs()) + (2 * d + 2 ** -19) * (w @ v.abs())
+            tol = tol + n * 2 ** -30 * sv.amax(1, keepdim=True)
             off = (out[b].double() - want).abs()
             assert (off <= tol).all(), (b, n, (off / tol).max().item())
 
@@ -245,3 +248,35 @@ def test_serving_steps_over_a_4bit_cache():
             assert far < 4 * 2 ** -8
             assert math.isfinite(far) and (got[[b for b in range(3) if not new[b]]] == 0).all()
     F.check_status(st)
+
+
+def test_scales_and_queries_from_one_end_of_their_range_to_the_other():
+    """Column groups whose scales differ by 2^60 and grow from key to key, and query heads as far apart."""
+    x = Batch([200, 45], 2, 4, 128, 16, seed=21)
+    step = torch.linspace(-40, 40, x.pages * 16).reshape(x.pages, 16)
+    for group, sign in ((0, 1), (1, -1), (3, 0)):        # group 2 as it was
+        v = torch.randn(x.pages, 16, 2, 128, generator=torch.Generator().manual_seed(group)).cuda()
+        v = v * 2.0 ** (sign * step.cuda() if sign else torch.full_like(step, -55.0).cuda())[..., None, None]
+        rec = cache4.encode(v, True)
+        meta = 64 + 2 * group
+        x.pools[1][..., meta:meta + 2] = rec[..., meta:meta + 2]
+        x.pools[1][..., meta + 8:meta + 10] = rec[..., meta + 8:meta + 10]
+        for piece in range(8):                            # the group's 16-bit word of each piece
+            b = 8 * piece + 2 * group
+            x.pools[1][..., b:b + 2] = rec[..., b:b + 2]
+    x.q = x.q * torch.tensor([2.0 ** -50, 1.0, 2.0 ** -10, 2.0 ** 3], device="cuda")[:, None].bfloat16()
+    out = F.decode_attention_4bit(x.q, *x.pools, x.table, x.seq_lens, scale=x.scale)
+    x.check(out)
+    x.q[0, 0] *= 2.0 ** 40                                # and with a scale that brings them back
+    x.q[1, 1] *= 2.0 ** 40
+    out = F.decode_attention_4bit(x.q, *x.pools, x.table, x.seq_lens, scale=x.scale * 2.0 ** -40)
+    x.scale *= 2.0 ** -40
+    x.check(out)
+
+
+def test_a_scale_of_zero_weighs_all_keys_alike():
+    x = Batch([70, 33], 2, 4, 64, 16, seed=23)
+    x.q *= 2.0 ** -30
+    out = F.decode_attention_4bit(x.q, *x.pools, x.table, x.seq_lens, scale=0.0)
+    x.scale = 0.0
+    x.check(out)

@@ -114,7 +114,10 @@ def pool_of(bits, pages, page, Hkv, D, layout):
 @pytest.mark.parametrize("T,Hq,Hkv,D,rot,pairs,page,layout", [
     (1, 4, 1, 64, 64, False, 16, "head"), (1, 32, 8, 128, 128, False, 16, "page"), (19, 0, 3, 128, 64, True, 1, "head"),
     (70, 6, 2, 64, 16, False, 24, "slots"), (777, 8, 5, 128, 128, False, 16, "head"),
-    (1500, 0, 8, 64, 32, True, 64, "page"), (2049, 12, 4, 128, 96, False, 7, "slots")])
+    (1500, 0, 8, 64, 32, True, 64, "page"), (2049, 12, 4, 128, 96, False, 7, "slots"),
+    (300, 4, 2, 128, 64, False, 16, "head"), (90, 0, 2, 128, 32, False, 16, "head"), (333, 2, 1, 128, 16, False, 8, "page"),
+    (410, 2, 3, 64, 32, False, 16, "head"), (2100, 9, 3, 64, 48, False, 16, "slots"), (65, 5, 2, 128, 16, True, 32, "head"),
+    (2300, 8, 8, 128, 48, True, 16, "page"), (2500, 16, 8, 64, 64, True, 16, "head")])
 def test_append_bits(bits, T, Hq, Hkv, D, rot, pairs, page, layout):
     q, k, v = rows(T, max(Hq, 1), Hkv, D, T + 5)
     k[0], v[0] = 2.5, -0.75                              # groups of one value
@@ -308,6 +311,8 @@ def test_refusals():
         (ValueError, lambda: F.kv_gather_4bit(k_pool, v_pool, blocks, i32(0, 4, 4), 4)),
         (ValueError, lambda: F.kv_gather_4bit(k_pool, v_pool, blocks, i32(0, 4), -1)),
         (ValueError, lambda: F.kv_gather_4bit(k_pool, v_pool, blocks, i32(0, 4), 4, k_out=bf(5, 2, 64))),
+        (ValueError, lambda: F.kv_gather_4bit(k_pool, v_pool, blocks, i32(0, 4), 4, k_out=big[:, :2], v_out=big[:, :2])),
+        (ValueError, lambda: F.kv_gather_4bit(k_pool, v_pool, blocks, i32(0, 4), 4, k_out=bf(2, 64).expand(4, 2, 64))),
         (TypeError, lambda: F.decode_attention_4bit(bf(1, 2, 2, 64), k16, k16, blocks, i32(4))),
         (ValueError, lambda: F.decode_attention_4bit(bf(1, 2, 2, 128), k_pool, v_pool, blocks, i32(4))),
         (ValueError, lambda: F.decode_attention_4bit(bf(1, 1, 2, 64), k_pool, v_pool, blocks, i32(4))),
@@ -330,3 +335,36 @@ def test_no_rows():
     assert F.kv_append_rotary(k, v, k_pool, v_pool, none, none, table, q=q).shape == (0, 2, 64)
     cu = torch.zeros(2, dtype=torch.int32, device="cuda")
     assert F.kv_gather_4bit(k_pool, v_pool, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), cu, 0)[0].shape == (0, 2, 64)
+
+
+def test_a_step_in_a_graph_on_another_stream():
+    """Append with the norm, in place for q, then gather, recorded once and replayed on new rows."""
+    T, Hq, Hkv, D = 37, 8, 2, 128
+    q, k, v = rows(T, Hq, Hkv, D, 50)
+    table, w = cache4.rotary_table(64, D), torch.ones(D, device="cuda")
+    pos = torch.arange(T, dtype=torch.int32, device="cuda")
+    blocks, cu = torch.arange(3, device="cuda").int()[None], torch.tensor([0, T], dtype=torch.int32, device="cuda")
+    pools = F.kv_cache_4bit(3, 16, Hkv, D)
+    qs = q.clone()
+
+    def step(pools, q):
+        F.kv_append_rotary(k, v, *pools, pos, pos, table, q=q, q_weight=w, k_weight=w, q_out=q)
+        return F.kv_gather_4bit(*pools, blocks, cu, T)
+
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        got = step(pools, qs)
+    for seed in (51, 52):
+        fresh = rows(T, Hq, Hkv, D, seed)
+        qs.copy_(fresh[0])
+        k.copy_(fresh[1])
+        v.copy_(fresh[2])
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            graph.replay()
+        torch.cuda.synchronize()
+        other = F.kv_cache_4bit(3, 16, Hkv, D)
+        want_q = fresh[0].clone()
+        want = step(other, want_q)
+        assert torch.equal(qs, want_q) and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        assert all(torch.equal(a, b) for a, b in zip(pools, other))
