@@ -5,8 +5,8 @@
 //   o       = sum_g sum_j (p_j sV_jg) (cV_jg - 8) + sum_g sum_j p_j zV_jg,    p_j = 2^(score_j - m),
 // so a cache row is never unpacked to its values. A code in bits 0..3 (4..7) of an fp16 whose other bits are zero is the
 // subnormal number c 2^-24 (16 c 2^-24), which a matrix instruction multiplies exactly: one AND makes two operands of
-// codes, and the products, in fp32, are ordinary numbers again. Query rows, times a power of two that brings them into fp16's
-// range, are exact as well. Scales are applied to the scores of a group and to the weights; the 8 comes off where it was
+// codes, and the products, in fp32, are ordinary numbers again. Query rows, times a power of two that brings them into
+// fp16's range, are exact as well. Scales are applied to the scores of a group and to the weights; the 8 comes off where it was
 // added: scores get -8 sum(q) with each scale, and weights meet a constant -8 in a product of their own.
 //
 // Bound by HBM, 5/8 byte per value, if the instructions keep up: an SM has to take some 40 values a clock, its integer pipe
@@ -27,14 +27,14 @@ namespace lf {
 
 constexpr int kD4Warps = 4;
 constexpr int kD4Stages = 2;  // groups of a warp's ring: one is copied while one is computed
-constexpr int kD4Group = 32;   // tokens that a warp takes at a time
-constexpr int kD4Run = 1;      // groups of a warp, at least
+constexpr int kD4Group = 32;  // tokens that a warp takes at a time
+constexpr int kD4Run = 1;     // groups of a warp, at least
+constexpr int kD4Heads = 8;   // query heads that a warp computes together: the columns of a matrix instruction
+constexpr int kD4Scan = 128;  // up to so many requests, the join adds their lengths up itself
 // CTAs of an SM: as many as fit without spilled registers (D = 128, 16 requests of up to 65536 keys: four 157 us, three
 // 149; D = 64, 32 of 8192: three 63, four 52).
 constexpr int d4_ctas(int D) { return D == 128 ? 3 : 4; }
 
-constexpr int kD4Heads = 8;     // query heads that a warp computes together: the columns of a matrix instruction
-constexpr int kD4Scan = 128;    // up to so many requests, the join adds their lengths up itself
 
 struct Decode4Params {
   const __nv_bfloat16* q;
@@ -63,7 +63,7 @@ struct Decode4Params {
 
   // Keys of a request that count: never more than the caller said.
   __device__ __forceinline__ int length(int b) const { return min(max(seq_lens[b], 0), max_len); }
-  // Of those, the first that the groups begin with: that of the window, or of the sixteen it lies in (pages of 16 and more
+  // Of those, the first that the groups begin with: that of the sixteen which the window's first lies in (pages of 16, 32, ...
   // then hold whole halves of a group).
   __device__ __forceinline__ int first_token(int end) const {
     return window > 0 && end > window ? (end - window) & ~15 : 0;
@@ -185,7 +185,7 @@ struct D4Walk {
 //           are keys g, g + 8 of query heads 2c, 2c + 1.
 //   output  rows: 16 columns of V, inner dimension: 16 keys. Lane (g, c) reads piece g of keys 2c, 2c + 1, 2c + 8,
 //           2c + 9 and pairs halfwords of two keys. The weights, times the scale of a column group and rounded to
-//           bf16, get from the first product's layout to the second's by two 8 x 8 transposes.
+//           fp16, get from the first product's layout to the second's by two 8 x 8 transposes.
 //
 // EVEN: pages of a power of two of slots, 16 or more, whose rows lie next to each other: half a group is then one run
 // of bytes, and its place takes few operations (a lane's own row for each piece took 60 of a group's 820).
@@ -300,9 +300,10 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
       if constexpr (EVEN) {
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
-          const char* base = (kv ? p.v : p.k) + static_cast<int64_t>(x.kvh) * p.even_stride[2 * kv + 1] + lane * R::kAlign;
-          const char* lo = base + static_cast<int64_t>(x.page[0]) * p.even_stride[2 * kv] + x.slot[0] * R::kBytes;
-          const char* hi = base + static_cast<int64_t>(x.page[1]) * p.even_stride[2 * kv] + (x.slot[1] - 16) * R::kBytes;
+          const int64_t of_page = p.even_stride[2 * kv], of_head = p.even_stride[2 * kv + 1];
+          const char* base = (kv ? p.v : p.k) + x.kvh * of_head + lane * R::kAlign;
+          const char* lo = base + x.page[0] * of_page + x.slot[0] * R::kBytes;
+          const char* hi = base + x.page[1] * of_page + (x.slot[1] - 16) * R::kBytes;
           const char* mid = lane < 16 ? lo : hi;  // (a half is 2.5 pieces of each lane)
 #pragma unroll
           for (int i = 0; i < 5; ++i)
@@ -323,9 +324,10 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
     cp_async_commit();
   };
 
-  // The query heads of a unit: columns of the first product, in the order that the codes have (in shared memory: registers
-  // are what bounds the warps of an SM); and the sums of the columns, which go with the midpoints (sum_z) and, times -8, with the scales (sum_s), as two or three bf16 each.
-  // Scores are in units of a power of two of each row until they are scaled.
+  // The query heads of a unit: columns of the first product, in the order that the codes have (in shared memory:
+  // registers are what bounds the warps of an SM); and the sums of the columns, which go with the midpoints (sum_z) and,
+  // times -8, with the scales (sum_s), as two or three bf16 each. Scores are in units of a power of two, of each
+  // row, until they are scaled.
   uint4* qf = reinterpret_cast<uint4*>(smem + kD4Warps * kD4Stages * kStageBytes) + warp * (32 * NG) + lane;
   uint32_t sum_z, sum_s;
   float row_a[2], row_c2[2];  // query heads 2c, 2c + 1: score = row_c2 x, or row_c2 tanh(row_a x)
@@ -500,8 +502,9 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t of = (top[n] >> (16 * i)) & 0xffffu, before = (most[n] >> (16 * i)) & 0xffffu;
-          // (Up to four times as large, none moves it again. From 2^-114 to 2^127; what is beyond is zero or not a number.)
-          const uint32_t field = of > before ? min(max(max(((of & 0x7fffu) >> 7) + 3u, before >> 7), 13u), 254u) : before >> 7;
+          // (Up to four times as large, none moves it again. From 2^-114 to 2^127; what is beyond is zero or no number.)
+          const uint32_t wanted = min(max(((of & 0x7fffu) >> 7) + 3u, 13u), 254u);
+          const uint32_t field = of > before ? max(wanted, before >> 7) : before >> 7;
           now |= (field << 7) << (16 * i);
           if (of > before) {
             const float f = power(254 + kFactor - static_cast<int>(field)), by = f * over(factor[2 * n + i]);
@@ -622,7 +625,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
     int g0;
     kv_head(at.head, &g0);
     const bool done = at.t >= at.end;
-    if (left > 0) {  // (the next one's queries come in under what is left to do: 64 requests of 1500 keys 39 -> 36.5 us)
+    if (left > 0) {  // (the next one's queries come in under what is left to do: 64 requests of 1500 keys 39 -> 36 us)
       at.next_unit(p, lane);
       query = load_q();
     }
@@ -766,7 +769,8 @@ __global__ void __launch_bounds__(128) decode4_join_kernel(const Decode4Params p
   const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
   __nv_bfloat16* dst = p.out + b * p.o_stride[0] + kvh * p.o_stride[1] + head * p.o_stride[2] + lane * EPL;
   if constexpr (EPL == 4)
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
+    *reinterpret_cast<uint2*>(dst) =
+        make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
   else
     *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(o[0] * inv, o[1] * inv);
 }

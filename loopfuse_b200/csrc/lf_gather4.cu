@@ -32,7 +32,7 @@ __device__ __forceinline__ uint32_t value2(uint32_t codes, uint32_t s, uint32_t 
   return fma_bf16x2(c, s, z);
 }
 
-// Tokens of a warp, CTAs of an SM, and rows of a lane whose loads are in flight together. 55 thousand tokens of 8 heads,
+// Tokens of a warp, CTAs of an SM, rows of a lane whose loads are in flight together. 55 thousand tokens of 8 heads,
 // D = 128: 51 us; three CTAs of two rows 53 (four of them 59), eight tokens 58, sixteen 61.
 constexpr int kGatherTokens = 4, kGatherCtas = 2, kGatherRows = 4;
 

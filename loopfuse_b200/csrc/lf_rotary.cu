@@ -327,8 +327,10 @@ __global__ void __launch_bounds__(256, rotary_ctas(NORM)) rotary_kernel(const Ro
           if (is_v) {
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              *reinterpret_cast<uint16_t*>(to + (2 * ia + j) * R::kValuePiece + 2 * ga) = static_cast<uint16_t>(wx >> (16 * j));
-              *reinterpret_cast<uint16_t*>(to + (2 * ib + j) * R::kValuePiece + 2 * gb) = static_cast<uint16_t>(wy >> (16 * j));
+              char* pa = to + (2 * ia + j) * R::kValuePiece + 2 * ga;
+              char* pb = to + (2 * ib + j) * R::kValuePiece + 2 * gb;
+              *reinterpret_cast<uint16_t*>(pa) = static_cast<uint16_t>(wx >> (16 * j));
+              *reinterpret_cast<uint16_t*>(pb) = static_cast<uint16_t>(wy >> (16 * j));
             }
           } else {
             *reinterpret_cast<uint32_t*>(to + ia * R::kKeyPiece + 4 * ga) = wx;
@@ -480,8 +482,10 @@ static bool rotary_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(
 
 template <int D, int STORE, int LAYOUT>
 static void launch_rotary(const RotaryParams& p, bool few, unsigned grid, cudaStream_t st) {
-  const auto normed = few ? rotary_kernel<D, 1, STORE, true, LAYOUT> : rotary_kernel<D, rotary_heads(true), STORE, true, LAYOUT>;
-  const auto plain = few ? rotary_kernel<D, 1, STORE, false, LAYOUT> : rotary_kernel<D, rotary_heads(false), STORE, false, LAYOUT>;
+  const auto normed = few ? rotary_kernel<D, 1, STORE, true, LAYOUT>
+                          : rotary_kernel<D, rotary_heads(true), STORE, true, LAYOUT>;
+  const auto plain = few ? rotary_kernel<D, 1, STORE, false, LAYOUT>
+                         : rotary_kernel<D, rotary_heads(false), STORE, false, LAYOUT>;
   launch_pdl(p.q_weight || p.k_weight ? normed : plain, dim3(grid), 256, 0, st, p);
 }
 
