@@ -305,22 +305,28 @@ __global__ void __launch_bounds__(256, rotary_ctas(NORM)) rotary_kernel(const Ro
       float lo[2], hi[2];
       range8(x, lo[0], hi[0]);
       range8(y, lo[1], hi[1]);
-      if (!piece) {
-        lo[0] = lo[1] = min_nan(lo[0], lo[1]);
-        hi[0] = hi[1] = max_nan(hi[0], hi[1]);
+      // A lane makes one group, of either piece or of both, and has the other's numbers from the lane that makes that.
+      const bool second = piece && (sub & 2);
+      float low = piece ? (second ? lo[1] : lo[0]) : min_nan(lo[0], lo[1]);
+      float high = piece ? (second ? hi[1] : hi[0]) : max_nan(hi[0], hi[1]);
+      const float low2 = __shfl_xor_sync(0xffffffffu, second ? lo[0] : lo[1], 2);
+      const float high2 = __shfl_xor_sync(0xffffffffu, second ? hi[0] : hi[1], 2);
+      if (piece) {
+        low = min_nan(low, low2);
+        high = max_nan(high, high2);
       }
-#pragma unroll
-      for (int d = 1; d <= 2; d <<= 1)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float a = __shfl_xor_sync(0xffffffffu, lo[i], d), b = __shfl_xor_sync(0xffffffffu, hi[i], d);
-          if (d == 1 || piece) {
-            lo[i] = min_nan(lo[i], a);
-            hi[i] = max_nan(hi[i], b);
-          }
+      low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, 1));
+      high = max_nan(high, __shfl_xor_sync(0xffffffffu, high, 1));
+      const Group4 mine = group_of(low, high);
+      Group4 gx = mine, gy = mine;
+      {
+        const float z = __shfl_xor_sync(0xffffffffu, mine.z, 2), inv = __shfl_xor_sync(0xffffffffu, mine.inv, 2);
+        if (piece) {
+          gx.z = second ? z : mine.z, gx.inv = second ? inv : mine.inv;
+          gy.z = second ? mine.z : z, gy.inv = second ? mine.inv : inv;
         }
+      }
       if (!is_q) {
-        const Group4 gx = group_of(lo[0], hi[0]), gy = piece ? group_of(lo[1], hi[1]) : gx;
         const uint32_t wx = codes8(x, gx), wy = codes8(y, gy);
         const int ga = ca / 32, ia = ca / 8 % 4, gb = cb / 32, ib = cb / 8 % 4;
         if (store) {
@@ -337,8 +343,6 @@ __global__ void __launch_bounds__(256, rotary_ctas(NORM)) rotary_kernel(const Ro
             *reinterpret_cast<uint32_t*>(to + ib * R::kKeyPiece + 4 * gb) = wy;
           }
           // (A lane each for the scale and the midpoint of a group.)
-          const bool second = piece && (sub & 2);
-          const Group4& mine = second ? gy : gx;
           *reinterpret_cast<uint16_t*>(to + (sub & 1 ? R::kMids : R::kScales) + 2 * (second ? gb : ga)) =
               sub & 1 ? mine.mid : mine.scale;
         }
@@ -562,8 +566,12 @@ extern "C" int lf_rotary_bf16(const LfRotaryArgs* a, void* stream) {
     p.page_size = a->page_size;
     p.page_shift = cache_page_shift(a->page_size);
   }
-  int dev = 0, sms = 148;
-  if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  static thread_local int cached_dev = -1, sms = 148;
+  int dev = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && dev != cached_dev) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) sms = 148;
+    cached_dev = dev;
+  }
   // Several heads an item: what is read for the token serves them all. One where that leaves threads without work.
   const int store = !pools ? kStoreRows : four ? kStorePool4 : kStorePool16;
   const bool norm = p.q_weight || p.k_weight;
