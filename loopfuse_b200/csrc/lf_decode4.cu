@@ -2,19 +2,19 @@
 //
 // With codes c, scales s and midpoints z of the groups g of 32 columns (include/lf_sm100.h has the format),
 //   score_j = sum_g sK_jg (q_g . (cK_jg - 8)) + sum_g zK_jg sum(q_g)
-//   o       = sum_g sum_j (p_j sV_jg) (cV_jg - 8) + sum_g sum_j p_j zV_jg,    p_j = 2^(score_j - m),
+//   o       = sum_g sum_j (p_j sV_jg) cV_jg + sum_g sum_j p_j (zV_jg - 8 sV_jg),    p_j = 2^(score_j - m),
 // so a cache row is never unpacked to its values. A code in bits 0..3 (4..7) of an fp16 whose other bits are zero is the
 // subnormal number c 2^-24 (16 c 2^-24), which a matrix instruction multiplies exactly: one AND makes two operands of
 // codes, and the products, in fp32, are ordinary numbers again. Query rows, times a power of two that brings them into
-// fp16's range, are exact as well. Scales are applied to the scores of a group and to the weights; the 8 comes off where it was
-// added: scores get -8 sum(q) with each scale, and weights meet a constant -8 in a product of their own.
+// fp16's range, are exact as well. Scales are applied to the scores of a group and to the weights.
 //
 // Bound by HBM, 5/8 byte per value, if the instructions keep up: an SM has to take some 40 values a clock, its integer pipe
-// does 64 operations and its matrix instructions, 50 for 32 keys, 2 clocks each. 16 requests of up to 65536 keys, 32 heads on
-// 8, D = 128: 155 us, 4.7 TB/s (bytes once at HBM's rate 112); 64 of up to 4096 39 (19).
-// Built before, at 16 x 35700 keys: codes with an exponent set above them, 128 + c and 16 + c three bits up, 187 us (7
-// operations for 8 codes where this takes 5, and offsets that cost long sums their last bits: an error of 0.015 for 65536
-// keys); codes as subnormal bf16 161, with an error of 0.0024 from the weights' rounding where this has 0.0017.
+// does 64 operations and its matrix instructions, 34 for 32 keys, 2 clocks each. 16 requests of up to 65536 keys, 32 heads on
+// 8, D = 128: 149 us, 4.9 TB/s (bytes once at HBM's rate 112); 64 of up to 4096 38 (19).
+// Built before: codes with an exponent set above them, 128 + c and 16 + c three bits up, 187 us (7 operations for 8 codes
+// where this takes 5, and offsets that cost long sums their last bits: an error of 0.015); codes as subnormal bf16 151,
+// with an error of 0.0024 from the weights' rounding where this has 0.0017; c - 8 by a product of the weights with a
+// constant in each step, 155.
 #include "lf_cache4.cuh"
 #include "lf_packed.cuh"
 
@@ -121,11 +121,11 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
 // The codes of both halves of a word as fp16: nibbles 0 and 4 in units of 2^-24, 1 and 5 in units of 2^-20.
 __device__ __forceinline__ uint32_t codes_even(uint32_t w) { return w & 0x000f000fu; }
 __device__ __forceinline__ uint32_t codes_odd(uint32_t w) { return w & 0x00f000f0u; }
-constexpr uint32_t kMinus8Even = 0x80088008u, kMinus8Odd = 0x80808080u;  // -8 in either unit
 // Weights are at most 2^4 (the reference of a row moves when a score rises further above it), a scale times its column
 // group's factor at most 2^11, so that their product is an fp16; weights below 2^-33 of the largest are lost.
 constexpr float kRise = 4.f;
 constexpr int kFactor = 11;
+constexpr int kMeet = 16;  // groups after which the sums of codes and bottoms meet (8 and 64: within 1 %)
 
 template <int BYTES>
 __device__ __forceinline__ void cp_async_piece(uint32_t dst, const void* src) {
@@ -405,7 +405,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
   // Query heads 2c, 2c + 1; this lane's keys, until the end of the unit. A pair: keys g, and g + 8, of every sixteen.
   float m_run[2];
   uint64_t l_run[2];
-  float mids[NG][2];
+  float bottoms[NG][2];  // weights times what codes of 0 stand for
   // Of a column group of V: 2^11 over a power of two that no scale so far is above; those powers, as bf16.
   float factor[NG];
   uint32_t most[NG / 2];
@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
       m_run[r] = -INFINITY;
       l_run[r] = 0;
 #pragma unroll
-      for (int n = 0; n < NG; ++n) mids[n][r] = 0;
+      for (int n = 0; n < NG; ++n) bottoms[n][r] = 0.f;
     }
 #pragma unroll
     for (int n = 0; n < NG; ++n) {
@@ -427,6 +427,28 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
     for (int n = 0; n < 2 * NG; ++n)
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[n].x[e] = 0.f;
+  };
+
+  auto over_keys = [](float x) {
+#pragma unroll
+    for (int d = 4; d <= 16; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
+    return x;
+  };
+  // The sums of codes, which are all positive, and of the bottoms, about minus that, become one of the size of the result.
+  // (Only at the end of a long run, the result would be left with what the roundings of sums many times its size leave.)
+  auto meet = [&] {
+#pragma unroll
+    for (int n = 0; n < NG; ++n)
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float x = over_keys(bottoms[n][r]) * factor[n];
+        bottoms[n][r] = 0.f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          o[2 * n + t].x[r] = fmaf(x, 0x1p-24f, o[2 * n + t].x[r]);
+          o[2 * n + t].x[2 + r] = fmaf(x, 0x1p-20f, o[2 * n + t].x[2 + r]);
+        }
+      }
   };
 
   // The products of the group at.t, which lies in `stage`. EDGE: not all of its keys are seen, but [from, at.end).
@@ -528,7 +550,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
         const uint64_t alpha2 = pack2(alpha, alpha);
         l_run[r] = mul2(l_run[r], alpha2);
 #pragma unroll
-        for (int n = 0; n < NG; ++n) mids[n][r] *= alpha;
+        for (int n = 0; n < NG; ++n) bottoms[n][r] *= alpha;
 #pragma unroll
         for (int n = 0; n < 2 * NG; ++n) {
           o[n].x[r] *= alpha;
@@ -567,7 +589,8 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
         const float b = n & 1 ? bf16hi_to_f32(s1[n / 2]) : bf16lo_to_f32(s1[n / 2]);
         const float za = n & 1 ? bf16hi_to_f32(s0[NG / 2 + n / 2]) : bf16lo_to_f32(s0[NG / 2 + n / 2]);
         const float zb = n & 1 ? bf16hi_to_f32(s1[NG / 2 + n / 2]) : bf16lo_to_f32(s1[NG / 2 + n / 2]);
-        float x0, y0, x1, y1;
+        float x0, y0, x1, y1, bottom_a, bottom_b;  // (bottom: what a code of 0 stands for)
+        unpack2(fma2(pack2(a, b), pack2(-8.f, -8.f), pack2(za, zb)), bottom_a, bottom_b);
         const uint64_t scaled = mul2(pack2(a, b), pack2(factor[n], factor[n]));
         unpack2(mul2(pr[0], scaled), x0, y0);
         unpack2(mul2(pr[1], scaled), x1, y1);
@@ -575,7 +598,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
         for (int r = 0; r < 2; ++r) {
           float pa, pb;
           unpack2(pr[r], pa, pb);
-          mids[n][r] = fmaf(pa, za, fmaf(pb, zb, mids[n][r]));
+          bottoms[n][r] = fmaf(pa, bottom_a, fmaf(pb, bottom_b, bottoms[n][r]));
         }
         const uint32_t pb0 = transpose_8x8(pack_f16x2(x0, x1));
         const uint32_t pb1 = transpose_8x8(pack_f16x2(y0, y1));
@@ -586,7 +609,6 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
         for (int e = 0; e < 2; ++e) {
           const uint32_t ux = e ? x >> 8 : x, uy = e ? y >> 8 : y;
           Acc& d = o[2 * n + e];
-          d = mma_f16(kMinus8Even, kMinus8Odd, kMinus8Even, kMinus8Odd, pb0, pb1, d);
           d = mma_f16(codes_even(ux), codes_odd(ux), codes_even(uy), codes_odd(uy), pb0, pb1, d);
         }
       }
@@ -619,6 +641,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
         compute(stage, std::false_type{});
       __syncwarp();  // every lane is done with this stage before it is refilled
       it ^= 1;
+      if (here % kMeet == 1) meet();
     }
 
     // This warp is done with the unit: its rows and their (maximum, sum) go to the join.
@@ -630,19 +653,11 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
       query = load_q();
     }
     if (lane == 0 && done) p.warps[unit].y = static_cast<int>(w);
-    auto over_keys = [](float x) {
-#pragma unroll
-      for (int d = 4; d <= 16; d <<= 1) x += __shfl_xor_sync(0xffffffffu, x, d);
-      return x;
-    };
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       float la, lb;
       unpack2(l_run[r], la, lb);
       const float l = over_keys(la + lb);
-      float z[NG];
-#pragma unroll
-      for (int n = 0; n < NG; ++n) z[n] = over_keys(mids[n][r]);
       if (g0 + 2 * c + r < p.G) {
         const int64_t place = (static_cast<int64_t>(w) + unit) * kD4Heads + 2 * c + r;
         float* dst = p.part_o + place * D + 4 * g;
@@ -650,8 +665,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
         for (int n = 0; n < NG; ++n) {
           const float back = over(factor[n]), even = 0x1p24f * back, odd = 0x1p20f * back;
           *reinterpret_cast<float4*>(dst + 32 * n) =
-              make_float4(fmaf(o[2 * n].x[r], even, z[n]), fmaf(o[2 * n].x[2 + r], odd, z[n]),
-                          fmaf(o[2 * n + 1].x[r], even, z[n]), fmaf(o[2 * n + 1].x[2 + r], odd, z[n]));
+              make_float4(o[2 * n].x[r] * even, o[2 * n].x[2 + r] * odd, o[2 * n + 1].x[r] * even, o[2 * n + 1].x[2 + r] * odd);
         }
         if (g == 0) p.part_ml[place] = make_float2(m_run[r], l);
       }
