@@ -380,7 +380,7 @@ typedef struct {
   int32_t n_mod;
   int32_t mod_op[LF_MAX_MODS];
   float mod_arg[LF_MAX_MODS];
-  void* workspace;        /* device, >= lf_decode_4bit_workspace_bytes(...), 16-byte aligned */
+  void* workspace;        /* device, >= lf_decode_4bit_workspace_bytes(...) (may be 0), 16-byte aligned */
   size_t workspace_bytes;
   int32_t* status;
 } LfDecode4Args;

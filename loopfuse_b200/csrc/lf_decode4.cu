@@ -3,18 +3,18 @@
 // With codes c, scales s and midpoints z of the groups g of 32 columns (include/lf_sm100.h has the format),
 //   score_j = sum_g sK_jg (q_g . (cK_jg - 8)) + sum_g zK_jg sum(q_g)
 //   o       = sum_g sum_j (p_j sV_jg) cV_jg + sum_g sum_j p_j (zV_jg - 8 sV_jg),    p_j = 2^(score_j - m),
-// so a cache row is never unpacked to its values. A code in bits 0..3 (4..7) of an fp16 whose other bits are zero is the
-// subnormal number c 2^-24 (16 c 2^-24), which a matrix instruction multiplies exactly: one AND makes two operands of
-// codes, and the products, in fp32, are ordinary numbers again. Query rows, times a power of two that brings them into
-// fp16's range, are exact as well. Scales are applied to the scores of a group and to the weights.
+// so a cache row is never unpacked to its values. A code in bits 0..3 (4..7) of an fp16 whose other bits are zero is
+// the subnormal number c 2^-24 (16 c 2^-24), which a matrix instruction multiplies exactly: one AND makes two operands
+// of codes, and the products, in fp32, are ordinary numbers again. Query rows, times a power of two that brings them
+// into fp16's range, are exact as well. Scales are applied to the scores of a group and to the weights.
 //
-// Bound by HBM, 5/8 byte per value, if the instructions keep up: an SM has to take some 40 values a clock, its integer pipe
-// does 64 operations and its matrix instructions, 34 for 32 keys, 2 clocks each. 16 requests of up to 65536 keys, 32 heads on
-// 8, D = 128: 149 us, 4.9 TB/s (bytes once at HBM's rate 112); 64 of up to 4096 38 (19).
-// Built before: codes with an exponent set above them, 128 + c and 16 + c three bits up, 187 us (7 operations for 8 codes
-// where this takes 5, and offsets that cost long sums their last bits: an error of 0.015); codes as subnormal bf16 151,
-// with an error of 0.0024 from the weights' rounding where this has 0.0017; c - 8 by a product of the weights with a
-// constant in each step, 155.
+// Bound by HBM, 5/8 byte per value, if the instructions keep up: an SM has to take some 40 values a clock, its integer
+// pipe does 64 operations and its matrix instructions, 34 for 32 keys, 2 clocks each. 16 requests of up to 65536 keys,
+// 32 heads on 8, D = 128: 149 us, 4.9 TB/s (bytes once at HBM's rate 112); 64 of up to 4096 38 (19).
+// Built before: codes with an exponent set above them, 128 + c and 16 + c three bits up, 187 us (7 operations for 8
+// codes where this takes 5, and offsets that cost long sums their last bits: an error of 0.015); codes as subnormal
+// bf16 151, with an error of 0.0024 from the weights' rounding where this has 0.0017; c - 8 by a product of the weights
+// with a constant in each step, 155.
 #include "lf_cache4.cuh"
 #include "lf_packed.cuh"
 
@@ -25,7 +25,9 @@
 
 namespace lf {
 
-constexpr int kD4Warps = 4;
+constexpr int kD4Warps = 4, kD4DirectWarps = 8;  // of a CTA
+constexpr int d4_warps(bool direct) { return direct ? kD4DirectWarps : kD4Warps; }
+constexpr int kD4DirectGroups = 2 * kD4DirectWarps;  // of the longest unit, for DIRECT
 constexpr int kD4Stages = 2;  // groups of a warp's ring: one is copied while one is computed
 constexpr int kD4Group = 32;  // tokens that a warp takes at a time
 constexpr int kD4Run = 1;     // groups of a warp, at least
@@ -34,7 +36,6 @@ constexpr int kD4Scan = 128;  // up to so many requests, the join adds their len
 // CTAs of an SM: as many as fit without spilled registers (D = 128, 16 requests of up to 65536 keys: four 157 us, three
 // 149; D = 64, 32 of 8192: three 63, four 52).
 constexpr int d4_ctas(int D) { return D == 128 ? 3 : 4; }
-
 
 struct Decode4Params {
   const __nv_bfloat16* q;
@@ -63,8 +64,8 @@ struct Decode4Params {
 
   // Keys of a request that count: never more than the caller said.
   __device__ __forceinline__ int length(int b) const { return min(max(seq_lens[b], 0), max_len); }
-  // Of those, the first that the groups begin with: that of the sixteen which the window's first lies in (pages of 16, 32, ...
-  // then hold whole halves of a group).
+  // Of those, the first that the groups begin with: that of the sixteen which the window's first lies in (pages of
+  // 16, 32, ... then hold whole halves of a group).
   __device__ __forceinline__ int first_token(int end) const {
     return window > 0 && end > window ? (end - window) & ~15 : 0;
   }
@@ -187,10 +188,14 @@ struct D4Walk {
 //           2c + 9 and pairs halfwords of two keys. The weights, times the scale of a column group and rounded to
 //           fp16, get from the first product's layout to the second's by two 8 x 8 transposes.
 //
+// DIRECT: a CTA has one unit, its warps equal runs of that, and joins them itself: one launch where the units are few
+// and short.
 // EVEN: pages of a power of two of slots, 16 or more, whose rows lie next to each other: half a group is then one run
 // of bytes, and its place takes few operations (a lane's own row for each piece took 60 of a group's 820).
-template <int D, bool SOFTCAP, bool EVEN>
-__global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(const Decode4Params p) {
+template <int D, bool SOFTCAP, bool EVEN, bool DIRECT>
+__global__ void __launch_bounds__(d4_warps(DIRECT) * 32, DIRECT ? 1 : d4_ctas(D))
+    decode4_kernel(const Decode4Params p) {
+  constexpr int WARPS = DIRECT ? kD4DirectWarps : kD4Warps;
   using R = Record4<D>;
   constexpr int NG = R::kGroups;
   constexpr int kHalf = kD4Group * R::kBytes;  // keys, then values
@@ -206,42 +211,56 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
   const uint32_t w = warp * gridDim.x + blockIdx.x;
 
   D4Walk at;  // what is computed
-  // Groups of the requests [b, b + 32), one per lane.
-  auto groups_at = [&](int b) { return b + lane < p.B ? static_cast<uint32_t>(p.groups_of(p.length(b + lane))) : 0u; };
-  uint32_t all = 0, groups = 0;
-#pragma unroll 4
-  for (int b = 0; b < p.B; b += 32) {
-    groups = groups_at(b);
-    all += groups;
-  }
-  all = __reduce_add_sync(0xffffffffu, all) * p.heads;
-  const uint32_t run = p.run(all);
-  if (all <= w * run) return;  // (run times the warps is below 2^31 and 2^31 more)
-  int left = static_cast<int>(min(all - w * run, run));  // groups of this warp
-  {
-    uint32_t skip = w * run;  // of the requests ahead, then of the units ahead
-    uint32_t incl = 0;
-    unsigned past = 0;
-    int from = 0;
-    for (int b = 0; b < p.B && !past; b += 32) {
-      if (b) skip -= __shfl_sync(0xffffffffu, incl, 31);
-      if (p.B > 32) groups = groups_at(b);
-      from = b;
-      incl = groups * p.heads;
-#pragma unroll
-      for (int d = 1; d < 32; d <<= 1) {
-        const uint32_t x = __shfl_up_sync(0xffffffffu, incl, d);
-        if (lane >= d) incl += x;
-      }
-      past = __ballot_sync(0xffffffffu, incl > skip);
-    }
-    const int l = __ffs(past) - 1;
-    const uint32_t n = __shfl_sync(0xffffffffu, groups, l);
-    const uint32_t into = skip - __shfl_sync(0xffffffffu, incl, l) + n * p.heads;
-    at.b = from + l;
-    at.head = static_cast<int>(into / n);
+  int left;   // groups of this warp
+  if constexpr (DIRECT) {
+    at.b = blockIdx.x / p.heads;
+    at.head = blockIdx.x - at.b * p.heads;
     at.end = p.length(at.b);
-    at.t = p.first_token(at.end) + static_cast<int>(into - at.head * n) * kD4Group;
+    const int all = p.groups_of(at.end), run = (all + WARPS - 1) / WARPS;
+    at.t = p.first_token(at.end) + warp * run * kD4Group;
+    left = max(min(all - warp * run, run), 0);
+    if (p.status && at.head == 0 && threadIdx.x == 0) {
+      const int len = p.seq_lens[at.b];
+      if (len < 0 || len > p.max_len) atomicCAS(p.status, 0, LF_DEV_BAD_LENGTHS);
+    }
+  } else {
+    // Groups of the requests [b, b + 32), one per lane.
+    auto groups_at = [&](int b) { return b + lane < p.B ? static_cast<uint32_t>(p.groups_of(p.length(b + lane))) : 0u; };
+    uint32_t all = 0, groups = 0;
+#pragma unroll 4
+    for (int b = 0; b < p.B; b += 32) {
+      groups = groups_at(b);
+      all += groups;
+    }
+    all = __reduce_add_sync(0xffffffffu, all) * p.heads;
+    const uint32_t run = p.run(all);
+    if (all <= w * run) return;  // (run times the warps is below 2^31 and 2^31 more)
+    left = static_cast<int>(min(all - w * run, run));
+    {
+      uint32_t skip = w * run;  // of the requests ahead, then of the units ahead
+      uint32_t incl = 0;
+      unsigned past = 0;
+      int from = 0;
+      for (int b = 0; b < p.B && !past; b += 32) {
+        if (b) skip -= __shfl_sync(0xffffffffu, incl, 31);
+        if (p.B > 32) groups = groups_at(b);
+        from = b;
+        incl = groups * p.heads;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+          const uint32_t x = __shfl_up_sync(0xffffffffu, incl, d);
+          if (lane >= d) incl += x;
+        }
+        past = __ballot_sync(0xffffffffu, incl > skip);
+      }
+      const int l = __ffs(past) - 1;
+      const uint32_t n = __shfl_sync(0xffffffffu, groups, l);
+      const uint32_t into = skip - __shfl_sync(0xffffffffu, incl, l) + n * p.heads;
+      at.b = from + l;
+      at.head = static_cast<int>(into / n);
+      at.end = p.length(at.b);
+      at.t = p.first_token(at.end) + static_cast<int>(into - at.head * n) * kD4Group;
+    }
   }
   auto kv_head = [&](int head, int* g0) {
     const int kvh = static_cast<int>(p.div_groups.div(head));
@@ -328,7 +347,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
   // registers are what bounds the warps of an SM); and the sums of the columns, which go with the midpoints (sum_z) and,
   // times -8, with the scales (sum_s), as two or three bf16 each. Scores are in units of a power of two, of each
   // row, until they are scaled.
-  uint4* qf = reinterpret_cast<uint4*>(smem + kD4Warps * kD4Stages * kStageBytes) + warp * (32 * NG) + lane;
+  uint4* qf = reinterpret_cast<uint4*>(smem + WARPS * kD4Stages * kStageBytes) + warp * (32 * NG) + lane;
   uint32_t sum_z, sum_s;
   float row_a[2], row_c2[2];  // query heads 2c, 2c + 1: score = row_c2 x, or row_c2 tanh(row_a x)
   struct Query {
@@ -616,6 +635,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
   };
 
   // A group is looked up while the one before it is copied, and that while the one before that is computed.
+  if constexpr (DIRECT) clear();  // (for a warp without a group)
   Query query = load_q();
   copy_group(look_up(), 0);
   Place next = look_up();
@@ -625,7 +645,7 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
     take_q(query);
     clear();
     const int unit = at.b * p.heads + at.head, first = p.first_token(at.end);
-    if (lane == 0 && at.t == first) p.warps[unit].x = static_cast<int>(w);  // where the join finds the unit's parts
+    if (!DIRECT && lane == 0 && at.t == first) p.warps[unit].x = static_cast<int>(w);  // where the join finds its parts
     from = p.window > 0 ? at.end - p.window : 0;
     int here = min(left, (at.end - at.t + kD4Group - 1) / kD4Group);
     left -= here;
@@ -647,11 +667,12 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
     // This warp is done with the unit: its rows and their (maximum, sum) go to the join.
     int g0;
     kv_head(at.head, &g0);
-    const bool done = at.t >= at.end;
+    [[maybe_unused]] const bool done = at.t >= at.end;
     if (left > 0) {  // (the next one's queries come in under what is left to do: 64 requests of 1500 keys 39 -> 36 us)
       at.next_unit(p, lane);
       query = load_q();
     }
+    if constexpr (DIRECT) break;  // (a warp has one unit; its sums go to the others below)
     if (lane == 0 && done) p.warps[unit].y = static_cast<int>(w);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
@@ -672,6 +693,52 @@ __global__ void __launch_bounds__(kD4Warps * 32, d4_ctas(D)) decode4_kernel(cons
     }
   }
   cp_async_wait<0>();
+  if constexpr (DIRECT) {
+    constexpr int kPart = D + 2;
+    float* s_part = reinterpret_cast<float*>(smem);  // [warp][query head][D, maximum, sum], where the rings were
+    static_assert(WARPS * kD4Heads * kPart * 4 <= WARPS * kD4Stages * kStageBytes, "the parts lie in the rings");
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      float la, lb;
+      unpack2(l_run[r], la, lb);
+      const float l = over_keys(la + lb);
+      float* dst = s_part + (warp * kD4Heads + 2 * c + r) * kPart;
+#pragma unroll
+      for (int n = 0; n < NG; ++n) {
+        const float back = over(factor[n]), even = 0x1p24f * back, odd = 0x1p20f * back;
+        dst[32 * n + 4 * g] = o[2 * n].x[r] * even;
+        dst[32 * n + 4 * g + 1] = o[2 * n].x[2 + r] * odd;
+        dst[32 * n + 4 * g + 2] = o[2 * n + 1].x[r] * even;
+        dst[32 * n + 4 * g + 3] = o[2 * n + 1].x[2 + r] * odd;
+      }
+      if (g == 0) {
+        dst[D] = m_run[r];
+        dst[D + 1] = l;
+      }
+    }
+    __syncthreads();
+    int g0;
+    const int kvh = kv_head(blockIdx.x - at.b * p.heads, &g0);
+    for (int i = threadIdx.x; i < kD4Heads * D; i += WARPS * 32) {
+      const int head = i / D, col = i - head * D;
+      if (g0 + head >= p.G) break;
+      const float* src = s_part + head * kPart;
+      float m = -INFINITY;
+#pragma unroll
+      for (int x = 0; x < WARPS; ++x) m = fmaxf(m, src[x * kD4Heads * kPart + D]);
+      const float m_safe = m == -INFINITY ? 0.f : m;
+      float l = 0.f, y = 0.f;
+#pragma unroll
+      for (int x = 0; x < WARPS; ++x) {
+        const float wt = ex2_approx(src[x * kD4Heads * kPart + D] - m_safe);
+        l = fmaf(src[x * kD4Heads * kPart + D + 1], wt, l);
+        y = fmaf(src[x * kD4Heads * kPart + col], wt, y);
+      }
+      p.out[at.b * p.o_stride[0] + kvh * p.o_stride[1] + (g0 + head) * p.o_stride[2] + col] =
+          __float2bfloat16_rn(l == 0.f ? 0.f : y / l);
+    }
+  }
 }
 
 // out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the parts of a row's unit, which WARPS warps share. Bound by the
@@ -791,6 +858,7 @@ __global__ void __launch_bounds__(128) decode4_join_kernel(const Decode4Params p
 
 // How a call is cut, and the room for its parts.
 struct Decode4Cut {
+  bool direct = false;
   int ctas = 0, heads = 1;
   int64_t units = 0;
   size_t parts = 0;  // rows
@@ -814,20 +882,29 @@ static Decode4Cut cut_decode4(int B, int Hkv, int G, int D, int window, int max_
   if (max_len <= 0) return c;
   c.heads = Hkv * ((G + kD4Heads - 1) / kD4Heads);
   c.units = static_cast<int64_t>(B) * c.heads;
+  // One launch, a CTA of eight warps a unit, where units have an SM each and are short (8 kv heads, D = 128): 4 requests
+  // of 100 keys 4.6 us a call instead of 7.8, 4 of 500 6.6 instead of 7.8, 16 of 500 6.7 instead of 10.0, but 4 of 1000
+  // 9.4 instead of 8.5. With twelve warps 5.1, 7.0 and 7.0.
+  if (c.units <= cached && most_groups(window, max_len) <= kD4DirectGroups) {
+    c.direct = true;
+    c.ctas = static_cast<int>(c.units);
+    c.units = 0;
+    return c;
+  }
   const int64_t runs = (c.units * most_groups(window, max_len) + kD4Run - 1) / kD4Run;
   c.ctas = static_cast<int>(std::min<int64_t>(runs, static_cast<int64_t>(d4_ctas(D)) * cached));
   c.parts = static_cast<size_t>(c.units + c.ctas * kD4Warps) * kD4Heads;
   return c;
 }
 
-template <int D, bool SOFTCAP, bool EVEN>
+template <int D, bool SOFTCAP, bool EVEN, bool DIRECT>
 static int launch_decode4(const Decode4Params& p, unsigned grid, cudaStream_t st) {
-  constexpr size_t smem = static_cast<size_t>(kD4Warps) * (kD4Stages * 2 * kD4Group * Record4<D>::kBytes + 16 * D);
+  constexpr size_t smem = static_cast<size_t>(d4_warps(DIRECT)) * (kD4Stages * 2 * kD4Group * Record4<D>::kBytes + 16 * D);
   static thread_local int configured_dev = -1;
-  const auto kernel = decode4_kernel<D, SOFTCAP, EVEN>;
+  const auto kernel = decode4_kernel<D, SOFTCAP, EVEN, DIRECT>;
   const int rc = packed_configure(kernel, smem, &configured_dev);
   if (rc != LF_OK) return rc;
-  launch_pdl(kernel, dim3(grid), kD4Warps * 32, smem, st, p);
+  launch_pdl(kernel, dim3(grid), d4_warps(DIRECT) * 32, smem, st, p);
   return check_launch("decode4_kernel");
 }
 
@@ -911,10 +988,14 @@ int lf_decode_4bit(const LfDecode4Args* a, void* stream) {
   auto with_d = [&](auto d) {
     constexpr int D = decltype(d)::value;
     if (cut.ctas > 0) {
-      const auto run = score.softcap ? (even ? launch_decode4<D, true, true> : launch_decode4<D, true, false>)
-                                     : (even ? launch_decode4<D, false, true> : launch_decode4<D, false, false>);
+      auto pick = [&](auto direct) {
+        constexpr bool DIRECT = decltype(direct)::value;
+        return score.softcap ? (even ? launch_decode4<D, true, true, DIRECT> : launch_decode4<D, true, false, DIRECT>)
+                             : (even ? launch_decode4<D, false, true, DIRECT> : launch_decode4<D, false, false, DIRECT>);
+      };
+      const auto run = cut.direct ? pick(std::true_type{}) : pick(std::false_type{});
       const int r = run(p, static_cast<unsigned>(cut.ctas), st);
-      if (r != LF_OK) return r;
+      if (r != LF_OK || cut.direct) return r;
     }
     if (p.n_warps > 6 * units)
       launch_pdl(decode4_join_kernel<D, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, st, p);

@@ -195,6 +195,54 @@ def test_lengths_and_pages_that_make_no_sense():
     assert (out == 0).all()
 
 
+@pytest.mark.parametrize("lens,Hkv,G,D,page,layout,cap,window", [
+    ([0, 1, 512, 257, 33], 2, 4, 128, 16, "head", 30.0, 0),
+    ([511, 480, 31, 0], 1, 11, 64, 32, "page", 0.0, 0),
+    ([512, 100, 0, 7], 2, 3, 128, 24, "slots", 0.0, 0),
+    ([3000, 1, 0, 496, 497, 498], 2, 8, 128, 16, "head", 0.0, 497),      # the longest that 16 groups hold
+    ([3000, 1, 0, 497, 498, 499], 2, 8, 64, 16, "page", 20.0, 498),
+])
+def test_few_short_requests_and_the_same_among_many(lens, Hkv, G, D, page, layout, cap, window):
+    """Few short requests take one launch; repeated until there are more of them than SMs, they take two. Lengths past
+    the longest that the caller gives, or below zero, are cut and reported in both."""
+    x = Batch(lens, Hkv, G, D, page, seed=7 + G, layout=layout)
+    longest = max(lens)
+    for times in (1, 80):
+        tile = lambda t: t.repeat(times, *[1] * (t.dim() - 1))  # noqa: E731, B023
+        q, table, seq_lens = tile(x.q), tile(x.table), tile(x.seq_lens)
+        for bad in (False, True):
+            st = F.new_status("cuda")
+            if bad:
+                seq_lens[seq_lens == longest], seq_lens[seq_lens == 0] = 2 ** 31 - 1, -1
+            out = F.decode_attention_4bit(q, *x.pools, table, seq_lens, window=window, scale=x.scale,
+                                          mods=softcap(cap), max_seq_len=longest, status=st)
+            if bad:
+                with pytest.raises(RuntimeError, match="max_seq_len"):
+                    F.check_status(st)
+            else:
+                F.check_status(st)
+            for t in (0, times - 1):
+                x.check(out[t * len(lens):(t + 1) * len(lens)], cap, window)
+    # a group that is infinite, in one request alone; a page that is not there
+    st = F.new_status("cuda")
+    short = lens.index(min(n for n in lens if n > 0))
+    last = lens[short] - 1
+    x.pools[1][x.table[short, last // page].item(), last % page, 0, D // 2:D // 2 + 2] = \
+        torch.tensor([0x80, 0x7f], dtype=torch.uint8, device="cuda")     # its first scale
+    out = F.decode_attention_4bit(x.q, *x.pools, x.table, x.seq_lens, window=window, scale=x.scale,
+                                  mods=softcap(cap), max_seq_len=longest, status=st)
+    F.check_status(st)
+    assert not out[short, 0, :, :32].isfinite().any() and out[short, 0, :, 32:].isfinite().all()
+    rest = [b for b in range(len(lens)) if b != short]
+    assert out[rest].isfinite().all() and out[short, 1:].isfinite().all()
+    x.table[0, 0] = 10 ** 6
+    x.table[short, last // page] = -4
+    F.decode_attention_4bit(x.q, *x.pools, x.table, x.seq_lens, window=window, scale=x.scale, mods=softcap(cap),
+                            max_seq_len=longest, status=st)
+    with pytest.raises(RuntimeError, match="page id"):
+        F.check_status(st)
+
+
 def test_a_key_with_an_infinite_group_reaches_only_its_request_and_columns():
     x = Batch([20, 20], 1, 2, 64, 16, seed=12)
     at = x.table[0, 0].item()

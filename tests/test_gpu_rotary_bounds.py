@@ -20,7 +20,7 @@ def test_rotary_and_4bit_entry_points_stay_in_range():
     code = ("import sys, pytest; sys.path.insert(0, '.'); from loopfuse_b200 import _native; "
             "assert _native.load().lf_debug_bounds() == 1; "
             "sys.exit(pytest.main(['-q', '-x', '-m', 'gpu', '-p', 'no:cacheprovider', '-k', "
-            "'append or gather or rotation_bits or test_decode or window or sense or serving', "
+            "'append or gather or rotation_bits or test_decode or few_short or window or sense or serving', "
             "'tests/test_gpu_rotary.py', 'tests/test_gpu_decode4.py']))")
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, env=env, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and " passed" in r.stdout, r.stdout[-3000:] + r.stderr[-2000:]

@@ -82,7 +82,7 @@ def test_decode_refusals(native_lib):
     call = lambda a: native_lib.lf_decode_4bit(C.byref(a), None)  # noqa: E731
     assert call(_native.LfDecode4Args()) == INVALID
     for code, change in [
-            (UNSUPPORTED, dict(D=32)), (UNSUPPORTED, dict(G=129)), (INVALID, dict(max_seq_len=129)),
+            (UNSUPPORTED, dict(D=32)), (UNSUPPORTED, dict(G=129)), (INVALID, dict(max_seq_len=1025)),
             (INVALID, dict(window=-1)), (INVALID, dict(B=0)), (TOO_LARGE, dict(B=65536)),
             (ALIGNMENT, dict(k=0x1002)), (ALIGNMENT, dict(k_stride=(640, 20, 320))),
             (ALIGNMENT, dict(q_stride=(384, 192, 60))), (ALIGNMENT, dict(o_stride=(384, 192, 62))),
@@ -91,7 +91,7 @@ def test_decode_refusals(native_lib):
         a = _native.LfDecode4Args()
         for name in ("q", "k", "v", "out", "block_table", "seq_lens"):
             setattr(a, name, 0x1000)
-        fill(a, B=4, Hkv=2, G=3, D=64, bt_blocks=8, page_size=16, n_pages=64, max_seq_len=128, scale=0.125,
+        fill(a, B=4, Hkv=2, G=3, D=64, bt_blocks=64, page_size=16, n_pages=64, max_seq_len=1024, scale=0.125,
              q_stride=(384, 192, 64), o_stride=(384, 192, 64), k_stride=(1280, 40, 640), v_stride=(1280, 40, 640))
         assert call(fill(a, **change)) == code, change
 
@@ -100,8 +100,9 @@ def test_workspace_holds_a_part_for_every_warp_and_unit(native_lib):
     size = native_lib.lf_decode_4bit_workspace_bytes
     assert size(4, 8, 4, 128, 0, 0) == 0
     assert size(4, 8, 129, 128, 0, 64) == 0
-    for B, Hkv, G, D, window, longest in ((1, 1, 1, 64, 0, 1), (4, 8, 4, 128, 0, 500), (37, 4, 3, 64, 100, 1500),
-                                          (3, 2, 17, 128, 0, 70)):
+    assert size(4, 8, 4, 128, 0, 500) == 0               # few short units: their CTAs join them
+    for B, Hkv, G, D, window, longest in ((1, 1, 1, 64, 0, 1000), (64, 8, 4, 128, 0, 500), (37, 5, 3, 64, 100, 1500),
+                                          (3, 2, 17, 128, 0, 700)):
         units = B * Hkv * -(-G // 8)
         assert size(B, Hkv, G, D, window, longest) >= (units + 4) * 8 * (D + 2) * 4 + units * 8
 
