@@ -1192,13 +1192,7 @@ Tensor run_decode4(const Tensor& q, const Tensor& k, const Tensor& v, const Tens
   if (max_len < 0) max_len = held;
   if (max_len > held)
     value_error("max_seq_len must lie in what the block table holds (" + std::to_string(held) + " tokens)");
-  if (!out.defined()) {
-    out = new_bf16(q.sizes(), dev);
-  } else {
-    require_cuda(out, dev);
-    check_bf16(out, "out");
-    if (out.sizes() != q.sizes()) value_error("out must have the shape of q");
-  }
+  out = out_like(std::move(out), q, dev, "out");
   LfDecode4Args a;
   std::memset(&a, 0, sizeof(a));
   a.q = q.data_ptr();

@@ -465,6 +465,7 @@ def decode_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.T
     128; request b sees its ``seq_lens[b]`` keys (int32 ``[B]``, its new one among them), with ``window`` the last
     ``window`` of those. A request of length 0 (a row of a padded batch) gets zeros.
 
-    ``max_seq_len`` and ``mods`` as for ``shared_prefix_decode_attention``."""
+    ``max_seq_len`` and ``mods`` as for ``shared_prefix_decode_attention``. ``out`` may be ``q``, but not lie across
+    it."""
     return _native.host().decode_4bit(q, k_pool, v_pool, block_table, seq_lens, window, max_seq_len, out,
                                       workspace, status, scale, mods)

@@ -358,3 +358,20 @@ def test_a_scale_of_zero_weighs_all_keys_alike():
     out = F.decode_attention_4bit(x.q, *x.pools, x.table, x.seq_lens, scale=0.0)
     x.scale = 0.0
     x.check(out)
+
+
+def test_output_in_place_of_the_queries_or_apart_from_them():
+    for lens in ([300, 12, 500], [2000, 12, 0]):         # one launch, and two
+        x = Batch(lens, 2, 3, 64, 16, seed=41)
+        args = (x.q, *x.pools, x.table, x.seq_lens)
+        want = F.decode_attention_4bit(*args, scale=x.scale, max_seq_len=max(lens))
+        room = torch.zeros(4, 2, 3, 64, dtype=BF16, device="cuda")
+        room[:3] = x.q
+        for out in (room[1:], room[:1].expand(3, -1, -1, -1), room[:3, :1].expand(-1, 2, -1, -1)):
+            with pytest.raises(ValueError, match="out "):
+                F.decode_attention_4bit(room[:3], *args[1:], scale=x.scale, max_seq_len=max(lens), out=out)
+        with pytest.raises(ValueError, match="out "):
+            F.decode_attention_4bit(*args, scale=x.scale, out=room)
+        assert F.decode_attention_4bit(room[:3], *args[1:], scale=x.scale, max_seq_len=max(lens),
+                                       out=room[:3]).data_ptr() == room.data_ptr()
+        assert torch.equal(room[:3], want) and (room[3] == 0).all()
