@@ -550,11 +550,11 @@ __global__ void __launch_bounds__(d4_warps(DIRECT) * 32, DIRECT ? 1 : d4_ctas(D)
           if (of > before) {
             const float f = power(254 + kFactor - static_cast<int>(field)), by = f * over(factor[2 * n + i]);
             factor[2 * n + i] = f;
-            if (before)
+            // (With the first scale above zero too: the sums of bottoms may have met, in units of the factor before.)
 #pragma unroll
-              for (int t = 0; t < 2; ++t)
+            for (int t = 0; t < 2; ++t)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[4 * n + 2 * i + t].x[e] *= by;
+              for (int e = 0; e < 4; ++e) o[4 * n + 2 * i + t].x[e] *= by;
           }
         }
         most[n] = now;

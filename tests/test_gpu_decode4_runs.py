@@ -1,0 +1,137 @@
+"""Decode attention over a 4-bit cache where a warp has many groups of 32 keys in a row, against float64 on the values
+that the records stand for: sums that meet in the middle of a run, scales and scores that move after they did.
+
+All requests read the same pages, so that a batch of many groups takes little memory; their lengths differ, so that
+units begin anywhere in a warp's run.
+
+Tolerance of an output column, with w the softmax weights, u those over the largest of them and S their sum:
+  2^-8 |o|                                    its own rounding to bf16
+  sum_j e_j (c_j + 8)                         e_j, of a key's weight times its scale: rounded to fp16, 2^-11 w_j s_j, or
+                                              where that is subnormal half a step, 2^-33 of the column group's largest
+                                              scale (a step is 2^-24 where that scale is 2^8 or more) over S
+  2 d sum_j w_j |v_j|                         what an error d of the scores does to the weights: the sums of the query
+                                              row enter with 16 bits, 2^-16 of 8 |q| s and of |q| |z|, and sums in fp32
+                                              are within 2^-20 of products of up to 15 |q| s
+  n_g 2^-21 sum_j w_j (|v_j| + s_j (c_j + 8)) sums in fp32 over n_g groups: four additions of a column per group (of
+                                              matrix products, which may cut instead of rounding: 2^-23), as many of the
+                                              bottoms and of the weights
+"""
+import pytest
+import torch
+
+from loopfuse_b200 import functional as F
+from tests import cache4
+
+pytestmark = pytest.mark.gpu
+BF16 = torch.bfloat16
+PAGE = 16
+
+
+def batch_for(run, D, Hkv, groups):
+    """Requests whose units give each warp of the GPU `run` groups (12 warps an SM at D = 128, 16 at 64)."""
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    return -(-run * sms * (12 if D == 128 else 16) // (Hkv * groups))
+
+
+class Shared:
+    """Requests that see the first lens[b] of the same keys, k and v [n, Hkv, D]."""
+
+    def __init__(self, k, v, lens, G, seed, page=PAGE, layout="head"):
+        n, Hkv, D = k.shape
+        g = torch.Generator().manual_seed(seed)
+        self.D, self.n, self.page = D, n, page
+        pages = -(-n // page)
+        ids = torch.randperm(pages + 2, generator=g)[:pages].cuda()
+        self.rec, self.pools = [], []
+        for x, value in ((k, False), (v, True)):
+            rec = cache4.encode(x.float().cuda(), value)
+            pool = torch.full((pages + 2, page, Hkv, rec.shape[-1]), 0xFF, dtype=torch.uint8, device="cuda")
+            j = torch.arange(n, device="cuda")
+            pool[ids[j // page], j % page] = rec
+            if layout == "head":
+                pool = pool.transpose(1, 2).contiguous().transpose(1, 2)
+            self.rec.append(rec)
+            self.pools.append(pool)
+        self.lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        self.table = ids.int()[None].expand(len(lens), -1)
+        self.q = torch.randn(len(lens), Hkv, G, D, generator=g).to(BF16).cuda()
+        self.scale = D ** -0.5
+
+    def run(self, **kw):
+        st = F.new_status("cuda")
+        out = F.decode_attention_4bit(self.q, *self.pools, self.table, self.lens, max_seq_len=self.n, scale=self.scale,
+                                      status=st, **kw)
+        F.check_status(st)
+        return out
+
+    def check(self, out, window=0):
+        ck, sk, zk = (x.transpose(0, 1) for x in cache4.parts(self.rec[0], self.D, False))    # Hkv, n, D
+        cv, sv, zv = (x.transpose(0, 1) for x in cache4.parts(self.rec[1], self.D, True))
+        keys, v = (zk + sk * ck).transpose(1, 2), zv + sv * cv
+        j = torch.arange(self.n, device="cuda")
+        for lo in range(0, len(self.lens), 32):
+            lens = self.lens[lo:lo + 32, None]
+            seen = j < lens
+            if window:
+                seen &= j >= lens - window
+            seen = seen[:, None, None]                                              # B, 1, 1, n
+            q = self.q[lo:lo + 32].double()                                         # B, Hkv, G, D
+            s = (q @ keys * self.scale).masked_fill(~seen, -torch.inf)
+            u = torch.exp(s - s.amax(-1, keepdim=True))
+            total = u.sum(-1, keepdim=True)
+            w = u / total
+            d = (2 ** -13 + 15 * 2 ** -20) * (q.abs() @ sk.transpose(1, 2)) + 2 ** -16 * (q.abs() @ zk.abs().transpose(1, 2))
+            d = (d * self.scale).masked_fill(~seen, 0).amax(-1, keepdim=True)
+            want = w @ v
+            # rounded weights: normal ones, and subnormal ones as if all were
+            highest = torch.where(seen[:, :, 0, :, None], sv[None], 0.0).amax(2)     # B, Hkv, D
+            e = torch.zeros_like(want)
+            for g in range(0, self.D, 32):
+                each = torch.maximum(2 ** -11 * w * sv[:, None, :, g], 2 ** -33 * highest[:, :, None, g, None] / total)
+                e[..., g:g + 32] = (each * seen) @ (cv + 8)[..., g:g + 32]
+            groups = -(-self.n // 32)
+            size = w @ (v.abs() + sv * (cv + 8))
+            tol = 2 ** -8 * want.abs() + e + 2 * d * (w @ v.abs()) + groups * 2 ** -21 * size
+            off = (out[lo:lo + 32].double() - want).abs()
+            assert (off <= tol).all(), (lo, (off / tol).nan_to_num(torch.inf).amax((1, 2, 3)).argmax().item(),
+                                        (off / tol).nan_to_num(torch.inf).max().item())
+
+
+def contexts(kind, n, Hkv, D, seed):
+    """Keys and values: what changes along a context, in its first third and behind it."""
+    g = torch.Generator().manual_seed(seed)
+    k, v = torch.randn(2, n, Hkv, D, generator=g)
+    j = torch.arange(n)[:, None, None].float()
+    first = j < n // 3
+    flat = torch.randn(n, Hkv, D // 32, generator=g).bfloat16().float().repeat_interleave(32, -1)  # one value a group
+    if kind == "growing":            # scales over 2^16, and scores that rise (or fall) along the context
+        v = v * 2.0 ** (16.0 * j / n - 8)
+        k[..., 0] += 12.0 * j[..., 0] / n
+    elif kind == "constant first":   # scales of zero and midpoints, until a meeting of the sums has come
+        v = torch.where(first, flat, v)
+    elif kind == "constant":
+        v = flat
+    elif kind == "constant, then tiny":
+        v = torch.where(first, 8 * flat, v * 2.0 ** -115)
+    elif kind == "tiny, then constant":
+        v = torch.where(first, v * 2.0 ** -115, flat * 2.0 ** 40)
+    elif kind == "tiny":
+        v = v * 2.0 ** -80
+    elif kind == "huge":
+        v = v * 2.0 ** 80
+    else:
+        assert kind == "plain"
+    return k, v
+
+
+@pytest.mark.parametrize("run,D,Hkv,G,n,page,layout,window", [
+    (17, 128, 8, 1, 1900, 16, "head", 0), (33, 64, 8, 1, 1900, 16, "head", 0), (80, 128, 8, 1, 1900, 16, "head", 0),
+    (18, 128, 8, 4, 1900, 16, "head", 0), (35, 128, 4, 9, 1900, 24, "page", 0), (20, 64, 8, 3, 1500, 24, "page", 0),
+    (21, 128, 8, 8, 1900, 16, "head", 1000), (100, 64, 8, 4, 3300, 16, "head", 0), (100, 128, 16, 2, 3300, 16, "head", 0)])
+@pytest.mark.parametrize("kind", ["plain", "growing", "constant first", "constant"])
+def test_long_runs(kind, run, D, Hkv, G, n, page, layout, window):
+    k, v = contexts(kind, n, Hkv, D, run)
+    B = -(-batch_for(run, D, Hkv, (window or n - 100) // 32) // -(-G // 8))
+    x = Shared(k, v, [n - 7 * b % 100 for b in range(B)], G, seed=run, page=page, layout=layout)
+    x.q[..., 0] = torch.where(x.q[..., 0] < 0, -8.0, 8.0)           # up or down with the keys' first column
+    x.check(x.run(window=window), window)
