@@ -586,7 +586,7 @@ int lf_kv_gather_4bit(const LfGather4Args* args, void* stream);
  * times its scale is rounded to fp16 once per group of columns; weights below 2^-33 of the largest are lost, and
  * columns of q below 2^-24 of the row's largest). Score functions as for
  * lf_packed_prefill_bf16. A request of length 0 gets zeros. With a window, table entries in front of its first
- * key are not read. Values of keys that a request sees must be finite. B up to 65535. The last bits
+ * key are not read. Values of keys that a request sees must be finite, those of V below 2^90. B up to 65535. The last bits
  * may change with the batch, never between two calls of the same one. */
 int lf_decode_4bit(const LfDecode4Args* args, void* stream);
 size_t lf_decode_4bit_workspace_bytes(int32_t B, int32_t Hkv, int32_t G, int32_t D, int32_t window,

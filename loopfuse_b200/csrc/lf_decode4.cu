@@ -126,6 +126,9 @@ __device__ __forceinline__ uint32_t codes_odd(uint32_t w) { return w & 0x00f000f
 // group's factor at most 2^11, so that their product is an fp16; weights below 2^-33 of the largest are lost.
 constexpr float kRise = 4.f;
 constexpr int kFactor = 11;
+constexpr int kLargestFactorLog2 = 125;  // of a column group
+constexpr int kLargestSumLog2 = 100;     // of what becomes a column's sum at a time
+constexpr float kLargestSum = 0x1p100f;
 constexpr int kMeet = 16;  // groups after which the sums of codes and bottoms meet (8 and 64: within 1 %)
 
 template <int BYTES>
@@ -455,19 +458,51 @@ __global__ void __launch_bounds__(d4_warps(DIRECT) * 32, DIRECT ? 1 : d4_ctas(D)
   };
   // The sums of codes, which are all positive, and of the bottoms, about minus that, become one of the size of the result.
   // (Only at the end of a long run, the result would be left with what the roundings of sums many times its size leave.)
+  // A sum of bottoms times its group's factor has to stay in fp32: midpoints of 8 over scales of 2^-115 would be infinite
+  // with the factor that follows from these alone. A sum that is past the limit lowers the factor to what it bears; the
+  // first that is not zero sets one where there was no scale yet, so that what has met is never brought up.
   auto meet = [&] {
+    bool past = false;
 #pragma unroll
-    for (int n = 0; n < NG; ++n)
+    for (int n = 0; n < NG; ++n) {
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float x = over_keys(bottoms[n][r]) * factor[n];
-        bottoms[n][r] = 0.f;
+      for (int r = 0; r < 2; ++r) bottoms[n][r] = over_keys(bottoms[n][r]);
+      const float big = fmaxf(fabsf(bottoms[n][0]), fabsf(bottoms[n][1]));
+      past = past || big * 0x1p-20f * factor[n] > kLargestSum || (!(most[n / 2] & 0xffffu << (16 * (n & 1))) && big > 0.f);
+    }
+    if (__any_sync(0xffffffffu, past)) {
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-          o[2 * n + t].x[r] = fmaf(x, 0x1p-24f, o[2 * n + t].x[r]);
-          o[2 * n + t].x[2 + r] = fmaf(x, 0x1p-20f, o[2 * n + t].x[2 + r]);
+      for (int n = 0; n < NG; ++n) {
+        float big = fmaxf(fabsf(bottoms[n][0]), fabsf(bottoms[n][1]));
+#pragma unroll
+        for (int d = 1; d <= 2; d <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, d));
+        // (big < 2^(e - 126), e its exponent's field.)
+        const int e = __float_as_int(big) >> 23, f = min(kLargestSumLog2 + 20 + 126 - e, kLargestFactorLog2);
+        const uint32_t half = 0xffffu << (16 * (n & 1));
+        if (most[n / 2] & half ? power(127 + f) < factor[n] : big > 0.f) {
+          const float by = power(127 + f) * over(factor[n]);
+          factor[n] = power(127 + f);
+          most[n / 2] = (most[n / 2] & ~half) | (127u + kFactor - f) << (7 + 16 * (n & 1));
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[2 * n + t].x[i] *= by;
         }
       }
+    }
+#pragma unroll
+    for (int n = 0; n < NG; ++n) {
+      const float even = 0x1p-24f * factor[n], odd = 0x1p-20f * factor[n];
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          o[2 * n + t].x[r] = fmaf(bottoms[n][r], even, o[2 * n + t].x[r]);
+          o[2 * n + t].x[2 + r] = fmaf(bottoms[n][r], odd, o[2 * n + t].x[2 + r]);
+        }
+        bottoms[n][r] = 0.f;
+      }
+    }
   };
 
   // The products of the group at.t, which lies in `stage`. EDGE: not all of its keys are seen, but [from, at.end).
@@ -543,14 +578,14 @@ __global__ void __launch_bounds__(d4_warps(DIRECT) * 32, DIRECT ? 1 : d4_ctas(D)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const uint32_t of = (top[n] >> (16 * i)) & 0xffffu, before = (most[n] >> (16 * i)) & 0xffffu;
-          // (Up to four times as large, none moves it again. From 2^-114 to 2^127; what is beyond is zero or no number.)
-          const uint32_t wanted = min(max(((of & 0x7fffu) >> 7) + 3u, 13u), 254u);
+          // (Up to four times as large, none moves it again. From 2^-114 to 2^127; scales below lose bits.)
+          const uint32_t wanted = min(max(((of & 0x7fffu) >> 7) + 3u, 127u + kFactor - kLargestFactorLog2), 254u);
           const uint32_t field = of > before ? max(wanted, before >> 7) : before >> 7;
           now |= (field << 7) << (16 * i);
           if (of > before) {
             const float f = power(254 + kFactor - static_cast<int>(field)), by = f * over(factor[2 * n + i]);
             factor[2 * n + i] = f;
-            // (With the first scale above zero too: the sums of bottoms may have met, in units of the factor before.)
+            // (With the first scale above zero too, where o is zero or holds sums that met before it.)
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll

@@ -135,3 +135,13 @@ def test_long_runs(kind, run, D, Hkv, G, n, page, layout, window):
     x = Shared(k, v, [n - 7 * b % 100 for b in range(B)], G, seed=run, page=page, layout=layout)
     x.q[..., 0] = torch.where(x.q[..., 0] < 0, -8.0, 8.0)           # up or down with the keys' first column
     x.check(x.run(window=window), window)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("kind", ["constant, then tiny", "tiny, then constant", "tiny", "huge"])
+def test_midpoints_and_scales_of_other_sizes(kind, D):
+    """Midpoints that are many times all scales of their columns, in front of these and behind them."""
+    k, v = contexts(kind, 1900, 8, D, 3)
+    B = batch_for(40, D, 8, 56)
+    x = Shared(k, v, [1900 - 7 * b % 100 for b in range(B)], 1, seed=4)
+    x.check(x.run())
