@@ -381,14 +381,16 @@ __global__ void __launch_bounds__(d4_warps(DIRECT) * 32, DIRECT ? 1 : d4_ctas(D)
     }
 #pragma unroll
     for (int d = 1; d <= 2; d <<= 1) top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, d));
-    const int field = min(max(static_cast<int>(max(top >> 16, top & 0xffffu) >> 7), 30), 220);
-    const float up = power(268 - field), unit = power(field + 10);
+    const int field = min(max(static_cast<int>(max(top >> 16, top & 0xffffu) >> 7), 14), 254);  // (`up` is a number)
+    const float up = power(268 - field);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const float of_row = __shfl_sync(0xffffffffu, unit, 8 * c + 4 * r);
-      row_a[r] = p.a * of_row;
+      // (In two factors: the unit of a row of columns past 2^117 is no fp32.)
+      const int unit = __shfl_sync(0xffffffffu, field, 8 * c + 4 * r) + 10;
+      const float of_row = power(min(unit, 254)), rest = power(127 + max(unit - 254, 0));
       // (Neither zero nor infinite: with a masked score, or a score of zero, either would be NaN.)
-      row_c2[r] = SOFTCAP ? p.c2 : fminf(fmaxf(p.c2 * of_row, FLT_MIN), FLT_MAX);
+      row_a[r] = fminf(fmaxf(p.a * of_row * rest, -FLT_MAX), FLT_MAX);
+      row_c2[r] = SOFTCAP ? p.c2 : fminf(fmaxf(p.c2 * of_row * rest, FLT_MIN), FLT_MAX);
     }
     float sum[NG];
 #pragma unroll

@@ -145,3 +145,14 @@ def test_midpoints_and_scales_of_other_sizes(kind, D):
     B = batch_for(40, D, 8, 56)
     x = Shared(k, v, [1900 - 7 * b % 100 for b in range(B)], 1, seed=4)
     x.check(x.run())
+
+
+def test_queries_of_every_size():
+    """The largest column of a query row anywhere in the range of bfloat16, and a scale that brings the scores back."""
+    for n, D in ((300, 128), (2500, 64)):               # one launch, and two
+        k, v = contexts("plain", n, 2, D, 6)
+        for power in (-117, -100, -60, 90, 95, 100, 112, 120):
+            x = Shared(k, v, [n, n - 50], 4, seed=7)
+            x.q = (x.q.float() * 2.0 ** power).to(BF16)
+            x.scale *= 2.0 ** min(-power, 96)           # (a scale is below 10^30)
+            x.check(x.run())
