@@ -572,7 +572,7 @@ size_t lf_shared_prefix_workspace_bytes(int32_t B, int32_t Hkv, int32_t G, int32
  * norm each product and sum of the rotation is rounded once in fp32, so that the stored bits are defined. A
  * position outside the table is reported as LF_DEV_BAD_POSITION and takes the nearest row, a slot outside
  * the pool as LF_DEV_BAD_PAGE and is not written; slots must differ. q_out may be q and k_out k (same strides);
- * apart from that outputs must not overlap inputs. */
+ * apart from that outputs must not overlap inputs or each other, and the pools must lie apart (not checked here). */
 int lf_rotary_bf16(const LfRotaryArgs* args, void* stream);
 
 /* Keys and values of requests from a 4-bit cache as packed bf16 rows: what lf_packed_prefill_bf16 takes as

@@ -976,6 +976,42 @@ std::pair<Tensor, Tensor> new_bf16_pair(std::array<int64_t, 3> a, std::array<int
 
 std::array<int64_t, 3> sizes3(const Tensor& t) { return {t.size(0), t.size(1), t.size(2)}; }
 
+// Whether two tensors are the same rows.
+bool same_rows(const Tensor& a, const Tensor& b) {
+  if (a.data_ptr() != b.data_ptr() || a.sizes() != b.sizes()) return false;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1 && a.stride(i) != b.stride(i)) return false;
+  return true;
+}
+
+// Whether two bf16 tensors share no element, as far as addresses and strides tell: they lie behind one another, or, as
+// parts of one buffer (q, k and v of a projection), in turn: with S a stride of either, what remains of each modulo S is
+// an interval, and the two are apart on a circle of length S.
+bool rows_apart(const Tensor& a, const Tensor& b) {
+  const auto x = extent(a), y = extent(b);
+  if (x.first >= y.second || y.first >= x.second) return true;
+  const int64_t d = (y.first - x.first) / a.element_size();
+  auto interval = [](const Tensor& t, int64_t S) {
+    int64_t n = t.size(-1);
+    for (int64_t i = 0; i + 1 < t.dim(); ++i)
+      if (t.size(i) > 1 && t.stride(i) % S) n += (t.size(i) - 1) * t.stride(i);
+    return n;
+  };
+  for (const Tensor* t : {&a, &b})
+    for (int64_t i = 0; i + 1 < t->dim(); ++i) {
+      const int64_t S = t->stride(i);
+      if (S <= 0) continue;
+      const int64_t at = (d % S + S) % S;
+      if (at >= interval(a, S) && at + interval(b, S) <= S) return true;
+    }
+  return false;
+}
+
+void check_apart(const Tensor& out, const char* name, const Tensor& other, const char* other_name) {
+  if (!rows_apart(out, other))
+    value_error(std::string(name) + " and " + other_name + " share memory: an output has to lie apart from it");
+}
+
 // An output of `like`'s shape: made here, or the caller's, which may be `like` itself but not lie across it.
 Tensor out_like(Tensor out, const Tensor& like, const c10::Device& dev, const char* name) {
   if (!out.defined()) return new_bf16(like.sizes(), dev);
@@ -983,9 +1019,7 @@ Tensor out_like(Tensor out, const Tensor& like, const c10::Device& dev, const ch
   check_bf16(out, name);
   if (out.sizes() != like.sizes()) value_error(std::string(name) + " must have the shape of its input");
   check_rows_apart(out, name);
-  const auto x = extent(out), y = extent(like);
-  if (x.first < y.second && y.first < x.second &&
-      (out.data_ptr() != like.data_ptr() || out.strides() != like.strides()))
+  if (!same_rows(out, like) && !rows_apart(out, like))
     value_error(std::string(name) + " must be its input itself or lie apart from it");
   return out;
 }
@@ -1038,7 +1072,9 @@ void fill_rotary(LfRotaryArgs& a, const Tensor* q, const Tensor& k, const Tensor
     if (q->dim() != 3 || q->size(0) != T || q->size(2) != D || q->size(1) == 0)
       value_error("q must be [T, Hq, D] with the rows of k, got " + shape_text(q->sizes()) + " and " +
                   shape_text(k.sizes()));
+    const bool given = q_out.defined();
     q_out = out_like(std::move(q_out), *q, dev, "q_out");
+    if (given) check_apart(q_out, "q_out", k, "k");
     a.q = q->data_ptr();
     a.q_out = q_out.data_ptr();
     a.Hq = narrow_i32(q->size(1), "Hq");
@@ -1072,10 +1108,14 @@ std::pair<Tensor, Tensor> run_qk_norm_rotary(const Tensor& q, const Tensor& k, c
                                              const RotaryOptions& o) {
   const c10::Device dev = k.device();
   LfRotaryArgs a;
-  if (!q_out.defined() && !k_out.defined() && q.dim() == 3 && k.dim() == 3 && k.is_cuda())
-    std::tie(q_out, k_out) = new_bf16_pair(sizes3(q), sizes3(k), dev);
+  const bool made = !q_out.defined() && !k_out.defined() && q.dim() == 3 && k.dim() == 3 && k.is_cuda();
+  if (made) std::tie(q_out, k_out) = new_bf16_pair(sizes3(q), sizes3(k), dev);
   fill_rotary(a, &q, k, positions, table, q_weight, k_weight, o, q_out, status);
   k_out = out_like(std::move(k_out), k, dev, "k_out");
+  if (!made) {
+    check_apart(k_out, "k_out", q, "q");
+    check_apart(k_out, "k_out", q_out, "q_out");
+  }
   a.k_out = k_out.data_ptr();
   for (int i = 0; i < 2; ++i) a.ko_stride[i] = k_out.stride(i);
   check_rc(launch(dev, [&](void* st) { return lib.rotary(&a, st); }), "lf_rotary_bf16");
@@ -1088,12 +1128,14 @@ Tensor run_kv_append_rotary(const Tensor& k, const Tensor& v, const Tensor& k_po
                             const RotaryOptions& o) {
   const c10::Device dev = k.device();
   LfRotaryArgs a;
+  const bool given = q_out.defined();
   fill_rotary(a, q, k, positions, table, q_weight, k_weight, o, q_out, status);
   require_cuda(v, dev);
   check_bf16(v, "v_new");
   if (v.sizes() != k.sizes())
     value_error("k_new and v_new must be [T, Hkv, D], got " + shape_text(k.sizes()) + " and " +
                 shape_text(v.sizes()));
+  if (given) check_apart(q_out, "q_out", v, "v_new");
   check_i32(slots, dev, "slots", -1);
   if (slots.size(0) < k.size(0)) value_error("slots must have an entry for each new row");
   require_cuda(k_pool, dev);
@@ -1153,7 +1195,7 @@ std::pair<Tensor, Tensor> run_kv_gather4(const Tensor& k_pool, const Tensor& v_p
       value_error("k_out and v_out must be [num_tokens, Hkv, D], got " + shape_text(t->sizes()));
     check_rows_apart(*t, "k_out or v_out");
   }
-  if (T > 0 && k_out.data_ptr() == v_out.data_ptr()) value_error("k_out and v_out must not be the same rows");
+  if (!rows_apart(k_out, v_out)) value_error("k_out and v_out must not share rows");
   LfGather4Args a;
   std::memset(&a, 0, sizeof(a));
   a.k_pool = k_pool.data_ptr();

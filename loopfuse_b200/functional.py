@@ -407,8 +407,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, ta
     multiple of 16, columns are turned: column i with i + rot / 2, or with ``interleaved`` column 2 i with 2 i + 1.
     The others stay as they are. ``q_weight`` / ``k_weight`` (``[D]``, bfloat16 or float32):
     ``x * rsqrt(mean(x^2) + eps) * weight`` in front of it; without one that tensor's rows are only turned.
-    All in float32, rounded once. ``q_out`` may be ``q`` and ``k_out`` ``k``; apart from that the outputs must not
-    overlap the inputs. A position that the table has no row for takes the nearest (reported in ``status``)."""
+    All in float32, rounded once. ``q_out`` may be ``q`` and ``k_out`` ``k``; apart from that, outputs that share
+    rows with ``q``, ``k`` or each other are refused. A position that the table has no row for takes the nearest (reported in ``status``)."""
     return _native.host().qk_norm_rotary(q, k, positions, table, q_weight, k_weight, eps, interleaved, q_out,
                                          k_out, status)
 
@@ -424,7 +424,8 @@ def kv_append_rotary(k_new: torch.Tensor, v_new: torch.Tensor, k_pool: torch.Ten
     which hold bfloat16 ``[pages, page_size, Hkv, D]`` or 4 bits (``kv_cache_4bit``). A negative slot is skipped,
     the others must differ. ``slots`` and ``positions`` are those of ``plan_pages``.
 
-    With ``q`` ``[T, Hq, D]``, its normed and turned rows are returned (in ``q_out``, which may be ``q``): all that
+    With ``q`` ``[T, Hq, D]``, its normed and turned rows are returned (in ``q_out``, which may be ``q``, but not share
+    rows with it otherwise, nor with ``k_new`` or ``v_new``; the pools must lie apart from all of them): all that
     a step does between its projections and its attention, in one launch."""
     return _native.host().kv_append_rotary(k_new, v_new, k_pool, v_pool, slots, positions, table, q, q_weight,
                                            k_weight, eps, interleaved, q_out, status)
