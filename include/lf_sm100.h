@@ -582,9 +582,14 @@ int lf_rotary_bf16(const LfRotaryArgs* args, void* stream);
 int lf_kv_gather_4bit(const LfGather4Args* args, void* stream);
 
 /* Decode attention of requests of different lengths over a 4-bit paged cache, one token per request: what
- * lf_decode_paged_bf16 gives on the values that the records stand for, up to rounding (the weight of a key
- * times its scale is rounded to fp16 once per group of columns; weights below 2^-33 of the largest are lost, and
- * columns of q below 2^-24 of the row's largest). Score functions as for
+ * lf_decode_paged_bf16 gives on the values that the records stand for, up to rounding. In fewer than 32 bits are:
+ *   - the weight of a key (over the largest of its row) times its scale, rounded to fp16 once per group of columns: 11
+ *     bits where that product is at least 2^-22 of the largest scale which the group of columns has in the request, and
+ *     otherwise within 2^-33 of that scale, however small the weight of the key which has it;
+ *   - the sums of a query row over a group of columns, which multiply the midpoints and scales of K: 16 bits (D = 64: 24);
+ *   - tanh of a softcap: within 2^-11, as in lf_decode_bf16;
+ *   - columns of q below 2^-22 of the row's largest, which lose bits.
+ * Score functions as for
  * lf_packed_prefill_bf16. A request of length 0 gets zeros. With a window, table entries in front of its first
  * key are not read. Values of keys that a request sees must be finite, those of V below 2^90. B up to 65535. The last bits
  * may change with the batch, never between two calls of the same one. */

@@ -123,7 +123,9 @@ __device__ __forceinline__ uint32_t transpose_8x8(uint32_t x) {
 __device__ __forceinline__ uint32_t codes_even(uint32_t w) { return w & 0x000f000fu; }
 __device__ __forceinline__ uint32_t codes_odd(uint32_t w) { return w & 0x00f000f0u; }
 // Weights are at most 2^4 (the reference of a row moves when a score rises further above it), a scale times its column
-// group's factor at most 2^11, so that their product is an fp16; weights below 2^-33 of the largest are lost.
+// group's factor at most 2^11, so that their product is an fp16: with all its 11 bits down to 2^-22 of the group's largest
+// scale, and half a step, 2^-33 of that scale, off below. (The factor follows the largest scale alone: with the weights in
+// it, every rise of a score would move it.)
 constexpr float kRise = 4.f;
 constexpr int kFactor = 11;
 constexpr int kLargestFactorLog2 = 125;  // of a column group
@@ -348,8 +350,8 @@ __global__ void __launch_bounds__(d4_warps(DIRECT) * 32, DIRECT ? 1 : d4_ctas(D)
 
   // The query heads of a unit: columns of the first product, in the order that the codes have (in shared memory:
   // registers are what bounds the warps of an SM); and the sums of the columns, which go with the midpoints (sum_z) and,
-  // times -8, with the scales (sum_s), as two or three bf16 each. Scores are in units of a power of two, of each
-  // row, until they are scaled.
+  // times -8, with the scales (sum_s), as two or three bf16 each: as many as one more instruction has room for, 2^-17 of
+  // a group's share of a score or less. Scores are in units of a power of two, of each row, until they are scaled.
   uint4* qf = reinterpret_cast<uint4*>(smem + WARPS * kD4Stages * kStageBytes) + warp * (32 * NG) + lane;
   uint32_t sum_z, sum_s;
   float row_a[2], row_c2[2];  // query heads 2c, 2c + 1: score = row_c2 x, or row_c2 tanh(row_a x)

@@ -467,6 +467,8 @@ def decode_attention_4bit(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.T
     ``window`` of those. A request of length 0 (a row of a padded batch) gets zeros.
 
     ``max_seq_len`` and ``mods`` as for ``shared_prefix_decode_attention``. ``out`` may be ``q``, but not lie across
-    it."""
+    it. Weights times scales of V are rounded to 11 bits, against the largest scale of a request's column group
+    (``lf_decode_4bit`` in ``include/lf_sm100.h`` has this and what else is held in fewer than 32 bits); cached values
+    have to be finite, those of V below 2^90."""
     return _native.host().decode_4bit(q, k_pool, v_pool, block_table, seq_lens, window, max_seq_len, out,
                                       workspace, status, scale, mods)

@@ -156,3 +156,19 @@ def test_queries_of_every_size():
             x.q = (x.q.float() * 2.0 ** power).to(BF16)
             x.scale *= 2.0 ** min(-power, 96)           # (a scale is below 10^30)
             x.check(x.run())
+
+
+@pytest.mark.parametrize("ratio", [10, 16, 22, 26, 40])
+@pytest.mark.parametrize("D,n,B", [(128, 450, 3), (64, 1900, 4), (128, 1900, 0)])
+def test_weights_on_keys_whose_scales_are_far_below_the_largest(ratio, D, n, B):
+    """A third of the keys, in front or behind, has scales 2^ratio times the others' and weights of 2^-40: what the
+    others' weights lose is what the largest scale says, and up to a ratio of 2^16 or so it is nothing."""
+    for front in (True, False):
+        k, v = contexts("plain", n, 8, D, ratio)
+        far = torch.arange(n) < n // 3 if front else torch.arange(n) >= n - n // 3
+        k[far, :, 0] = -40.0 if D == 128 else -28.0
+        v[far] *= 2.0 ** ratio
+        lens = [n - 7 * b % 20 for b in range(B or batch_for(20, D, 8, 58))]
+        x = Shared(k, v, lens, 1, seed=ratio)
+        x.q[..., 0] = 8.0
+        x.check(x.run())
