@@ -309,6 +309,8 @@ typedef struct {
  * and column d stands for z + s * (c - 8), z and s those of group d / 32. A row x is stored as
  *   s = bf16((max - min) * (1/15)), z = bf16(min + 8 s), c = clamp(rint((x - z) * (1/s)) + 8, 0, 15),
  * each step rounded once in fp32 (s = 0: c = 8), so that every column is at most 0.51 s + |z| 2^-8 away.
+ * In all of this numbers below 2^-126 count as zeros: a group whose range is under 15 of those has s = 0, and its
+ * columns are 2^-122 away at most.
  * Groups with a NaN or infinity, or a range above the largest fp32, stand for NaN or infinities.
  * Order of the codes: those of a key's columns 32 g + 8 i .. + 7 are the 32-bit word g of piece i (of four,
  * D/8 bytes each), those of a value's columns 32 g + 4 i .. + 3 the 16-bit word g of piece i (of eight, D/16

@@ -368,3 +368,25 @@ def test_a_step_in_a_graph_on_another_stream():
         want = step(other, want_q)
         assert torch.equal(qs, want_q) and torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
         assert all(torch.equal(a, b) for a, b in zip(pools, other))
+
+
+def test_groups_of_the_smallest_numbers():
+    """Below 2^-126 numbers count as zeros: a group whose range is under 15 of these keeps its smallest column alone."""
+    T, Hkv, D = 64, 4, 128
+    _, k, v = rows(T, 1, Hkv, D, 60)
+    i = torch.arange(T, dtype=torch.int32, device="cuda")
+    table = cache4.rotary_table(T, D)
+    cos, sin = table.chunk(2, -1)
+    for power in (-112, -118, -121, -122, -123, -124, -126, -130):
+        kk, vv = ((x.double() * 2.0 ** power).to(BF16) for x in (k, v))
+        k_pool, v_pool = F.kv_cache_4bit(4, 16, Hkv, D)
+        F.kv_append_rotary(kk, vv, k_pool, v_pool, i, i, table)
+        for want, pool, value in ((cache4.turn(kk.double(), cos.double(), sin.double(), False), k_pool, False),
+                                  (vv.double(), v_pool, True)):
+            rec = pool.reshape(T, Hkv, -1)
+            _, s, z = cache4.parts(rec, D, value)
+            off = (cache4.decode(rec, D, value) - want).abs()
+            assert (off <= 0.51 * s + 2 ** -8 * z.abs() + 2.0 ** -122 + 2 ** -20 * want.abs().amax()).all(), power
+            if power == -112:
+                x = cache4.turn(kk.float(), cos, sin, False) if not value else vv.float()
+                assert torch.equal(rec, cache4.encode(x, value))
