@@ -21,10 +21,4 @@ inline bool record4_aligned(const void* p, const int64_t (&stride)[3], int D) {
   return reinterpret_cast<uintptr_t>(p) % a == 0 && stride[0] % a == 0 && stride[1] % a == 0 && stride[2] % a == 0;
 }
 
-inline int cache_page_shift(int page_size) {
-  for (int sh = 0; sh < 31; ++sh)
-    if ((1 << sh) == page_size) return sh;
-  return -1;
-}
-
 }  // namespace lf

@@ -18,6 +18,15 @@ namespace lf {
 void set_cuda_error(cudaError_t e, const char* where);
 int check_launch(const char* where);
 
+inline bool aligned_16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// n = 2^shift, or -1.
+inline int shift_of(int n) {
+  for (int sh = 0; sh < 31; ++sh)
+    if ((1 << sh) == n) return sh;
+  return -1;
+}
+
 // Division by a divisor fixed at launch time: q = (mulhi(n, mul) + n) >> shift (Granlund &
 // Montgomery's round-up method; exact for every 0 <= n < 2^31). The item decode of the
 // persistent kernels runs on one warp that gets few issue slots; real divisions (a few dozen

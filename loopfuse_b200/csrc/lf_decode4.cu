@@ -975,7 +975,7 @@ int lf_decode_4bit(const LfDecode4Args* a, void* stream) {
   const int64_t units = static_cast<int64_t>(a->B) * a->Hkv * head_groups;
   if (a->B > 65535 || units > (1 << 26) || units * most_groups(a->window, a->max_seq_len) > 0x7fffffff)
     return LF_ERR_TOO_LARGE;
-  if (!packed_aligned(a->q) || !packed_aligned(a->out) || !record4_aligned(a->k, a->k_stride, a->D) ||
+  if (!aligned_16(a->q) || !aligned_16(a->out) || !record4_aligned(a->k, a->k_stride, a->D) ||
       !record4_aligned(a->v, a->v_stride, a->D))
     return LF_ERR_ALIGNMENT;
   for (int i = 0; i < 3; ++i)
@@ -983,7 +983,7 @@ int lf_decode_4bit(const LfDecode4Args* a, void* stream) {
   const Decode4Cut cut = cut_decode4(a->B, a->Hkv, a->G, a->D, a->window, a->max_seq_len);
   const size_t need = cut.bytes(a->D);
   if (need && (!a->workspace || a->workspace_bytes < need)) return LF_ERR_WORKSPACE;
-  if (!packed_aligned(a->workspace)) return LF_ERR_ALIGNMENT;
+  if (!aligned_16(a->workspace)) return LF_ERR_ALIGNMENT;
 
   Decode4Params p = {};
   p.part_o = static_cast<float*>(a->workspace);
@@ -1009,7 +1009,7 @@ int lf_decode_4bit(const LfDecode4Args* a, void* stream) {
   p.max_len = a->max_seq_len;
   p.bt_blocks = a->bt_blocks;
   p.page_size = a->page_size;
-  p.page_shift = cache_page_shift(a->page_size);
+  p.page_shift = shift_of(a->page_size);
   p.n_pages = a->n_pages;
   p.a = score.a;
   p.c2 = score.c2;

@@ -180,7 +180,7 @@ extern "C" int lf_kv_gather_4bit(const LfGather4Args* a, void* stream) {
   p.T = a->T;
   p.Hkv = a->Hkv;
   p.page_size = a->page_size;
-  p.page_shift = cache_page_shift(a->page_size);
+  p.page_shift = shift_of(a->page_size);
   p.n_pages = a->n_pages;
   p.bt_blocks = a->bt_blocks;
   p.status = a->status;

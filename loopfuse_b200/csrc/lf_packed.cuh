@@ -1055,19 +1055,11 @@ inline int packed_score(float scale, int n_mod, const int32_t* op, const float* 
   return LF_OK;
 }
 
-inline bool packed_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 // Largest power of two that divides the page, up to a block: a copy of that many keys stays in one page.
 inline int packed_box(int page_size) {
   int box = 1;
   while (box < kPackedKeys && page_size % (box * 2) == 0) box *= 2;
   return box;
-}
-
-inline int packed_page_shift(int page_size) {
-  for (int sh = 0; sh < 31; ++sh)
-    if ((1 << sh) == page_size) return sh;
-  return -1;
 }
 
 // Maps of the pools [n_pages, page_size, Hkv, D] with strides (page, slot, kv head). Where both pools' groups
@@ -1083,7 +1075,7 @@ inline int packed_pool_maps(CUtensorMap* mk, CUtensorMap* mv, const void* k, con
   p->page_groups = even ? page_size / 8 : 0;
   p->box = packed_box(page_size);
   if (!even && p->box > 8) p->box = 8;
-  p->box_shift = packed_page_shift(p->box);
+  p->box_shift = shift_of(p->box);
   for (int i = 0; i < 2; ++i) {
     const int64_t* st = i ? v_st : k_st;
     TileMapSpec spec;

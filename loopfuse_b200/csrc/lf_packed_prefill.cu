@@ -317,7 +317,7 @@ int lf_packed_prefill_bf16(const LfPackedArgs* a, void* stream) {
   const bool no_keys = !paged && a->Tk == 0;
   const void* kv[2] = {no_keys ? a->q : a->k, no_keys ? a->q : a->v};
   if (!kv[0] || !kv[1]) return LF_ERR_INVALID_ARG;
-  if (!packed_aligned(a->q) || !packed_aligned(kv[0]) || !packed_aligned(kv[1]) || !packed_aligned(a->out))
+  if (!aligned_16(a->q) || !aligned_16(kv[0]) || !aligned_16(kv[1]) || !aligned_16(a->out))
     return LF_ERR_ALIGNMENT;
   if (a->o_stride[0] % 8 || a->o_stride[1] % 8) return LF_ERR_ALIGNMENT;
 
@@ -346,7 +346,7 @@ int lf_packed_prefill_bf16(const LfPackedArgs* a, void* stream) {
   p.m_first = score.m_first;
   p.bt_blocks = a->bt_blocks;
   p.page_size = paged ? a->page_size : 1;
-  p.page_shift = packed_page_shift(p.page_size);
+  p.page_shift = shift_of(p.page_size);
   p.n_pages = a->n_pages;
   p.status = a->status;
 

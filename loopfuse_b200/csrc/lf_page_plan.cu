@@ -210,14 +210,6 @@ __global__ void __launch_bounds__(256) kv_append_packed_kernel(const AppendPacke
   }
 }
 
-static bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-static int shift_of(int page_size) {
-  for (int sh = 0; sh < 31; ++sh)
-    if ((1 << sh) == page_size) return sh;
-  return -1;
-}
-
 static int sm_count_or(int fallback) {
   int dev = 0, n = fallback;
   if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev);
@@ -284,7 +276,7 @@ int lf_kv_append_packed_bf16(const LfKvAppendPackedArgs* a, void* stream) {
   if (a->D != 64 && a->D != 128) return LF_ERR_UNSUPPORTED;
   if (a->T == 0) return LF_OK;
   if (!a->k_new || !a->v_new || !a->k_pool || !a->v_pool || !a->slots) return LF_ERR_INVALID_ARG;
-  if (!aligned16(a->k_new) || !aligned16(a->v_new) || !aligned16(a->k_pool) || !aligned16(a->v_pool))
+  if (!aligned_16(a->k_new) || !aligned_16(a->v_new) || !aligned_16(a->k_pool) || !aligned_16(a->v_pool))
     return LF_ERR_ALIGNMENT;
   for (int i = 0; i < 3; ++i)
     if ((i < 2 && (a->kn_stride[i] % 8 || a->vn_stride[i] % 8)) || a->kp_stride[i] % 8 ||

@@ -482,8 +482,6 @@ __global__ void __launch_bounds__(256) rotary_odd_kernel(const RotaryParams p) {
   }
 }
 
-static bool rotary_aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 template <int D, int STORE, int LAYOUT>
 static void launch_rotary(const RotaryParams& p, bool few, unsigned grid, cudaStream_t st) {
   const auto normed = few ? rotary_kernel<D, 1, STORE, true, LAYOUT>
@@ -511,7 +509,7 @@ extern "C" int lf_rotary_bf16(const LfRotaryArgs* a, void* stream) {
   const bool four = pools && a->bits == 4;
   for (const void* ptr : {a->q, a->k, a->v, static_cast<const void*>(a->q_out), static_cast<const void*>(a->k_out),
                           static_cast<const void*>(a->table), a->q_weight, a->k_weight})
-    if (!rotary_aligned(ptr)) return LF_ERR_ALIGNMENT;
+    if (!aligned_16(ptr)) return LF_ERR_ALIGNMENT;
   for (int i = 0; i < 2; ++i) {
     if (a->k_stride[i] % 8) return LF_ERR_ALIGNMENT;
     if (a->q && (a->q_stride[i] % 8 || a->qo_stride[i] % 8)) return LF_ERR_ALIGNMENT;
@@ -522,7 +520,7 @@ extern "C" int lf_rotary_bf16(const LfRotaryArgs* a, void* stream) {
     if (!record4_aligned(a->k_pool, a->kp_stride, a->D) || !record4_aligned(a->v_pool, a->vp_stride, a->D))
       return LF_ERR_ALIGNMENT;
   } else if (pools) {
-    if (!rotary_aligned(a->k_pool) || !rotary_aligned(a->v_pool)) return LF_ERR_ALIGNMENT;
+    if (!aligned_16(a->k_pool) || !aligned_16(a->v_pool)) return LF_ERR_ALIGNMENT;
     for (int i = 0; i < 3; ++i)
       if (a->kp_stride[i] % 8 || a->vp_stride[i] % 8) return LF_ERR_ALIGNMENT;
   }
@@ -564,7 +562,7 @@ extern "C" int lf_rotary_bf16(const LfRotaryArgs* a, void* stream) {
   if (pools) {
     p.n_slots = a->n_pages * a->page_size;
     p.page_size = a->page_size;
-    p.page_shift = cache_page_shift(a->page_size);
+    p.page_shift = shift_of(a->page_size);
   }
   static thread_local int cached_dev = -1, sms = 148;
   int dev = 0;

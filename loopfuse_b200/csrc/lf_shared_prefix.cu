@@ -598,7 +598,7 @@ int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* a, void* stream) {
   if (rc != LF_OK) return rc;
   const int head_groups = (a->G + kOwnHeads - 1) / kOwnHeads;
   if (a->B > 65535 || static_cast<int64_t>(a->B) * a->Hkv * head_groups > (1 << 26)) return LF_ERR_TOO_LARGE;
-  if (!packed_aligned(a->q) || !packed_aligned(a->k) || !packed_aligned(a->v) || !packed_aligned(a->out))
+  if (!aligned_16(a->q) || !aligned_16(a->k) || !aligned_16(a->v) || !aligned_16(a->out))
     return LF_ERR_ALIGNMENT;
   for (int i = 0; i < 3; ++i)
     if (a->q_stride[i] % 8 || a->k_stride[i] % 8 || a->v_stride[i] % 8 || a->o_stride[i] % 4)
@@ -619,7 +619,7 @@ int lf_shared_prefix_decode_bf16(const LfSharedPrefixArgs* a, void* stream) {
   OwnParams po = {};
   CUtensorMap mq = {}, mk = {}, mv = {};
   int64_t prefix_ctas = 0;
-  const int page_shift = packed_page_shift(a->page_size);
+  const int page_shift = shift_of(a->page_size);
   if (cut.prefix_splits > 0) {
     pp.kv_lens = a->seq_lens;
     pp.table = a->block_table;
