@@ -11,7 +11,8 @@ Tolerance of an output column, with w the softmax weights, u those over the larg
                                               scale (a step is 2^-24 where that scale is 2^8 or more) over S
   2 d sum_j w_j |v_j|                         what an error d of the scores does to the weights: the sums of the query
                                               row enter with 16 bits, 2^-16 of 8 |q| s and of |q| |z|, and sums in fp32
-                                              are within 2^-20 of products of up to 15 |q| s
+                                              are within 2^-20 of products of up to 15 |q| s; with a softcap 2^-10
+                                              of the largest score (the unit's tanh is within 2^-11)
   n_g 2^-21 sum_j w_j (|v_j| + s_j (c_j + 8)) sums in fp32 over n_g groups: four additions of a column per group (of
                                               matrix products, which may cut instead of rounding: 2^-23), as many of the
                                               bottoms and of the weights
@@ -19,7 +20,9 @@ Tolerance of an output column, with w the softmax weights, u those over the larg
 import pytest
 import torch
 
+from loopfuse_b200 import _native
 from loopfuse_b200 import functional as F
+from loopfuse_b200 import spec as S
 from tests import cache4
 
 pytestmark = pytest.mark.gpu
@@ -57,14 +60,16 @@ class Shared:
         self.q = torch.randn(len(lens), Hkv, G, D, generator=g).to(BF16).cuda()
         self.scale = D ** -0.5
 
-    def run(self, **kw):
+    def run(self, cap=0.0, **kw):
         st = F.new_status("cuda")
+        if cap:
+            kw["mods"] = (S.ScoreMod(S.MOD_DIV, cap), S.ScoreMod(S.MOD_TANH), S.ScoreMod(S.MOD_MUL, cap))
         out = F.decode_attention_4bit(self.q, *self.pools, self.table, self.lens, max_seq_len=self.n, scale=self.scale,
                                       status=st, **kw)
         F.check_status(st)
         return out
 
-    def check(self, out, window=0):
+    def check(self, out, window=0, cap=0.0):
         ck, sk, zk = (x.transpose(0, 1) for x in cache4.parts(self.rec[0], self.D, False))    # Hkv, n, D
         cv, sv, zv = (x.transpose(0, 1) for x in cache4.parts(self.rec[1], self.D, True))
         keys, v = (zk + sk * ck).transpose(1, 2), zv + sv * cv
@@ -76,12 +81,18 @@ class Shared:
                 seen &= j >= lens - window
             seen = seen[:, None, None]                                              # B, 1, 1, n
             q = self.q[lo:lo + 32].double()                                         # B, Hkv, G, D
-            s = (q @ keys * self.scale).masked_fill(~seen, -torch.inf)
+            s = q @ keys * self.scale
+            if cap:
+                s = cap * torch.tanh(s / cap)
+            largest = s.masked_fill(~seen, 0).abs().amax(-1, keepdim=True)
+            s = s.masked_fill(~seen, -torch.inf)
             u = torch.exp(s - s.amax(-1, keepdim=True))
             total = u.sum(-1, keepdim=True)
             w = u / total
             d = (2 ** -13 + 15 * 2 ** -20) * (q.abs() @ sk.transpose(1, 2)) + 2 ** -16 * (q.abs() @ zk.abs().transpose(1, 2))
             d = (d * self.scale).masked_fill(~seen, 0).amax(-1, keepdim=True)
+            if cap:
+                d = d + 2 ** -10 * largest
             want = w @ v
             # rounded weights: normal ones, and subnormal ones as if all were
             highest = torch.where(seen[:, :, 0, :, None], sv[None], 0.0).amax(2)     # B, Hkv, D
@@ -137,6 +148,14 @@ def test_long_runs(kind, run, D, Hkv, G, n, page, layout, window):
     x.check(x.run(window=window), window)
 
 
+@pytest.mark.parametrize("D,G,page", [(64, 4, 16), (128, 1, 16), (128, 3, 24)])
+@pytest.mark.parametrize("kind", ["plain", "constant first"])
+def test_long_runs_under_a_softcap(kind, D, G, page):
+    k, v = contexts(kind, 1900, 8, D, 11)
+    x = Shared(k, v, [1900 - 7 * b % 100 for b in range(batch_for(25, D, 8, 56))], G, seed=12, page=page)
+    x.check(x.run(cap=20.0), cap=20.0)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("kind", ["constant, then tiny", "tiny, then constant", "tiny", "huge"])
 def test_midpoints_and_scales_of_other_sizes(kind, D):
@@ -156,6 +175,11 @@ def test_queries_of_every_size():
             x.q = (x.q.float() * 2.0 ** power).to(BF16)
             x.scale *= 2.0 ** min(-power, 96)           # (a scale is below 10^30)
             x.check(x.run())
+            if x.scale / 5.0 >= 1e6:                    # (what tanh takes is refused from there)
+                with pytest.raises(_native.LfError):
+                    x.run(cap=5.0)
+            elif power < 115:                           # (scale over cap is an fp32 above 2^-126)
+                x.check(x.run(cap=5.0), cap=5.0)
 
 
 @pytest.mark.parametrize("ratio", [10, 16, 22, 26, 40])
