@@ -8,13 +8,14 @@
 // of codes, and the products, in fp32, are ordinary numbers again. Query rows, times a power of two that brings them
 // into fp16's range, are exact as well. Scales are applied to the scores of a group and to the weights.
 //
-// Bound by HBM, 5/8 byte per value, if the instructions keep up: an SM has to take some 40 values a clock, its integer
-// pipe does 64 operations and its matrix instructions, 34 for 32 keys, 2 clocks each. 16 requests of up to 65536 keys,
-// 32 heads on 8, D = 128: 149 us, 4.9 TB/s (bytes once at HBM's rate 112); 64 of up to 4096 38 (19).
-// Built before: codes with an exponent set above them, 128 + c and 16 + c three bits up, 187 us (7 operations for 8
-// codes where this takes 5, and offsets that cost long sums their last bits: an error of 0.015); codes as subnormal
-// bf16 151, with an error of 0.0024 from the weights' rounding where this has 0.0017; c - 8 by a product of the weights
-// with a constant in each step, 155.
+// Bound by HBM, 5/8 byte per value, if the instructions keep up: an SM has to take some 40 values a clock. They do not
+// quite, though no pipe is full (issue slots 57 %, integer 49 %, tensor 21 %): the chains of dependent instructions in
+// 2.7 warps a scheduler, at 168 registers, leave slots empty. 16 requests of up to 65536 keys, 32 heads on 8, D = 128:
+// 149 to 165 us from box to box, 4.4 to 4.9 TB/s (bytes once at HBM's rate 112); 64 of up to 4096 38 to 42 (19).
+// Built before: codes with an exponent set above them, 128 + c and 16 + c three bits up, 187 us where this took 149 (7
+// operations for 8 codes where this takes 5, and offsets that cost long sums their last bits: an error of 0.015); codes
+// as subnormal bf16, as fast, with an error of 0.0024 from the weights' rounding where this has 0.0017; c - 8 by a
+// product of the weights with a constant in each step, 155.
 #include "lf_cache4.cuh"
 #include "lf_packed.cuh"
 
@@ -34,7 +35,7 @@ constexpr int kD4Run = 1;     // groups of a warp, at least
 constexpr int kD4Heads = 8;   // query heads that a warp computes together: the columns of a matrix instruction
 constexpr int kD4Scan = 128;  // up to so many requests, the join adds their lengths up itself
 // CTAs of an SM: as many as fit without spilled registers (D = 128, 16 requests of up to 65536 keys: four 157 us, three
-// 149; D = 64, 32 of 8192: three 63, four 52).
+// 149; D = 64, 32 of 8192: three 63, four 52), but for a softcap over pages of any kind at D = 128, which spills a word.
 constexpr int d4_ctas(int D) { return D == 128 ? 3 : 4; }
 
 struct Decode4Params {
@@ -781,9 +782,9 @@ __global__ void __launch_bounds__(d4_warps(DIRECT) * 32, DIRECT ? 1 : d4_ctas(D)
 }
 
 // out = sum_s o_s 2^(m_s - m) / sum_s l_s 2^(m_s - m) over the parts of a row's unit, which WARPS warps share. Bound by the
-// latency of its loads: which parts there are follows from the lengths, which it adds up while the products still run,
-// so that behind them there is one round trip to memory. Up to some eight parts a row, one warp each; four where there
-// are more (one request of 32768 keys: 1776 parts for 32 rows).
+// latency of its loads: which parts there are follows from the lengths, which it adds up while the products still run
+// (they are read in front of pdl_wait: the products' kernel waits for what is before it ahead of letting this one start),
+// so that behind them there is one round trip to memory.
 template <int D, int WARPS>
 __global__ void __launch_bounds__(128) decode4_join_kernel(const Decode4Params p) {
   constexpr int EPL = D / 32;
@@ -1036,6 +1037,10 @@ int lf_decode_4bit(const LfDecode4Args* a, void* stream) {
       const int r = run(p, static_cast<unsigned>(cut.ctas), st);
       if (r != LF_OK || cut.direct) return r;
     }
+    // Four warps a row where a unit has more than six warps' parts on average. Calls back to back, four / one, 8 kv heads
+    // of D = 128: 1 request of 32768 keys (222 parts a unit) 19.7 / 29.4 us, 9 of 2048 (25) 13.8 / 15.5, 32 of 2048 (7)
+    // 25.5 / 31.3, 64 of 2048 (3.5) 45.1 / 42.0. It does not fit everywhere: 16 of 4096 (14) 32.0 / 28.4, 37 of 2048
+    // (6) 28.6 / 35.4.
     if (p.n_warps > 6 * units)
       launch_pdl(decode4_join_kernel<D, 4>, dim3(static_cast<unsigned>(rows)), 128, 0, st, p);
     else

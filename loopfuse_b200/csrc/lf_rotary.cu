@@ -138,7 +138,10 @@ __device__ __forceinline__ uint32_t codes8(const float (&y)[8], const Group4& g)
 }
 
 // Heads of an item, and CTAs of an SM, with a norm and without: 21 thousand rows of 40 heads with a norm, four heads and
-// three CTAs 78 us, two and four 80; the append of 33 thousand rows, two and four 124, four and three 126.
+// three CTAs 78 us, two and four 80; the append of 33 thousand rows, two and four 124, four and three 126. (Chosen on
+// whole rotations without pools. Normed forms of four heads spill 24 to 140 bytes a thread at these registers, most of
+// them where a part is turned and pools are written: the append of 33 thousand rows with a norm takes 150 us whole, 156 in
+// pairs, 172 for a part, where it takes 127 to 131 without.)
 constexpr int rotary_heads(bool norm) { return norm ? 4 : 2; }
 constexpr int rotary_ctas(bool norm) { return norm ? 3 : 4; }
 

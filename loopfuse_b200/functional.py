@@ -408,7 +408,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, ta
     The others stay as they are. ``q_weight`` / ``k_weight`` (``[D]``, bfloat16 or float32):
     ``x * rsqrt(mean(x^2) + eps) * weight`` in front of it; without one that tensor's rows are only turned.
     All in float32, rounded once. ``q_out`` may be ``q`` and ``k_out`` ``k``; apart from that, outputs that share
-    rows with ``q``, ``k`` or each other are refused. A position that the table has no row for takes the nearest (reported in ``status``)."""
+    rows with ``q``, ``k`` or each other are refused. Outputs that are made here are one allocation: who keeps (or saves)
+    one keeps both. A position that the table has no row for takes the nearest (reported in ``status``)."""
     return _native.host().qk_norm_rotary(q, k, positions, table, q_weight, k_weight, eps, interleaved, q_out,
                                          k_out, status)
 
@@ -451,7 +452,8 @@ def kv_gather_4bit(k_pool: torch.Tensor, v_pool: torch.Tensor, block_table: torc
     """Keys and values of requests from a 4-bit cache as packed bfloat16 ``[num_tokens, Hkv, D]``: key j of
     request b, ``cu_seqlens_k[b + 1] - cu_seqlens_k[b]`` of them, is row ``cu_seqlens_k[b] + j``. With the same
     ``cu_seqlens_k`` they are the keys of ``packed_prefill_attention``: chunks of prompts over a 4-bit cache. Rows
-    that no request has are not written. A page that the table does not name reads as zeros (reported)."""
+    that no request has are not written. A page that the table does not name reads as zeros (reported). Outputs that are
+    made here are one allocation, of which either keeps the whole; ``k_out`` and ``v_out`` must not share rows."""
     return _native.host().kv_gather_4bit(k_pool, v_pool, block_table, cu_seqlens_k, num_tokens, k_out, v_out,
                                          status)
 
